@@ -1,7 +1,8 @@
 """Python wrappers over ``torch.ops.cuda_transformer`` with fake (meta)
 implementations -- the same ten functions, names and argument meaning as the
 reference's ``cuda_transformer/ops.py:4-139``, plus this implementation's
-LayerNorm and precision-explicit variants.
+LayerNorm and precision-explicit variants and the token-generation operators
+(paged key/value cache, one-token attention, logits processing).
 
 ``precision`` (the ``*_ex`` functions): 0 = 3xTF32 (FP32-accurate, the default
 of the plain functions), 1 = TF32, 2 = FP32 on the CUDA cores.  The plain
@@ -19,6 +20,8 @@ __all__ = [
     "flash_attention_fwd_ex", "flash_attention_bwd_ex", "cuda_fma_ex",
     "layernorm_fwd", "layernorm_bwd",
     "linear_fused", "linear_accumulate_", "cross_entropy_fwd_bwd_",
+    "kv_append_", "rotary_tables", "paged_attention", "paged_attention_workspace",
+    "logits_process",
 ]
 
 PRECISION_3XTF32 = 0
@@ -281,3 +284,98 @@ def cross_entropy_fwd_bwd_(logits: Tensor, targets: Tensor, ignore_index: int = 
 @torch.library.register_fake("cuda_transformer::cross_entropy_fwd_bwd_")
 def _(logits, targets, ignore_index):
     return logits.new_empty(logits.size(0))
+
+
+# ------------------------------------------------------------ token generation
+def rotary_tables(positions: int, rot: int, base: float = 10000.0, device=None):
+    """cos and sin of position * base^(-2i/rot), i < rot/2, for kv_append_:
+    FP32 [positions, rot/2], formed in FP64 (an FP32 angle loses its low bits
+    as the position grows)."""
+    inv = base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv
+    return angle.cos().float(), angle.sin().float()
+
+
+def kv_append_(k_cache: Tensor, v_cache: Tensor, k: Tensor, v: Tensor, block_table: Tensor,
+               positions: Tensor, seq_ids: Tensor | None = None, q: Tensor | None = None,
+               cos: Tensor | None = None, sin: Tensor | None = None, interleaved: bool = False,
+               want_k: bool = False) -> tuple[Tensor, Tensor]:
+    """Appends k, v [tokens, kv_heads, hs] to a paged cache, turning k (and q
+    [tokens, nh, hs]) by the rotary angles of their positions on the way.
+
+    k_cache, v_cache: [pages, kv_heads, page_size, hs], any order of the first
+    three in memory, float32, bfloat16 or float16 (k, v, q: float32 or the
+    cache's type).  block_table: int32 [batch, max_pages], the pages of each
+    sequence in order.  Token t goes to position positions[t] (int32) of
+    sequence seq_ids[t] (int32; default: sequence t).  cos, sin: float32
+    [positions, rot/2] (rotary_tables); element i pairs with i + rot/2, or 2i
+    with 2i + 1 when interleaved; None: no rotation.  A negative position is
+    padding (nothing appended, zero outputs); a token that has no place in the
+    cache gives NaN outputs.  Returns (turned q, turned k if want_k); unused
+    ones are empty."""
+    return torch.ops.cuda_transformer.kv_append_.default(
+        k_cache, v_cache, k, v, block_table, positions, seq_ids, q, cos, sin, interleaved, want_k)
+
+
+@torch.library.register_fake("cuda_transformer::kv_append_")
+def _(k_cache, v_cache, k, v, block_table, positions, seq_ids, q, cos, sin, interleaved, want_k):
+    _same_device(k, v, k_cache, v_cache, block_table, positions)
+    torch._check(k.dtype == v.dtype and k_cache.dtype == v_cache.dtype)
+    q_out = q.new_empty(q.shape) if q is not None else k.new_empty(0)
+    return q_out, k.new_empty(k.shape) if want_k else k.new_empty(0)
+
+
+def paged_attention_workspace(nh: int, kv_heads: int, hs: int, device=None) -> Tensor:
+    """The workspace of paged_attention for these heads, whatever the batch and
+    lengths: cleared once here, it serves any number of calls, but not two that
+    can run at the same time on different streams."""
+    size = torch.ops.cuda_transformer.paged_attention_workspace_size.default(nh, kv_heads, hs)
+    return torch.zeros(size, dtype=torch.uint8, device="cuda" if device is None else device)
+
+
+def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
+                    seq_lens: Tensor, scale: float | None = None,
+                    workspace: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """Attention of one new token per sequence, q [batch, nh, hs], over the
+    first seq_lens[b] (int32) tokens of a paged cache (kv_append_'s layout; nh
+    a multiple of kv_heads; cache rows 16-byte aligned).  Returns O
+    [batch, nh, hs] and L = logsumexp [batch, nh]; a length of 0 gives O = 0,
+    L = -inf, one that the table cannot hold gives NaN.  scale: hs^-0.5 by
+    default.  workspace: paged_attention_workspace's; a temporary one is
+    cleared for the call when it is not given."""
+    s = q.shape[-1] ** -0.5 if scale is None else scale
+    return torch.ops.cuda_transformer.paged_attention.default(q, k_cache, v_cache, block_table,
+                                                              seq_lens, s, workspace)
+
+
+@torch.library.register_fake("cuda_transformer::paged_attention")
+def _(q, k_cache, v_cache, block_table, seq_lens, scale, workspace):
+    _same_device(q, k_cache, v_cache, block_table, seq_lens)
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+def logits_process(logits: Tensor, tokens: Tensor | None = None, lens: Tensor | None = None,
+                   prompt_lens: Tensor | None = None, repetition: Tensor | None = None,
+                   frequency: Tensor | None = None, presence: Tensor | None = None,
+                   bias_ids: Tensor | None = None, bias_values: Tensor | None = None,
+                   mask: Tensor | None = None) -> Tensor:
+    """Sampling penalties, biases and a grammar mask on logits [rows, vocab]
+    (float32, bfloat16 or float16); returns new float32 logits.
+
+    tokens: int64 [rows, max_len] histories, lens (int32 [rows]) their lengths
+    (default: all of max_len), prompt_lens (int32 [rows]) how many of them are
+    the prompt (default: none).  repetition (float32 [rows]): x / r for x > 0,
+    else x * r, for every token of the history; frequency, presence (float32
+    [rows]): subtracted once per occurrence, and once, for tokens of the part
+    after the prompt.  bias_ids, bias_values (int64, float32 [rows, n]): added.
+    mask (int32 [rows, ceil(vocab/32)]): -inf where bit i % 32 of word i / 32
+    is 0.  Ids outside [0, vocab) are ignored."""
+    return torch.ops.cuda_transformer.logits_process.default(
+        logits, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values,
+        mask)
+
+
+@torch.library.register_fake("cuda_transformer::logits_process")
+def _(logits, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values,
+      mask):
+    return logits.new_empty(logits.shape, dtype=torch.float32)

@@ -31,6 +31,9 @@ PRECISION_FP32 = 2
 EPILOGUE_NONE = 0
 EPILOGUE_GELU = 1
 EPILOGUE_GELU_GRAD = 2
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+DTYPE_F16 = 2
 CT_FA2_BWD_NOALLOC_MAX_ROWS = 2097152  # batch * heads * seq_len limit of ct_fa2_bwd_noalloc
 CT_DEVSTAT_TIMEOUT = 1  # watchdog word bit: a bounded device-side wait ran out
 CT_WAIT_LIMIT_MIN_NS = 100000
@@ -79,6 +82,15 @@ SIGNATURES = {
     "ct_layernorm_bwd": ([_fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _i64, _i64, _fp, _sz, _fp],
                          _int),
     "ct_cross_entropy_fwd_bwd": ([_fp, _i64, _i64, _i64, _fp, _i64, _fp, _fp], _int),
+    "ct_kv_append": ([_fp, _i64p, _fp, _i64p, _fp, _i64p, _fp, _fp, _fp, _fp, _fp, _i64p, _fp,
+                      _i64p, _fp, _i64, _fp, _fp, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64,
+                      _i64, _i64, _i64, _int, _int, _fp], _int),
+    "ct_paged_attention_workspace_size": ([_i64, _i64, _i64], _sz),
+    "ct_paged_attention": ([_fp, _i64p, _fp, _i64p, _fp, _i64p, _fp, _i64, _fp, _fp, _fp, _i64,
+                            _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _int, _int, _fp,
+                            _sz, _fp], _int),
+    "ct_logits_process": ([_fp, _i64, _int, _fp, _i64, _i64, _i64, _fp, _i64, _i64, _fp, _fp, _fp,
+                           _fp, _fp, _fp, _i64, _fp, _i64, _i64, _fp, _i64, _fp], _int),
     "ct_set_wait_limit_ns": ([_int, ctypes.c_ulonglong], _int),
     "ct_get_wait_limit_ns": ([_int, ctypes.POINTER(ctypes.c_ulonglong)], _int),
     "ct_watchdog_selftest": ([_fp], _int),

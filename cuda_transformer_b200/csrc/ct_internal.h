@@ -178,6 +178,61 @@ int launch_layernorm_bwd(const float* x, const float* g, const float* mean, cons
 int launch_cross_entropy(float* x, int64_t ld, int64_t rows, int64_t vocab, const int64_t* targets,
                          int64_t ignore, float* loss_rows, cudaStream_t st);
 
+// -------------------------------------------------- token generation (decode)
+// A paged cache: [page, kv_head, slot, head_dim], unit stride along head_dim.
+struct PagedKv {
+  void* k;
+  void* v;
+  int64_t ks[3], vs[3];  // page, head, slot strides (elements)
+  const int32_t* table;  // [batch, max_pages]
+  int64_t table_s;
+  int64_t pages, max_pages;
+  int page_size;
+  int dtype;  // CT_DTYPE_*
+};
+struct KvAppend {
+  const void *q, *k, *v;
+  int64_t qs[3], ks[3], vs[3];  // token, head, dim
+  void *q_out, *k_out;
+  const float *cos, *sin;
+  PagedKv kv;
+  const int32_t *seq_ids, *positions;
+  int64_t tokens, q_heads, kv_heads, batch, max_positions;
+  int head_dim, rot_dim, act_dtype;
+  bool interleaved;
+};
+int launch_kv_append(const KvAppend& p, cudaStream_t st);
+struct PagedAttention {
+  const void* q;
+  int64_t qs[3];  // sequence, head, dim
+  PagedKv kv;
+  const int32_t* seq_lens;
+  void* out;
+  float* lse;
+  int64_t batch, q_heads, kv_heads;
+  int head_dim, act_dtype;
+  float scale;
+  void* ws;
+};
+size_t paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+int launch_paged_attention(const PagedAttention& p, const DeviceInfo& dev, cudaStream_t st);
+struct LogitsProcess {
+  const void* logits;
+  float* out;
+  int64_t ld, out_ld, rows, vocab;
+  const int64_t* tokens;
+  int64_t tokens_ld, max_len;
+  const int32_t *lens, *prompt_lens;
+  const float *repetition, *frequency, *presence;
+  const int64_t* bias_ids;
+  const float* bias_values;
+  int64_t bias_ld, bias_values_ld, bias_n;
+  const uint32_t* mask;
+  int64_t mask_ld;
+  int dtype;
+};
+int launch_logits_process(const LogitsProcess& p, cudaStream_t st);
+
 // ------------------------------------------------------------ watchdog
 // One CTA whose waits on a barrier phase that nothing completes run out after
 // the device's wait limit, followed by the kernels' abort teardown.

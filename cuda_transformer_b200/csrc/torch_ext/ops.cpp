@@ -429,6 +429,228 @@ std::tuple<Tensor, Tensor, Tensor> layernorm_bwd(Tensor x, Tensor gamma, Tensor 
   return {dx, dg, db};
 }
 
+// ---------------------------------------------------------- token generation
+int dtype_code(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return CT_DTYPE_F32;
+    case at::kBFloat16: return CT_DTYPE_BF16;
+    case at::kHalf: return CT_DTYPE_F16;
+    default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16");
+  }
+}
+
+void check_on(const Tensor& t, const Tensor& first, at::ScalarType type, const char* name) {
+  TORCH_CHECK(t.device() == first.device(), name, " must be on ", first.device());
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type);
+}
+
+// A dense 1-D operand of n elements (copied once if it is not dense); a null
+// pointer when it is absent.
+template <class T>
+const T* vector_of(const std::optional<Tensor>& t, int64_t n, const Tensor& first,
+                   at::ScalarType type, const char* name, Tensor* keep) {
+  if (!t.has_value()) return nullptr;
+  check_on(*t, first, type, name);
+  TORCH_CHECK(t->dim() == 1 && t->size(0) == n, name, " must have ", n, " elements");
+  *keep = t->contiguous();
+  return keep->const_data_ptr<T>();
+}
+
+// A [rows, n] operand with unit column stride (copied once if it has another).
+Tensor matrix_of(const Tensor& t, int64_t rows, const Tensor& first, at::ScalarType type,
+                 const char* name) {
+  check_on(t, first, type, name);
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows, name, " must be 2-D with ", rows, " rows");
+  return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous();
+}
+
+struct CacheArgs {
+  int64_t pages, heads, page_size, dim, batch, max_pages;
+  int dtype;
+  Tensor table;
+};
+
+CacheArgs check_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
+                      const Tensor& first) {
+  TORCH_CHECK(k_cache.is_cuda(), "k_cache must be a CUDA tensor");
+  TORCH_CHECK(k_cache.device() == first.device(), "k_cache must be on ", first.device());
+  TORCH_CHECK(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes(),
+              "k_cache, v_cache must be [pages, kv_heads, page_size, hs] of equal shape");
+  check_on(v_cache, k_cache, k_cache.scalar_type(), "v_cache");
+  check_on(table, k_cache, at::kInt, "block_table");
+  TORCH_CHECK(table.dim() == 2, "block_table must be [batch, max_pages]");
+  TORCH_CHECK(k_cache.stride(3) == 1 && v_cache.stride(3) == 1,
+              "k_cache, v_cache must have unit stride along hs");
+  CacheArgs a;
+  a.pages = k_cache.size(0);
+  a.heads = k_cache.size(1);
+  a.page_size = k_cache.size(2);
+  a.dim = k_cache.size(3);
+  a.batch = table.size(0);
+  a.max_pages = table.size(1);
+  a.dtype = dtype_code(k_cache, "k_cache");
+  a.table = table.stride(1) == 1 || a.max_pages <= 1 ? table : table.contiguous();
+  return a;
+}
+
+void strides3(const Tensor& t, int64_t out[3]) {
+  for (int i = 0; i < 3; ++i) out[i] = t.stride(i);
+}
+
+Tensor unit_last(const Tensor& t) { return t.stride(2) == 1 ? t : t.contiguous(); }
+
+// One new token's keys and values (and queries) into / beside the cache.
+std::tuple<Tensor, Tensor> kv_append_(Tensor k_cache, Tensor v_cache, Tensor k0, Tensor v0,
+                                      Tensor table0, Tensor positions,
+                                      std::optional<Tensor> seq_ids0, std::optional<Tensor> q0,
+                                      std::optional<Tensor> cos0, std::optional<Tensor> sin0,
+                                      bool interleaved, bool want_k) {
+  const CacheArgs c = check_cache(k_cache, v_cache, table0, k0);
+  const int act = dtype_code(k0, "k");
+  check_on(v0, k0, k0.scalar_type(), "v");
+  TORCH_CHECK(act == c.dtype || act == CT_DTYPE_F32, "k, v must be float32 or of the cache's type");
+  TORCH_CHECK(k0.dim() == 3 && v0.sizes() == k0.sizes() && k0.size(1) == c.heads &&
+                  k0.size(2) == c.dim,
+              "k, v must be [tokens, kv_heads, hs]");
+  c10::cuda::CUDAGuard guard(k0.device());
+  const int64_t tokens = k0.size(0);
+  const Tensor k = unit_last(k0), v = unit_last(v0);
+  Tensor keep_pos, keep_seq, q, cos, sin;
+  const int32_t* pos = vector_of<int32_t>(positions, tokens, k, at::kInt, "positions", &keep_pos);
+  const int32_t* seq = vector_of<int32_t>(seq_ids0, tokens, k, at::kInt, "seq_ids", &keep_seq);
+  int64_t q_heads = 0, rot = 0, max_positions = 0;
+  int64_t qs[3] = {0, 0, 1}, ks[3], vs[3], kcs[4], vcs[4];
+  Tensor q_out = at::empty({0}, k.options()), k_out = q_out;
+  if (q0.has_value()) {
+    check_on(*q0, k, k.scalar_type(), "q");
+    TORCH_CHECK(q0->dim() == 3 && q0->size(0) == tokens && q0->size(2) == c.dim,
+                "q must be [tokens, nh, hs]");
+    q = unit_last(*q0);
+    q_heads = q.size(1);
+    q_out = at::empty({tokens, q_heads, c.dim}, k.options());
+    strides3(q, qs);
+  }
+  if (want_k) k_out = at::empty({tokens, c.heads, c.dim}, k.options());
+  TORCH_CHECK(cos0.has_value() == sin0.has_value(), "cos and sin go together");
+  if (cos0.has_value()) {
+    check_on(*cos0, k, at::kFloat, "cos");
+    check_on(*sin0, k, at::kFloat, "sin");
+    TORCH_CHECK(cos0->dim() == 2 && sin0->sizes() == cos0->sizes() && 2 * cos0->size(1) <= c.dim,
+                "cos, sin must be [positions, rot/2] of equal shape, rot <= hs");
+    cos = cos0->contiguous();
+    sin = sin0->contiguous();
+    rot = 2 * cos.size(1);
+    max_positions = cos.size(0);
+  }
+  strides3(k, ks);
+  strides3(v, vs);
+  strides4(k_cache, kcs);
+  strides4(v_cache, vcs);
+  check_rc(ct_kv_append(q_heads ? q.const_data_ptr() : nullptr, qs, k.const_data_ptr(), ks,
+                        v.const_data_ptr(), vs, q_heads ? q_out.data_ptr() : nullptr,
+                        want_k ? k_out.data_ptr() : nullptr,
+                        rot ? cos.const_data_ptr<float>() : nullptr,
+                        rot ? sin.const_data_ptr<float>() : nullptr, k_cache.data_ptr(), kcs,
+                        v_cache.data_ptr(), vcs, c.table.const_data_ptr<int32_t>(),
+                        c.table.stride(0), seq, pos, tokens, q_heads, c.heads, c.dim, rot,
+                        interleaved ? 1 : 0, max_positions, c.batch, c.pages, c.page_size,
+                        c.max_pages, act, c.dtype, cur_stream()),
+           "kv_append_");
+  return {q_out, k_out};
+}
+
+int64_t paged_attention_workspace_size(int64_t nh, int64_t kv_heads, int64_t hs) {
+  return (int64_t)ct_paged_attention_workspace_size(nh, kv_heads, hs);
+}
+
+std::tuple<Tensor, Tensor> paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor table,
+                                           Tensor seq_lens, double scale,
+                                           std::optional<Tensor> workspace) {
+  const CacheArgs c = check_cache(k_cache, v_cache, table, q);
+  const int act = dtype_code(q, "q");
+  TORCH_CHECK(act == c.dtype || act == CT_DTYPE_F32, "q must be float32 or of the cache's type");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == c.dim, "q must be [batch, nh, hs]");
+  TORCH_CHECK(q.size(0) == c.batch, "block_table must have a row for each row of q");
+  c10::cuda::CUDAGuard guard(q.device());
+  const int64_t batch = q.size(0), heads = q.size(1);
+  Tensor keep_lens;
+  const int32_t* lens = vector_of<int32_t>(seq_lens, batch, q, at::kInt, "seq_lens", &keep_lens);
+  const int64_t need = paged_attention_workspace_size(heads, c.heads, c.dim);
+  Tensor ws;
+  if (workspace.has_value()) {
+    ws = *workspace;
+    check_on(ws, q, at::kByte, "workspace");
+    TORCH_CHECK(ws.is_contiguous() && ws.numel() >= need, "workspace must be dense, of ", need,
+                " bytes or more");
+  } else {
+    ws = at::zeros({need}, q.options().dtype(at::kByte));
+  }
+  Tensor out = at::empty({batch, heads, c.dim}, q.options());
+  Tensor lse = at::empty({batch, heads}, q.options().dtype(at::kFloat));
+  int64_t qs[3], kcs[4], vcs[4];
+  strides3(q, qs);
+  strides4(k_cache, kcs);
+  strides4(v_cache, vcs);
+  check_rc(ct_paged_attention(q.const_data_ptr(), qs, k_cache.const_data_ptr(), kcs,
+                              v_cache.const_data_ptr(), vcs, c.table.const_data_ptr<int32_t>(),
+                              c.table.stride(0), lens, out.data_ptr(), lse.data_ptr<float>(),
+                              batch, heads, c.heads, c.dim, c.pages, c.page_size, c.max_pages,
+                              (float)scale, act, c.dtype, ws.data_ptr(), (size_t)ws.numel(),
+                              cur_stream()),
+           "paged_attention");
+  return {out, lse};
+}
+
+Tensor logits_process(Tensor logits0, std::optional<Tensor> tokens0, std::optional<Tensor> lens0,
+                      std::optional<Tensor> prompt_lens0, std::optional<Tensor> repetition0,
+                      std::optional<Tensor> frequency0, std::optional<Tensor> presence0,
+                      std::optional<Tensor> bias_ids0, std::optional<Tensor> bias_values0,
+                      std::optional<Tensor> mask0) {
+  TORCH_CHECK(logits0.is_cuda(), "logits must be a CUDA tensor");
+  TORCH_CHECK(logits0.dim() == 2, "logits must be (rows, vocab)");
+  const int dtype = dtype_code(logits0, "logits");
+  c10::cuda::CUDAGuard guard(logits0.device());
+  const int64_t rows = logits0.size(0), vocab = logits0.size(1);
+  Tensor logits = matrix_of(logits0, rows, logits0, logits0.scalar_type(), "logits");
+  if (rows > 1 && logits.stride(0) < vocab) logits = logits.contiguous();  // a broadcast row
+  Tensor keep[5], tokens, ids, values, mask;
+  if (tokens0.has_value()) tokens = matrix_of(*tokens0, rows, logits, at::kLong, "tokens");
+  const int32_t* lens = vector_of<int32_t>(lens0, rows, logits, at::kInt, "lens", &keep[0]);
+  const int32_t* plens =
+      vector_of<int32_t>(prompt_lens0, rows, logits, at::kInt, "prompt_lens", &keep[1]);
+  const float* rep =
+      vector_of<float>(repetition0, rows, logits, at::kFloat, "repetition", &keep[2]);
+  const float* freq = vector_of<float>(frequency0, rows, logits, at::kFloat, "frequency", &keep[3]);
+  const float* pres = vector_of<float>(presence0, rows, logits, at::kFloat, "presence", &keep[4]);
+  TORCH_CHECK(bias_ids0.has_value() == bias_values0.has_value(),
+              "bias_ids and bias_values go together");
+  int64_t bias_n = 0;
+  if (bias_ids0.has_value()) {
+    ids = matrix_of(*bias_ids0, rows, logits, at::kLong, "bias_ids");
+    values = matrix_of(*bias_values0, rows, logits, at::kFloat, "bias_values");
+    bias_n = ids.size(1);
+    TORCH_CHECK(values.size(1) == bias_n, "bias_values must have bias_ids' shape");
+  }
+  if (mask0.has_value()) {
+    mask = matrix_of(*mask0, rows, logits, at::kInt, "mask");
+    TORCH_CHECK(mask.size(1) >= (vocab + 31) / 32, "mask must have ceil(vocab / 32) words a row");
+  }
+  Tensor out = at::empty({rows, vocab}, logits.options().dtype(at::kFloat));
+  check_rc(ct_logits_process(logits.const_data_ptr(), rows > 1 ? logits.stride(0) : vocab, dtype,
+                             out.data_ptr<float>(), vocab, rows, vocab,
+                             tokens.defined() ? tokens.const_data_ptr<int64_t>() : nullptr,
+                             tokens.defined() ? tokens.stride(0) : 0,
+                             tokens.defined() ? tokens.size(1) : 0, lens, plens, rep, freq, pres,
+                             bias_n ? ids.const_data_ptr<int64_t>() : nullptr,
+                             bias_n ? ids.stride(0) : 0,
+                             bias_n ? values.const_data_ptr<float>() : nullptr,
+                             bias_n ? values.stride(0) : 0, bias_n,
+                             mask.defined() ? mask.const_data_ptr<int32_t>() : nullptr,
+                             mask.defined() ? mask.stride(0) : 0, cur_stream()),
+           "logits_process");
+  return out;
+}
+
 // ------------------------------------------- materialised (naive) attention
 // Kept registered so cuda_autograd_fns imports; composed from this library's
 // own GEMM and softmax kernels.  qkv: (B, T, 3C) contiguous.
@@ -503,6 +725,10 @@ TORCH_LIBRARY(cuda_transformer, m) {
   m.def("linear_fused(Tensor x, Tensor weights, Tensor bias, int precision, int epilogue, Tensor? act_in, bool want_colsum) -> (Tensor, Tensor, Tensor)");
   m.def("linear_accumulate_(Tensor(a!) out, Tensor(b!)? colsum, Tensor x, Tensor weights, Tensor bias, int precision) -> ()");
   m.def("cross_entropy_fwd_bwd_(Tensor(a!) logits, Tensor targets, int ignore_index) -> Tensor");
+  m.def("kv_append_(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor k, Tensor v, Tensor block_table, Tensor positions, Tensor? seq_ids, Tensor? q, Tensor? cos, Tensor? sin, bool interleaved, bool want_k) -> (Tensor, Tensor)");
+  m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, float scale, Tensor(a!)? workspace) -> (Tensor, Tensor)");
+  m.def("paged_attention_workspace_size(int nh, int kv_heads, int hs) -> int", &paged_attention_workspace_size);
+  m.def("logits_process(Tensor logits, Tensor? tokens, Tensor? lens, Tensor? prompt_lens, Tensor? repetition, Tensor? frequency, Tensor? presence, Tensor? bias_ids, Tensor? bias_values, Tensor? mask) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(cuda_transformer, CUDA, m) {
@@ -524,6 +750,9 @@ TORCH_LIBRARY_IMPL(cuda_transformer, CUDA, m) {
   m.impl("linear_fused", &linear_fused);
   m.impl("linear_accumulate_", &linear_accumulate_);
   m.impl("cross_entropy_fwd_bwd_", &cross_entropy_fwd_bwd_);
+  m.impl("kv_append_", &kv_append_);
+  m.impl("paged_attention", &paged_attention);
+  m.impl("logits_process", &logits_process);
 }
 
 }  // namespace cuda_transformer

@@ -10,7 +10,7 @@
  * errors only.  Device-side watchdog failures (a bounded wait that ran out)
  * are recorded in a per-device status word read by ct_device_status().
  *
- * Tensors are FP32.  Four-dimensional attention tensors are indexed
+ * Tensors are FP32 unless a declaration takes a CT_DTYPE_*.  Four-dimensional attention tensors are indexed
  * [batch, head, seq, head_dim]; strides are in elements.  Outputs are written
  * densely (contiguous) exactly as the reference launchers allocate them.
  *
@@ -331,6 +331,103 @@ int ct_layernorm_bwd(const float* x, const float* gamma, const float* mean,
 int ct_cross_entropy_fwd_bwd(float* logits, int64_t ld, int64_t rows, int64_t vocab,
                              const int64_t* targets, int64_t ignore_index, float* loss_rows,
                              void* stream);
+
+/* ======================================================================== */
+/* Token generation: paged key/value cache, one-token attention, logits       */
+/* ======================================================================== */
+
+/* Element types of the generation operators.  Activations (q, k, v, outputs)
+ * are FP32, or of the cache's type. */
+enum { CT_DTYPE_F32 = 0, CT_DTYPE_BF16 = 1, CT_DTYPE_F16 = 2 };
+
+/* A paged cache is a pool of `pages` pages of `page_size` token slots:
+ * k_cache and v_cache are indexed [page, kv_head, slot, head_dim] through
+ * their element strides (any order of the first three; unit stride along
+ * head_dim, no negative strides).  Row s of block_table ([batch, max_pages]
+ * int32, row stride table_stride) lists the pages of sequence s in order:
+ * its token j lives in page block_table[s][j / page_size], slot
+ * j % page_size.  head_dim in {32, 64, 128};
+ * max_pages * page_size < 2^31. */
+
+/* Appends `tokens` new keys and values (k, v indexed [token, kv_head,
+ * head_dim] through their strides) to the cache: token t goes to position
+ * positions[t] of sequence seq_ids[t] (NULL: sequence t).  With rot_dim > 0
+ * (even, <= head_dim) the first rot_dim elements of each key are turned by the
+ * position's angles on the way: cos and sin are dense [max_positions,
+ * rot_dim / 2] FP32 tables, and element i pairs with i + rot_dim / 2, or
+ * 2i with 2i + 1 when `interleaved`.  q (NULL when q_heads is 0), indexed
+ * [token, q_head, head_dim], is turned the same way into q_out; k_out, when
+ * not NULL, also receives the turned keys.  Both are dense and of the
+ * activations' type; they may not overlap the inputs.  A token with a negative position is
+ * padding: nothing is appended and its q_out and k_out rows are zero.  A token
+ * with no place (sequence, page table entry or angle row out of range) is not
+ * appended and its q_out and k_out rows are NaN.  Two tokens with the same place leave either's values
+ * there.  No reference counterpart (the reference keeps no cache). */
+int ct_kv_append(const void* q, const int64_t q_stride[3],
+                 const void* k, const int64_t k_stride[3],
+                 const void* v, const int64_t v_stride[3],
+                 void* q_out, void* k_out, const float* cos, const float* sin,
+                 void* k_cache, const int64_t kc_stride[4],
+                 void* v_cache, const int64_t vc_stride[4],
+                 const int32_t* block_table, int64_t table_stride,
+                 const int32_t* seq_ids, const int32_t* positions,
+                 int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                 int64_t rot_dim, int interleaved, int64_t max_positions,
+                 int64_t batch, int64_t pages, int64_t page_size, int64_t max_pages,
+                 int act_dtype, int cache_dtype, void* stream);
+
+/* Bytes of workspace ct_paged_attention needs; they do not depend on the batch
+ * or the lengths. */
+size_t ct_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+
+/* Attention of one new token per sequence over the paged cache:
+ *   O = sum_j softmax_j(scale q . k_j) v_j,  LSE = ln sum_j exp(scale q . k_j)
+ * over the first seq_lens[b] cached tokens of sequence b.  q is indexed
+ * [batch, q_head, head_dim] through its strides; q_heads is a multiple of
+ * kv_heads and query head h reads key/value head h / (q_heads / kv_heads).
+ * out is dense [batch, q_heads, head_dim] of q's type; lse (may be NULL) dense
+ * [batch, q_heads].  A length of zero or below gives O = 0 and LSE = -inf; one
+ * beyond max_pages * page_size, or a page out of range, gives NaN.  Slots past
+ * the length are not read.  The cache's base and strides must be multiples of
+ * 16 bytes (CT_ERR_UNSUPPORTED_LAYOUT otherwise).
+ * The workspace must be zero before its first use and every call leaves it
+ * ready for the next, of whatever sizes (it needs no clearing in between); it
+ * must be 16-byte aligned and not be used by another call that can run
+ * concurrently.  Deterministic.  No reference counterpart
+ * (the reference keeps no cache). */
+int ct_paged_attention(const void* q, const int64_t q_stride[3],
+                       const void* k_cache, const int64_t kc_stride[4],
+                       const void* v_cache, const int64_t vc_stride[4],
+                       const int32_t* block_table, int64_t table_stride,
+                       const int32_t* seq_lens, void* out, float* lse,
+                       int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                       int64_t pages, int64_t page_size, int64_t max_pages, float scale,
+                       int act_dtype, int cache_dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Sampling penalties, biases and a grammar mask on `rows` rows of logits of
+ * length `vocab` (type `dtype`, row stride ld), into FP32 out (row stride
+ * out_ld).  With h = tokens[r][0 .. lens[r]) (lens NULL: max_len; clamped to
+ * [0, max_len]), of which the first prompt_lens[r] (NULL: 0) are the prompt,
+ * and count(i) the occurrences of token i in the rest of h:
+ *   x = logit(i);  where i occurs in h: x = x > 0 ? x / repetition : x * repetition
+ *   x -= frequency * count(i) + presence * (count(i) > 0)
+ *   x += bias_values of the row's entries with bias_ids == i
+ *   x = -inf where bit i % 32 of mask[r][i / 32] is 0
+ * tokens NULL: no penalties; repetition, frequency and presence are FP32
+ * [rows], NULL: 1, 0 and 0; bias_n entries a row (0: none); mask NULL: none.
+ * Ids outside [0, vocab) are ignored.  out may be logits itself when dtype is
+ * CT_DTYPE_F32 and out_ld == ld; any other overlap is not allowed.
+ * Deterministic.  The reference's GPT.generate samples from the plain softmax of
+ * the logits (gpt/gpt.py:184). */
+int ct_logits_process(const void* logits, int64_t ld, int dtype, float* out, int64_t out_ld,
+                      int64_t rows, int64_t vocab,
+                      const int64_t* tokens, int64_t tokens_ld, int64_t max_len,
+                      const int32_t* lens, const int32_t* prompt_lens,
+                      const float* repetition, const float* frequency, const float* presence,
+                      const int64_t* bias_ids, int64_t bias_ids_ld,
+                      const float* bias_values, int64_t bias_values_ld, int64_t bias_n,
+                      const int32_t* mask, int64_t mask_ld, void* stream);
 
 #ifdef __cplusplus
 }
