@@ -7,6 +7,8 @@ using namespace ct;
 namespace {
 
 constexpr int64_t kLim = 1ll << 31;
+// longest sequence: the kernels count past the last key by less than a unit
+constexpr int64_t kMaxTokens = kLim - 256;
 
 bool in_range(int64_t v, int64_t low) { return v >= low && v < kLim; }
 
@@ -21,7 +23,7 @@ int check_cache(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_d
                 int64_t page_size, int64_t max_pages, int act, int cache) {
   if (!in_range(batch, 0) || !in_range(q_heads, 0) || !in_range(kv_heads, 1) ||
       !in_range(pages, 0) || !in_range(page_size, 1) || !in_range(max_pages, 0) ||
-      max_pages * page_size >= kLim || !valid_types(act, cache))
+      max_pages * page_size > kMaxTokens || !valid_types(act, cache))
     return CT_ERR_INVALID_ARGUMENT;
   if (!(head_dim == 32 || head_dim == 64 || head_dim == 128)) return CT_ERR_UNSUPPORTED_HEAD_DIM;
   return CT_OK;
