@@ -7,8 +7,8 @@ using namespace ct;
 namespace {
 
 constexpr int64_t kLim = 1ll << 31;
-// longest sequence: the kernels count past the last key by less than a unit
-constexpr int64_t kMaxTokens = kLim - 256;
+// longest sequence: the tiles of 32 are counted in 32 bits
+constexpr int64_t kMaxTokens = (1ll << 30) - 256;
 
 bool in_range(int64_t v, int64_t low) { return v >= low && v < kLim; }
 

@@ -6,25 +6,28 @@
 //
 // Every cached value is read once and used for 2 * group FLOPs, so the bound
 // is HBM.  The design follows from that:
-//  * Work is cut into units of a few dozen keys of one (sequence, key/value
-//    head), and every CTA takes an equal share of the units, counted on the
-//    device from seq_lens (the host knows no lengths).  Ragged batches and one
-//    long sequence load the GPU alike.  A share that starts or ends inside a
-//    sequence leaves a partial (max, sum, O) in the workspace; the CTA that
-//    arrives last joins the partials in their order, so results do not depend
-//    on timing and no CTA waits for another.
-//  * Each warp streams its own keys through a private cp.async ring (16-byte
-//    copies gather pages of any size and layout), across sequence borders, with
-//    no block barrier until a sequence's end.
-//  * Products run on mma.sync m16n8k8 TF32 with FP32 accuracy: 8 heads fill
-//    rows 0-7 with the high part of q (or of the probabilities) and rows 8-15
-//    with the low part.  16-bit cache values are exact in TF32; FP32 ones are
-//    split too.  High and low sums of a head sit in the same lane, and the
-//    order of keys and dims inside a product is chosen so that every operand
-//    is a 16-byte shared-memory vector: no shuffles, no transposes.  tcgen05
-//    would take 8 heads as 128 rows (or as a column operand that has to be
-//    written to shared memory); at 4 * group FLOPs a value the tensor pipe is
-//    not what bounds this kernel.
+//  * Work is cut into tiles of 8 or 16 keys of one (sequence, key/value head),
+//    and every CTA takes an equal share of the tiles, counted on the device
+//    from seq_lens (the host knows no lengths).  Ragged batches and one long
+//    sequence load the GPU alike.  Short items stay whole and belong to one
+//    warp, which needs nobody else; the four warps of a CTA take turns at the
+//    tiles of a long one and join at its end.  A share that starts or ends
+//    inside a long item leaves a partial (maximum, sum, O) in the workspace;
+//    the CTA that arrives last joins the partials in their order, so results
+//    do not depend on timing and no CTA waits for another.
+//  * Each warp streams q and its keys and values through a private cp.async
+//    ring (16-byte copies gather pages of any size and layout) that runs ahead
+//    across items; a block barrier comes only where a long item ends.
+//  * Products run on mma.sync with FP32 accuracy: 16-bit cache values go in as
+//    they are, q and the probabilities as two or three 16-bit terms; FP32
+//    caches take three TF32 products.  Up to 8 heads put two terms into the 16
+//    rows of one product (high and low sums of a head then sit in the same
+//    lane), 16 heads fill the rows.  The order of keys and dims inside a
+//    product is chosen so that every operand is a 16-byte shared-memory
+//    vector: no shuffles, no transposes.  tcgen05 would take 8 heads as 128
+//    rows; at 4 * group FLOPs a value the tensor pipe is not what bounds this
+//    kernel.  One or two heads on an FP32 cache are cheaper as plain FMAs (64
+//    a lane, head and 8 KB of cache, against 64 products and 128 splits).
 #include "decode_common.cuh"
 
 namespace ct {
@@ -32,8 +35,13 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxCtas = 448;  // counters (two levels) and partial slots in the workspace
-constexpr int kGroup = 16;     // partials that are joined at a time
+constexpr int kMaxCtas = 448;  // counters (of each level) and partial slots in the workspace
+constexpr int kFan = 8;        // partials that are joined at a time
+constexpr int kLevels = 3;     // kFan^kLevels >= kMaxCtas
+// Items of no more tiles than a warp's part of its CTA's share (and no more
+// than this) are one warp's.
+constexpr int kShortMax = 16;
+constexpr int kMinShare = 4;   // tiles of a CTA, unless there are fewer in all
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum is raised only when a score passes it by this much (in
@@ -41,17 +49,26 @@ constexpr float kLn2 = 0.6931471805599453f;
 // as values below 1, and most tiles skip the rescaling of O.
 constexpr float kMaxSlack = 6.0f;
 
-// C: the cache's type; F32ACT: q and out are FP32, else of type C; R: blocks
-// of 8 query heads a CTA works on (1: high and low parts share a product's
-// rows; 2: 16 heads fill them and the parts are products of their own).
-template <class C, bool F32ACT, int D, int R>
+#pragma nv_diag_suppress 177  // not every configuration refers to every member
+template <class C, bool F32ACT>
+constexpr int q_terms() {
+  return sizeof(C) == 4 ? 2 : !F32ACT ? 1 : std::is_same<C, __nv_bfloat16>::value ? 3 : 2;
+}
+
+// C: the cache's type; F32ACT: q and out are FP32, else of type C; M: query
+// heads a CTA works on.  8: high and low parts share a product's rows; 16: the
+// heads fill them and the parts are products of their own; 1 and 2 (FP32
+// caches): plain FMAs.
+template <class C, bool F32ACT, int D, int M>
 struct Cfg {
+  static constexpr bool kLanes = M <= 2;                    // no tensor cores
+  static constexpr int R = M == 16 ? 2 : 1;                 // heads of a lane's rows
+  using A = std::conditional_t<F32ACT, float, C>;           // type of q and out
   static constexpr bool kF32 = sizeof(C) == 4;
   static constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
   static constexpr int kVec = 16 / (int)sizeof(C);          // elements of a 16-byte chunk
   static constexpr int kKeys = kF32 ? 8 : 16;                // keys of a warp's tile
   static constexpr int kNt = kKeys / 8;
-  static constexpr int kUnit = kWarps * kKeys;               // keys of a work unit
   static constexpr int kRowBytes = D * (int)sizeof(C);
   static constexpr int kRowChunks = kRowBytes / 16;
   static constexpr int kCopies = kKeys * kRowChunks / 32;    // of a lane, for K or V
@@ -65,7 +82,7 @@ struct Cfg {
   // is exact as it is, and two terms of p leave an error (2^-16 in bf16) far
   // below the output's own rounding; FP32 activations take as many as hold 22
   // bits or more.
-  static constexpr int kQTerms = kF32 ? 2 : !F32ACT ? 1 : kBf16 ? 3 : 2;
+  static constexpr int kQTerms = q_terms<C, F32ACT>();
   static constexpr int kPTerms = F32ACT && kBf16 ? 3 : 2;
   // The exponent's base lies this far below the running maximum (in powers of
   // two): f16 probabilities reach up to 2^14 instead of 1, so that the many
@@ -76,18 +93,20 @@ struct Cfg {
   static constexpr int kQOps = R == 1 ? (kQTerms + 1) / 2 : kQTerms;
   static constexpr int kPOps = R == 1 ? (kPTerms + 1) / 2 : kPTerms;
   static constexpr int kSteps = kF32 ? D / 8 : D / 16;
-  static constexpr int kQRegs = kSteps * kQOps * 4;
-  static constexpr bool kQInRegs = kQRegs <= 64;             // else in shared memory
-  // Registers: q, O (D / 2) and about 72 more.  Three CTAs an SM where that
-  // fits 168 a thread, with two stages of 8 KB or as many smaller ones.
-  static constexpr int kCtas = (kQInRegs ? kQRegs : 0) + D / 2 + 72 <= 168 ? 3 : 2;
+  static constexpr int kQRegs = kLanes ? M * D / 4 : kSteps * kQOps * 4;
+  // Registers: q, O and about 72 more.  Three CTAs an SM where that fits 168 a
+  // thread, with two stages of 8 KB or as many smaller ones.
+  static constexpr int kCtas = kQRegs + (kLanes ? kQRegs : D / 2) + 72 <= 168 ? 3 : 2;
   static constexpr int kRing = kCtas == 3 ? 16384 : 24576;
   static constexpr int kStages = kRing / kStageBytes > 6 ? 6 : kRing / kStageBytes;
   static constexpr int kJoinDims = D < 64 ? D : 64;          // dims of one joining pass
-  static constexpr int kJoinBytes = kWarps * 8 * kJoinDims * 4;
-  static constexpr int kQBytes = kQInRegs ? 0 : kQRegs * 32 * 4;
+  static constexpr int kRows = kLanes ? M : 8;               // heads of one joining pass
+  static constexpr int kJoinBytes = kWarps * kRows * kJoinDims * 4;
+  static constexpr int kQRowChunks = D * (int)sizeof(A) / 16;
+  static constexpr int kQChunks = M * kQRowChunks;
+  static_assert(kQChunks * 16 <= kStageBytes, "q passes through a stage of the ring");
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-  static constexpr int kSmem = kRingBytes + (kJoinBytes > kQBytes ? kJoinBytes : kQBytes);
+  static constexpr int kSmem = kRingBytes + kJoinBytes;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
@@ -130,6 +149,12 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   hi = __float_as_uint(x) & 0xffffe000u;
   lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
 }
+// The same of a cached value: the tensor core drops the 13 low bits of what it
+// is given, so x itself is the high part and the low part is not rounded (the
+// error is below 2^-21 of x).
+__device__ __forceinline__ uint32_t low_tf32(uint32_t x) {
+  return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u));
+}
 // The next 16-bit term of x and y (x in the low half); x and y keep the rest.
 template <class C>
 __device__ __forceinline__ uint32_t take_term(float& x, float& y) {
@@ -160,52 +185,60 @@ __device__ __forceinline__ int chunk_pos(int r, int c) {
     return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (r & 6)) << 4);
 }
 
+// Position of 16-byte chunk c of q's row h in its stage.
+template <int ROW_CHUNKS>
+__device__ __forceinline__ int q_pos(int h, int c) {
+  return (h * ROW_CHUNKS + (c ^ (h & (ROW_CHUNKS < 8 ? ROW_CHUNKS - 1 : 7)))) * 16;
+}
+
 __device__ __forceinline__ void store_act4(void* p, int64_t i, int dtype, float4 x) {
   if (dtype == CT_DTYPE_F32) {
     *reinterpret_cast<float4*>((float*)p + i) = x;
   } else if (dtype == CT_DTYPE_BF16) {
-    __nv_bfloat162 v[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
+    alignas(8) __nv_bfloat162 v[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
     *reinterpret_cast<uint2*>((__nv_bfloat16*)p + i) = *reinterpret_cast<uint2*>(v);
   } else {
-    __half2 v[2] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(x.z, x.w)};
+    alignas(8) __half2 v[2] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(x.z, x.w)};
     *reinterpret_cast<uint2*>((__half*)p + i) = *reinterpret_cast<uint2*>(v);
   }
 }
 
-// Floats of a partial: O [heads][D], then maximum and sum [heads] each.
-constexpr int64_t partial_floats(int heads, int D) { return (int64_t)heads * (D + 2); }
+// Floats of a partial: O [heads][D], then maximum and sum [heads] each; a
+// multiple of 4 (16 bytes).
+constexpr int64_t partial_floats(int heads, int D) { return ((int64_t)heads * (D + 2) + 3) / 4 * 4; }
 
 struct Launch {
   PagedAttention p;
-  int group, blocks;  // query heads of a key/value head; its blocks of 8 R heads
+  int group, blocks;  // query heads of a key/value head; its blocks of M heads
   int items;          // (key/value head, block) pairs of a sequence
   int page_shift;     // log2 of page_size, -1 when it is no power of two
   bool whole_tiles;   // a tile's keys lie in one page
+  bool q_vectors;     // q's rows are 16-byte vectors
   uint32_t* counters;
   float* partials;
 };
 
-// Where a CTA stands in the list of units: sequence, item, unit in the item.
+// A place in the list of tiles: sequence, item, tile in the item.
 struct Cursor {
   int64_t b;
-  int item, unit, units, len;
+  int item, tile, tiles, len;
   bool bad;
 };
 
-template <int UNIT>
+// A long item that other CTAs work on too: its tiles, its row of the output.
+struct Split {
+  int64_t first;
+  int tiles;
+  int64_t row;
+  int heads;
+};
+
+template <int KEYS>
 __device__ __forceinline__ void read_length(const Launch& a, Cursor& c) {
   const int n = a.p.seq_lens[c.b];
   c.bad = n > a.p.kv.max_pages * a.p.kv.page_size;
   c.len = n < 0 || c.bad ? 0 : n;
-  c.units = c.len > UNIT ? (c.len + UNIT - 1) / UNIT : 1;  // one, empty, at length 0
-}
-template <int UNIT>
-__device__ __forceinline__ void advance(const Launch& a, Cursor& c) {
-  if (++c.unit < c.units) return;
-  c.unit = 0;
-  if (++c.item < a.items) return;
-  c.item = 0;
-  if (++c.b < a.p.batch) read_length<UNIT>(a, c);
+  c.tiles = c.len > KEYS ? (c.len + KEYS - 1) / KEYS : 1;  // one, empty, at length 0
 }
 
 // A head's result from its unnormalised O and its maximum and sum.
@@ -214,6 +247,11 @@ __device__ __forceinline__ void write_out(const PagedAttention& p, int64_t row, 
   const float r = l == 0.0f ? 0.0f : 1.0f / l;
   store_act4(p.out, row * D + d, p.act_dtype, make_float4(x.x * r, x.y * r, x.z * r, x.w * r));
   if (d == 0 && p.lse) p.lse[row] = (m + log2f(l)) * kLn2;
+}
+
+// a / b of non-negative numbers, quickly where 32 bits hold them.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
 __device__ __forceinline__ float exp2_diff(float m, float top) {
@@ -235,191 +273,278 @@ __device__ __forceinline__ bool arrive_last(uint32_t* counter, int n, int* flag)
   return *flag != 0;
 }
 
-// Joins the partials k0, k0 + step, .. (n of them) of the item that CTA c0
-// starts, in that order, eight loads in flight: into partial k0 or the output.
+// Joins the partials k0, k0 + step, .. (n <= kFan of them) of the item that CTA
+// c0 starts, in that order and with all their loads in flight: into partial k0
+// or the output.
 template <int HEADS, int D>
-__device__ void join_partials(const Launch& a, int64_t c0, int k0, int step, int n, bool to_partial,
-                              int64_t row, int heads) {
+__device__ __forceinline__ void join_partials(const Launch& a, int64_t c0, int k0, int step, int n,
+                                              bool to_partial, int64_t row, int heads) {
   constexpr int64_t kSize = partial_floats(HEADS, D);
-  constexpr int kBatch = 8;
+  constexpr int kItems = HEADS * D / 4;  // float4s, two to a thread at a time
+  constexpr int kPart = kItems > kThreads ? 2 : 1;
   auto at = [&](int k) { return a.partials + (k == 0 ? 2 * c0 + 1 : 2 * (c0 + k)) * kSize; };
-  for (int i = threadIdx.x; i < HEADS * D / 4; i += kThreads) {
-    const int h = i / (D / 4), d = i % (D / 4) * 4;
-    float m = -INFINITY, l = 0.0f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int b = 0; b < n; b += kBatch) {
-      float km[kBatch], kl[kBatch];
-      float4 y[kBatch];
+#pragma unroll 1
+  for (int base = 0; base < kItems; base += kPart * kThreads) {
+    const int first = base + threadIdx.x < kItems ? base + threadIdx.x : 0;
+    float m[kPart][kFan], l[kPart][kFan];
+    float4 y[kPart][kFan];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        km[j] = -INFINITY;
-        kl[j] = 0.0f;
-        y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (b + j < n) {
-          const float* s = at(k0 + (b + j) * step);
-          km[j] = __ldcg(s + HEADS * D + h);
-          kl[j] = __ldcg(s + HEADS * D + HEADS + h);
-          y[j] = __ldcg(reinterpret_cast<const float4*>(s + h * D + d));
-        }
-      }
-      float top = m;
+    for (int j = 0; j < kFan; ++j) {
+      const float* s = at(k0 + (j < n ? j : 0) * step);
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) top = fmaxf(top, km[j]);
-      const float f0 = exp2_diff(m, top);
-      m = top;
-      l *= f0;
-      x.x *= f0;
-      x.y *= f0;
-      x.z *= f0;
-      x.w *= f0;
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const float f = exp2_diff(km[j], top);
-        x.x = fmaf(y[j].x, f, x.x);
-        x.y = fmaf(y[j].y, f, x.y);
-        x.z = fmaf(y[j].z, f, x.z);
-        x.w = fmaf(y[j].w, f, x.w);
-        l = fmaf(kl[j], f, l);
+      for (int i = 0; i < kPart; ++i) {
+        const int id = first + i * kThreads, h = id / (D / 4);
+        m[i][j] = __ldcg(s + HEADS * D + h);
+        l[i][j] = __ldcg(s + HEADS * D + HEADS + h);
+        y[i][j] = __ldcg(reinterpret_cast<const float4*>(s + id * 4));
       }
     }
-    if (to_partial) {
-      // heads' maxima and sums are read by all threads of the head: write
-      // them after everyone has read
-      float* s = at(k0);
-      __syncwarp();
-      *reinterpret_cast<float4*>(s + h * D + d) = x;
-      if (d == 0) {
-        s[HEADS * D + h] = m;
-        s[HEADS * D + HEADS + h] = l;
+    // heads' maxima and sums are read by the lanes of one warp; partial k0 is
+    // overwritten after they have them
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kPart; ++i) {
+      const int id = first + i * kThreads, h = id / (D / 4), d = id % (D / 4) * 4;
+      float top = m[i][0], sum = 0.0f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 1; j < kFan; ++j) top = fmaxf(top, j < n ? m[i][j] : -INFINITY);
+#pragma unroll
+      for (int j = 0; j < kFan; ++j) {
+        if (j >= n) continue;
+        const float f = exp2_diff(m[i][j], top);
+        x.x = fmaf(y[i][j].x, f, x.x);
+        x.y = fmaf(y[i][j].y, f, x.y);
+        x.z = fmaf(y[i][j].z, f, x.z);
+        x.w = fmaf(y[i][j].w, f, x.w);
+        sum = fmaf(l[i][j], f, sum);
       }
-    } else if (h < heads) {
-      write_out(a.p, row + h, d, D, x, m, l);
+      if (base + (int)threadIdx.x >= kItems) continue;
+      if (to_partial) {
+        float* s = at(k0);
+        *reinterpret_cast<float4*>(s + id * 4) = x;
+        if (d == 0) {
+          s[HEADS * D + h] = top;
+          s[HEADS * D + HEADS + h] = sum;
+        }
+      } else if (h < heads) {
+        write_out(a.p, row + h, d, D, x, top, sum);
+      }
     }
   }
 }
 
-template <class C, bool F32ACT, int D, int R>
-__global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, R>::kCtas)
+template <class C, bool F32ACT, int D, int M>
+__global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     paged_attention_kernel(const __grid_constant__ Launch a) {
-  using F = Cfg<C, F32ACT, D, R>;
+  using F = Cfg<C, F32ACT, D, M>;
+  using A = typename F::A;
+  constexpr int R = F::R;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t s_scan[kWarps];
-  __shared__ Cursor s_start;
-  __shared__ float s_m[kWarps][8 * R], s_l[kWarps][8 * R];
+  __shared__ uint32_t s_scan[kWarps];
+  __shared__ int64_t s_rest[kWarps];
+  __shared__ Cursor s_edge[2];
+  __shared__ float s_m[kWarps][M], s_l[kWarps][M], s_top[M], s_sum[M];
   __shared__ int s_last;
   const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const PagedAttention& p = a.p;
 
-  // ---- this CTA's share of the units
-  int64_t mine = 0;
-  for (int64_t b = tid; b < p.batch; b += kThreads) {
-    Cursor c;
-    c.b = b;
-    read_length<F::kUnit>(a, c);
-    mine += c.units;
+  // ---- this CTA's share of the tiles: a scan of the sequences' tiles, a
+  // block's worth at a time (nearly always one)
+  Cursor c{};
+  c.b = tid;
+  if (c.b < p.batch) read_length<F::kKeys>(a, c);
+  int64_t rest = 0;  // tiles of the sequences past the first block's worth
+  if (p.batch > kThreads) {
+    for (int64_t b = tid + kThreads; b < p.batch; b += kThreads) {
+      Cursor x;
+      x.b = b;
+      read_length<F::kKeys>(a, x);
+      rest += x.tiles;
+    }
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+    if (lane == 0) s_rest[w] = rest;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) s_scan[w] = mine;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) total += s_scan[i];
-  total *= a.items;
-  const int64_t ctas = total < gridDim.x ? total : gridDim.x;
-  if (blockIdx.x >= ctas) return;
-  const int64_t first = total * blockIdx.x / ctas, last = total * (blockIdx.x + 1) / ctas;
-  __syncthreads();
-  for (int64_t b0 = 0, before = 0; b0 < p.batch; b0 += kThreads) {
-    Cursor c{};
-    c.b = b0 + tid;
-    if (c.b < p.batch) read_length<F::kUnit>(a, c);
-    int64_t upto = c.units;
+  auto warp_scan = [&]() {  // 32 sequences have fewer than 2^32 tiles
+    uint32_t x = c.tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    if (lane == 31) s_scan[w] = upto;
-    __syncthreads();
-    int64_t chunk = 0;
+    if (lane == 31) s_scan[w] = x;
+    return (int64_t)x;
+  };
+  int64_t upto = warp_scan(), block = 0, before = 0;
+  __syncthreads();
 #pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < w) upto += s_scan[i];
+    block += s_scan[i];
+  }
+  rest = 0;
+  if (p.batch > kThreads)
+    for (int i = 0; i < kWarps; ++i) rest += s_rest[i];
+  const int64_t total = (block + rest) * a.items;
+  int64_t ctas = divide(total + kMinShare - 1, kMinShare);
+  if (ctas > gridDim.x) ctas = gridDim.x;
+  if (blockIdx.x >= ctas) return;
+  // the first `longer` CTAs take one tile more than the others
+  const int64_t share = divide(total, ctas), longer = total - share * ctas;
+  auto cta_of = [&](int64_t tile) {
+    return tile < longer * (share + 1) ? divide(tile, share + 1)
+                                       : longer + divide(tile - longer * (share + 1), share);
+  };
+  int64_t edge[2];
+  edge[0] = blockIdx.x * share + (blockIdx.x < longer ? blockIdx.x : longer);
+  edge[1] = edge[0] + share + (blockIdx.x < longer ? 1 : 0);
+  while (true) {
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+      const int64_t from = edge[e] - (before + upto - c.tiles) * a.items;
+      if (from >= 0 && from < (int64_t)c.tiles * a.items) {
+        Cursor x = c;
+        x.item = (int)divide(from, c.tiles);
+        x.tile = (int)(from - (int64_t)x.item * c.tiles);
+        s_edge[e] = x;
+      }
+    }
+    before += block;
+    __syncthreads();
+    if (before * a.items > edge[1] || before * a.items == total) break;
+    c = Cursor{c.b + kThreads, 0, 0, 0, 0, false};
+    if (c.b < p.batch) read_length<F::kKeys>(a, c);
+    upto = warp_scan();
+    __syncthreads();
+    block = 0;
     for (int i = 0; i < kWarps; ++i) {
       if (i < w) upto += s_scan[i];
-      chunk += s_scan[i];
+      block += s_scan[i];
     }
-    const int64_t from = first - (before + upto - c.units) * a.items;
-    if (from >= 0 && from < (int64_t)c.units * a.items) {
-      c.item = (int)(from / c.units);
-      c.unit = (int)(from % c.units);
-      s_start = c;
-    }
-    before += chunk;
-    __syncthreads();
-    if (before * a.items > first) break;
   }
-  Cursor cur = s_start, ahead = cur;
+  // an edge inside a short item moves to the item's start
+  const int brief = (int)(share / kWarps < kShortMax ? share / kWarps : kShortMax);
+  Cursor cur = s_edge[0];
+  if (cur.tiles <= brief) {
+    edge[0] -= cur.tile;
+    cur.tile = 0;
+  }
+  if (edge[1] < total && s_edge[1].tiles <= brief) edge[1] -= s_edge[1].tile;
+  int64_t left = edge[1] - edge[0];
+  const int64_t end = edge[1];
 
-  // ---- the copy side: tiles of this warp, kStages - 1 ahead of the products
+  // Walks the share item by item: true with `seg`, the tiles of the item that
+  // lie in the share, and whether it is this warp's alone; false at the end.
+  // Short items of other warps are passed over.
+  auto next_item = [&](Cursor& x, int64_t& todo, int& seg, bool& own, bool fresh) {
+    while (true) {
+      if (!fresh) {
+        todo -= seg;
+        if (todo <= 0) return false;
+        x.tile = 0;
+        if (++x.item == a.items) {
+          x.item = 0;
+          ++x.b;
+          read_length<F::kKeys>(a, x);
+        }
+      }
+      fresh = false;
+      seg = (int)(todo < x.tiles - x.tile ? todo : x.tiles - x.tile);
+      own = x.tiles <= brief;
+      if (!own || ((x.b * a.items + x.item) & (kWarps - 1)) == w) return true;
+    }
+  };
+  if (left <= 0) return;
+
+  // ---- the copy side: q, then the tiles of this warp, kStages - 1 ahead of
+  // the products
   const uint32_t ring = smem_addr(smem) + w * (F::kStages * F::kStageBytes);
   const uint8_t* ring_ptr = smem + w * (F::kStages * F::kStageBytes);
   const bool second = (lane / F::kKeys) & 1;  // this lane addresses V rows, else K rows
   const int my_row = lane % F::kKeys;
-  // The lane's part of a copy instruction: row copy_row + i * kCopyRows, chunk
-  // lane % kRowChunks.  The row's bits and i's do not meet, so the chunk's
-  // position is the xor of a part of each (chunk_pos).
   const int copy_row = lane / F::kRowChunks, copy_chunk = lane % F::kRowChunks;
   const int64_t k_step = p.kv.ks[2] * (int64_t)sizeof(C), v_step = p.kv.vs[2] * (int64_t)sizeof(C);
+  const int64_t k_page = p.kv.ks[0] * (int64_t)sizeof(C), v_page = p.kv.vs[0] * (int64_t)sizeof(C);
   const uint8_t* k_lane = (const uint8_t*)p.kv.k + copy_row * k_step + copy_chunk * 16;
   const uint8_t* v_lane = (const uint8_t*)p.kv.v + copy_row * v_step + copy_chunk * 16;
-  int64_t to_issue = last - first;
-  int next_page = -1, next_slot = 0, next_head = 0;
+  Cursor ahead = cur;
+  int64_t ahead_left = left;
+  int ahead_seg = 0;
+  bool ahead_own = false;
+  // of the item that is being copied: this warp's tiles still to go, the key of
+  // the lane's row in the next, the end of the keys, where its head and its row
+  // of the table begin
+  int tiles_left = 0, key = 0, key_end = 0;
+  const uint8_t *k_item = k_lane, *v_item = v_lane;
+  const int32_t* pages = p.kv.table;
+  // What the next issue copies: nothing, q, or a tile whose rows' pages and
+  // slots have been looked up
+  enum { kNothing, kQuery, kTile };
+  int next = kNothing, next_page = -1, next_slot = 0;
   bool next_there = false;
-  auto look_up = [&]() {  // page and slot of the lane's row of the next tile
-    next_there = false;
-    if (to_issue <= 0) return;
-    const int key = ahead.unit * F::kUnit + w * F::kKeys + my_row;
-    next_there = key < ahead.len;
+  auto look_up = [&]() {
+    next_there = key < key_end;
     if (next_there) {
       const int index = a.page_shift >= 0 ? key >> a.page_shift : key / p.kv.page_size;
       next_slot = key - index * p.kv.page_size;
-      next_page = p.kv.table[ahead.b * p.kv.table_s + index];
-      next_head = ahead.item / a.blocks;
+      next_page = pages[index];
     }
-    --to_issue;
-    if (to_issue > 0) advance<F::kUnit>(a, ahead);
   };
+  auto begin_item = [&]() {
+    next = kQuery;
+    tiles_left = ahead_own ? ahead_seg : (ahead_seg + kWarps - 1) / kWarps;
+    key = (ahead.tile + (ahead_own ? 0 : w)) * F::kKeys + my_row;
+    key_end = (ahead.tile + ahead_seg) * F::kKeys;
+    if (key_end > ahead.len) key_end = ahead.len;
+    const int64_t head = ahead.item / a.blocks;
+    k_item = k_lane + head * p.kv.ks[1] * (int64_t)sizeof(C);
+    v_item = v_lane + head * p.kv.vs[1] * (int64_t)sizeof(C);
+    pages = p.kv.table + ahead.b * p.kv.table_s;
+  };
+  auto step_ahead = [&]() {  // past what has been issued
+    if (next == kTile && --tiles_left > 0) {
+      key += (ahead_own ? 1 : kWarps) * F::kKeys;
+      look_up();
+    } else if (next == kQuery) {
+      next = kTile;
+      look_up();
+    } else if (next == kTile) {
+      next = kNothing;
+      if (next_item(ahead, ahead_left, ahead_seg, ahead_own, false)) begin_item();
+    }
+  };
+  if (next_item(ahead, ahead_left, ahead_seg, ahead_own, true)) begin_item();
   auto issue = [&](int stage) {
-    const bool fine = next_there && (unsigned)next_page < (unsigned)p.kv.pages;
     const uint32_t base = ring + stage * F::kStageBytes;
-    if (a.whole_tiles && __all_sync(0xffffffffu, fine)) {
-      // all rows are there and follow one another in one page
-      const int slot = next_slot - my_row;
-      const uint8_t* src[2] = {
-          k_lane + (next_page * p.kv.ks[0] + next_head * p.kv.ks[1]) * (int64_t)sizeof(C) + slot * k_step,
-          v_lane + (next_page * p.kv.vs[0] + next_head * p.kv.vs[1]) * (int64_t)sizeof(C) + slot * v_step};
+    if (next == kTile) {
+      const bool fine = next_there && (unsigned)next_page < (unsigned)p.kv.pages;
+      if (a.whole_tiles && __all_sync(0xffffffffu, fine)) {
+        // all rows are there and follow one another in one page
+        const int slot = next_slot - my_row;
+        const uint8_t* src[2] = {
+            k_item + next_page * k_page + slot * k_step,
+            v_item + next_page * v_page + slot * v_step};
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int64_t step = F::kCopyRows * (kv ? v_step : k_step);
-        const uint32_t dst = base + kv * (F::kKeys * F::kRowBytes);
+        for (int kv = 0; kv < 2; ++kv) {
+          const int64_t step = F::kCopyRows * (kv ? v_step : k_step);
 #pragma unroll
-        for (int i = 0; i < F::kCopies; ++i)
-          cp_async16(dst + chunk_pos<F::kRowBytes>(i * F::kCopyRows + copy_row, copy_chunk),
-                     src[kv] + i * step, 16);
-      }
-    } else if (__any_sync(0xffffffffu, next_there)) {
-      int64_t off = -1;  // past the length: zeros
-      if (next_there) {
-        const int64_t* s = second ? p.kv.vs : p.kv.ks;
-        off = !fine ? -2  // no such page: NaN keys
-                    : (next_page * s[0] + next_head * s[1] + next_slot * s[2]) * (int64_t)sizeof(C);
-      }
+          for (int i = 0; i < F::kCopies; ++i)
+            cp_async16(base + kv * (F::kKeys * F::kRowBytes) +
+                           chunk_pos<F::kRowBytes>(i * F::kCopyRows + copy_row, copy_chunk),
+                       src[kv] + i * step, 16);
+        }
+      } else if (__any_sync(0xffffffffu, next_there)) {
+        int64_t off = -1;  // past the length: zeros
+        if (next_there) {
+          off = !fine    ? -2  // no such page: NaN
+                : second ? next_page * v_page + next_slot * v_step
+                         : next_page * k_page + next_slot * k_step;
+        }
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const uint8_t* from = (const uint8_t*)(kv ? p.kv.v : p.kv.k);
-#pragma unroll
-        for (int i = 0; i < F::kCopies; ++i) {
-          const int r = i * F::kCopyRows + copy_row;
+        for (int i = 0; i < 2 * F::kCopies; ++i) {
+          const int kv = i / F::kCopies, r = i % F::kCopies * F::kCopyRows + copy_row;
+          const uint8_t* from = kv ? v_item - copy_row * v_step : k_item - copy_row * k_step;
           const int64_t o = __shfl_sync(0xffffffffu, off, kv * F::kKeys + r);
           const uint32_t dst =
               base + kv * (F::kKeys * F::kRowBytes) + chunk_pos<F::kRowBytes>(r, copy_chunk);
@@ -427,127 +552,204 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, R>::kCtas)
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0x7fc07fc0u)
                          : "memory");  // NaN in each of the three types
           else
-            cp_async16(dst, o < 0 ? from : from + o + copy_chunk * 16, o < 0 ? 0 : 16);
+            cp_async16(dst, o < 0 ? p.kv.k : from + o, o < 0 ? 0 : 16);
+        }
+      }
+    } else if (next == kQuery) {
+      const int head = ahead.item / a.blocks, head0 = (ahead.item % a.blocks) * M;
+      const A* q = (const A*)p.q + ahead.b * p.qs[0] + ((int64_t)head * a.group + head0) * p.qs[1];
+#pragma unroll 1
+      for (int i = lane; i < F::kQChunks; i += 32) {
+        const int h = i / F::kQRowChunks, ch = i % F::kQRowChunks;
+        const bool there = head0 + h < a.group;
+        const A* row = there ? q + h * p.qs[1] + ch * (16 / (int)sizeof(A)) * p.qs[2] : q;
+        const uint32_t dst = base + q_pos<F::kQRowChunks>(h, ch);
+        if (a.q_vectors) {
+          cp_async16(dst, row, there ? 16 : 0);
+        } else {
+          alignas(16) A x[16 / sizeof(A)];
+#pragma unroll
+          for (int e = 0; e < 16 / (int)sizeof(A); ++e) x[e] = there ? row[e * p.qs[2]] : A(0.0f);
+          const uint4 v = *reinterpret_cast<const uint4*>(x);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y),
+                       "r"(v.z), "r"(v.w)
+                       : "memory");
         }
       }
     }
     cp_async_commit();
-    look_up();
+    step_ahead();
   };
-  look_up();
-#pragma unroll
-  for (int s = 0; s < F::kStages - 1; ++s) issue(s);
 
   float* join = reinterpret_cast<float*>(smem + F::kRingBytes);
-  uint32_t* q_smem = reinterpret_cast<uint32_t*>(smem + F::kRingBytes);
-  uint32_t q_regs[F::kQInRegs ? F::kSteps : 1][F::kQOps][4];
-  int stage = 0;
+  // q, O, maxima and sums: of a lane's rows of the products, or (plain FMAs) of
+  // keys g, g + 8, .. and the dims of chunks t + 4 i
+  uint32_t q_regs[F::kLanes ? 1 : F::kSteps][F::kQOps][4];
+  float o_acc[F::kLanes ? 1 : F::kOTiles][4];
+  constexpr int kChunks = F::kLanes ? D / 16 : 1, kHeads = F::kLanes ? M : 1;
+  alignas(16) float q_lane[kHeads][kChunks][4], o_lane[kHeads][kChunks][4];
+  constexpr int kMine = F::kLanes ? M : R;
+  float m_run[kMine], l_run[kMine], s_mul[kMine];
+  int stage = 0;  // the next to fill
+  int filled = 0;
+  Split split[2] = {};
 
-  for (int64_t at = first; at < last;) {
-    // ---- one segment: units cur.unit .. end of the item, or of the share
-    const int kv_head = cur.item / a.blocks, head0 = (cur.item % a.blocks) * 8 * R;
-    const int heads = a.group - head0 < 8 * R ? a.group - head0 : 8 * R;
-    const int64_t q_head = (int64_t)kv_head * a.group + head0;
-    const int64_t item_first = at - cur.unit;
-    const int seg = (int)(last - at < cur.units - cur.unit ? last - at : cur.units - cur.unit);
+  int seg = 0;  // tiles of the item in this share
+  bool own = false;
+  for (bool more = next_item(cur, left, seg, own, true); more;
+       more = next_item(cur, left, seg, own, false)) {
+    const int kv_head = cur.item / a.blocks, head0 = (cur.item % a.blocks) * M;
+    const int heads = a.group - head0 < M ? a.group - head0 : M;
+    const int64_t row = cur.b * p.q_heads + (int64_t)kv_head * a.group + head0;
+    const int steps = own ? seg : (seg + kWarps - 1) / kWarps;
+    int key0 = (cur.tile + (own ? 0 : w)) * F::kKeys;
+    int end_key = (cur.tile + seg) * F::kKeys;
+    if (end_key > cur.len) end_key = cur.len;
 
-    // q in the order of the products' A operands: the dims that lane t of step
-    // s multiplies; rows g and g + 8 are two terms (R = 1) or two heads.
-    using A = std::conditional_t<F32ACT, float, C>;
-    const A* q_row[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r)  // a head past the group's last reads another's row, and then zero
-      q_row[r] = (const A*)p.q + cur.b * p.qs[0] +
-                 (q_head + (r * 8 + g < heads ? r * 8 + g : 0)) * p.qs[1];
-    auto q_at = [&](int r, int d) {
-      const float x = to_f32(q_row[r][d * p.qs[2]]);
-      return r * 8 + g < heads ? x : 0.0f;
-    };
-    // FP32 q in f16 terms is scaled by a power of two that brings the head's
-    // largest element to 2^14 .. 2^15: what falls below the f16 range is then
-    // below 2^-38 of it.  s_mul undoes it, with the softmax scale.
-    float s_mul[R], q_mul[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      q_mul[r] = 1.0f;
-      s_mul[r] = p.scale * kLog2e;
-      if constexpr (!F::kF32 && !F::kBf16 && F32ACT) {
-        float top = 0.0f;
-#pragma unroll
-        for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(q_at(r, d)));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (top > 0.0f && top < INFINITY) {
-          int e;
-          frexpf(top, &e);
-          e = 15 - e < 120 ? 15 - e : 120;  // 2^e and 2^-e are normal
-          q_mul[r] = __int_as_float((127 + e) << 23);
-          s_mul[r] *= __int_as_float((127 - e) << 23);
-        }
+    for (int u = -1; u < steps;) {
+      // fill a stage; the one to work on is the kStages - 1 filled before it
+      if (filled == F::kStages - 1) cp_async_wait<F::kStages - 2>();
+      __syncwarp();
+      issue(stage);
+      stage = stage + 1 == F::kStages ? 0 : stage + 1;
+      if (filled < F::kStages - 1) {
+        ++filled;
+        continue;
       }
-    }
-    auto q_ops = [&](int s, uint32_t (&op)[F::kQOps][4]) {
-      const int i = s / (F::kVec / (F::kF32 ? 2 : 4)), e = s % (F::kVec / (F::kF32 ? 2 : 4));
-      const int d = (t + 4 * i) * F::kVec + e * (F::kF32 ? 2 : 4);
+      const uint8_t* tile = ring_ptr + stage * F::kStageBytes;
+      if (u < 0) {
+        // ---- the item's start: q in the order of the products' A operands,
+        // the dims that lane t of step s multiplies; rows g and g + 8 are two
+        // terms (R = 1) or two heads
+        u = 0;
+        auto q_at = [&](int r, int d) {
+          return to_f32(*reinterpret_cast<const A*>(
+              tile + q_pos<F::kQRowChunks>(r * 8 + g, d * (int)sizeof(A) / 16) +
+              d * (int)sizeof(A) % 16));
+        };
+        // FP32 q in f16 terms is scaled by a power of two that brings the
+        // head's largest element to 2^14 .. 2^15: what falls below the f16
+        // range is then below 2^-38 of it.  s_mul undoes it, with the softmax
+        // scale.
+        float q_mul[kMine];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if constexpr (F::kF32) {
-          uint32_t term[2][2];
-          split_tf32(q_at(r, d), term[0][0], term[1][0]);
-          split_tf32(q_at(r, d + 1), term[0][1], term[1][1]);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            op[R == 1 ? 0 : k][R == 1 ? k : r] = term[k][0];
-            op[R == 1 ? 0 : k][(R == 1 ? k : r) + 2] = term[k][1];
+        for (int r = 0; r < kMine; ++r) {
+          m_run[r] = -INFINITY;
+          l_run[r] = 0.0f;
+          q_mul[r] = 1.0f;
+          s_mul[r] = p.scale * kLog2e;
+          if constexpr (!F::kF32 && !F::kBf16 && F32ACT) {
+            float top = 0.0f;
+#pragma unroll 4
+            for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(q_at(r, d)));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (top > 0.0f && top < INFINITY) {
+              int e;
+              frexpf(top, &e);
+              e = 15 - e < 120 ? 15 - e : 120;  // 2^e and 2^-e are normal
+              q_mul[r] = __int_as_float((127 + e) << 23);
+              s_mul[r] *= __int_as_float((127 - e) << 23);
+            }
           }
+        }
+        if constexpr (F::kLanes) {
+#pragma unroll
+          for (int h = 0; h < M; ++h)
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+              *reinterpret_cast<float4*>(q_lane[h][i]) = *reinterpret_cast<const float4*>(
+                  tile + q_pos<F::kQRowChunks>(h, t + 4 * i));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o_lane[h][i][e] = 0.0f;
+            }
         } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x = q_at(r, d + 2 * h) * q_mul[r];
-            float y = q_at(r, d + 2 * h + 1) * q_mul[r];
+          for (int s = 0; s < F::kSteps; ++s) {
+            constexpr int kPart = F::kF32 ? 2 : 4;  // dims of a lane in a step
+            const int d = (t + 4 * (s / (F::kVec / kPart))) * F::kVec + s % (F::kVec / kPart) * kPart;
 #pragma unroll
-            for (int k = 0; k < F::kQTerms; ++k)
-              op[R == 1 ? k / 2 : k][(R == 1 ? k % 2 : r) + 2 * h] = take_term<C>(x, y);
-            if (R == 1 && F::kQTerms % 2) op[F::kQTerms / 2][1 + 2 * h] = 0u;
+            for (int r = 0; r < R; ++r) {
+              if constexpr (F::kF32) {
+                uint32_t term[2][2];
+                split_tf32(q_at(r, d), term[0][0], term[1][0]);
+                split_tf32(q_at(r, d + 1), term[0][1], term[1][1]);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  q_regs[s][R == 1 ? 0 : k][R == 1 ? k : r] = term[k][0];
+                  q_regs[s][R == 1 ? 0 : k][(R == 1 ? k : r) + 2] = term[k][1];
+                }
+              } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  float x = q_at(r, d + 2 * h) * q_mul[r], y = q_at(r, d + 2 * h + 1) * q_mul[r];
+#pragma unroll
+                  for (int k = 0; k < F::kQTerms; ++k)
+                    q_regs[s][R == 1 ? k / 2 : k][(R == 1 ? k % 2 : r) + 2 * h] = take_term<C>(x, y);
+                  if (R == 1 && F::kQTerms % 2) q_regs[s][F::kQTerms / 2][1 + 2 * h] = 0u;
+                }
+              }
+            }
           }
+#pragma unroll
+          for (int j = 0; j < F::kOTiles; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o_acc[j][e] = 0.0f;
         }
+        continue;
       }
-    };
-    if constexpr (F::kQInRegs) {
-#pragma unroll
-      for (int s = 0; s < F::kSteps; ++s) q_ops(s, q_regs[s]);
-    } else {
-      for (int s = w; s < F::kSteps; s += kWarps) {
-        uint32_t op[F::kQOps][4];
-        q_ops(s, op);
-#pragma unroll
-        for (int k = 0; k < F::kQOps; ++k)
-          *reinterpret_cast<uint4*>(q_smem + ((s * F::kQOps + k) * 32 + lane) * 4) =
-              make_uint4(op[k][0], op[k][1], op[k][2], op[k][3]);
-      }
-      __syncthreads();
-    }
+      const int first_key = key0;
+      key0 += (own ? 1 : kWarps) * F::kKeys;
+      ++u;
+      if (first_key >= end_key) continue;
 
-    float o_acc[F::kOTiles][4], m_run[R], l_run[R];
+      if constexpr (F::kLanes) {
+        // ---- key g of the tile, the dims of chunks t + 4 i
+        float s[M];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      m_run[r] = -INFINITY;
-      l_run[r] = 0.0f;
-    }
+        for (int h = 0; h < M; ++h) s[h] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < F::kOTiles; ++j)
+        for (int i = 0; i < kChunks; ++i) {
+          alignas(16) float x[4];
+          *reinterpret_cast<float4*>(x) =
+              *reinterpret_cast<const float4*>(tile + chunk_pos<F::kRowBytes>(g, t + 4 * i));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o_acc[j][e] = 0.0f;
-
-    for (int u = 0; u < seg; ++u) {
-      cp_async_wait<F::kStages - 2>();
-      __syncwarp();
-      issue(stage == 0 ? F::kStages - 1 : stage - 1);
-      const int key0 = (cur.unit + u) * F::kUnit + w * F::kKeys;
-      const uint8_t* tile = ring_ptr + stage * F::kStageBytes;
-      stage = stage + 1 == F::kStages ? 0 : stage + 1;
-      if (key0 >= cur.len) continue;
-
+          for (int h = 0; h < M; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[h] = fmaf(q_lane[h][i][e], x[e], s[h]);
+        }
+        float pr[M];
+#pragma unroll
+        for (int h = 0; h < M; ++h) {
+          s[h] += __shfl_xor_sync(0xffffffffu, s[h], 1);
+          s[h] += __shfl_xor_sync(0xffffffffu, s[h], 2);
+          s[h] *= s_mul[h];
+          if (first_key + g >= end_key) s[h] = -INFINITY;
+          // each lane has a maximum of its own keys
+          if (__any_sync(0xffffffffu, s[h] > m_run[h] + kMaxSlack)) {
+            const float top = fmaxf(s[h], m_run[h]), f = exp2_diff(m_run[h], top);
+            m_run[h] = top;
+            l_run[h] *= f;
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o_lane[h][i][e] *= f;
+          }
+          pr[h] = exp2f(s[h] - (m_run[h] == -INFINITY ? 0.0f : m_run[h]));
+          l_run[h] += pr[h];
+        }
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          alignas(16) float x[4];
+          *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(
+              tile + F::kKeys * F::kRowBytes + chunk_pos<F::kRowBytes>(g, t + 4 * i));
+#pragma unroll
+          for (int h = 0; h < M; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o_lane[h][i][e] = fmaf(pr[h], x[e], o_lane[h][i][e]);
+        }
+        continue;
+      } else {
       // ---- S = q k^T, in two chains for each 8 keys
       float s_acc[F::kNt][2][4];
 #pragma unroll
@@ -556,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, R>::kCtas)
         for (int e = 0; e < 4; ++e) s_acc[n][0][e] = s_acc[n][1][e] = 0.0f;
 #pragma unroll
       for (int i = 0; i < F::kKIter; ++i) {
-        uint32_t kw[F::kNt][4];
+        alignas(16) uint32_t kw[F::kNt][4];
 #pragma unroll
         for (int n = 0; n < F::kNt; ++n)
           *reinterpret_cast<uint4*>(kw[n]) = *reinterpret_cast<const uint4*>(
@@ -564,30 +766,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, R>::kCtas)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int s = 2 * i + e;
-          uint32_t qa[F::kQOps][4];
-#pragma unroll
-          for (int k = 0; k < F::kQOps; ++k) {
-            if constexpr (F::kQInRegs) {
-#pragma unroll
-              for (int x = 0; x < 4; ++x) qa[k][x] = q_regs[s][k][x];
-            } else {
-              *reinterpret_cast<uint4*>(qa[k]) =
-                  *reinterpret_cast<const uint4*>(q_smem + ((s * F::kQOps + k) * 32 + lane) * 4);
-            }
-          }
 #pragma unroll
           for (int n = 0; n < F::kNt; ++n) {
             if constexpr (F::kF32) {
-              uint32_t xh, xl, yh, yl;
-              split_tf32(__uint_as_float(kw[n][2 * e]), xh, xl);
-              split_tf32(__uint_as_float(kw[n][2 * e + 1]), yh, yl);
-              mma<C>(s_acc[n][0], qa[0], xh, yh);
-              mma<C>(s_acc[n][1], qa[0], xl, yl);
-              if constexpr (R == 2) mma<C>(s_acc[n][1], qa[1], xh, yh);
+              const uint32_t x = kw[n][2 * e], y = kw[n][2 * e + 1];
+              mma<C>(s_acc[n][0], q_regs[s][0], x, y);
+              mma<C>(s_acc[n][1], q_regs[s][0], low_tf32(x), low_tf32(y));
+              if constexpr (R == 2) mma<C>(s_acc[n][1], q_regs[s][1], x, y);
             } else {
 #pragma unroll
               for (int k = 0; k < F::kQOps; ++k)
-                mma<C>(s_acc[n][(e + k) & 1], qa[k], kw[n][2 * e], kw[n][2 * e + 1]);
+                mma<C>(s_acc[n][(e + k) & 1], q_regs[s][k], kw[n][2 * e], kw[n][2 * e + 1]);
             }
           }
         }
@@ -606,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, R>::kCtas)
             v[n][e] = R == 1 ? (x[0][e] + x[1][e]) + (x[0][e + 2] + x[1][e + 2])
                              : x[0][2 * r + e] + x[1][2 * r + e];
             v[n][e] *= s_mul[r];
-            if (key0 + n * 8 + 2 * t + e >= cur.len) v[n][e] = -INFINITY;
+            if (first_key + n * 8 + 2 * t + e >= end_key) v[n][e] = -INFINITY;
             top = fmaxf(top, v[n][e]);
           }
         if (__any_sync(0xffffffffu, top > m_run[r] + (F::kBelow + kMaxSlack))) {
@@ -651,7 +840,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, R>::kCtas)
       const uint8_t* vt = tile + F::kKeys * F::kRowBytes;
 #pragma unroll
       for (int i = 0; i < F::kVIter; ++i) {
-        uint32_t vw[2 * F::kNt][4];
+        alignas(16) uint32_t vw[2 * F::kNt][4];
 #pragma unroll
         for (int n = 0; n < 2 * F::kNt; ++n) {
           const int r = (n / 2) * 8 + 2 * t + n % 2;
@@ -674,12 +863,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, R>::kCtas)
             c[3] = o[3];
           }
           if constexpr (F::kF32) {
-            uint32_t xh, xl, yh, yl;
-            split_tf32(__uint_as_float(vw[0][e]), xh, xl);
-            split_tf32(__uint_as_float(vw[1][e]), yh, yl);
-            mma<C>(c, pa[0], xh, yh);
-            mma<C>(c, pa[0], xl, yl);
-            if constexpr (R == 2) mma<C>(c, pa[1], xh, yh);
+            const uint32_t x = vw[0][e], y = vw[1][e];
+            mma<C>(c, pa[0], low_tf32(x), low_tf32(y));
+            if constexpr (R == 2) mma<C>(c, pa[1], x, y);
+            mma<C>(c, pa[0], x, y);
           } else {
             // element e of keys 2 t and 2 t + 1 (and 8 further) in one word
             const uint32_t pick = e % 2 ? 0x7632u : 0x5410u;
@@ -692,171 +879,253 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, R>::kCtas)
           for (int x = 0; x < 4; ++x) o[x] = F32ACT && (R == 2 || x < 2) ? o[x] + c[x] : c[x];
         }
       }
-    }
-
-    // ---- the segment's end: join the warps, then write O or a partial
-    const bool whole = cur.unit == 0 && seg == cur.units;
-    const bool tail = cur.unit != 0;
-    float* slot =
-        a.partials + (2 * (int64_t)blockIdx.x + (tail ? 0 : 1)) * partial_floats(8 * R, D);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float l = l_run[r];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      if (t == 0) {
-        s_m[w][r * 8 + g] = m_run[r];
-        s_l[w][r * 8 + g] = l;
       }
     }
-    __syncthreads();
+
+    // ---- the item's end.  `each` passes the lane's part of O to its caller:
+    // head, dim, four values times the head's factor
+    if constexpr (F::kLanes) {
+      // join the eight key groups: halve the chunks with the partner while
+      // there are two or more, then add whole chunks
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float top = -INFINITY;
+      for (int h = 0; h < M; ++h) {
+        float top = m_run[h];
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_m[i][r * 8 + g]);
-      const float f = exp2_diff(m_run[r], top);
-      constexpr int J = F::kJoinDims, kPassIter = J / (8 * F::kVVec);
+        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float f = exp2_diff(m_run[h], top);
+        m_run[h] = top;
+        l_run[h] *= f;
 #pragma unroll
-      for (int pass = 0; pass < D / J; ++pass) {
+        for (int o = 4; o < 32; o <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], o);
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o_lane[h][i][e] *= f;
+#pragma unroll
+        for (int o = 16, n = kChunks; o >= 4; o >>= 1, n = n > 1 ? n / 2 : 1) {
+          const bool upper = lane & o;
+#pragma unroll
+          for (int i = 0; i < (n > 1 ? n / 2 : 1); ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float keep = n > 1 && upper ? o_lane[h][n > 1 ? i + n / 2 : 0][e] : o_lane[h][i][e];
+              const float give = n > 1 && !upper ? o_lane[h][n > 1 ? i + n / 2 : 0][e] : o_lane[h][i][e];
+              o_lane[h][i][e] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
+        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
+      }
+    }
+    if (cur.bad)
+#pragma unroll
+      for (int r = 0; r < kMine; ++r) l_run[r] = NAN;
+    // the head of row r of this lane, and whether the lane speaks for it
+    auto head_of = [&](int r) { return F::kLanes ? r : r * 8 + g; };
+    const bool speaks = F::kLanes ? lane == 0 : t == 0;
+    auto each = [&](int r, float f, int d_from, int d_to, auto&& put) {
+      if constexpr (F::kLanes) {
+        // the chunk that the halvings left: the group's high bits; groups that
+        // hold the same one leave it to the first
+        constexpr int kSame = 8 / kChunks;
+        const int d = (t + 4 * (g / kSame)) * 4;
+        if (g % kSame == 0 && d >= d_from && d < d_to) {
+          const float(&o)[4] = o_lane[r][0];
+          put(d, make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f));
+        }
+      } else {
         // lane (g, t) holds dims of chunks 2 t and 2 t + 1 (+ 8 i) of head g
 #pragma unroll
-        for (int i = 0; i < kPassIter; ++i)
+        for (int i = 0; i < F::kVIter; ++i) {
+          if (i * 8 * F::kVVec < d_from || i * 8 * F::kVVec >= d_to) continue;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
             for (int e = 0; e < F::kVVec; e += 4) {
               float4 x;
               float* xs = reinterpret_cast<float*>(&x);
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const float(&o)[4] = o_acc[(pass * kPassIter + i) * F::kVVec + e + k];
-                xs[k] = (R == 1 ? o[c] + o[c + 2] : o[2 * r + c]) * f;
+                const float(&o)[4] = o_acc[i * F::kVVec + e + k];
+                xs[k] = (R == 1 ? o[cc] + o[cc + 2] : o[2 * r + cc]) * f;
               }
-              *reinterpret_cast<float4*>(join + (w * 8 + g) * J + (2 * t + c + 8 * i) * F::kVVec +
-                                         e) = x;
+              put((2 * t + cc + 8 * i) * F::kVVec + e, x);
             }
+        }
+      }
+    };
+    if (own) {
+#pragma unroll
+      for (int r = 0; r < kMine; ++r) {
+        const int h = head_of(r);
+        if (h >= heads) continue;
+        const float f = l_run[r] == 0.0f ? 0.0f : 1.0f / l_run[r];
+        each(r, f, 0, D, [&](int d, float4 x) { store_act4(p.out, (row + h) * D + d, p.act_dtype, x); });
+        if (speaks && p.lse) p.lse[row + h] = (m_run[r] + log2f(l_run[r])) * kLn2;
+      }
+    } else {
+      const bool whole = cur.tile == 0 && seg == cur.tiles;
+      const bool tail = cur.tile != 0;
+      float* slot = a.partials + (2 * (int64_t)blockIdx.x + (tail ? 0 : 1)) * partial_floats(M, D);
+      if (speaks)
+#pragma unroll
+        for (int r = 0; r < kMine; ++r) {
+          s_m[w][head_of(r)] = m_run[r];
+          s_l[w][head_of(r)] = l_run[r];
+        }
+      __syncthreads();
+      float factor[kMine];
+#pragma unroll
+      for (int r = 0; r < kMine; ++r) {
+        const int h = head_of(r);
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_m[i][h]);
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) sum += s_l[i][h] * exp2_diff(s_m[i][h], top);
+        factor[r] = exp2_diff(m_run[r], top);
+        if (speaks && w == 0) {
+          s_top[h] = top;
+          s_sum[h] = sum;
+        }
+      }
+      // a pass: kRows heads, J dims
+      constexpr int J = F::kJoinDims, kR = F::kRows;
+#pragma unroll
+      for (int pass = 0; pass < M / kR * (D / J); ++pass) {
+        const int block = pass / (D / J), from = pass % (D / J) * J;
+#pragma unroll
+        for (int r = 0; r < kMine; ++r)
+          if (F::kLanes || r == block)
+            each(r, factor[r], from, from + J, [&](int d, float4 x) {
+              *reinterpret_cast<float4*>(join + (w * kR + head_of(r) - block * kR) * J + d - from) = x;
+            });
         __syncthreads();
-        for (int i = tid; i < 8 * J / 4; i += kThreads) {
-          const int h = i / (J / 4), dj = i % (J / 4) * 4, d = pass * J + dj;
+#pragma unroll 1
+        for (int i = tid; i < kR * J / 4; i += kThreads) {
+          const int hj = i / (J / 4), dj = i % (J / 4) * 4, h = block * kR + hj, d = from + dj;
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          float hm = -INFINITY, hl = 0.0f;
 #pragma unroll
           for (int k = 0; k < kWarps; ++k) {
-            const float4 y = *reinterpret_cast<const float4*>(join + (k * 8 + h) * J + dj);
+            const float4 y = *reinterpret_cast<const float4*>(join + (k * kR + hj) * J + dj);
             x.x += y.x;
             x.y += y.y;
             x.z += y.z;
             x.w += y.w;
-            hm = fmaxf(hm, s_m[k][r * 8 + h]);
           }
-#pragma unroll
-          for (int k = 0; k < kWarps; ++k)
-            hl += s_l[k][r * 8 + h] * exp2_diff(s_m[k][r * 8 + h], hm);
-          if (cur.bad) hl = NAN;
           if (!whole) {
-            *reinterpret_cast<float4*>(slot + (r * 8 + h) * D + d) = x;
+            *reinterpret_cast<float4*>(slot + h * D + d) = x;
             if (d == 0) {
-              slot[8 * R * D + r * 8 + h] = hm;
-              slot[8 * R * D + 8 * R + r * 8 + h] = hl;
+              slot[M * D + h] = s_top[h];
+              slot[M * D + M + h] = s_sum[h];
             }
-          } else if (r * 8 + h < heads) {
-            write_out(p, cur.b * p.q_heads + q_head + r * 8 + h, d, D, x, hm, hl);
+          } else if (h < heads) {
+            write_out(p, row + h, d, D, x, s_top[h], s_sum[h]);
           }
         }
         __syncthreads();
       }
-    }
-
-    if (!whole) {
-      // Contributors of this item: CTAs c0 (its first units, odd slot) .. c1.
-      // The last of each kGroup to arrive joins the group's partials into the
-      // group's first, the last group to arrive joins those: a few loads in
-      // flight at a time for one CTA, however many CTAs share the item.
-      const int64_t c0 = ((item_first + 1) * ctas - 1) / total;
-      const int n = (int)(((item_first + cur.units) * ctas - 1) / total - c0) + 1;
-      const int groups = (n + kGroup - 1) / kGroup, mine_at = (int)(blockIdx.x - c0) / kGroup;
-      const int members = n - mine_at * kGroup < kGroup ? n - mine_at * kGroup : kGroup;
-      // A group of one needs no counter, so a group's first CTA names it alone.
-      uint32_t* counter = a.counters + c0 + mine_at * kGroup;
-      if (members == 1 || arrive_last(counter, members, &s_last)) {
-        if (groups > 1) {
-          if (members > 1)
-            join_partials<8 * R, D>(a, c0, mine_at * kGroup, 1, members, true, 0, 0);
-          __syncthreads();
-          if (arrive_last(a.counters + kMaxCtas + c0, groups, &s_last))
-            join_partials<8 * R, D>(a, c0, 0, kGroup, groups, false,
-                                    cur.b * p.q_heads + q_head, heads);
-        } else {
-          join_partials<8 * R, D>(a, c0, 0, 1, n, false, cur.b * p.q_heads + q_head, heads);
-        }
-      }
-    }
-    at += seg;
-    if (at < last) {
-      cur.unit = cur.units - 1;  // the segment ended with its item
-      advance<F::kUnit>(a, cur);
+      if (!whole) split[tail ? 0 : 1] = Split{end - left - cur.tile, cur.tiles, row, heads};
     }
   }
   cp_async_wait<0>();
+
+  // ---- the items this share has a part of: its first and its last at most.
+  // Contributors of an item are CTAs c0 (its first tiles, odd slot) and on.
+  // They join in a tree: the last of kFan neighbours to arrive joins their
+  // partials into the first's and goes on to the next level with it.
+#pragma unroll 1
+  for (int e = 0; e < 2; ++e) {
+    const Split& s = split[e];
+    if (s.tiles == 0) continue;
+    const int64_t c0 = cta_of(s.first);
+    int n = (int)(cta_of(s.first + s.tiles - 1) - c0) + 1;  // partials on this level
+    int at = (int)(blockIdx.x - c0), span = 1;              // this one; CTAs in each
+    for (int level = 0; n > 1; ++level) {
+      const int first = at / kFan * kFan, members = n - first < kFan ? n - first : kFan;
+      if (members > 1) {
+        // a group of one needs no counter, so the first CTA names a group alone
+        __syncthreads();
+        if (!arrive_last(a.counters + level * kMaxCtas + c0 + first * span, members, &s_last)) break;
+        join_partials<M, D>(a, c0, first * span, span, members, n > kFan, s.row, s.heads);
+      }
+      at /= kFan;
+      span *= kFan;
+      n = (n + kFan - 1) / kFan;
+    }
+  }
 }
 
-template <class C, bool F32ACT, int D, int R>
+template <class C, bool F32ACT, int D, int M>
 int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
-  using F = Cfg<C, F32ACT, D, R>;
-  auto kernel = paged_attention_kernel<C, F32ACT, D, R>;
+  using F = Cfg<C, F32ACT, D, M>;
+  auto kernel = paged_attention_kernel<C, F32ACT, D, M>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) !=
       cudaSuccess)
     return CT_ERR_CUDA;
   Launch b = a;
+  b.blocks = (a.group + M - 1) / M;
+  b.items = (int)(a.p.kv_heads * b.blocks);
   b.whole_tiles = a.p.kv.page_size % F::kKeys == 0;
-  // no more CTAs than units the table can hold
+  // no more CTAs than the table can hold work for
   const int64_t keys = a.p.kv.max_pages * a.p.kv.page_size;
-  const int64_t units = a.p.batch * a.items * (keys > F::kUnit ? (keys + F::kUnit - 1) / F::kUnit : 1);
+  const int64_t tiles = a.p.batch * b.items * (keys > F::kKeys ? (keys + F::kKeys - 1) / F::kKeys : 1);
   int64_t ctas = (int64_t)dev.sm_count * F::kCtas;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
-  if (ctas > units) ctas = units;
+  if (ctas > (tiles + kMinShare - 1) / kMinShare) ctas = (tiles + kMinShare - 1) / kMinShare;
   kernel<<<(unsigned)ctas, kThreads, F::kSmem, st>>>(b);
   return check_launch();
 }
 
-constexpr size_t kCounterBytes = 2 * kMaxCtas * sizeof(uint32_t);
-int head_blocks(int64_t q_heads, int64_t kv_heads) { return q_heads / kv_heads > 8 ? 2 : 1; }
+constexpr size_t kCounterBytes = kLevels * kMaxCtas * sizeof(uint32_t);
+
+// Groups of more than 8 heads take 16 at a time where their q stays in
+// registers (64 at most), else 8: the cache is then read again, from L2.
+template <class C, bool F32ACT, int D>
+int launch_heads(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
+  if constexpr (sizeof(C) == 4) {
+    if (a.group == 1) return launch<C, F32ACT, D, 1>(a, dev, st);
+    if (a.group == 2) return launch<C, F32ACT, D, 2>(a, dev, st);
+  }
+  if constexpr (sizeof(C) == 4 ? D <= 64 : D * q_terms<C, F32ACT>() <= 256)
+    if (a.group > 8) return launch<C, F32ACT, D, 16>(a, dev, st);
+  return launch<C, F32ACT, D, 8>(a, dev, st);
+}
 
 template <class C, bool F32ACT>
-int launch_dims(const Launch& a, int r, const DeviceInfo& dev, cudaStream_t st) {
-  if (a.p.head_dim == 32)
-    return r == 1 ? launch<C, F32ACT, 32, 1>(a, dev, st) : launch<C, F32ACT, 32, 2>(a, dev, st);
-  if (a.p.head_dim == 64)
-    return r == 1 ? launch<C, F32ACT, 64, 1>(a, dev, st) : launch<C, F32ACT, 64, 2>(a, dev, st);
-  return r == 1 ? launch<C, F32ACT, 128, 1>(a, dev, st) : launch<C, F32ACT, 128, 2>(a, dev, st);
+int launch_dims(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
+  if (a.p.head_dim == 32) return launch_heads<C, F32ACT, 32>(a, dev, st);
+  if (a.p.head_dim == 64) return launch_heads<C, F32ACT, 64>(a, dev, st);
+  return launch_heads<C, F32ACT, 128>(a, dev, st);
 }
 
 }  // namespace
 
 size_t paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
   return kCounterBytes + 2 * kMaxCtas * sizeof(float) *
-                             partial_floats(8 * head_blocks(q_heads, kv_heads), (int)head_dim);
+                             partial_floats(q_heads / kv_heads > 8 ? 16 : 8, (int)head_dim);
 }
 
 int launch_paged_attention(const PagedAttention& p, const DeviceInfo& dev, cudaStream_t st) {
   Launch a{};
   a.p = p;
-  const int r = head_blocks(p.q_heads, p.kv_heads);
+  if (p.q_heads >= (1ll << 30)) return CT_ERR_INVALID_ARGUMENT;
   a.group = (int)(p.q_heads / p.kv_heads);
-  a.blocks = (a.group + 8 * r - 1) / (8 * r);
-  const int64_t items = p.kv_heads * a.blocks;
-  if (items >= (1ll << 31)) return CT_ERR_INVALID_ARGUMENT;
-  a.items = (int)items;
   a.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (p.kv.page_size == 1 << s) a.page_shift = s;
+  const int q_vec = 16 / dtype_bytes(p.act_dtype);
+  a.q_vectors = aligned16(p.q) && p.qs[0] % q_vec == 0 && p.qs[1] % q_vec == 0 && p.qs[2] == 1;
   a.counters = static_cast<uint32_t*>(p.ws);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(p.ws) + kCounterBytes);
   return with_dtype(p.kv.dtype, [&](auto c) {
     using C = decltype(c);
-    if (p.act_dtype == CT_DTYPE_F32) return launch_dims<C, true>(a, r, dev, st);
-    if constexpr (sizeof(C) == 2) return launch_dims<C, false>(a, r, dev, st);
+    if (p.act_dtype == CT_DTYPE_F32) return launch_dims<C, true>(a, dev, st);
+    if constexpr (sizeof(C) == 2) return launch_dims<C, false>(a, dev, st);
     return (int)CT_ERR_INVALID_ARGUMENT;
   });
 }

@@ -347,7 +347,7 @@ enum { CT_DTYPE_F32 = 0, CT_DTYPE_BF16 = 1, CT_DTYPE_F16 = 2 };
  * int32, row stride table_stride) lists the pages of sequence s in order:
  * its token j lives in page block_table[s][j / page_size], slot
  * j % page_size.  head_dim in {32, 64, 128};
- * max_pages * page_size <= 2^31 - 256. */
+ * max_pages * page_size <= 2^30 - 256. */
 
 /* Appends `tokens` new keys and values (k, v indexed [token, kv_head,
  * head_dim] through their strides) to the cache: token t goes to position
