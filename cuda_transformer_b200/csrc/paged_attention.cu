@@ -33,14 +33,13 @@
 namespace ct {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCtas = 448;  // counters (of each level) and partial slots in the workspace
-constexpr int kFan = 8;        // partials that are joined at a time
-constexpr int kLevels = 3;     // kFan^kLevels >= kMaxCtas
-// Items of no more tiles than a warp's part of its CTA's share (and no more
-// than this) are one warp's.
-constexpr int kShortMax = 16;
+constexpr int kFan = 32;       // partials that are joined at a time
+constexpr int kLevels = 2;     // kFan^kLevels >= kMaxCtas
+// Items of at most so many tiles are never split between CTAs: joining the
+// parts costs more than the tiles.  Those of no more tiles than a warp's part
+// of its CTA's share are one warp's.
+constexpr int kWhole = 16;
 constexpr int kMinShare = 4;   // tiles of a CTA, unless there are fewer in all
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -58,8 +57,9 @@ constexpr int q_terms() {
 // C: the cache's type; F32ACT: q and out are FP32, else of type C; M: query
 // heads a CTA works on.  8: high and low parts share a product's rows; 16: the
 // heads fill them and the parts are products of their own; 1 and 2 (FP32
-// caches): plain FMAs.
-template <class C, bool F32ACT, int D, int M>
+// caches): plain FMAs.  WIDE: one CTA of 8 or 12 warps an SM instead of two or
+// three of four.
+template <class C, bool F32ACT, int D, int M, bool WIDE>
 struct Cfg {
   static constexpr bool kLanes = M <= 2;                    // no tensor cores
   static constexpr int R = M == 16 ? 2 : 1;                 // heads of a lane's rows
@@ -67,13 +67,8 @@ struct Cfg {
   static constexpr bool kF32 = sizeof(C) == 4;
   static constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
   static constexpr int kVec = 16 / (int)sizeof(C);          // elements of a 16-byte chunk
-  static constexpr int kKeys = kF32 ? 8 : 16;                // keys of a warp's tile
-  static constexpr int kNt = kKeys / 8;
   static constexpr int kRowBytes = D * (int)sizeof(C);
   static constexpr int kRowChunks = kRowBytes / 16;
-  static constexpr int kCopies = kKeys * kRowChunks / 32;    // of a lane, for K or V
-  static constexpr int kCopyRows = 32 / kRowChunks;          // rows of one copy instruction
-  static constexpr int kStageBytes = 2 * kKeys * kRowBytes;  // K tile, V tile
   static constexpr int kKIter = D / (4 * kVec);              // K chunks a lane reads per key
   static constexpr int kVVec = kVec < D / 8 ? kVec : D / 8;  // V elements a lane reads at once
   static constexpr int kVIter = D / (8 * kVVec);
@@ -94,10 +89,24 @@ struct Cfg {
   static constexpr int kPOps = R == 1 ? (kPTerms + 1) / 2 : kPTerms;
   static constexpr int kSteps = kF32 ? D / 8 : D / 16;
   static constexpr int kQRegs = kLanes ? M * D / 4 : kSteps * kQOps * 4;
+  // Keys of a warp's tile: 8 KB of K and V, 32 at most; a smaller one (8 keys in
+  // TF32, 16 in the 16-bit types) where q and O leave no registers for the
+  // larger one's scores.
+  static constexpr int kLeast = kF32 ? 8 : 16;
+  static constexpr int kMost = 4096 / kRowBytes < 32 ? 4096 / kRowBytes : 32;
+  static constexpr int kKeys = kLanes || kQRegs + D / 2 <= 48 ? kMost : kLeast;
+  static constexpr int kRun = kKeys < 16 ? kKeys : 16;       // keys that are copied from one page
+  static constexpr int kNt = kKeys / 8;
+  static constexpr int kCopies = kKeys * kRowChunks / 32;    // of a lane, for K or V
+  static constexpr int kCopyRows = 32 / kRowChunks;          // rows of one copy instruction
+  static constexpr int kStageBytes = 2 * kKeys * kRowBytes;  // K tile, V tile
   // Registers: q, O and about 72 more.  Three CTAs an SM where that fits 168 a
   // thread, with two stages of 8 KB or as many smaller ones.
-  static constexpr int kCtas = kQRegs + (kLanes ? kQRegs : D / 2) + 72 <= 168 ? 3 : 2;
-  static constexpr int kRing = kCtas == 3 ? 16384 : 24576;
+  static constexpr int kPerSm = kQRegs + (kLanes ? kQRegs : D / 2) + 72 <= 168 ? 3 : 2;
+  static constexpr int kCtas = WIDE ? 1 : kPerSm;
+  static constexpr int kWarps = WIDE ? 4 * kPerSm : 4;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kRing = kPerSm == 3 ? 16384 : 24576;
   static constexpr int kStages = kRing / kStageBytes > 6 ? 6 : kRing / kStageBytes;
   static constexpr int kJoinDims = D < 64 ? D : 64;          // dims of one joining pass
   static constexpr int kRows = kLanes ? M : 8;               // heads of one joining pass
@@ -212,7 +221,7 @@ struct Launch {
   int group, blocks;  // query heads of a key/value head; its blocks of M heads
   int items;          // (key/value head, block) pairs of a sequence
   int page_shift;     // log2 of page_size, -1 when it is no power of two
-  bool whole_tiles;   // a tile's keys lie in one page
+  bool whole_tiles;   // a tile's keys (runs of 16) lie in one page
   bool q_vectors;     // q's rows are 16-byte vectors
   uint32_t* counters;
   float* partials;
@@ -225,12 +234,11 @@ struct Cursor {
   bool bad;
 };
 
-// A long item that other CTAs work on too: its tiles, its row of the output.
+// A long item that other CTAs work on too: the first of them, how many, the
+// item's row of the output.
 struct Split {
-  int64_t first;
-  int tiles;
   int64_t row;
-  int heads;
+  int first, n, heads;
 };
 
 template <int KEYS>
@@ -254,98 +262,108 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
   return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
-__device__ __forceinline__ float exp2_diff(float m, float top) {
-  return m == -INFINITY ? 0.0f : exp2f(m - top);
+// 2^x to 2 ulp (0 for -inf and for results below the normal range).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+// Reference point of a maximum: sums that have seen no key are 0 to any.
+__device__ __forceinline__ float finite(float top) { return top == -INFINITY ? 0.0f : top; }
 
-// Counts a CTA in; true in all threads of the one that completes `n`, which
-// leaves the counter at zero for the next launch.  Writes made before it by
-// any CTA that was counted are visible after it.
-__device__ __forceinline__ bool arrive_last(uint32_t* counter, int n, int* flag) {
-  if (threadIdx.x == 0) {
-    __threadfence();
-    const bool last = atomicAdd(counter, 1u) == (uint32_t)(n - 1);
-    if (last) *counter = 0u;
-    *flag = last;
-    __threadfence();
-  }
-  __syncthreads();
-  return *flag != 0;
-}
-
-// Joins the partials k0, k0 + step, .. (n <= kFan of them) of the item that CTA
-// c0 starts, in that order and with all their loads in flight: into partial k0
-// or the output.
-template <int HEADS, int D>
-__device__ __forceinline__ void join_partials(const Launch& a, int64_t c0, int k0, int step, int n,
+// Joins the partials k0, k0 + step, .. (n of them) of the item that CTA c0
+// starts, in that order, 8 or 16 at a time: into partial k0 or the output.
+template <int HEADS, int D, int THREADS>
+__device__ __forceinline__ void join_partials(const Launch& a, int c0, int k0, int step, int n,
                                               bool to_partial, int64_t row, int heads) {
   constexpr int64_t kSize = partial_floats(HEADS, D);
-  constexpr int kItems = HEADS * D / 4;  // float4s, two to a thread at a time
-  constexpr int kPart = kItems > kThreads ? 2 : 1;
+  constexpr int kItems = HEADS * D / 4;  // float4s, one or two to a thread at a time
+  constexpr int kPart = kItems > THREADS ? 2 : 1, kBatch = 16 / kPart;
   auto at = [&](int k) { return a.partials + (k == 0 ? 2 * c0 + 1 : 2 * (c0 + k)) * kSize; };
 #pragma unroll 1
-  for (int base = 0; base < kItems; base += kPart * kThreads) {
-    const int first = base + threadIdx.x < kItems ? base + threadIdx.x : 0;
-    float m[kPart][kFan], l[kPart][kFan];
-    float4 y[kPart][kFan];
+  for (int base = 0; base < kItems; base += kPart * THREADS) {
+    float m[kPart], l[kPart];
+    float4 x[kPart];
 #pragma unroll
-    for (int j = 0; j < kFan; ++j) {
-      const float* s = at(k0 + (j < n ? j : 0) * step);
+    for (int i = 0; i < kPart; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll 1
+    for (int b = 0; b < n; b += kBatch) {
+      float km[kPart][kBatch], kl[kPart][kBatch];
+      float4 y[kPart][kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (b + j >= n) continue;
+        const float* s = at(k0 + (b + j) * step);
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) {
+          const int id = base + threadIdx.x + i * THREADS;
+          if (id >= kItems) continue;
+          km[i][j] = __ldcg(s + HEADS * D + id / (D / 4));
+          kl[i][j] = __ldcg(s + HEADS * D + HEADS + id / (D / 4));
+          y[i][j] = __ldcg(reinterpret_cast<const float4*>(s + id * 4));
+        }
+      }
 #pragma unroll
       for (int i = 0; i < kPart; ++i) {
-        const int id = first + i * kThreads, h = id / (D / 4);
-        m[i][j] = __ldcg(s + HEADS * D + h);
-        l[i][j] = __ldcg(s + HEADS * D + HEADS + h);
-        y[i][j] = __ldcg(reinterpret_cast<const float4*>(s + id * 4));
+        float top = m[i];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (b + j < n) top = fmaxf(top, km[i][j]);
+        const float ref = finite(top), f0 = exp2_fast(m[i] - ref);
+        m[i] = top;
+        l[i] *= f0;
+        x[i] = make_float4(x[i].x * f0, x[i].y * f0, x[i].z * f0, x[i].w * f0);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          if (b + j >= n) continue;
+          const float f = exp2_fast(km[i][j] - ref);
+          x[i].x = fmaf(y[i][j].x, f, x[i].x);
+          x[i].y = fmaf(y[i][j].y, f, x[i].y);
+          x[i].z = fmaf(y[i][j].z, f, x[i].z);
+          x[i].w = fmaf(y[i][j].w, f, x[i].w);
+          l[i] = fmaf(kl[i][j], f, l[i]);
+        }
       }
     }
-    // heads' maxima and sums are read by the lanes of one warp; partial k0 is
+    // a head's maxima and sums are read by the lanes of one warp; partial k0 is
     // overwritten after they have them
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kPart; ++i) {
-      const int id = first + i * kThreads, h = id / (D / 4), d = id % (D / 4) * 4;
-      float top = m[i][0], sum = 0.0f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int j = 1; j < kFan; ++j) top = fmaxf(top, j < n ? m[i][j] : -INFINITY);
-#pragma unroll
-      for (int j = 0; j < kFan; ++j) {
-        if (j >= n) continue;
-        const float f = exp2_diff(m[i][j], top);
-        x.x = fmaf(y[i][j].x, f, x.x);
-        x.y = fmaf(y[i][j].y, f, x.y);
-        x.z = fmaf(y[i][j].z, f, x.z);
-        x.w = fmaf(y[i][j].w, f, x.w);
-        sum = fmaf(l[i][j], f, sum);
-      }
-      if (base + (int)threadIdx.x >= kItems) continue;
+      const int id = base + threadIdx.x + i * THREADS, h = id / (D / 4), d = id % (D / 4) * 4;
+      if (id >= kItems) continue;
       if (to_partial) {
         float* s = at(k0);
-        *reinterpret_cast<float4*>(s + id * 4) = x;
+        *reinterpret_cast<float4*>(s + id * 4) = x[i];
         if (d == 0) {
-          s[HEADS * D + h] = top;
-          s[HEADS * D + HEADS + h] = sum;
+          s[HEADS * D + h] = m[i];
+          s[HEADS * D + HEADS + h] = l[i];
         }
       } else if (h < heads) {
-        write_out(a.p, row + h, d, D, x, top, sum);
+        write_out(a.p, row + h, d, D, x[i], m[i], l[i]);
       }
     }
   }
 }
 
-template <class C, bool F32ACT, int D, int M>
-__global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
+template <class C, bool F32ACT, int D, int M, bool WIDE>
+__global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
+                                  Cfg<C, F32ACT, D, M, WIDE>::kCtas)
     paged_attention_kernel(const __grid_constant__ Launch a) {
-  using F = Cfg<C, F32ACT, D, M>;
+  using F = Cfg<C, F32ACT, D, M, WIDE>;
   using A = typename F::A;
-  constexpr int R = F::R;
+  constexpr int R = F::R, kWarps = F::kWarps, kThreads = F::kThreads;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t s_scan[kWarps];
   __shared__ int64_t s_rest[kWarps];
   __shared__ Cursor s_edge[2];
   __shared__ float s_m[kWarps][M], s_l[kWarps][M], s_top[M], s_sum[M];
-  __shared__ int s_last;
+  __shared__ bool s_last[2];
+  __shared__ Split s_split[2];
   const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const PagedAttention& p = a.p;
 
@@ -424,15 +442,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     }
   }
   // an edge inside a short item moves to the item's start
-  const int brief = (int)(share / kWarps < kShortMax ? share / kWarps : kShortMax);
   Cursor cur = s_edge[0];
-  if (cur.tiles <= brief) {
+  if (cur.tiles <= kWhole) {
     edge[0] -= cur.tile;
     cur.tile = 0;
   }
-  if (edge[1] < total && s_edge[1].tiles <= brief) edge[1] -= s_edge[1].tile;
+  if (edge[1] < total && s_edge[1].tiles <= kWhole) edge[1] -= s_edge[1].tile;
+  const int brief = (int)(share / kWarps < kWhole ? share / kWarps : kWhole);
   int64_t left = edge[1] - edge[0];
-  const int64_t end = edge[1];
 
   // Walks the share item by item: true with `seg`, the tiles of the item that
   // lie in the share, and whether it is this warp's alone; false at the end.
@@ -452,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
       fresh = false;
       seg = (int)(todo < x.tiles - x.tile ? todo : x.tiles - x.tile);
       own = x.tiles <= brief;
-      if (!own || ((x.b * a.items + x.item) & (kWarps - 1)) == w) return true;
+      if (!own || (uint32_t)(x.b * a.items + x.item) % kWarps == w) return true;
     }
   };
   if (left <= 0) return;
@@ -461,7 +478,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
   // the products
   const uint32_t ring = smem_addr(smem) + w * (F::kStages * F::kStageBytes);
   const uint8_t* ring_ptr = smem + w * (F::kStages * F::kStageBytes);
-  const bool second = (lane / F::kKeys) & 1;  // this lane addresses V rows, else K rows
   const int my_row = lane % F::kKeys;
   const int copy_row = lane / F::kRowChunks, copy_chunk = lane % F::kRowChunks;
   const int64_t k_step = p.kv.ks[2] * (int64_t)sizeof(C), v_step = p.kv.vs[2] * (int64_t)sizeof(C);
@@ -520,39 +536,48 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     if (next == kTile) {
       const bool fine = next_there && (unsigned)next_page < (unsigned)p.kv.pages;
       if (a.whole_tiles && __all_sync(0xffffffffu, fine)) {
-        // all rows are there and follow one another in one page
-        const int slot = next_slot - my_row;
-        const uint8_t* src[2] = {
-            k_item + next_page * k_page + slot * k_step,
-            v_item + next_page * v_page + slot * v_step};
+        // all rows are there and follow one another in one page (or two)
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int64_t step = F::kCopyRows * (kv ? v_step : k_step);
+        for (int run = 0; run < F::kKeys / F::kRun; ++run) {
+          const int64_t page = F::kKeys == F::kRun ? next_page
+                                                   : __shfl_sync(0xffffffffu, next_page, run * F::kRun);
+          const int slot = F::kKeys == F::kRun ? next_slot - my_row
+                                               : __shfl_sync(0xffffffffu, next_slot, run * F::kRun);
 #pragma unroll
-          for (int i = 0; i < F::kCopies; ++i)
-            cp_async16(base + kv * (F::kKeys * F::kRowBytes) +
-                           chunk_pos<F::kRowBytes>(i * F::kCopyRows + copy_row, copy_chunk),
-                       src[kv] + i * step, 16);
+          for (int kv = 0; kv < 2; ++kv) {
+            const int64_t row_step = kv ? v_step : k_step, step = F::kCopyRows * row_step;
+            const uint8_t* src = (kv ? v_item : k_item) + page * (kv ? v_page : k_page) + slot * row_step;
+#pragma unroll
+            for (int i = 0; i < F::kRun / F::kCopyRows; ++i)
+              cp_async16(base + kv * (F::kKeys * F::kRowBytes) +
+                             chunk_pos<F::kRowBytes>(run * F::kRun + i * F::kCopyRows + copy_row,
+                                                     copy_chunk),
+                         src + i * step, 16);
+          }
         }
       } else if (__any_sync(0xffffffffu, next_there)) {
-        int64_t off = -1;  // past the length: zeros
-        if (next_there) {
-          off = !fine    ? -2  // no such page: NaN
-                : second ? next_page * v_page + next_slot * v_step
-                         : next_page * k_page + next_slot * k_step;
+        // bytes from the item's first row: -1 past the length (zeros), -2 where
+        // there is no such page (NaN)
+        int64_t off[2] = {next_there ? -2 : -1, next_there ? -2 : -1};
+        if (fine) {
+          off[0] = next_page * k_page + next_slot * k_step;
+          off[1] = next_page * v_page + next_slot * v_step;
         }
 #pragma unroll
-        for (int i = 0; i < 2 * F::kCopies; ++i) {
-          const int kv = i / F::kCopies, r = i % F::kCopies * F::kCopyRows + copy_row;
+        for (int kv = 0; kv < 2; ++kv) {
           const uint8_t* from = kv ? v_item - copy_row * v_step : k_item - copy_row * k_step;
-          const int64_t o = __shfl_sync(0xffffffffu, off, kv * F::kKeys + r);
-          const uint32_t dst =
-              base + kv * (F::kKeys * F::kRowBytes) + chunk_pos<F::kRowBytes>(r, copy_chunk);
-          if (o == -2)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0x7fc07fc0u)
-                         : "memory");  // NaN in each of the three types
-          else
-            cp_async16(dst, o < 0 ? p.kv.k : from + o, o < 0 ? 0 : 16);
+#pragma unroll
+          for (int i = 0; i < F::kCopies; ++i) {
+            const int r = i * F::kCopyRows + copy_row;
+            const int64_t o = __shfl_sync(0xffffffffu, off[kv], r);
+            const uint32_t dst =
+                base + kv * (F::kKeys * F::kRowBytes) + chunk_pos<F::kRowBytes>(r, copy_chunk);
+            if (o == -2)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0x7fc07fc0u)
+                           : "memory");  // NaN in each of the three types
+            else
+              cp_async16(dst, o < 0 ? p.kv.k : from + o, o < 0 ? 0 : 16);
+          }
         }
       }
     } else if (next == kQuery) {
@@ -581,6 +606,27 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     step_ahead();
   };
 
+  // while the first copies are on their way: the items that the share has a
+  // part of, the one it starts in (if that began before it or goes on after
+  // it) and the one it ends in
+  if (tid < 2) {
+    const Cursor& x = s_edge[tid];
+    const int64_t first = edge[tid] - x.tile;
+    Split s{};
+    bool part = tid == 0 || edge[1] < total;
+    if (part) part = x.tiles > kWhole;  // (short ones lie in one share)
+    if (part)
+      part = tid == 0 ? x.tile > 0 || first + x.tiles > edge[1] : x.tile > 0 && first > edge[0];
+    if (part) {
+      s.first = (int)cta_of(first);
+      s.n = (int)cta_of(first + x.tiles - 1) - s.first + 1;
+      const int head0 = (x.item % a.blocks) * M;
+      s.row = x.b * p.q_heads + (int64_t)(x.item / a.blocks) * a.group + head0;
+      s.heads = a.group - head0 < M ? a.group - head0 : M;
+    }
+    s_split[tid] = s;
+  }
+
   float* join = reinterpret_cast<float*>(smem + F::kRingBytes);
   // q, O, maxima and sums: of a lane's rows of the products, or (plain FMAs) of
   // keys g, g + 8, .. and the dims of chunks t + 4 i
@@ -592,7 +638,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
   float m_run[kMine], l_run[kMine], s_mul[kMine];
   int stage = 0;  // the next to fill
   int filled = 0;
-  Split split[2] = {};
 
   int seg = 0;  // tiles of the item in this share
   bool own = false;
@@ -682,7 +727,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
               } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                  float x = q_at(r, d + 2 * h) * q_mul[r], y = q_at(r, d + 2 * h + 1) * q_mul[r];
+                  if constexpr (!F32ACT) {  // exact as it is
+                  q_regs[s][0][r + 2 * h] = *reinterpret_cast<const uint32_t*>(
+                      tile + q_pos<F::kQRowChunks>(r * 8 + g, (d + 2 * h) * 2 / 16) +
+                      (d + 2 * h) * 2 % 16);
+                  if (R == 1) q_regs[s][0][1 + 2 * h] = 0u;
+                  continue;
+                }
+                float x = q_at(r, d + 2 * h) * q_mul[r], y = q_at(r, d + 2 * h + 1) * q_mul[r];
 #pragma unroll
                   for (int k = 0; k < F::kQTerms; ++k)
                     q_regs[s][R == 1 ? k / 2 : k][(R == 1 ? k % 2 : r) + 2 * h] = take_term<C>(x, y);
@@ -704,49 +756,52 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
       if (first_key >= end_key) continue;
 
       if constexpr (F::kLanes) {
-        // ---- key g of the tile, the dims of chunks t + 4 i
-        float s[M];
+        // ---- key n * 8 + g of the tile, the dims of chunks t + 4 i
 #pragma unroll
-        for (int h = 0; h < M; ++h) s[h] = 0.0f;
+        for (int n = 0; n < F::kNt; ++n) {
+          float s[M];
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-          alignas(16) float x[4];
-          *reinterpret_cast<float4*>(x) =
-              *reinterpret_cast<const float4*>(tile + chunk_pos<F::kRowBytes>(g, t + 4 * i));
+          for (int h = 0; h < M; ++h) s[h] = 0.0f;
 #pragma unroll
-          for (int h = 0; h < M; ++h)
+          for (int i = 0; i < kChunks; ++i) {
+            alignas(16) float x[4];
+            *reinterpret_cast<float4*>(x) =
+                *reinterpret_cast<const float4*>(tile + chunk_pos<F::kRowBytes>(n * 8 + g, t + 4 * i));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[h] = fmaf(q_lane[h][i][e], x[e], s[h]);
-        }
-        float pr[M];
+            for (int h = 0; h < M; ++h)
 #pragma unroll
-        for (int h = 0; h < M; ++h) {
-          s[h] += __shfl_xor_sync(0xffffffffu, s[h], 1);
-          s[h] += __shfl_xor_sync(0xffffffffu, s[h], 2);
-          s[h] *= s_mul[h];
-          if (first_key + g >= end_key) s[h] = -INFINITY;
-          // each lane has a maximum of its own keys
-          if (__any_sync(0xffffffffu, s[h] > m_run[h] + kMaxSlack)) {
-            const float top = fmaxf(s[h], m_run[h]), f = exp2_diff(m_run[h], top);
-            m_run[h] = top;
-            l_run[h] *= f;
-#pragma unroll
-            for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o_lane[h][i][e] *= f;
+              for (int e = 0; e < 4; ++e) s[h] = fmaf(q_lane[h][i][e], x[e], s[h]);
           }
-          pr[h] = exp2f(s[h] - (m_run[h] == -INFINITY ? 0.0f : m_run[h]));
-          l_run[h] += pr[h];
-        }
+          float pr[M];
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-          alignas(16) float x[4];
-          *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(
-              tile + F::kKeys * F::kRowBytes + chunk_pos<F::kRowBytes>(g, t + 4 * i));
+          for (int h = 0; h < M; ++h) {
+            s[h] += __shfl_xor_sync(0xffffffffu, s[h], 1);
+            s[h] += __shfl_xor_sync(0xffffffffu, s[h], 2);
+            s[h] *= s_mul[h];
+            if (first_key + n * 8 + g >= end_key) s[h] = -INFINITY;
+            // each lane has a maximum of its own keys
+            if (__any_sync(0xffffffffu, s[h] > m_run[h] + kMaxSlack)) {
+              const float top = fmaxf(s[h], m_run[h]), f = exp2_fast(m_run[h] - finite(top));
+              m_run[h] = top;
+              l_run[h] *= f;
 #pragma unroll
-          for (int h = 0; h < M; ++h)
+              for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o_lane[h][i][e] = fmaf(pr[h], x[e], o_lane[h][i][e]);
+                for (int e = 0; e < 4; ++e) o_lane[h][i][e] *= f;
+            }
+            pr[h] = exp2_fast(s[h] - finite(m_run[h]));
+            l_run[h] += pr[h];
+          }
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i) {
+            alignas(16) float x[4];
+            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(
+                tile + F::kKeys * F::kRowBytes + chunk_pos<F::kRowBytes>(n * 8 + g, t + 4 * i));
+#pragma unroll
+            for (int h = 0; h < M; ++h)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o_lane[h][i][e] = fmaf(pr[h], x[e], o_lane[h][i][e]);
+          }
         }
         continue;
       } else {
@@ -783,7 +838,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
       }
 
       // ---- probabilities of keys n * 8 + 2 t and + 1; heads g (and g + 8)
-      uint32_t pa[F::kPOps][4];
+      constexpr int kKSteps = F::kF32 ? F::kNt : F::kNt / 2;  // products over the tile's keys
+      uint32_t pa[kKSteps][F::kPOps][4];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float v[F::kNt][2], top = -INFINITY;
@@ -802,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           top = fmaxf(top - F::kBelow, m_run[r]);
-          const float f = exp2_diff(m_run[r], top);
+          const float f = exp2_fast(m_run[r] - finite(top));
           m_run[r] = top;
           l_run[r] *= f;
 #pragma unroll
@@ -811,10 +867,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
             for (int e = 0; e < 4; ++e)
               if (R == 1 || e / 2 == r) o_acc[j][e] *= f;
         }
-        const float m = m_run[r] == -INFINITY ? 0.0f : m_run[r];
+        const float m = finite(m_run[r]);
 #pragma unroll
         for (int n = 0; n < F::kNt; ++n) {
-          float x = exp2f(v[n][0] - m), y = exp2f(v[n][1] - m);
+          float x = exp2_fast(v[n][0] - m), y = exp2_fast(v[n][1] - m);
           l_run[r] += x + y;
           if constexpr (F::kF32) {
             uint32_t term[2][2];
@@ -822,14 +878,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
             split_tf32(y, term[0][1], term[1][1]);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              pa[R == 1 ? 0 : k][R == 1 ? k : r] = term[k][0];
-              pa[R == 1 ? 0 : k][(R == 1 ? k : r) + 2] = term[k][1];
+              pa[n][R == 1 ? 0 : k][R == 1 ? k : r] = term[k][0];
+              pa[n][R == 1 ? 0 : k][(R == 1 ? k : r) + 2] = term[k][1];
             }
           } else {
 #pragma unroll
             for (int k = 0; k < F::kPTerms; ++k)
-              pa[R == 1 ? k / 2 : k][(R == 1 ? k % 2 : r) + 2 * n] = take_term<C>(x, y);
-            if (R == 1 && F::kPTerms % 2) pa[F::kPTerms / 2][1 + 2 * n] = 0u;
+              pa[n / 2][R == 1 ? k / 2 : k][(R == 1 ? k % 2 : r) + 2 * (n % 2)] = take_term<C>(x, y);
+            if (R == 1 && F::kPTerms % 2) pa[n / 2][F::kPTerms / 2][1 + 2 * (n % 2)] = 0u;
           }
         }
       }
@@ -840,44 +896,50 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
       const uint8_t* vt = tile + F::kKeys * F::kRowBytes;
 #pragma unroll
       for (int i = 0; i < F::kVIter; ++i) {
-        alignas(16) uint32_t vw[2 * F::kNt][4];
+        float c[F::kVVec][4];
 #pragma unroll
-        for (int n = 0; n < 2 * F::kNt; ++n) {
-          const int r = (n / 2) * 8 + 2 * t + n % 2;
-          if constexpr (F::kVVec == F::kVec)
-            *reinterpret_cast<uint4*>(vw[n]) = *reinterpret_cast<const uint4*>(
-                vt + chunk_pos<F::kRowBytes>(r, g + 8 * i));
-          else  // 64-byte rows: half a chunk to a lane
-            *reinterpret_cast<uint2*>(vw[n]) = *reinterpret_cast<const uint2*>(
-                vt + chunk_pos<F::kRowBytes>(r, g >> 1) + (g & 1) * 8);
-        }
+        for (int e = 0; e < F::kVVec; ++e)
 #pragma unroll
-        for (int e = 0; e < F::kVVec; ++e) {
-          float(&o)[4] = o_acc[i * F::kVVec + e];
-          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (!F32ACT) {
+          for (int x = 0; x < 4; ++x)  // (the low part's sum may be cut off)
+            c[e][x] = !F32ACT || (R == 1 && x >= 2) ? o_acc[i * F::kVVec + e][x] : 0.0f;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) c[x] = o[x];
-          } else if constexpr (R == 1) {  // the low part's sum may be cut off
-            c[2] = o[2];
-            c[3] = o[3];
-          }
-          if constexpr (F::kF32) {
-            const uint32_t x = vw[0][e], y = vw[1][e];
-            mma<C>(c, pa[0], low_tf32(x), low_tf32(y));
-            if constexpr (R == 2) mma<C>(c, pa[1], x, y);
-            mma<C>(c, pa[0], x, y);
-          } else {
-            // element e of keys 2 t and 2 t + 1 (and 8 further) in one word
-            const uint32_t pick = e % 2 ? 0x7632u : 0x5410u;
-            const uint32_t b0 = __byte_perm(vw[0][e / 2], vw[1][e / 2], pick);
-            const uint32_t b1 = __byte_perm(vw[2][e / 2], vw[3][e / 2], pick);
+        for (int ks = 0; ks < kKSteps; ++ks) {
+          constexpr int kV = F::kF32 ? 2 : 4;  // of the lane's keys in a product
+          alignas(16) uint32_t vw[kV][4];
 #pragma unroll
-            for (int k = 0; k < F::kPOps; ++k) mma<C>(c, pa[k], b0, b1);
+          for (int n = 0; n < kV; ++n) {
+            const int r = ks * 4 * kV + (n / 2) * 8 + 2 * t + n % 2;
+            if constexpr (F::kVVec == F::kVec)
+              *reinterpret_cast<uint4*>(vw[n]) = *reinterpret_cast<const uint4*>(
+                  vt + chunk_pos<F::kRowBytes>(r, g + 8 * i));
+            else  // 64-byte rows: half a chunk to a lane
+              *reinterpret_cast<uint2*>(vw[n]) = *reinterpret_cast<const uint2*>(
+                  vt + chunk_pos<F::kRowBytes>(r, g >> 1) + (g & 1) * 8);
           }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[x] = F32ACT && (R == 2 || x < 2) ? o[x] + c[x] : c[x];
+          for (int e = 0; e < F::kVVec; ++e) {
+            if constexpr (F::kF32) {
+              const uint32_t x = vw[0][e], y = vw[1][e];
+              mma<C>(c[e], pa[ks][0], low_tf32(x), low_tf32(y));
+              if constexpr (R == 2) mma<C>(c[e], pa[ks][1], x, y);
+              mma<C>(c[e], pa[ks][0], x, y);
+            } else {
+              // element e of keys 2 t and 2 t + 1 (and 8 further) in one word
+              const uint32_t pick = e % 2 ? 0x7632u : 0x5410u;
+              const uint32_t b0 = __byte_perm(vw[0][e / 2], vw[1][e / 2], pick);
+              const uint32_t b1 = __byte_perm(vw[2][e / 2], vw[3][e / 2], pick);
+#pragma unroll
+              for (int k = 0; k < F::kPOps; ++k) mma<C>(c[e], pa[ks][k], b0, b1);
+            }
+          }
         }
+#pragma unroll
+        for (int e = 0; e < F::kVVec; ++e)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float& o = o_acc[i * F::kVVec + e][x];
+            o = F32ACT && (R == 2 || x < 2) ? o + c[e][x] : c[e][x];
+          }
       }
       }
     }
@@ -892,7 +954,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
         float top = m_run[h];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float f = exp2_diff(m_run[h], top);
+        const float f = exp2_fast(m_run[h] - finite(top));
         m_run[h] = top;
         l_run[h] *= f;
 #pragma unroll
@@ -982,13 +1044,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
 #pragma unroll
       for (int r = 0; r < kMine; ++r) {
         const int h = head_of(r);
-        float top = -INFINITY, sum = 0.0f;
+        float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_m[i][h]);
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) sum += s_l[i][h] * exp2_diff(s_m[i][h], top);
-        factor[r] = exp2_diff(m_run[r], top);
+        const float ref = finite(top);
+        factor[r] = exp2_fast(m_run[r] - ref);
         if (speaks && w == 0) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kWarps; ++i) sum = fmaf(s_l[i][h], exp2_fast(s_m[i][h] - ref), sum);
           s_top[h] = top;
           s_sum[h] = sum;
         }
@@ -1029,71 +1093,111 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
         }
         __syncthreads();
       }
-      if (!whole) split[tail ? 0 : 1] = Split{end - left - cur.tile, cur.tiles, row, heads};
     }
   }
   cp_async_wait<0>();
 
   // ---- the items this share has a part of: its first and its last at most.
-  // Contributors of an item are CTAs c0 (its first tiles, odd slot) and on.
+  // Contributors of an item are CTAs `first` (its first tiles, odd slot) and on.
   // They join in a tree: the last of kFan neighbours to arrive joins their
   // partials into the first's and goes on to the next level with it.
-#pragma unroll 1
+  // Both items of a CTA climb together: a CTA that joins one would be late for
+  // the other.
+  __syncthreads();
+  int c0[2], n[2], at[2];  // partials on this level (0: no part in it), this CTA's
+#pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const Split& s = split[e];
-    if (s.tiles == 0) continue;
-    const int64_t c0 = cta_of(s.first);
-    int n = (int)(cta_of(s.first + s.tiles - 1) - c0) + 1;  // partials on this level
-    int at = (int)(blockIdx.x - c0), span = 1;              // this one; CTAs in each
-    for (int level = 0; n > 1; ++level) {
-      const int first = at / kFan * kFan, members = n - first < kFan ? n - first : kFan;
-      if (members > 1) {
+    c0[e] = s_split[e].first;
+    n[e] = s_split[e].n;
+    at[e] = (int)blockIdx.x - c0[e];
+  }
+  for (int level = 0, span = 1; n[0] + n[1] > 0; ++level, span *= kFan) {
+    int members[2];
+    __syncthreads();
+    if (tid == 0) {
+      // Counts this CTA in; the one that completes a group leaves its counter
+      // at zero for the next launch.  Writes made before by any CTA that was
+      // counted are visible after.
+      __threadfence();
+      uint32_t old[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int first = at[e] / kFan * kFan;
+        members[e] = n[e] - first < kFan ? n[e] - first : kFan;
         // a group of one needs no counter, so the first CTA names a group alone
-        __syncthreads();
-        if (!arrive_last(a.counters + level * kMaxCtas + c0 + first * span, members, &s_last)) break;
-        join_partials<M, D>(a, c0, first * span, span, members, n > kFan, s.row, s.heads);
+        old[e] = members[e] > 1
+                     ? atomicAdd(a.counters + level * kMaxCtas + c0[e] + first * span, 1u)
+                     : 0u;
       }
-      at /= kFan;
-      span *= kFan;
-      n = (n + kFan - 1) / kFan;
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool last = old[e] + 1 == (uint32_t)members[e];
+        if (last && members[e] > 1)
+          a.counters[level * kMaxCtas + c0[e] + at[e] / kFan * kFan * span] = 0u;
+        s_last[e] = last;
+        any = any || last;
+      }
+      if (any) __threadfence();
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+      if (n[e] == 0) continue;
+      const int first = at[e] / kFan * kFan, of = n[e] - first < kFan ? n[e] - first : kFan;
+      const bool top = n[e] <= kFan;
+      if (s_last[e] && of > 1)
+        join_partials<M, D, kThreads>(a, c0[e], first * span, span, of, !top, s_split[e].row,
+                            s_split[e].heads);
+      at[e] /= kFan;
+      n[e] = top || !s_last[e] ? 0 : (n[e] + kFan - 1) / kFan;
     }
   }
 }
 
-template <class C, bool F32ACT, int D, int M>
+template <class C, bool F32ACT, int D, int M, bool WIDE>
 int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
-  using F = Cfg<C, F32ACT, D, M>;
-  auto kernel = paged_attention_kernel<C, F32ACT, D, M>;
+  using F = Cfg<C, F32ACT, D, M, WIDE>;
+  auto kernel = paged_attention_kernel<C, F32ACT, D, M, WIDE>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) !=
       cudaSuccess)
     return CT_ERR_CUDA;
   Launch b = a;
   b.blocks = (a.group + M - 1) / M;
   b.items = (int)(a.p.kv_heads * b.blocks);
-  b.whole_tiles = a.p.kv.page_size % F::kKeys == 0;
+  b.whole_tiles = a.p.kv.page_size % F::kRun == 0;
   // no more CTAs than the table can hold work for
   const int64_t keys = a.p.kv.max_pages * a.p.kv.page_size;
   const int64_t tiles = a.p.batch * b.items * (keys > F::kKeys ? (keys + F::kKeys - 1) / F::kKeys : 1);
   int64_t ctas = (int64_t)dev.sm_count * F::kCtas;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   if (ctas > (tiles + kMinShare - 1) / kMinShare) ctas = (tiles + kMinShare - 1) / kMinShare;
-  kernel<<<(unsigned)ctas, kThreads, F::kSmem, st>>>(b);
+  kernel<<<(unsigned)ctas, F::kThreads, F::kSmem, st>>>(b);
   return check_launch();
 }
 
 constexpr size_t kCounterBytes = kLevels * kMaxCtas * sizeof(uint32_t);
+
+template <class C, bool F32ACT, int D, int M>
+int launch_width(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
+  // Fewer items than SMs: nearly all are split, and one large CTA an SM leaves
+  // a third of the partials to join.
+  if (a.p.batch * a.p.kv_heads * ((a.group + M - 1) / M) < dev.sm_count)
+    return launch<C, F32ACT, D, M, true>(a, dev, st);
+  return launch<C, F32ACT, D, M, false>(a, dev, st);
+}
 
 // Groups of more than 8 heads take 16 at a time where their q stays in
 // registers (64 at most), else 8: the cache is then read again, from L2.
 template <class C, bool F32ACT, int D>
 int launch_heads(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   if constexpr (sizeof(C) == 4) {
-    if (a.group == 1) return launch<C, F32ACT, D, 1>(a, dev, st);
-    if (a.group == 2) return launch<C, F32ACT, D, 2>(a, dev, st);
+    if (a.group == 1) return launch_width<C, F32ACT, D, 1>(a, dev, st);
+    if (a.group == 2) return launch_width<C, F32ACT, D, 2>(a, dev, st);
   }
   if constexpr (sizeof(C) == 4 ? D <= 64 : D * q_terms<C, F32ACT>() <= 256)
-    if (a.group > 8) return launch<C, F32ACT, D, 16>(a, dev, st);
-  return launch<C, F32ACT, D, 8>(a, dev, st);
+    if (a.group > 8) return launch_width<C, F32ACT, D, 16>(a, dev, st);
+  return launch_width<C, F32ACT, D, 8>(a, dev, st);
 }
 
 template <class C, bool F32ACT>
