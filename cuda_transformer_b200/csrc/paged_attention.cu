@@ -6,15 +6,15 @@
 //
 // Every cached value is read once and used for 2 * group FLOPs, so the bound
 // is HBM.  The design follows from that:
-//  * Work is cut into tiles of 8 or 16 keys of one (sequence, key/value head),
-//    and every CTA takes an equal share of the tiles, counted on the device
-//    from seq_lens (the host knows no lengths).  Ragged batches and one long
-//    sequence load the GPU alike.  Short items stay whole and belong to one
-//    warp, which needs nobody else; the four warps of a CTA take turns at the
-//    tiles of a long one and join at its end.  A share that starts or ends
-//    inside a long item leaves a partial (maximum, sum, O) in the workspace;
-//    the CTA that arrives last joins the partials in their order, so results
-//    do not depend on timing and no CTA waits for another.
+//  * Work is cut into tiles of 8 to 32 keys of one item (a sequence and a
+//    key/value head), and every CTA takes an equal share of the tiles, counted
+//    on the device from seq_lens (the host knows no lengths).  Ragged batches
+//    and one long sequence load the GPU alike.  Short items stay whole; the
+//    shortest belong to one warp, which needs nobody else, at the others the
+//    four warps of a CTA take turns and join at the end.  A share that starts
+//    or ends inside a long item leaves a partial (maximum, sum, O) in the
+//    workspace; the CTA that arrives last joins the partials in their order,
+//    so results do not depend on timing and no CTA waits for another.
 //  * Each warp streams q and its keys and values through a private cp.async
 //    ring (16-byte copies gather pages of any size and layout) that runs ahead
 //    across items; a block barrier comes only where a long item ends.
@@ -34,12 +34,16 @@ namespace ct {
 namespace {
 
 constexpr int kMaxCtas = 448;  // counters (of each level) and partial slots in the workspace
-constexpr int kFan = 32;       // partials that are joined at a time
-constexpr int kLevels = 2;     // kFan^kLevels >= kMaxCtas
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kFan = 8;        // partials that are joined at a time
+constexpr int kLevels = 3;     // kFan^kLevels >= kMaxCtas
 // Items of at most so many tiles are never split between CTAs: joining the
 // parts costs more than the tiles.  Those of no more tiles than a warp's part
 // of its CTA's share are one warp's.
 constexpr int kWhole = 16;
+// What an item costs beside its tiles (q, the end), in tiles.
+constexpr int kItemCost = 3;
 constexpr int kMinShare = 4;   // tiles of a CTA, unless there are fewer in all
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -57,9 +61,8 @@ constexpr int q_terms() {
 // C: the cache's type; F32ACT: q and out are FP32, else of type C; M: query
 // heads a CTA works on.  8: high and low parts share a product's rows; 16: the
 // heads fill them and the parts are products of their own; 1 and 2 (FP32
-// caches): plain FMAs.  WIDE: one CTA of 8 or 12 warps an SM instead of two or
-// three of four.
-template <class C, bool F32ACT, int D, int M, bool WIDE>
+// caches): plain FMAs.
+template <class C, bool F32ACT, int D, int M>
 struct Cfg {
   static constexpr bool kLanes = M <= 2;                    // no tensor cores
   static constexpr int R = M == 16 ? 2 : 1;                 // heads of a lane's rows
@@ -102,20 +105,14 @@ struct Cfg {
   static constexpr int kStageBytes = 2 * kKeys * kRowBytes;  // K tile, V tile
   // Registers: q, O and about 72 more.  Three CTAs an SM where that fits 168 a
   // thread, with two stages of 8 KB or as many smaller ones.
-  static constexpr int kPerSm = kQRegs + (kLanes ? kQRegs : D / 2) + 72 <= 168 ? 3 : 2;
-  static constexpr int kCtas = WIDE ? 1 : kPerSm;
-  static constexpr int kWarps = WIDE ? 4 * kPerSm : 4;
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int kRing = kPerSm == 3 ? 16384 : 24576;
+  static constexpr int kCtas = kQRegs + (kLanes ? kQRegs : D / 2) + 72 <= 168 ? 3 : 2;
+  static constexpr int kRing = kCtas == 3 ? 16384 : 24576;
   static constexpr int kStages = kRing / kStageBytes > 6 ? 6 : kRing / kStageBytes;
-  static constexpr int kJoinDims = D < 64 ? D : 64;          // dims of one joining pass
-  static constexpr int kRows = kLanes ? M : 8;               // heads of one joining pass
-  static constexpr int kJoinBytes = kWarps * kRows * kJoinDims * 4;
+  static_assert(M * D * 4 <= kStageBytes, "the warps' O meet in stages of their rings");
   static constexpr int kQRowChunks = D * (int)sizeof(A) / 16;
   static constexpr int kQChunks = M * kQRowChunks;
   static_assert(kQChunks * 16 <= kStageBytes, "q passes through a stage of the ring");
-  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-  static constexpr int kSmem = kRingBytes + kJoinBytes;
+  static constexpr int kSmem = kWarps * kStages * kStageBytes;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
@@ -273,15 +270,15 @@ __device__ __forceinline__ float finite(float top) { return top == -INFINITY ? 0
 
 // Joins the partials k0, k0 + step, .. (n of them) of the item that CTA c0
 // starts, in that order, 8 or 16 at a time: into partial k0 or the output.
-template <int HEADS, int D, int THREADS>
+template <int HEADS, int D>
 __device__ __forceinline__ void join_partials(const Launch& a, int c0, int k0, int step, int n,
                                               bool to_partial, int64_t row, int heads) {
   constexpr int64_t kSize = partial_floats(HEADS, D);
   constexpr int kItems = HEADS * D / 4;  // float4s, one or two to a thread at a time
-  constexpr int kPart = kItems > THREADS ? 2 : 1, kBatch = 16 / kPart;
+  constexpr int kPart = kItems > kThreads ? 2 : 1, kBatch = 16 / kPart;
   auto at = [&](int k) { return a.partials + (k == 0 ? 2 * c0 + 1 : 2 * (c0 + k)) * kSize; };
 #pragma unroll 1
-  for (int base = 0; base < kItems; base += kPart * THREADS) {
+  for (int base = 0; base < kItems; base += kPart * kThreads) {
     float m[kPart], l[kPart];
     float4 x[kPart];
 #pragma unroll
@@ -300,7 +297,7 @@ __device__ __forceinline__ void join_partials(const Launch& a, int c0, int k0, i
         const float* s = at(k0 + (b + j) * step);
 #pragma unroll
         for (int i = 0; i < kPart; ++i) {
-          const int id = base + threadIdx.x + i * THREADS;
+          const int id = base + threadIdx.x + i * kThreads;
           if (id >= kItems) continue;
           km[i][j] = __ldcg(s + HEADS * D + id / (D / 4));
           kl[i][j] = __ldcg(s + HEADS * D + HEADS + id / (D / 4));
@@ -334,7 +331,7 @@ __device__ __forceinline__ void join_partials(const Launch& a, int c0, int k0, i
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kPart; ++i) {
-      const int id = base + threadIdx.x + i * THREADS, h = id / (D / 4), d = id % (D / 4) * 4;
+      const int id = base + threadIdx.x + i * kThreads, h = id / (D / 4), d = id % (D / 4) * 4;
       if (id >= kItems) continue;
       if (to_partial) {
         float* s = at(k0);
@@ -350,25 +347,28 @@ __device__ __forceinline__ void join_partials(const Launch& a, int c0, int k0, i
   }
 }
 
-template <class C, bool F32ACT, int D, int M, bool WIDE>
-__global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
-                                  Cfg<C, F32ACT, D, M, WIDE>::kCtas)
+template <class C, bool F32ACT, int D, int M>
+__global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     paged_attention_kernel(const __grid_constant__ Launch a) {
-  using F = Cfg<C, F32ACT, D, M, WIDE>;
+  using F = Cfg<C, F32ACT, D, M>;
   using A = typename F::A;
-  constexpr int R = F::R, kWarps = F::kWarps, kThreads = F::kThreads;
+  constexpr int R = F::R;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t s_scan[kWarps];
   __shared__ int64_t s_rest[kWarps];
   __shared__ Cursor s_edge[2];
-  __shared__ float s_m[kWarps][M], s_l[kWarps][M], s_top[M], s_sum[M];
+  __shared__ int64_t s_first[2];
+  __shared__ float s_m[kWarps][M], s_l[kWarps][M];
+  __shared__ int s_area[kWarps];
   __shared__ bool s_last[2];
   __shared__ Split s_split[2];
   const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const PagedAttention& p = a.p;
 
-  // ---- this CTA's share of the tiles: a scan of the sequences' tiles, a
-  // block's worth at a time (nearly always one)
+  // ---- this CTA's share of the tiles: a scan of the sequences' tiles (and
+  // items' costs), a block's worth at a time (nearly always one)
+  if (tid == 0) s_edge[1].b = p.batch;  // where the last share ends
+  if (tid < 2) s_split[tid] = Split{};
   Cursor c{};
   c.b = tid;
   if (c.b < p.batch) read_length<F::kKeys>(a, c);
@@ -378,14 +378,14 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
       Cursor x;
       x.b = b;
       read_length<F::kKeys>(a, x);
-      rest += x.tiles;
+      rest += x.tiles + kItemCost;
     }
 #pragma unroll 1
     for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
     if (lane == 0) s_rest[w] = rest;
   }
   auto warp_scan = [&]() {  // 32 sequences have fewer than 2^32 tiles
-    uint32_t x = c.tiles;
+    uint32_t x = c.b < p.batch ? c.tiles + kItemCost : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
@@ -418,13 +418,18 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
   edge[0] = blockIdx.x * share + (blockIdx.x < longer ? blockIdx.x : longer);
   edge[1] = edge[0] + share + (blockIdx.x < longer ? 1 : 0);
   while (true) {
+    const int cost = c.tiles + kItemCost;
+    const int64_t start = (before + upto - cost) * a.items;
 #pragma unroll 1
     for (int e = 0; e < 2; ++e) {
-      const int64_t from = edge[e] - (before + upto - c.tiles) * a.items;
-      if (from >= 0 && from < (int64_t)c.tiles * a.items) {
+      const int64_t from = edge[e] - start;
+      if (c.b < p.batch && from >= 0 && from < (int64_t)cost * a.items) {
         Cursor x = c;
-        x.item = (int)divide(from, c.tiles);
-        x.tile = (int)(from - (int64_t)x.item * c.tiles);
+        x.item = (int)divide(from, cost);
+        x.tile = (int)(from - (int64_t)x.item * cost) - kItemCost;
+        s_first[e] = edge[e] - x.tile;  // the item's first tile, in the count
+        // an edge in the item's cost, or inside a short item, moves to its start
+        if (x.tile < 0 || x.tiles <= kWhole) x.tile = 0;
         s_edge[e] = x;
       }
     }
@@ -441,38 +446,33 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
       block += s_scan[i];
     }
   }
-  // an edge inside a short item moves to the item's start
   Cursor cur = s_edge[0];
-  if (cur.tiles <= kWhole) {
-    edge[0] -= cur.tile;
-    cur.tile = 0;
-  }
-  if (edge[1] < total && s_edge[1].tiles <= kWhole) edge[1] -= s_edge[1].tile;
+  const int64_t end_b = s_edge[1].b;
+  const int end_item = end_b < p.batch ? s_edge[1].item : 0;
+  const int end_tile = end_b < p.batch ? s_edge[1].tile : 0;
+  if (cur.b == end_b && cur.item == end_item && cur.tile >= end_tile) return;
   const int brief = (int)(share / kWarps < kWhole ? share / kWarps : kWhole);
-  int64_t left = edge[1] - edge[0];
 
   // Walks the share item by item: true with `seg`, the tiles of the item that
   // lie in the share, and whether it is this warp's alone; false at the end.
   // Short items of other warps are passed over.
-  auto next_item = [&](Cursor& x, int64_t& todo, int& seg, bool& own, bool fresh) {
+  auto next_item = [&](Cursor& x, int& seg, bool& own, bool fresh) {
     while (true) {
       if (!fresh) {
-        todo -= seg;
-        if (todo <= 0) return false;
+        if (x.b == end_b && x.item == end_item) return false;
         x.tile = 0;
         if (++x.item == a.items) {
           x.item = 0;
-          ++x.b;
-          read_length<F::kKeys>(a, x);
+          if (++x.b < p.batch) read_length<F::kKeys>(a, x);
         }
       }
       fresh = false;
-      seg = (int)(todo < x.tiles - x.tile ? todo : x.tiles - x.tile);
+      seg = (x.b == end_b && x.item == end_item ? end_tile : x.tiles) - x.tile;
+      if (seg <= 0 || x.b >= p.batch) return false;
       own = x.tiles <= brief;
       if (!own || (uint32_t)(x.b * a.items + x.item) % kWarps == w) return true;
     }
   };
-  if (left <= 0) return;
 
   // ---- the copy side: q, then the tiles of this warp, kStages - 1 ahead of
   // the products
@@ -485,7 +485,6 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
   const uint8_t* k_lane = (const uint8_t*)p.kv.k + copy_row * k_step + copy_chunk * 16;
   const uint8_t* v_lane = (const uint8_t*)p.kv.v + copy_row * v_step + copy_chunk * 16;
   Cursor ahead = cur;
-  int64_t ahead_left = left;
   int ahead_seg = 0;
   bool ahead_own = false;
   // of the item that is being copied: this warp's tiles still to go, the key of
@@ -527,10 +526,10 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
       look_up();
     } else if (next == kTile) {
       next = kNothing;
-      if (next_item(ahead, ahead_left, ahead_seg, ahead_own, false)) begin_item();
+      if (next_item(ahead, ahead_seg, ahead_own, false)) begin_item();
     }
   };
-  if (next_item(ahead, ahead_left, ahead_seg, ahead_own, true)) begin_item();
+  if (next_item(ahead, ahead_seg, ahead_own, true)) begin_item();
   auto issue = [&](int stage) {
     const uint32_t base = ring + stage * F::kStageBytes;
     if (next == kTile) {
@@ -572,11 +571,12 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
             const int64_t o = __shfl_sync(0xffffffffu, off[kv], r);
             const uint32_t dst =
                 base + kv * (F::kKeys * F::kRowBytes) + chunk_pos<F::kRowBytes>(r, copy_chunk);
-            if (o == -2)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0x7fc07fc0u)
-                           : "memory");  // NaN in each of the three types
+            if (o < 0)  // (0x7fc07fc0 is NaN in each of the three types)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst),
+                           "r"(o == -2 ? 0x7fc07fc0u : 0u)
+                           : "memory");
             else
-              cp_async16(dst, o < 0 ? p.kv.k : from + o, o < 0 ? 0 : 16);
+              cp_async16(dst, from + o, 16);
           }
         }
       }
@@ -606,28 +606,29 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
     step_ahead();
   };
 
-  // while the first copies are on their way: the items that the share has a
+  // While the first copies are on their way: the items that the share has a
   // part of, the one it starts in (if that began before it or goes on after
-  // it) and the one it ends in
-  if (tid < 2) {
+  // it) and the one it ends in.
+  auto find_splits = [&]() {
+    if (tid >= 2) return;
     const Cursor& x = s_edge[tid];
-    const int64_t first = edge[tid] - x.tile;
-    Split s{};
-    bool part = tid == 0 || edge[1] < total;
+    bool part = tid == 0 || end_b < p.batch;
     if (part) part = x.tiles > kWhole;  // (short ones lie in one share)
-    if (part)
-      part = tid == 0 ? x.tile > 0 || first + x.tiles > edge[1] : x.tile > 0 && first > edge[0];
     if (part) {
-      s.first = (int)cta_of(first);
-      s.n = (int)cta_of(first + x.tiles - 1) - s.first + 1;
-      const int head0 = (x.item % a.blocks) * M;
-      s.row = x.b * p.q_heads + (int64_t)(x.item / a.blocks) * a.group + head0;
-      s.heads = a.group - head0 < M ? a.group - head0 : M;
+      const bool same = x.b == end_b && x.item == end_item;
+      part = tid == 0 ? x.tile > 0 || same
+                      : x.tile > 0 && !(x.b == s_edge[0].b && x.item == s_edge[0].item);
     }
+    if (!part) return;
+    Split s;
+    s.first = (int)cta_of(s_first[tid]);
+    s.n = (int)cta_of(s_first[tid] + x.tiles - 1) - s.first + 1;
+    const int head0 = (x.item % a.blocks) * M;
+    s.row = x.b * p.q_heads + (int64_t)(x.item / a.blocks) * a.group + head0;
+    s.heads = a.group - head0 < M ? a.group - head0 : M;
     s_split[tid] = s;
-  }
+  };
 
-  float* join = reinterpret_cast<float*>(smem + F::kRingBytes);
   // q, O, maxima and sums: of a lane's rows of the products, or (plain FMAs) of
   // keys g, g + 8, .. and the dims of chunks t + 4 i
   uint32_t q_regs[F::kLanes ? 1 : F::kSteps][F::kQOps][4];
@@ -641,8 +642,8 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
 
   int seg = 0;  // tiles of the item in this share
   bool own = false;
-  for (bool more = next_item(cur, left, seg, own, true); more;
-       more = next_item(cur, left, seg, own, false)) {
+  for (bool more = next_item(cur, seg, own, true); more;
+       more = next_item(cur, seg, own, false)) {
     const int kv_head = cur.item / a.blocks, head0 = (cur.item % a.blocks) * M;
     const int heads = a.group - head0 < M ? a.group - head0 : M;
     const int64_t row = cur.b * p.q_heads + (int64_t)kv_head * a.group + head0;
@@ -658,7 +659,7 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
       issue(stage);
       stage = stage + 1 == F::kStages ? 0 : stage + 1;
       if (filled < F::kStages - 1) {
-        ++filled;
+        if (++filled == F::kStages - 1) find_splits();
         continue;
       }
       const uint8_t* tile = ring_ptr + stage * F::kStageBytes;
@@ -989,13 +990,13 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
     // the head of row r of this lane, and whether the lane speaks for it
     auto head_of = [&](int r) { return F::kLanes ? r : r * 8 + g; };
     const bool speaks = F::kLanes ? lane == 0 : t == 0;
-    auto each = [&](int r, float f, int d_from, int d_to, auto&& put) {
+    auto each = [&](int r, float f, auto&& put) {
       if constexpr (F::kLanes) {
         // the chunk that the halvings left: the group's high bits; groups that
         // hold the same one leave it to the first
         constexpr int kSame = 8 / kChunks;
         const int d = (t + 4 * (g / kSame)) * 4;
-        if (g % kSame == 0 && d >= d_from && d < d_to) {
+        if (g % kSame == 0) {
           const float(&o)[4] = o_lane[r][0];
           put(d, make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f));
         }
@@ -1003,7 +1004,6 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
         // lane (g, t) holds dims of chunks 2 t and 2 t + 1 (+ 8 i) of head g
 #pragma unroll
         for (int i = 0; i < F::kVIter; ++i) {
-          if (i * 8 * F::kVVec < d_from || i * 8 * F::kVVec >= d_to) continue;
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
@@ -1026,73 +1026,57 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
         const int h = head_of(r);
         if (h >= heads) continue;
         const float f = l_run[r] == 0.0f ? 0.0f : 1.0f / l_run[r];
-        each(r, f, 0, D, [&](int d, float4 x) { store_act4(p.out, (row + h) * D + d, p.act_dtype, x); });
+        each(r, f, [&](int d, float4 x) { store_act4(p.out, (row + h) * D + d, p.act_dtype, x); });
         if (speaks && p.lse) p.lse[row + h] = (m_run[r] + log2f(l_run[r])) * kLn2;
       }
     } else {
       const bool whole = cur.tile == 0 && seg == cur.tiles;
       const bool tail = cur.tile != 0;
       float* slot = a.partials + (2 * (int64_t)blockIdx.x + (tail ? 0 : 1)) * partial_floats(M, D);
-      if (speaks)
-#pragma unroll
-        for (int r = 0; r < kMine; ++r) {
-          s_m[w][head_of(r)] = m_run[r];
-          s_l[w][head_of(r)] = l_run[r];
-        }
-      __syncthreads();
-      float factor[kMine];
+      // the warps' O meet in the stages that they worked on last (the next
+      // copies into those come after the joining)
+      float* area = reinterpret_cast<float*>(smem + (w * F::kStages + stage) * F::kStageBytes);
+      __syncwarp();
+      if (lane == 0) s_area[w] = (w * F::kStages + stage) * F::kStageBytes;
 #pragma unroll
       for (int r = 0; r < kMine; ++r) {
         const int h = head_of(r);
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_m[i][h]);
-        const float ref = finite(top);
-        factor[r] = exp2_fast(m_run[r] - ref);
-        if (speaks && w == 0) {
-          float sum = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kWarps; ++i) sum = fmaf(s_l[i][h], exp2_fast(s_m[i][h] - ref), sum);
-          s_top[h] = top;
-          s_sum[h] = sum;
+        if (speaks) {
+          s_m[w][h] = m_run[r];
+          s_l[w][h] = l_run[r];
         }
+        each(r, 1.0f, [&](int d, float4 x) { *reinterpret_cast<float4*>(area + h * D + d) = x; });
       }
-      // a pass: kRows heads, J dims
-      constexpr int J = F::kJoinDims, kR = F::kRows;
-#pragma unroll
-      for (int pass = 0; pass < M / kR * (D / J); ++pass) {
-        const int block = pass / (D / J), from = pass % (D / J) * J;
-#pragma unroll
-        for (int r = 0; r < kMine; ++r)
-          if (F::kLanes || r == block)
-            each(r, factor[r], from, from + J, [&](int d, float4 x) {
-              *reinterpret_cast<float4*>(join + (w * kR + head_of(r) - block * kR) * J + d - from) = x;
-            });
-        __syncthreads();
+      __syncthreads();
 #pragma unroll 1
-        for (int i = tid; i < kR * J / 4; i += kThreads) {
-          const int hj = i / (J / 4), dj = i % (J / 4) * 4, h = block * kR + hj, d = from + dj;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = tid; i < M * D / 4; i += kThreads) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float top = -INFINITY, sum = 0.0f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int k = 0; k < kWarps; ++k) {
-            const float4 y = *reinterpret_cast<const float4*>(join + (k * kR + hj) * J + dj);
-            x.x += y.x;
-            x.y += y.y;
-            x.z += y.z;
-            x.w += y.w;
-          }
-          if (!whole) {
-            *reinterpret_cast<float4*>(slot + h * D + d) = x;
-            if (d == 0) {
-              slot[M * D + h] = s_top[h];
-              slot[M * D + M + h] = s_sum[h];
-            }
-          } else if (h < heads) {
-            write_out(p, row + h, d, D, x, s_top[h], s_sum[h]);
-          }
+        for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s_m[k][h]);
+        const float ref = finite(top);
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+          const float4 y = *reinterpret_cast<const float4*>(smem + s_area[k] + i * 16);
+          const float f = exp2_fast(s_m[k][h] - ref);
+          x.x = fmaf(y.x, f, x.x);
+          x.y = fmaf(y.y, f, x.y);
+          x.z = fmaf(y.z, f, x.z);
+          x.w = fmaf(y.w, f, x.w);
+          sum = fmaf(s_l[k][h], f, sum);
         }
-        __syncthreads();
+        if (!whole) {
+          *reinterpret_cast<float4*>(slot + h * D + d) = x;
+          if (d == 0) {
+            slot[M * D + h] = top;
+            slot[M * D + M + h] = sum;
+          }
+        } else if (h < heads) {
+          write_out(p, row + h, d, D, x, top, sum);
+        }
       }
+      __syncthreads();
     }
   }
   cp_async_wait<0>();
@@ -1107,9 +1091,9 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
   int c0[2], n[2], at[2];  // partials on this level (0: no part in it), this CTA's
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    c0[e] = s_split[e].first;
     n[e] = s_split[e].n;
-    at[e] = (int)blockIdx.x - c0[e];
+    c0[e] = n[e] > 0 ? s_split[e].first : 0;
+    at[e] = n[e] > 0 ? (int)blockIdx.x - c0[e] : 0;
   }
   for (int level = 0, span = 1; n[0] + n[1] > 0; ++level, span *= kFan) {
     int members[2];
@@ -1147,7 +1131,7 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
       const int first = at[e] / kFan * kFan, of = n[e] - first < kFan ? n[e] - first : kFan;
       const bool top = n[e] <= kFan;
       if (s_last[e] && of > 1)
-        join_partials<M, D, kThreads>(a, c0[e], first * span, span, of, !top, s_split[e].row,
+        join_partials<M, D>(a, c0[e], first * span, span, of, !top, s_split[e].row,
                             s_split[e].heads);
       at[e] /= kFan;
       n[e] = top || !s_last[e] ? 0 : (n[e] + kFan - 1) / kFan;
@@ -1155,10 +1139,10 @@ __global__ void __launch_bounds__(Cfg<C, F32ACT, D, M, WIDE>::kThreads,
   }
 }
 
-template <class C, bool F32ACT, int D, int M, bool WIDE>
+template <class C, bool F32ACT, int D, int M>
 int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
-  using F = Cfg<C, F32ACT, D, M, WIDE>;
-  auto kernel = paged_attention_kernel<C, F32ACT, D, M, WIDE>;
+  using F = Cfg<C, F32ACT, D, M>;
+  auto kernel = paged_attention_kernel<C, F32ACT, D, M>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) !=
       cudaSuccess)
     return CT_ERR_CUDA;
@@ -1168,36 +1152,28 @@ int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   b.whole_tiles = a.p.kv.page_size % F::kRun == 0;
   // no more CTAs than the table can hold work for
   const int64_t keys = a.p.kv.max_pages * a.p.kv.page_size;
-  const int64_t tiles = a.p.batch * b.items * (keys > F::kKeys ? (keys + F::kKeys - 1) / F::kKeys : 1);
+  const int64_t tiles =
+      a.p.batch * b.items * (kItemCost + (keys > F::kKeys ? (keys + F::kKeys - 1) / F::kKeys : 1));
   int64_t ctas = (int64_t)dev.sm_count * F::kCtas;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   if (ctas > (tiles + kMinShare - 1) / kMinShare) ctas = (tiles + kMinShare - 1) / kMinShare;
-  kernel<<<(unsigned)ctas, F::kThreads, F::kSmem, st>>>(b);
+  kernel<<<(unsigned)ctas, kThreads, F::kSmem, st>>>(b);
   return check_launch();
 }
 
 constexpr size_t kCounterBytes = kLevels * kMaxCtas * sizeof(uint32_t);
-
-template <class C, bool F32ACT, int D, int M>
-int launch_width(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
-  // Fewer items than SMs: nearly all are split, and one large CTA an SM leaves
-  // a third of the partials to join.
-  if (a.p.batch * a.p.kv_heads * ((a.group + M - 1) / M) < dev.sm_count)
-    return launch<C, F32ACT, D, M, true>(a, dev, st);
-  return launch<C, F32ACT, D, M, false>(a, dev, st);
-}
 
 // Groups of more than 8 heads take 16 at a time where their q stays in
 // registers (64 at most), else 8: the cache is then read again, from L2.
 template <class C, bool F32ACT, int D>
 int launch_heads(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   if constexpr (sizeof(C) == 4) {
-    if (a.group == 1) return launch_width<C, F32ACT, D, 1>(a, dev, st);
-    if (a.group == 2) return launch_width<C, F32ACT, D, 2>(a, dev, st);
+    if (a.group == 1) return launch<C, F32ACT, D, 1>(a, dev, st);
+    if (a.group == 2) return launch<C, F32ACT, D, 2>(a, dev, st);
   }
   if constexpr (sizeof(C) == 4 ? D <= 64 : D * q_terms<C, F32ACT>() <= 256)
-    if (a.group > 8) return launch_width<C, F32ACT, D, 16>(a, dev, st);
-  return launch_width<C, F32ACT, D, 8>(a, dev, st);
+    if (a.group > 8) return launch<C, F32ACT, D, 16>(a, dev, st);
+  return launch<C, F32ACT, D, 8>(a, dev, st);
 }
 
 template <class C, bool F32ACT>

@@ -121,7 +121,8 @@ def test_attention_groups(cuda_device, ops, heads, kv):
     check_attention(q, k, v, table, lens, 16, got, 0.125)
 
 
-@pytest.mark.parametrize("lens", [[20000], [4096, 1], [1] * 300, [0] * 5, [9000, 0, 0, 33]])
+@pytest.mark.parametrize("lens", [[20000], [4096, 1], [1] * 300, [0] * 5, [9000, 0, 0, 33],
+                                  [(7 * i * i) % 400 for i in range(300)] + [2000]])
 @pytest.mark.parametrize("kv,group,cache", [(1, 8, F16), (3, 2, F32)])
 def test_attention_lengths(cuda_device, ops, lens, kv, group, cache):
     """Few long rows (the length is split over the GPU), many short ones, none."""
@@ -186,6 +187,18 @@ def test_attention_bad_lengths_and_pages(cuda_device, ops):
     for b in (1, 2, 3):
         assert out[b].isnan().all() and lse[b].isnan().all()
     check_attention(q[[0, 4]], k, v, table[[0, 4]], [40, 0], 16, (out[[0, 4]], lse[[0, 4]]), 0.125)
+
+
+def test_attention_without_pages(cuda_device, ops):
+    """An empty pool and an empty table: nothing can be read."""
+    k = torch.zeros(0, 2, 8, 64, device="cuda")
+    q = torch.ones(2, 4, 64, device="cuda")
+    lens = torch.tensor([0, 5], dtype=torch.int32, device="cuda")
+    for table in (torch.zeros(2, 4, dtype=torch.int32, device="cuda"),
+                  torch.zeros(2, 0, dtype=torch.int32, device="cuda")):
+        out, lse = ops.paged_attention(q, k, k.clone(), table, lens)
+        assert torch.count_nonzero(out[0]) == 0 and torch.isneginf(lse[0]).all()
+        assert out[1].isnan().all() and lse[1].isnan().all()
 
 
 def test_attention_workspace_is_reusable(cuda_device, ops):
