@@ -104,9 +104,9 @@ int ct_kv_append(const void* q, const int64_t q_stride[3], const void* k, const 
   p.rot_dim = (int)rot_dim;
   p.act_dtype = act_dtype;
   p.interleaved = interleaved != 0;
-  current_device(&rc);
+  const DeviceInfo* dev = current_device(&rc);
   if (rc != CT_OK) return rc;
-  return launch_kv_append(p, reinterpret_cast<cudaStream_t>(stream));
+  return launch_kv_append(p, *dev, reinterpret_cast<cudaStream_t>(stream));
 }
 
 size_t ct_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim) {

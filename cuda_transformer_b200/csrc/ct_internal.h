@@ -201,7 +201,7 @@ struct KvAppend {
   int head_dim, rot_dim, act_dtype;
   bool interleaved;
 };
-int launch_kv_append(const KvAppend& p, cudaStream_t st);
+int launch_kv_append(const KvAppend& p, const DeviceInfo& dev, cudaStream_t st);
 struct PagedAttention {
   const void* q;
   int64_t qs[3];  // sequence, head, dim
