@@ -196,9 +196,9 @@ int ct_logits_process(const void* logits, int64_t ld, int dtype, float* out, int
   p.mask_ld = mask_ld;
   p.dtype = dtype;
   int rc = CT_OK;
-  current_device(&rc);
+  const DeviceInfo* dev = current_device(&rc);
   if (rc != CT_OK) return rc;
-  return launch_logits_process(p, reinterpret_cast<cudaStream_t>(stream));
+  return launch_logits_process(p, *dev, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

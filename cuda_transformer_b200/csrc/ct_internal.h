@@ -231,7 +231,7 @@ struct LogitsProcess {
   int64_t mask_ld;
   int dtype;
 };
-int launch_logits_process(const LogitsProcess& p, cudaStream_t st);
+int launch_logits_process(const LogitsProcess& p, const DeviceInfo& dev, cudaStream_t st);
 
 // ------------------------------------------------------------ watchdog
 // One CTA whose waits on a barrier phase that nothing completes run out after

@@ -6,6 +6,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "ct_internal.h"
 
 namespace ct {
@@ -32,6 +35,17 @@ inline int with_dtype(int dtype, F&& f) {
     case CT_DTYPE_F16: return f(__half{});
     default: return CT_ERR_INVALID_ARGUMENT;
   }
+}
+
+// Raises a kernel's limit of dynamic shared memory, once a device.
+template <auto KERNEL>
+inline int allow_shared(int bytes, const DeviceInfo& dev) {
+  static std::atomic<bool> done[64];
+  if (dev.device < 64 && done[dev.device].load(std::memory_order_acquire)) return CT_OK;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return CT_ERR_CUDA;
+  if (dev.device < 64) done[dev.device].store(true, std::memory_order_release);
+  return CT_OK;
 }
 
 inline int dtype_bytes(int dtype) { return dtype == CT_DTYPE_F32 ? 4 : 2; }

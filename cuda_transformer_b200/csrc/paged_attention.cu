@@ -1142,10 +1142,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
 template <class C, bool F32ACT, int D, int M>
 int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   using F = Cfg<C, F32ACT, D, M>;
-  auto kernel = paged_attention_kernel<C, F32ACT, D, M>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) !=
-      cudaSuccess)
-    return CT_ERR_CUDA;
+  constexpr auto kernel = paged_attention_kernel<C, F32ACT, D, M>;
+  const int rc = allow_shared<kernel>(F::kSmem, dev);
+  if (rc != CT_OK) return rc;
   Launch b = a;
   b.blocks = (a.group + M - 1) / M;
   b.items = (int)(a.p.kv_heads * b.blocks);
@@ -1161,7 +1160,8 @@ int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   return check_launch();
 }
 
-constexpr size_t kCounterBytes = kLevels * kMaxCtas * sizeof(uint32_t);
+constexpr size_t kCounterBytes = CT_PAGED_ATTENTION_COUNTER_BYTES;
+static_assert(kLevels * kMaxCtas * sizeof(uint32_t) <= kCounterBytes, "");
 
 // Groups of more than 8 heads take 16 at a time where their q stays in
 // registers (64 at most), else 8: the cache is then read again, from L2.

@@ -16,6 +16,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -430,6 +431,12 @@ std::tuple<Tensor, Tensor, Tensor> layernorm_bwd(Tensor x, Tensor gamma, Tensor 
 }
 
 // ---------------------------------------------------------- token generation
+// A dense CUDA tensor beside `of`, allocated without a trip through the
+// dispatcher (which costs as much as a kernel's launch).
+Tensor empty_like_of(at::IntArrayRef sizes, at::ScalarType type, const Tensor& of) {
+  return at::detail::empty_cuda(sizes, type, of.device(), std::nullopt);
+}
+
 int dtype_code(const Tensor& t, const char* name) {
   switch (t.scalar_type()) {
     case at::kFloat: return CT_DTYPE_F32;
@@ -520,17 +527,17 @@ std::tuple<Tensor, Tensor> kv_append_(Tensor k_cache, Tensor v_cache, Tensor k0,
   const int32_t* seq = vector_of<int32_t>(seq_ids0, tokens, k, at::kInt, "seq_ids", &keep_seq);
   int64_t q_heads = 0, rot = 0, max_positions = 0;
   int64_t qs[3] = {0, 0, 1}, ks[3], vs[3], kcs[4], vcs[4];
-  Tensor q_out = at::empty({0}, k.options()), k_out = q_out;
+  Tensor q_out = empty_like_of({0}, k.scalar_type(), k), k_out = q_out;
   if (q0.has_value()) {
     check_on(*q0, k, k.scalar_type(), "q");
     TORCH_CHECK(q0->dim() == 3 && q0->size(0) == tokens && q0->size(2) == c.dim,
                 "q must be [tokens, nh, hs]");
     q = unit_last(*q0);
     q_heads = q.size(1);
-    q_out = at::empty({tokens, q_heads, c.dim}, k.options());
+    q_out = empty_like_of({tokens, q_heads, c.dim}, k.scalar_type(), k);
     strides3(q, qs);
   }
-  if (want_k) k_out = at::empty({tokens, c.heads, c.dim}, k.options());
+  if (want_k) k_out = empty_like_of({tokens, c.heads, c.dim}, k.scalar_type(), k);
   TORCH_CHECK(cos0.has_value() == sin0.has_value(), "cos and sin go together");
   if (cos0.has_value()) {
     check_on(*cos0, k, at::kFloat, "cos");
@@ -583,10 +590,12 @@ std::tuple<Tensor, Tensor> paged_attention(Tensor q, Tensor k_cache, Tensor v_ca
     TORCH_CHECK(ws.is_contiguous() && ws.numel() >= need, "workspace must be dense, of ", need,
                 " bytes or more");
   } else {
-    ws = at::zeros({need}, q.options().dtype(at::kByte));
+    // only the counters at its start have to be clear
+    ws = empty_like_of({need}, at::kByte, q);
+    ws.narrow(0, 0, CT_PAGED_ATTENTION_COUNTER_BYTES).zero_();
   }
-  Tensor out = at::empty({batch, heads, c.dim}, q.options());
-  Tensor lse = at::empty({batch, heads}, q.options().dtype(at::kFloat));
+  Tensor out = empty_like_of({batch, heads, c.dim}, q.scalar_type(), q);
+  Tensor lse = empty_like_of({batch, heads}, at::kFloat, q);
   int64_t qs[3], kcs[4], vcs[4];
   strides3(q, qs);
   strides4(k_cache, kcs);
@@ -635,7 +644,7 @@ Tensor logits_process(Tensor logits0, std::optional<Tensor> tokens0, std::option
     mask = matrix_of(*mask0, rows, logits, at::kInt, "mask");
     TORCH_CHECK(mask.size(1) >= (vocab + 31) / 32, "mask must have ceil(vocab / 32) words a row");
   }
-  Tensor out = at::empty({rows, vocab}, logits.options().dtype(at::kFloat));
+  Tensor out = empty_like_of({rows, vocab}, at::kFloat, logits);
   check_rc(ct_logits_process(logits.const_data_ptr(), rows > 1 ? logits.stride(0) : vocab, dtype,
                              out.data_ptr<float>(), vocab, rows, vocab,
                              tokens.defined() ? tokens.const_data_ptr<int64_t>() : nullptr,

@@ -390,11 +390,12 @@ size_t ct_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int6
  * beyond max_pages * page_size, or a page out of range, gives NaN.  Slots past
  * the length are not read.  The cache's base and strides must be multiples of
  * 16 bytes (CT_ERR_UNSUPPORTED_LAYOUT otherwise).
- * The workspace must be zero before its first use and every call leaves it
- * ready for the next, of whatever sizes (it needs no clearing in between); it
- * must be 16-byte aligned and not be used by another call that can run
- * concurrently.  Deterministic.  No reference counterpart
+ * The first CT_PAGED_ATTENTION_COUNTER_BYTES of the workspace must be zero
+ * before its first use; every call leaves them so, ready for the next call of
+ * whatever sizes.  The workspace must be 16-byte aligned and not be used by
+ * another call that can run concurrently.  Deterministic.  No reference counterpart
  * (the reference keeps no cache). */
+#define CT_PAGED_ATTENTION_COUNTER_BYTES 8192
 int ct_paged_attention(const void* q, const int64_t q_stride[3],
                        const void* k_cache, const int64_t kc_stride[4],
                        const void* v_cache, const int64_t vc_stride[4],

@@ -425,6 +425,7 @@ def random_mask(rows, vocab, g, extra=0):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("rows,vocab,hist,bias", [(1, 1, 3, 2), (3, 65, 40, 5), (2, 8191, 300, 0),
                                                   (5, 8193, 9000, 40), (2, 50257, 1, 300),
+                                                  (40, 20001, 1500, 20), (1, 2000, 2000, 3000),
                                                   (1, 100256, 500, 16), (4, 33000, 0, 1)])
 @pytest.mark.parametrize("masked", [False, True])
 def test_logits(cuda_device, ops, dtype, rows, vocab, hist, bias, masked):
@@ -506,6 +507,24 @@ def test_logits_strides_and_streams(cuda_device, ops):
     for r in range(rows):
         one = ops.logits_process(*(None if t is None else t[r:r + 1] for t in args))
         assert torch.equal(one[0], got[r])
+
+
+def test_logits_edges_of_rows(cuda_device, ops):
+    """Rows of every length around the vectors' and pieces', each starting at
+    another offset, logits and outputs aligned alike and not."""
+    g = gen(25)
+    pool = torch.randn(1 << 16, generator=g, device="cuda")
+    for vocab in (*range(1, 12), 1021, 1022, 1023, 1024, 1025, 1026, 2047, 2050, 4099):
+        for pad in range(4):
+            rows, ld = 5, vocab + pad
+            x = pool[pad:pad + rows * ld].view(rows, ld)[:, :vocab]
+            mask = random_mask(rows, vocab, g)
+            for dtype in (F32, BF16):
+                y = x if dtype is F32 else pool.to(dtype)[pad:pad + rows * ld].view(rows, ld)[:, :vocab]
+                tokens = torch.randint(0, vocab, (rows, 3), generator=g, device="cuda")
+                freq = torch.ones(rows, device="cuda")
+                got = ops.logits_process(y, tokens, frequency=freq, mask=mask)
+                check_logits(got, y, tokens, None, None, None, freq, None, None, None, mask)
 
 
 def test_logits_in_place_through_the_c_abi(cuda_device):
