@@ -120,3 +120,22 @@ def test_rotary_tables():
         angle = p * 10000.0 ** (-2 * i / 8)
         assert abs(cos[p, i].item() - math.cos(angle)) < 1e-7
         assert abs(sin[p, i].item() - math.sin(angle)) < 1e-7
+
+
+def test_page_pool():
+    from cuda_transformer_b200.generate_case import PagePool
+
+    pool = PagePool(6, 4, 2, 4, "cpu")
+    pool.reserve(0, 9)
+    pool.reserve(0, 5)   # fewer than it has: nothing changes
+    pool.reserve(1, 1)
+    assert [len(p) for p in pool.owned] == [3, 1] and len(pool.free) == 2
+    assert pool.table[0, :3].tolist() == pool.owned[0] and len(set(sum(pool.owned, []))) == 4
+    pool.reserve(0, 16)
+    with pytest.raises(RuntimeError):
+        pool.reserve(1, 16)
+    with pytest.raises(ValueError):
+        pool.reserve(1, 17)
+    pool.release(0)
+    pool.reserve(1, 16)
+    assert len(pool.free) == 2 and pool.table[1].tolist() == pool.owned[1]
