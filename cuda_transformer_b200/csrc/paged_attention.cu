@@ -26,8 +26,8 @@
 //    product is chosen so that every operand is a 16-byte shared-memory
 //    vector: no shuffles, no transposes.  tcgen05 would take 8 heads as 128
 //    rows; at 4 * group FLOPs a value the tensor pipe is not what bounds this
-//    kernel.  One or two heads on an FP32 cache are cheaper as plain FMAs (64
-//    a lane, head and 8 KB of cache, against 64 products and 128 splits).
+//    kernel.  One or two heads are cheaper as plain FMAs of FP32 (a lane
+//    has a key's dims, so only the score is added up across lanes).
 #include "decode_common.cuh"
 
 namespace ct {
@@ -60,8 +60,7 @@ constexpr int q_terms() {
 
 // C: the cache's type; F32ACT: q and out are FP32, else of type C; M: query
 // heads a CTA works on.  8: high and low parts share a product's rows; 16: the
-// heads fill them and the parts are products of their own; 1 and 2 (FP32
-// caches): plain FMAs.
+// heads fill them and the parts are products of their own; 1 and 2: plain FMAs.
 template <class C, bool F32ACT, int D, int M>
 struct Cfg {
   static constexpr bool kLanes = M <= 2;                    // no tensor cores
@@ -178,6 +177,18 @@ __device__ __forceinline__ uint32_t take_term(float& x, float& y) {
     y -= f.y;
   }
   return w;
+}
+
+// Element e of a 16-byte chunk.
+template <class C>
+__device__ __forceinline__ float chunk_value(const uint32_t (&w)[4], int e) {
+  if constexpr (sizeof(C) == 4)
+    return __uint_as_float(w[e]);
+  else if constexpr (std::is_same<C, __nv_bfloat16>::value)
+    return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+  else
+    return e & 1 ? __high2float(*reinterpret_cast<const __half2*>(&w[e / 2]))
+                 : __low2float(*reinterpret_cast<const __half2*>(&w[e / 2]));
 }
 
 // Position of 16-byte chunk `c` of tile row `r`.  Chunks are permuted within
@@ -630,11 +641,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
   };
 
   // q, O, maxima and sums: of a lane's rows of the products, or (plain FMAs) of
-  // keys g, g + 8, .. and the dims of chunks t + 4 i
+  // keys g, g + 8, .. and the dims of chunks t + 4 i, in parts of four
   uint32_t q_regs[F::kLanes ? 1 : F::kSteps][F::kQOps][4];
   float o_acc[F::kLanes ? 1 : F::kOTiles][4];
   constexpr int kChunks = F::kLanes ? D / 16 : 1, kHeads = F::kLanes ? M : 1;
   alignas(16) float q_lane[kHeads][kChunks][4], o_lane[kHeads][kChunks][4];
+  auto lane_dim = [&](int part) {  // the first of part's four dims
+    constexpr int kParts = F::kVec / 4;
+    return (t + 4 * (part / kParts)) * F::kVec + part % kParts * 4;
+  };
   constexpr int kMine = F::kLanes ? M : R;
   float m_run[kMine], l_run[kMine], s_mul[kMine];
   int stage = 0;  // the next to fill
@@ -684,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
           l_run[r] = 0.0f;
           q_mul[r] = 1.0f;
           s_mul[r] = p.scale * kLog2e;
-          if constexpr (!F::kF32 && !F::kBf16 && F32ACT) {
+          if constexpr (!F::kLanes && !F::kF32 && !F::kBf16 && F32ACT) {
             float top = 0.0f;
 #pragma unroll 4
             for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(q_at(r, d)));
@@ -704,10 +719,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
           for (int h = 0; h < M; ++h)
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
-              *reinterpret_cast<float4*>(q_lane[h][i]) = *reinterpret_cast<const float4*>(
-                  tile + q_pos<F::kQRowChunks>(h, t + 4 * i));
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o_lane[h][i][e] = 0.0f;
+              for (int e = 0; e < 4; ++e) {
+                const int d = lane_dim(i) + e;
+                q_lane[h][i][e] = to_f32(*reinterpret_cast<const A*>(
+                    tile + q_pos<F::kQRowChunks>(h, d * (int)sizeof(A) / 16) +
+                    d * (int)sizeof(A) % 16));
+                o_lane[h][i][e] = 0.0f;
+              }
             }
         } else {
 #pragma unroll
@@ -757,53 +776,80 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
       if (first_key >= end_key) continue;
 
       if constexpr (F::kLanes) {
-        // ---- key n * 8 + g of the tile, the dims of chunks t + 4 i
+        // ---- keys n * 8 + g of the tile, the dims of chunks t + 4 i
+        constexpr int kSums = F::kNt == 1 ? 4 : 2;  // chains of a score
+        float s[F::kNt][M][kSums];
 #pragma unroll
-        for (int n = 0; n < F::kNt; ++n) {
-          float s[M];
+        for (int n = 0; n < F::kNt; ++n)
 #pragma unroll
-          for (int h = 0; h < M; ++h) s[h] = 0.0f;
+          for (int h = 0; h < M; ++h)
 #pragma unroll
-          for (int i = 0; i < kChunks; ++i) {
-            alignas(16) float x[4];
-            *reinterpret_cast<float4*>(x) =
-                *reinterpret_cast<const float4*>(tile + chunk_pos<F::kRowBytes>(n * 8 + g, t + 4 * i));
+            for (int e = 0; e < kSums; ++e) s[n][h][e] = 0.0f;
 #pragma unroll
-            for (int h = 0; h < M; ++h)
+        for (int i = 0; i < F::kKIter; ++i)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[h] = fmaf(q_lane[h][i][e], x[e], s[h]);
-          }
-          float pr[M];
+          for (int n = 0; n < F::kNt; ++n) {
+            alignas(16) uint32_t kw[4];
+            *reinterpret_cast<uint4*>(kw) =
+                *reinterpret_cast<const uint4*>(tile + chunk_pos<F::kRowBytes>(n * 8 + g, t + 4 * i));
 #pragma unroll
-          for (int h = 0; h < M; ++h) {
-            s[h] += __shfl_xor_sync(0xffffffffu, s[h], 1);
-            s[h] += __shfl_xor_sync(0xffffffffu, s[h], 2);
-            s[h] *= s_mul[h];
-            if (first_key + n * 8 + g >= end_key) s[h] = -INFINITY;
-            // each lane has a maximum of its own keys
-            if (__any_sync(0xffffffffu, s[h] > m_run[h] + kMaxSlack)) {
-              const float top = fmaxf(s[h], m_run[h]), f = exp2_fast(m_run[h] - finite(top));
-              m_run[h] = top;
-              l_run[h] *= f;
+            for (int e = 0; e < F::kVec; ++e) {
+              const float x = chunk_value<C>(kw, e);
 #pragma unroll
-              for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o_lane[h][i][e] *= f;
+              for (int h = 0; h < M; ++h)
+                s[n][h][e % kSums] =
+                    fmaf(q_lane[h][i * (F::kVec / 4) + e / 4][e % 4], x, s[n][h][e % kSums]);
             }
-            pr[h] = exp2_fast(s[h] - finite(m_run[h]));
-            l_run[h] += pr[h];
+          }
+        float pr[F::kNt][M];
+#pragma unroll
+        for (int h = 0; h < M; ++h) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < F::kNt; ++n) {
+            float& x = pr[n][h];
+            x = s[n][h][0] + s[n][h][1];
+            if constexpr (kSums == 4) x += s[n][h][2] + s[n][h][3];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            x *= s_mul[h];
+            if (first_key + n * 8 + g >= end_key) x = -INFINITY;
+            top = fmaxf(top, x);
+          }
+          // each lane has a maximum of its own keys
+          if (__any_sync(0xffffffffu, top > m_run[h] + kMaxSlack)) {
+            top = fmaxf(top, m_run[h]);
+            const float f = exp2_fast(m_run[h] - finite(top));
+            m_run[h] = top;
+            l_run[h] *= f;
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o_lane[h][i][e] *= f;
           }
 #pragma unroll
-          for (int i = 0; i < kChunks; ++i) {
-            alignas(16) float x[4];
-            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(
-                tile + F::kKeys * F::kRowBytes + chunk_pos<F::kRowBytes>(n * 8 + g, t + 4 * i));
-#pragma unroll
-            for (int h = 0; h < M; ++h)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o_lane[h][i][e] = fmaf(pr[h], x[e], o_lane[h][i][e]);
+          for (int n = 0; n < F::kNt; ++n) {
+            pr[n][h] = exp2_fast(pr[n][h] - finite(m_run[h]));
+            l_run[h] += pr[n][h];
           }
         }
+#pragma unroll
+        for (int i = 0; i < F::kKIter; ++i)
+#pragma unroll
+          for (int n = 0; n < F::kNt; ++n) {
+            alignas(16) uint32_t vw[4];
+            *reinterpret_cast<uint4*>(vw) = *reinterpret_cast<const uint4*>(
+                tile + F::kKeys * F::kRowBytes + chunk_pos<F::kRowBytes>(n * 8 + g, t + 4 * i));
+#pragma unroll
+            for (int e = 0; e < F::kVec; ++e) {
+              const float x = chunk_value<C>(vw, e);
+#pragma unroll
+              for (int h = 0; h < M; ++h) {
+                float& o = o_lane[h][i * (F::kVec / 4) + e / 4][e % 4];
+                o = fmaf(pr[n][h], x, o);
+              }
+            }
+          }
         continue;
       } else {
       // ---- S = q k^T, in two chains for each 8 keys
@@ -995,7 +1041,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
         // the chunk that the halvings left: the group's high bits; groups that
         // hold the same one leave it to the first
         constexpr int kSame = 8 / kChunks;
-        const int d = (t + 4 * (g / kSame)) * 4;
+        const int d = lane_dim(g / kSame);
         if (g % kSame == 0) {
           const float(&o)[4] = o_lane[r][0];
           put(d, make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f));
@@ -1156,6 +1202,9 @@ int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   int64_t ctas = (int64_t)dev.sm_count * F::kCtas;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   if (ctas > (tiles + kMinShare - 1) / kMinShare) ctas = (tiles + kMinShare - 1) / kMinShare;
+  // One sequence: as many whole CTAs to each item, so that none works on two
+  // (the one that does ends some 3 us after the others).
+  if (a.p.batch == 1 && b.items <= ctas / 8) ctas -= ctas % b.items;
   kernel<<<(unsigned)ctas, kThreads, F::kSmem, st>>>(b);
   return check_launch();
 }
@@ -1167,10 +1216,9 @@ static_assert(kLevels * kMaxCtas * sizeof(uint32_t) <= kCounterBytes, "");
 // registers (64 at most), else 8: the cache is then read again, from L2.
 template <class C, bool F32ACT, int D>
 int launch_heads(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
-  if constexpr (sizeof(C) == 4) {
-    if (a.group == 1) return launch<C, F32ACT, D, 1>(a, dev, st);
+  if (a.group == 1) return launch<C, F32ACT, D, 1>(a, dev, st);
+  if constexpr (sizeof(C) == 4 || (q_terms<C, F32ACT>() == 3 && D <= 64))
     if (a.group == 2) return launch<C, F32ACT, D, 2>(a, dev, st);
-  }
   if constexpr (sizeof(C) == 4 ? D <= 64 : D * q_terms<C, F32ACT>() <= 256)
     if (a.group > 8) return launch<C, F32ACT, D, 16>(a, dev, st);
   return launch<C, F32ACT, D, 8>(a, dev, st);
