@@ -111,7 +111,7 @@ int ct_kv_append(const void* q, const int64_t q_stride[3], const void* k, const 
 
 size_t ct_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
   if (!in_range(q_heads, 0) || !in_range(kv_heads, 1) || !in_range(head_dim, 1)) return 0;
-  return paged_attention_workspace(q_heads, kv_heads, head_dim);
+  return paged_attention_workspace(head_dim);
 }
 
 int ct_paged_attention(const void* q, const int64_t q_stride[3], const void* k_cache,
@@ -135,7 +135,7 @@ int ct_paged_attention(const void* q, const int64_t q_stride[3], const void* k_c
   bool ok = aligned16(k_cache) && aligned16(v_cache);
   for (int i = 0; i < 3; ++i) ok = ok && kc_stride[i] % align == 0 && vc_stride[i] % align == 0;
   if (!ok) return CT_ERR_UNSUPPORTED_LAYOUT;
-  if (workspace_bytes < paged_attention_workspace(q_heads, kv_heads, head_dim) ||
+  if (workspace_bytes < paged_attention_workspace(head_dim) ||
       (workspace_bytes > 0 && !workspace))
     return CT_ERR_WORKSPACE_TOO_SMALL;
   if (!aligned16(workspace)) return CT_ERR_INVALID_ARGUMENT;

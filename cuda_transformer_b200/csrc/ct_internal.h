@@ -214,7 +214,7 @@ struct PagedAttention {
   float scale;
   void* ws;
 };
-size_t paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+size_t paged_attention_workspace(int64_t head_dim);
 int launch_paged_attention(const PagedAttention& p, const DeviceInfo& dev, cudaStream_t st);
 struct LogitsProcess {
   const void* logits;

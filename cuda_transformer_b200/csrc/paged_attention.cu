@@ -20,9 +20,9 @@
 //    across items; a block barrier comes only where a long item ends.
 //  * Products run on mma.sync with FP32 accuracy: 16-bit cache values go in as
 //    they are, q and the probabilities as two or three 16-bit terms; FP32
-//    caches take three TF32 products.  Up to 8 heads put two terms into the 16
-//    rows of one product (high and low sums of a head then sit in the same
-//    lane), 16 heads fill the rows.  The order of keys and dims inside a
+//    caches take three TF32 products.  8 heads put two terms into the 16 rows of
+//    one product (high and low sums of a head then sit in the same lane).  The
+//    order of keys and dims inside a
 //    product is chosen so that every operand is a 16-byte shared-memory
 //    vector: no shuffles, no transposes.  tcgen05 would take 8 heads as 128
 //    rows; at 4 * group FLOPs a value the tensor pipe is not what bounds this
@@ -59,12 +59,11 @@ constexpr int q_terms() {
 }
 
 // C: the cache's type; F32ACT: q and out are FP32, else of type C; M: query
-// heads a CTA works on.  8: high and low parts share a product's rows; 16: the
-// heads fill them and the parts are products of their own; 1 and 2: plain FMAs.
+// heads a CTA works on.  8: on the tensor cores, high and low parts share a
+// product's rows; 1 and 2: plain FMAs.
 template <class C, bool F32ACT, int D, int M>
 struct Cfg {
   static constexpr bool kLanes = M <= 2;                    // no tensor cores
-  static constexpr int R = M == 16 ? 2 : 1;                 // heads of a lane's rows
   using A = std::conditional_t<F32ACT, float, C>;           // type of q and out
   static constexpr bool kF32 = sizeof(C) == 4;
   static constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
@@ -85,10 +84,9 @@ struct Cfg {
   // two): f16 probabilities reach up to 2^14 instead of 1, so that the many
   // small ones of a long sequence stay clear of the subnormals.
   static constexpr float kBelow = !kF32 && !kBf16 ? 8.0f : 0.0f;
-  // A operands of one step (8 dims in TF32, 16 in the 16-bit types).  R = 1:
-  // rows 0-7 and 8-15 hold two terms; R = 2: one term of 16 heads.
-  static constexpr int kQOps = R == 1 ? (kQTerms + 1) / 2 : kQTerms;
-  static constexpr int kPOps = R == 1 ? (kPTerms + 1) / 2 : kPTerms;
+  // A operands of one step (8 dims in TF32, 16 in the 16-bit types): rows 0-7
+  // and 8-15 hold two terms.
+  static constexpr int kQOps = (kQTerms + 1) / 2, kPOps = (kPTerms + 1) / 2;
   static constexpr int kSteps = kF32 ? D / 8 : D / 16;
   static constexpr int kQRegs = kLanes ? M * D / 4 : kSteps * kQOps * 4;
   // Keys of a warp's tile: 8 KB of K and V, 32 at most; a smaller one (8 keys in
@@ -363,7 +361,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     paged_attention_kernel(const __grid_constant__ Launch a) {
   using F = Cfg<C, F32ACT, D, M>;
   using A = typename F::A;
-  constexpr int R = F::R;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t s_scan[kWarps];
   __shared__ int64_t s_rest[kWarps];
@@ -650,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     constexpr int kParts = F::kVec / 4;
     return (t + 4 * (part / kParts)) * F::kVec + part % kParts * 4;
   };
-  constexpr int kMine = F::kLanes ? M : R;
+  constexpr int kMine = F::kLanes ? M : 1;  // heads of a lane
   float m_run[kMine], l_run[kMine], s_mul[kMine];
   int stage = 0;  // the next to fill
   int filled = 0;
@@ -681,11 +678,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
       if (u < 0) {
         // ---- the item's start: q in the order of the products' A operands,
         // the dims that lane t of step s multiplies; rows g and g + 8 are two
-        // terms (R = 1) or two heads
+        // terms
         u = 0;
-        auto q_at = [&](int r, int d) {
+        auto q_at = [&](int d) {
           return to_f32(*reinterpret_cast<const A*>(
-              tile + q_pos<F::kQRowChunks>(r * 8 + g, d * (int)sizeof(A) / 16) +
+              tile + q_pos<F::kQRowChunks>(g, d * (int)sizeof(A) / 16) +
               d * (int)sizeof(A) % 16));
         };
         // FP32 q in f16 terms is scaled by a power of two that brings the
@@ -702,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
           if constexpr (!F::kLanes && !F::kF32 && !F::kBf16 && F32ACT) {
             float top = 0.0f;
 #pragma unroll 4
-            for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(q_at(r, d)));
+            for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(q_at(d)));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             if (top > 0.0f && top < INFINITY) {
@@ -733,32 +730,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
           for (int s = 0; s < F::kSteps; ++s) {
             constexpr int kPart = F::kF32 ? 2 : 4;  // dims of a lane in a step
             const int d = (t + 4 * (s / (F::kVec / kPart))) * F::kVec + s % (F::kVec / kPart) * kPart;
+            if constexpr (F::kF32) {
+              split_tf32(q_at(d), q_regs[s][0][0], q_regs[s][0][1]);
+              split_tf32(q_at(d + 1), q_regs[s][0][2], q_regs[s][0][3]);
+            } else {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-              if constexpr (F::kF32) {
-                uint32_t term[2][2];
-                split_tf32(q_at(r, d), term[0][0], term[1][0]);
-                split_tf32(q_at(r, d + 1), term[0][1], term[1][1]);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  q_regs[s][R == 1 ? 0 : k][R == 1 ? k : r] = term[k][0];
-                  q_regs[s][R == 1 ? 0 : k][(R == 1 ? k : r) + 2] = term[k][1];
-                }
-              } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  if constexpr (!F32ACT) {  // exact as it is
-                  q_regs[s][0][r + 2 * h] = *reinterpret_cast<const uint32_t*>(
-                      tile + q_pos<F::kQRowChunks>(r * 8 + g, (d + 2 * h) * 2 / 16) +
-                      (d + 2 * h) * 2 % 16);
-                  if (R == 1) q_regs[s][0][1 + 2 * h] = 0u;
-                  continue;
-                }
-                float x = q_at(r, d + 2 * h) * q_mul[r], y = q_at(r, d + 2 * h + 1) * q_mul[r];
+              for (int h = 0; h < 2; ++h) {
+                if constexpr (!F32ACT) {  // exact as it is
+                  q_regs[s][0][2 * h] = *reinterpret_cast<const uint32_t*>(
+                      tile + q_pos<F::kQRowChunks>(g, (d + 2 * h) * 2 / 16) + (d + 2 * h) * 2 % 16);
+                  q_regs[s][0][1 + 2 * h] = 0u;
+                } else {
+                  float x = q_at(d + 2 * h) * q_mul[0], y = q_at(d + 2 * h + 1) * q_mul[0];
 #pragma unroll
                   for (int k = 0; k < F::kQTerms; ++k)
-                    q_regs[s][R == 1 ? k / 2 : k][(R == 1 ? k % 2 : r) + 2 * h] = take_term<C>(x, y);
-                  if (R == 1 && F::kQTerms % 2) q_regs[s][F::kQTerms / 2][1 + 2 * h] = 0u;
+                    q_regs[s][k / 2][k % 2 + 2 * h] = take_term<C>(x, y);
+                  if (F::kQTerms % 2) q_regs[s][F::kQTerms / 2][1 + 2 * h] = 0u;
                 }
               }
             }
@@ -874,7 +861,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
               const uint32_t x = kw[n][2 * e], y = kw[n][2 * e + 1];
               mma<C>(s_acc[n][0], q_regs[s][0], x, y);
               mma<C>(s_acc[n][1], q_regs[s][0], low_tf32(x), low_tf32(y));
-              if constexpr (R == 2) mma<C>(s_acc[n][1], q_regs[s][1], x, y);
             } else {
 #pragma unroll
               for (int k = 0; k < F::kQOps; ++k)
@@ -884,55 +870,45 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
         }
       }
 
-      // ---- probabilities of keys n * 8 + 2 t and + 1; heads g (and g + 8)
+      // ---- probabilities of keys n * 8 + 2 t and + 1; head g
       constexpr int kKSteps = F::kF32 ? F::kNt : F::kNt / 2;  // products over the tile's keys
       uint32_t pa[kKSteps][F::kPOps][4];
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
+      {
         float v[F::kNt][2], top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < F::kNt; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float(&x)[2][4] = s_acc[n];
-            v[n][e] = R == 1 ? (x[0][e] + x[1][e]) + (x[0][e + 2] + x[1][e + 2])
-                             : x[0][2 * r + e] + x[1][2 * r + e];
-            v[n][e] *= s_mul[r];
+            v[n][e] = ((x[0][e] + x[1][e]) + (x[0][e + 2] + x[1][e + 2])) * s_mul[0];
             if (first_key + n * 8 + 2 * t + e >= end_key) v[n][e] = -INFINITY;
             top = fmaxf(top, v[n][e]);
           }
-        if (__any_sync(0xffffffffu, top > m_run[r] + (F::kBelow + kMaxSlack))) {
+        if (__any_sync(0xffffffffu, top > m_run[0] + (F::kBelow + kMaxSlack))) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          top = fmaxf(top - F::kBelow, m_run[r]);
-          const float f = exp2_fast(m_run[r] - finite(top));
-          m_run[r] = top;
-          l_run[r] *= f;
+          top = fmaxf(top - F::kBelow, m_run[0]);
+          const float f = exp2_fast(m_run[0] - finite(top));
+          m_run[0] = top;
+          l_run[0] *= f;
 #pragma unroll
           for (int j = 0; j < F::kOTiles; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (R == 1 || e / 2 == r) o_acc[j][e] *= f;
+            for (int e = 0; e < 4; ++e) o_acc[j][e] *= f;
         }
-        const float m = finite(m_run[r]);
+        const float m = finite(m_run[0]);
 #pragma unroll
         for (int n = 0; n < F::kNt; ++n) {
           float x = exp2_fast(v[n][0] - m), y = exp2_fast(v[n][1] - m);
-          l_run[r] += x + y;
+          l_run[0] += x + y;
           if constexpr (F::kF32) {
-            uint32_t term[2][2];
-            split_tf32(x, term[0][0], term[1][0]);
-            split_tf32(y, term[0][1], term[1][1]);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              pa[n][R == 1 ? 0 : k][R == 1 ? k : r] = term[k][0];
-              pa[n][R == 1 ? 0 : k][(R == 1 ? k : r) + 2] = term[k][1];
-            }
+            split_tf32(x, pa[n][0][0], pa[n][0][1]);
+            split_tf32(y, pa[n][0][2], pa[n][0][3]);
           } else {
 #pragma unroll
             for (int k = 0; k < F::kPTerms; ++k)
-              pa[n / 2][R == 1 ? k / 2 : k][(R == 1 ? k % 2 : r) + 2 * (n % 2)] = take_term<C>(x, y);
-            if (R == 1 && F::kPTerms % 2) pa[n / 2][F::kPTerms / 2][1 + 2 * (n % 2)] = 0u;
+              pa[n / 2][k / 2][k % 2 + 2 * (n % 2)] = take_term<C>(x, y);
+            if (F::kPTerms % 2) pa[n / 2][F::kPTerms / 2][1 + 2 * (n % 2)] = 0u;
           }
         }
       }
@@ -948,7 +924,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
         for (int e = 0; e < F::kVVec; ++e)
 #pragma unroll
           for (int x = 0; x < 4; ++x)  // (the low part's sum may be cut off)
-            c[e][x] = !F32ACT || (R == 1 && x >= 2) ? o_acc[i * F::kVVec + e][x] : 0.0f;
+            c[e][x] = !F32ACT || x >= 2 ? o_acc[i * F::kVVec + e][x] : 0.0f;
 #pragma unroll
         for (int ks = 0; ks < kKSteps; ++ks) {
           constexpr int kV = F::kF32 ? 2 : 4;  // of the lane's keys in a product
@@ -968,7 +944,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
             if constexpr (F::kF32) {
               const uint32_t x = vw[0][e], y = vw[1][e];
               mma<C>(c[e], pa[ks][0], low_tf32(x), low_tf32(y));
-              if constexpr (R == 2) mma<C>(c[e], pa[ks][1], x, y);
               mma<C>(c[e], pa[ks][0], x, y);
             } else {
               // element e of keys 2 t and 2 t + 1 (and 8 further) in one word
@@ -985,7 +960,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             float& o = o_acc[i * F::kVVec + e][x];
-            o = F32ACT && (R == 2 || x < 2) ? o + c[e][x] : c[e][x];
+            o = F32ACT && x < 2 ? o + c[e][x] : c[e][x];
           }
       }
       }
@@ -1025,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
       }
     } else {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int r = 0; r < kMine; ++r) {
         l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
         l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
       }
@@ -1033,8 +1008,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     if (cur.bad)
 #pragma unroll
       for (int r = 0; r < kMine; ++r) l_run[r] = NAN;
-    // the head of row r of this lane, and whether the lane speaks for it
-    auto head_of = [&](int r) { return F::kLanes ? r : r * 8 + g; };
+    // this lane's head r, and whether the lane speaks for it
+    auto head_of = [&](int r) { return F::kLanes ? r : g; };
     const bool speaks = F::kLanes ? lane == 0 : t == 0;
     auto each = [&](int r, float f, auto&& put) {
       if constexpr (F::kLanes) {
@@ -1059,7 +1034,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const float(&o)[4] = o_acc[i * F::kVVec + e + k];
-                xs[k] = (R == 1 ? o[cc] + o[cc + 2] : o[2 * r + cc]) * f;
+                xs[k] = (o[cc] + o[cc + 2]) * f;
               }
               put((2 * t + cc + 8 * i) * F::kVVec + e, x);
             }
@@ -1212,15 +1187,16 @@ int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
 constexpr size_t kCounterBytes = CT_PAGED_ATTENTION_COUNTER_BYTES;
 static_assert(kLevels * kMaxCtas * sizeof(uint32_t) <= kCounterBytes, "");
 
-// Groups of more than 8 heads take 16 at a time where their q stays in
-// registers (64 at most), else 8: the cache is then read again, from L2.
+// Groups of more than 8 heads are blocks of 8, for each of which the cache is
+// read again, mostly from L2.  (16 heads at a time, a product's rows filled by
+// one term, spilled registers and was slower but for the most ragged batch:
+// 16 heads on one, 32 x 4096 tokens, in bf16 of 128 46.2 us against 28.6, in
+// FP32 of 64 45.2 against 36.9; f16 of 64, 128 x 1 .. 16384 27.5 against 28.7.)
 template <class C, bool F32ACT, int D>
 int launch_heads(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   if (a.group == 1) return launch<C, F32ACT, D, 1>(a, dev, st);
   if constexpr (sizeof(C) == 4 || (q_terms<C, F32ACT>() == 3 && D <= 64))
     if (a.group == 2) return launch<C, F32ACT, D, 2>(a, dev, st);
-  if constexpr (sizeof(C) == 4 ? D <= 64 : D * q_terms<C, F32ACT>() <= 256)
-    if (a.group > 8) return launch<C, F32ACT, D, 16>(a, dev, st);
   return launch<C, F32ACT, D, 8>(a, dev, st);
 }
 
@@ -1233,9 +1209,8 @@ int launch_dims(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
 
 }  // namespace
 
-size_t paged_attention_workspace(int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
-  return kCounterBytes + 2 * kMaxCtas * sizeof(float) *
-                             partial_floats(q_heads / kv_heads > 8 ? 16 : 8, (int)head_dim);
+size_t paged_attention_workspace(int64_t head_dim) {
+  return kCounterBytes + 2 * kMaxCtas * sizeof(float) * partial_floats(8, (int)head_dim);
 }
 
 int launch_paged_attention(const PagedAttention& p, const DeviceInfo& dev, cudaStream_t st) {
