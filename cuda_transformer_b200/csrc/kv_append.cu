@@ -15,6 +15,16 @@
 // position -> table -> page that the stores need.  A thread holds the two
 // vectors whose elements pair up; its part of a head is the same for every
 // head that it handles, so angles, page and slot are fetched once a thread.
+//
+// Device time on a B200 (floor: bytes at the 6.53 TB/s of a copy):
+//   12 prompts of 300 to 4096 tokens, 32 on 32 heads of 64, FP32 into a bf16
+//   cache                                      115.9 us  floor 114.6 (99 %)
+//   32 on 8 of 128 in bf16, turned / not       80 / 71.5 us   69.0 / 68.7
+//   7 prompts of 100 to 2000, 8 on 8 of 128, FP32, half of a head turned
+//                                               24.4 us  18.6 (76 %)
+//   one token each of 64 sequences, bf16         2.4 us  0.25 (the launch)
+// In bf16 with angles a thread's chain (angles, page, then the stores) is what
+// is left: its bytes are half and its latencies the same.
 #include "decode_common.cuh"
 
 namespace ct {
@@ -198,7 +208,8 @@ __global__ void __launch_bounds__(kThreads, 6)
   }
 }
 
-// 16-byte vectors of the activations: halves of the rotated part and of the
+// 16-byte vectors of the activations (FP32 into bf16: 115.9 us, in single
+// elements 247; bf16: 80 and 312): halves of the rotated part and of the
 // rest in whole vectors, all rows aligned to their vectors.  Otherwise single
 // elements.
 bool vectors_fit(const KvAppend& p) {
@@ -223,7 +234,8 @@ int launch(const KvAppend& p, const DeviceInfo& dev, cudaStream_t st) {
   while ((VEC << (unit_shift + 1)) < p.head_dim) ++unit_shift;
   const int64_t parts = (p.q_heads + 2 * p.kv_heads) << unit_shift;
   // Several parts a thread (fewer fetches of angles and pages) once there is
-  // work for every SM several times over; one for the shortest way through a
+  // work for every SM several times over (12 prompts, FP32 into bf16: 115.9 us,
+  // one part a thread 135.9; in bf16 80 and 92; the 7 FP32 prompts 24.4 and 23.0); one for the shortest way through a
   // decoding step.
   const int64_t rows = (parts + kThreads - 1) / kThreads;
   int items = 1;

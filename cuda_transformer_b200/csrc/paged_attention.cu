@@ -28,6 +28,20 @@
 //    rows; at 4 * group FLOPs a value the tensor pipe is not what bounds this
 //    kernel.  One or two heads are cheaper as plain FMAs of FP32 (a lane
 //    has a key's dims, so only the score is added up across lanes).
+//
+// Device time of a launch on a B200 (floor: the cached values at the 6.53 TB/s
+// of a copy); 32 heads on 8 of 128, bf16, unless it says otherwise:
+//   64 sequences of 4096 tokens            170 - 174 us   floor 164
+//   one of 131072                          92.5           82.2
+//   32 on 32 of 64, FP32 q, 16 x 3500..4096 81.9          76.0
+//   64 of 16 .. 4096                       46.9           30.4
+//   FP32, 8 on 8 of 128, 5 x 777..4097     26.4           13.2
+//   f16, 16 on 1 of 64, 128 x 1..16384     28.5           8.7
+//   one of 8192 / 1024 / 64                24 / 13.4 / 6.4  5.1 / 0.6 / 0.04
+// Long batches run at the copy's rate.  The rest is a fixed chain of latencies:
+// 2 us to start, 2 us for the lengths and the table, 2 to 3 us until the first
+// tile is worked on, 1 us at the end of an item and about 3 us (write, fence,
+// counter, read) for each level of joining, two of them from 9 parts on.
 #include "decode_common.cuh"
 
 namespace ct {
@@ -36,15 +50,24 @@ namespace {
 constexpr int kMaxCtas = 448;  // counters (of each level) and partial slots in the workspace
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kFan = 8;        // partials that are joined at a time
+// Partials that are joined at a time.  (32: 8192 tokens 32 us instead of 24,
+// 131072 105 instead of 96; 16, where a thread holds them: FP32, 8 on 8 of 128,
+// 5 x 777..4097 27.1 instead of 26.1.)
+constexpr int kFan = 8;
 constexpr int kLevels = 3;     // kFan^kLevels >= kMaxCtas
 // Items of at most so many tiles are never split between CTAs: joining the
-// parts costs more than the tiles.  Those of no more tiles than a warp's part
-// of its CTA's share are one warp's.
+// parts costs more than the tiles (64 sequences of 16 to 4096 tokens took 58 us
+// with 16, 70 with 8, when this was chosen).  Those of no more tiles than a
+// warp's part of its CTA's share are one warp's.
 constexpr int kWhole = 16;
-// What an item costs beside its tiles (q, the end), in tiles.
+// What an item costs beside its tiles (q, the end), in tiles (the same batch:
+// 54 us with 1, 48 with 3 or 4).
 constexpr int kItemCost = 3;
-constexpr int kMinShare = 4;   // tiles of a CTA, unless there are fewer in all
+// Tiles of a CTA, unless there are fewer in all: one for each warp.  (With 16,
+// one sequence of 1024 tokens takes 16.4 us instead of 13.3 and one of 64 9.6
+// instead of 6.4; 8192 tokens 21.7 instead of 23.2, 16 heads on one of 64 over
+// 128 x 490 tokens 11.4 instead of 13.4.)
+constexpr int kMinShare = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum is raised only when a score passes it by this much (in
@@ -91,7 +114,7 @@ struct Cfg {
   static constexpr int kQRegs = kLanes ? M * D / 4 : kSteps * kQOps * 4;
   // Keys of a warp's tile: 8 KB of K and V, 32 at most; a smaller one (8 keys in
   // TF32, 16 in the 16-bit types) where q and O leave no registers for the
-  // larger one's scores.
+  // larger one's scores (they would spill).
   static constexpr int kLeast = kF32 ? 8 : 16;
   static constexpr int kMost = 4096 / kRowBytes < 32 ? 4096 / kRowBytes : 32;
   static constexpr int kKeys = kLanes || kQRegs + D / 2 <= 48 ? kMost : kLeast;
@@ -1194,7 +1217,13 @@ static_assert(kLevels * kMaxCtas * sizeof(uint32_t) <= kCounterBytes, "");
 // FP32 of 64 45.2 against 36.9; f16 of 64, 128 x 1 .. 16384 27.5 against 28.7.)
 template <class C, bool F32ACT, int D>
 int launch_heads(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
+  // One head: plain FMAs.  (FP32, 8 on 8, 8 x 4096 tokens: 53 us against 72 of
+  // the tensor cores at 128 dims, 34 against 42 at 64; 32 on 32 of 64, FP32 q on
+  // bf16: 82 against 98.)
   if (a.group == 1) return launch<C, F32ACT, D, 1>(a, dev, st);
+  // Two: where q would take three terms or the cache is FP32.  (16 on 8 of 64,
+  // 32 x 4096, FP32 q on bf16: 54 us against 62; 16-bit q, and FP32 q on f16,
+  // take 54 to 55 either way, at 32 dims 63.)
   if constexpr (sizeof(C) == 4 || (q_terms<C, F32ACT>() == 3 && D <= 64))
     if (a.group == 2) return launch<C, F32ACT, D, 2>(a, dev, st);
   return launch<C, F32ACT, D, 8>(a, dev, st);
