@@ -16,10 +16,23 @@
 // still streams (programmatic dependent launch) and waits for it before it
 // touches an output.  A CTA of the second takes the token ids of a row that
 // leave one remainder, so that the small ids, which make up most of a text,
-// are spread.  Counting within the streaming kernel, a piece of the vocabulary
-// a CTA, took 90 us for 256 x 100256 logits with histories of 64 to 8192
-// tokens: every CTA waited for its own counts.
-// Integer counts do not depend on the order of the atomics.
+// are spread.  Integer counts do not depend on the order of the atomics.
+//
+// Device time on a B200 (floor: bytes at the 6.53 TB/s of a copy):
+//   256 x 100256 FP32, mask                     33.4 us   floor 31.9 (95 %)
+//   the same, histories of 64 / 64 .. 8192 / 8192 tokens, 64 biases
+//                            41 / 54.5 / 73     floor 32 to 34
+//   33 x 50257 bf16, histories up to 2048, mask 8.2       1.6
+//   1 x 100256, history of 256, 16 biases       5.0       0.1
+// The mending alone takes 8 / 23 / 52 us: a history of 8192 is counted in 8,
+// and its few thousand outputs are single sectors, read and written.  The
+// overlap saves 3 (256 x 100256: 54.5 us against 57.7).  What else was tried
+// with 256 x 100256 logits and histories of 64 to 8192: counting within the
+// streaming kernel, a piece of the vocabulary a CTA (90 us: each waits for its
+// own counts); a cluster for each row (103 to 141); and one mending CTA beside
+// three streaming ones on an SM, which counts all of its rows while they
+// stream and keeps the results in shared memory (73 to 99: the shared memory
+// is the L1 that the streaming loads pass through, 33 us becomes 47).
 #include "decode_common.cuh"
 
 namespace ct {
@@ -45,7 +58,7 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* mask, uint32_t id,
 // out = logits, -inf where the mask has a 0.  Rows start at any multiple of
 // the element size: the tokens up to the first whole vector are single
 // accesses, and so are all of a row whose logits and outputs are not aligned
-// alike (`vectors` false).
+// alike (`vectors` false: 39.3 us instead of 33.4 for 256 x 100256).
 template <class T>
 __device__ __forceinline__ void stream_piece(const LogitsProcess& p, int64_t item, int piece,
                                              int pieces, bool vectors) {
@@ -267,8 +280,10 @@ __global__ void __launch_bounds__(kMendThreads, 3)
     auto mended = [&](float x, uint32_t mark) {
       const uint32_t count = mark >> 1;
       // (x / rep to 1 ulp more: the reciprocal is rounded first)
-      const float y = x * (x > 0.0f ? inverse : rep);
-      return count ? y - (freq * (float)count + pres) : y;
+      // (the roundings are spelled out: a row's result does not depend on
+      // which of the two places mends it)
+      const float y = __fmul_rn(x, x > 0.0f ? inverse : rep);
+      return count ? __fsub_rn(y, fmaf(freq, (float)count, pres)) : y;
     };
     const int in_list = listed < kListed ? listed : kListed;
     for (int k0 = threadIdx.x; k0 < in_list; k0 += kMends * kMendThreads) {
@@ -321,7 +336,7 @@ __global__ void __launch_bounds__(kMendThreads, 3)
 template <class T>
 int launch_stream(const LogitsProcess& p, const DeviceInfo& dev, cudaStream_t st) {
   // Some rounds of loads a CTA, one or less where that would leave SMs without
-  // work.
+  // work (1 x 100256: 1.8 us against 2.4).
   int piece = kRounds * kLoads * kBlock;
   while (piece > kBlock && p.rows * ((p.vocab + piece - 1) / piece) < 4 * dev.sm_count) piece /= 2;
   const int64_t pieces = (p.vocab + piece - 1) / piece;
@@ -338,7 +353,8 @@ int launch_stream(const LogitsProcess& p, const DeviceInfo& dev, cudaStream_t st
 template <bool WIDE>
 int launch_mend(const LogitsProcess& p, bool dependent, const DeviceInfo& dev, cudaStream_t st) {
   // The fewest parts of a row (each reads its history) whose marks and list fit
-  // and that give every SM a CTA.
+  // and that give every SM a CTA (64 x 100256: 13.1 us, with the fewest that fit
+  // 13.8; 1 x 100256: 5.0 and 5.3).
   const int64_t most = p.tokens ? p.max_len : 0;
   int shift = 0;
   int64_t entries = p.vocab, bytes = 0;

@@ -450,6 +450,48 @@ def test_logits(cuda_device, ops, dtype, rows, vocab, hist, bias, masked):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("rows,vocab,hist,bias", [(310, 700, 900, 4), (300, 60000, 20000, 0),
+                                                  (300, 1001, 60, 700), (330, 40000, 40000, 400)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_logits_more_rows_than_sms(cuda_device, ops, rows, vocab, hist, bias, masked):
+    """Rows of which a block has several, whose tokens and biases fit its lists together, one
+    by one, or not at all; histories beyond 16-bit counts.  A row's result is the same
+    whichever rows it is computed with; some are compared with 64 bits."""
+    g = gen(rows + vocab)
+    x = 3 * torch.randn(rows, vocab, generator=g, device="cuda")
+    tokens = torch.randint(-2, vocab + 2, (rows, hist), generator=g, device="cuda")
+    tokens[::2] %= 90
+    lens = torch.randint(0, hist + 1, (rows,), generator=g, device="cuda").int()
+    plens = torch.randint(0, hist + 1, (rows,), generator=g, device="cuda").int()
+    rep, freq, pres = (torch.rand(rows, generator=g, device="cuda") + 0.6 for _ in range(3))
+    ids = values = None
+    if bias:
+        ids = torch.randint(-1, vocab + 1, (rows, bias), generator=g, device="cuda")
+        ids[:, bias // 2:] = ids[:, :bias - bias // 2]
+        values = torch.randn(rows, bias, generator=g, device="cuda")
+    mask = random_mask(rows, vocab, g) if masked else None
+    args = (x, tokens, lens, plens, rep, freq, pres, ids, values, mask)
+    got = ops.logits_process(*args)
+    some = list(range(0, rows, 47)) + [rows - 1]
+    check_logits(got[some], *(None if a is None else a[some] for a in args))
+    for r0 in range(0, rows, 110):
+        part = ops.logits_process(*(None if a is None else a[r0:r0 + 110] for a in args))
+        assert torch.equal(part, got[r0:r0 + 110])
+
+
+def test_logits_a_great_many_rows(cuda_device, ops):
+    g = gen(77)
+    rows, vocab = 80000, 40
+    x = torch.randn(rows, vocab, generator=g, device="cuda")
+    tokens = torch.randint(0, vocab, (rows, 9), generator=g, device="cuda")
+    pres = torch.rand(rows, generator=g, device="cuda")
+    got = ops.logits_process(x, tokens, presence=pres)
+    seen = torch.zeros(rows, vocab, dtype=torch.bool, device="cuda").scatter_(1, tokens, True)
+    ref = torch.where(seen, x.double() - pres.double()[:, None], x.double())
+    # one rounding, of a term below 8
+    assert bool(((got.double() - ref).abs() <= 2.0 ** -21).all())
+
+
 @pytest.mark.parametrize("keep", ["nothing", "penalties", "bias", "mask"])
 def test_logits_single_options(cuda_device, ops, keep):
     g = gen(21)
