@@ -34,14 +34,15 @@
 //   64 sequences of 4096 tokens            170 - 174 us   floor 164
 //   one of 131072                          92.5           82.2
 //   32 on 32 of 64, FP32 q, 16 x 3500..4096 81.9          76.0
-//   64 of 16 .. 4096                       46.9           30.4
-//   FP32, 8 on 8 of 128, 5 x 777..4097     26.4           13.2
-//   f16, 16 on 1 of 64, 128 x 1..16384     28.5           8.7
-//   one of 8192 / 1024 / 64                24 / 13.4 / 6.4  5.1 / 0.6 / 0.04
+//   64 of 16 .. 4096                       45.3           30.4
+//   FP32, 8 on 8 of 128, 5 x 777..4097     25.0           13.2
+//   f16, 16 on 1 of 64, 128 x 1..16384     28.2           8.7
+//   one of 8192 / 1024 / 64         19.5 / 13.9 / 6.5     5.1 / 0.6 / 0.04
 // Long batches run at the copy's rate.  The rest is a fixed chain of latencies:
 // 2 us to start, 2 us for the lengths and the table, 2 to 3 us until the first
 // tile is worked on, 1 us at the end of an item and about 3 us (write, fence,
-// counter, read) for each level of joining, two of them from 9 parts on.
+// counter, read) for each level of joining, two of them from 9 parts on.  Where
+// a choice below names a figure, both sides were measured on the code of its day.
 #include "decode_common.cuh"
 
 namespace ct {
@@ -56,13 +57,17 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kFan = 8;
 constexpr int kLevels = 3;     // kFan^kLevels >= kMaxCtas
 // Items of at most so many tiles are never split between CTAs: joining the
-// parts costs more than the tiles (64 sequences of 16 to 4096 tokens took 58 us
-// with 16, 70 with 8, when this was chosen).  Those of no more tiles than a
-// warp's part of its CTA's share are one warp's.
-constexpr int kWhole = 16;
-// What an item costs beside its tiles (q, the end), in tiles (the same batch:
-// 54 us with 1, 48 with 3 or 4).
-constexpr int kItemCost = 3;
+// parts costs more than the tiles, in short shares above all.  Those of no more
+// tiles than a warp's part of its CTA's share are one warp's.  (Whole up to 12
+// tiles against 16: 64 sequences of 16 to 4096 tokens, in six random orders, 48
+// us against 49 on average and 48 against 56 at most; FP32, 6 on 6 of 64,
+// 128 x 1..256, which have shares of 19 tiles, 13.5 against 11.5.)
+constexpr int kShortShare = 32;
+__device__ __forceinline__ int longest_whole(int64_t share) { return share < kShortShare ? 16 : 12; }
+// What an item costs beside its tiles (q, the end), in tiles.  (The same six,
+// 3 / 7 / 12: 52 / 49 / 51 us; FP32, 8 on 8 of 128, 5 x 777..4097 26.7 / 25.1 /
+// 24.9.)
+constexpr int kItemCost = 7;
 // Tiles of a CTA, unless there are fewer in all: one for each warp.  (With 16,
 // one sequence of 1024 tokens takes 16.4 us instead of 13.3 and one of 64 9.6
 // instead of 6.4; 8192 tokens 21.7 instead of 23.2, 16 heads on one of 64 over
@@ -439,15 +444,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
   int64_t ctas = divide(total + kMinShare - 1, kMinShare);
   if (ctas > gridDim.x) ctas = gridDim.x;
   if (blockIdx.x >= ctas) return;
-  // the first `longer` CTAs take one tile more than the others
-  const int64_t share = divide(total, ctas), longer = total - share * ctas;
-  auto cta_of = [&](int64_t tile) {
-    return tile < longer * (share + 1) ? divide(tile, share + 1)
-                                       : longer + divide(tile - longer * (share + 1), share);
-  };
+  // CTA c's share begins at tile c * total / ctas, rounded down
+  const int64_t share = divide(total, ctas);
+  const int whole = longest_whole(share);
+  auto cta_of = [&](int64_t tile) { return divide((tile + 1) * ctas - 1, total); };
   int64_t edge[2];
-  edge[0] = blockIdx.x * share + (blockIdx.x < longer ? blockIdx.x : longer);
-  edge[1] = edge[0] + share + (blockIdx.x < longer ? 1 : 0);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) edge[e] = divide((blockIdx.x + e) * total, ctas);
   while (true) {
     const int cost = c.tiles + kItemCost;
     const int64_t start = (before + upto - cost) * a.items;
@@ -460,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
         x.tile = (int)(from - (int64_t)x.item * cost) - kItemCost;
         s_first[e] = edge[e] - x.tile;  // the item's first tile, in the count
         // an edge in the item's cost, or inside a short item, moves to its start
-        if (x.tile < 0 || x.tiles <= kWhole) x.tile = 0;
+        if (x.tile < 0 || x.tiles <= whole) x.tile = 0;
         s_edge[e] = x;
       }
     }
@@ -482,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
   const int end_item = end_b < p.batch ? s_edge[1].item : 0;
   const int end_tile = end_b < p.batch ? s_edge[1].tile : 0;
   if (cur.b == end_b && cur.item == end_item && cur.tile >= end_tile) return;
-  const int brief = (int)(share / kWarps < kWhole ? share / kWarps : kWhole);
+  const int brief = (int)(share / kWarps < whole ? share / kWarps : whole);
 
   // Walks the share item by item: true with `seg`, the tiles of the item that
   // lie in the share, and whether it is this warp's alone; false at the end.
@@ -644,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
     if (tid >= 2) return;
     const Cursor& x = s_edge[tid];
     bool part = tid == 0 || end_b < p.batch;
-    if (part) part = x.tiles > kWhole;  // (short ones lie in one share)
+    if (part) part = x.tiles > whole;  // (short ones lie in one share)
     if (part) {
       const bool same = x.b == end_b && x.item == end_item;
       part = tid == 0 ? x.tile > 0 || same
@@ -1201,7 +1204,8 @@ int launch(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   if (ctas > (tiles + kMinShare - 1) / kMinShare) ctas = (tiles + kMinShare - 1) / kMinShare;
   // One sequence: as many whole CTAs to each item, so that none works on two
-  // (the one that does ends some 3 us after the others).
+  // (the one that does ends some 3 us after the others): 8192 tokens 19.5 us
+  // against 23.3, 131072 92.5 against 95.7.
   if (a.p.batch == 1 && b.items <= ctas / 8) ctas -= ctas % b.items;
   kernel<<<(unsigned)ctas, kThreads, F::kSmem, st>>>(b);
   return check_launch();
