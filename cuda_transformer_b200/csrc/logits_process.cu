@@ -21,9 +21,9 @@
 // Device time on a B200 (floor: bytes at the 6.53 TB/s of a copy):
 //   256 x 100256 FP32, mask                     33.4 us   floor 31.9 (95 %)
 //   the same, histories of 64 / 64 .. 8192 / 8192 tokens, 64 biases
-//                            41 / 54.5 / 73     floor 32 to 34
-//   33 x 50257 bf16, histories up to 2048, mask 8.2       1.6
-//   1 x 100256, history of 256, 16 biases       5.0       0.1
+//                            41.5 / 53.5 / 73     floor 32 to 34
+//   33 x 50257 bf16, histories up to 2048, mask 7.6       1.6
+//   1 x 100256, history of 256, 16 biases       4.9       0.1
 // The mending alone takes 8 / 23 / 52 us: a history of 8192 is counted in 8,
 // and its few thousand outputs are single sectors, read and written.  The
 // overlap saves 3 (256 x 100256: 54.5 us against 57.7).  What else was tried
@@ -32,7 +32,8 @@
 // own counts); a cluster for each row (103 to 141); and one mending CTA beside
 // three streaming ones on an SM, which counts all of its rows while they
 // stream and keeps the results in shared memory (73 to 99: the shared memory
-// is the L1 that the streaming loads pass through, 33 us becomes 47).
+// is the L1 that the streaming loads pass through, 33 us becomes 47).  Taking the
+// rows with the longest histories first gave less than finding them cost.
 #include "decode_common.cuh"
 
 namespace ct {
@@ -148,14 +149,16 @@ __global__ void __launch_bounds__(kStreamThreads, 5)
   stream_piece<T>(p, blockIdx.x, piece, pieces, vectors);
 }
 
-constexpr int kMendThreads = 512;
+// (256 x 100256, histories of 64 to 8192: 53.3 us; 512 threads and 8 reads 54.6,
+// 1024 threads 57 to 59)
+constexpr int kMendThreads = 768;
 constexpr int kMendShared = 108 * 1024;  // most of a CTA: two an SM
 constexpr int kListed = 4096;           // tokens that the list holds
 constexpr int kMends = 4;               // tokens of a thread that are on the way at once
 constexpr int kBiases = 512;            // of a CTA that are kept in shared memory
 constexpr int kMostEntries = 65536;     // (the list holds 16 bits)
 
-constexpr int kReads = 8;               // of the history, of a thread, likewise
+constexpr int kReads = 4;               // of the history, of a thread, likewise
 constexpr uint32_t kNoToken = 0xffffffffu;  // (ids are below 2^31)
 
 // A CTA: the tokens of row r with id % 2^shift == part, id >> shift their index;
@@ -165,7 +168,7 @@ constexpr uint32_t kNoToken = 0xffffffffu;  // (ids are below 2^31)
 // found, so that their outputs are fetched together; should there be more than
 // the list holds, the rest are looked for among the marks.
 template <bool WIDE>
-__global__ void __launch_bounds__(kMendThreads, 3)
+__global__ void __launch_bounds__(kMendThreads, 2)
     logits_mend_kernel(const __grid_constant__ LogitsProcess p, const int shift, const int entries,
                        const bool dependent) {
   extern __shared__ __align__(16) uint32_t marks[];
