@@ -31,13 +31,13 @@
 //
 // Device time of a launch on a B200 (floor: the cached values at the 6.53 TB/s
 // of a copy); 32 heads on 8 of 128, bf16, unless it says otherwise:
-//   64 sequences of 4096 tokens            170 - 174 us   floor 164
+//   64 sequences of 4096 tokens            175 us         floor 164
 //   one of 131072                          92.5           82.2
 //   32 on 32 of 64, FP32 q, 16 x 3500..4096 81.9          76.0
-//   64 of 16 .. 4096                       45.3           30.4
+//   64 of 16 .. 4096                       43.9           30.4
 //   FP32, 8 on 8 of 128, 5 x 777..4097     25.0           13.2
 //   f16, 16 on 1 of 64, 128 x 1..16384     28.2           8.7
-//   one of 8192 / 1024 / 64         19.5 / 13.9 / 6.5     5.1 / 0.6 / 0.04
+//   one of 8192 / 1024 / 64         18.1 / 13.5 / 6.6     5.1 / 0.6 / 0.04
 // Long batches run at the copy's rate.  The rest is a fixed chain of latencies:
 // 2 us to start, 2 us for the lengths and the table, 2 to 3 us until the first
 // tile is worked on, 1 us at the end of an item and about 3 us (write, fence,
@@ -128,9 +128,13 @@ struct Cfg {
   static constexpr int kCopies = kKeys * kRowChunks / 32;    // of a lane, for K or V
   static constexpr int kCopyRows = 32 / kRowChunks;          // rows of one copy instruction
   static constexpr int kStageBytes = 2 * kKeys * kRowBytes;  // K tile, V tile
-  // Registers: q, O and about 72 more.  Three CTAs an SM where that fits 168 a
-  // thread, with two stages of 8 KB or as many smaller ones.
-  static constexpr int kCtas = kQRegs + (kLanes ? kQRegs : D / 2) + 72 <= 168 ? 3 : 2;
+  // Three CTAs an SM of 168 registers a thread, with two stages of 8 KB or as
+  // many smaller ones; two CTAs with three stages where q and O of several heads
+  // of 128 dims leave too few registers.  (32 heads on 8 of 128: FP32 q on f16,
+  // 16 x 4096 tokens, 55 us instead of 72, which spilled; bf16, 64 x 16..4096
+  // 43.9 instead of 45.5, 64 x 64 9.7 instead of 11.9, 64 x 4096 174.9 instead of
+  // 173.  Two CTAs at 64 dims: FP32, 32 on 8, 16 x 4096 61.4 instead of 59.4.)
+  static constexpr int kCtas = D == 128 && M > 1 ? 2 : 3;
   static constexpr int kRing = kCtas == 3 ? 16384 : 24576;
   static constexpr int kStages = kRing / kStageBytes > 6 ? 6 : kRing / kStageBytes;
   static_assert(M * D * 4 <= kStageBytes, "the warps' O meet in stages of their rings");
