@@ -21,7 +21,7 @@
 //   cache                                      115.9 us  floor 114.6 (99 %)
 //   32 on 8 of 128 in bf16, turned / not       80 / 71.5 us   69.0 / 68.7
 //   7 prompts of 100 to 2000, 8 on 8 of 128, FP32, half of a head turned
-//                                               24.4 us  18.6 (76 %)
+//                                               23.0 us  18.6 (81 %)
 //   one token each of 64 sequences, bf16         2.4 us  0.25 (the launch)
 // In bf16 with angles a thread's chain (angles, page, then the stores) is what
 // is left: its bytes are half and its latencies the same.
@@ -233,13 +233,13 @@ int launch(const KvAppend& p, const DeviceInfo& dev, cudaStream_t st) {
   int unit_shift = 0;
   while ((VEC << (unit_shift + 1)) < p.head_dim) ++unit_shift;
   const int64_t parts = (p.q_heads + 2 * p.kv_heads) << unit_shift;
-  // Several parts a thread (fewer fetches of angles and pages) once there is
-  // work for every SM several times over (12 prompts, FP32 into bf16: 115.9 us,
-  // one part a thread 135.9; in bf16 80 and 92; the 7 FP32 prompts 24.4 and 23.0); one for the shortest way through a
-  // decoding step.
+  // Several parts a thread (fewer fetches of angles and pages) once every SM has
+  // work for many rounds (12 prompts of 300 to 4096 tokens, FP32 into bf16: 115.9
+  // us, one part a thread 135.9; in bf16, 54000 CTAs of one part, 80 and 92); one
+  // part below that (7 FP32 prompts, 15000 CTAs: 23.0 us, three parts 24.4).
   const int64_t rows = (parts + kThreads - 1) / kThreads;
   int items = 1;
-  if (p.tokens * rows >= (int64_t)dev.sm_count * 32)
+  if (p.tokens * rows >= (int64_t)dev.sm_count * 128)
     items = rows % 3 == 0 ? 3 : rows % 4 == 0 ? 4 : rows % 2 == 0 ? 2 : rows == 1 ? 1 : 3;
   const dim3 grid((unsigned)p.tokens, (unsigned)((rows + items - 1) / items));
   switch (items) {
