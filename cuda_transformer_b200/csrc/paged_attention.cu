@@ -22,12 +22,12 @@
 //    they are, q and the probabilities as two or three 16-bit terms; FP32
 //    caches take three TF32 products.  8 heads put two terms into the 16 rows of
 //    one product (high and low sums of a head then sit in the same lane).  The
-//    order of keys and dims inside a
-//    product is chosen so that every operand is a 16-byte shared-memory
-//    vector: no shuffles, no transposes.  tcgen05 would take 8 heads as 128
-//    rows; at 4 * group FLOPs a value the tensor pipe is not what bounds this
-//    kernel.  One or two heads are cheaper as plain FMAs of FP32 (a lane
-//    has a key's dims, so only the score is added up across lanes).
+//    order of keys and dims inside a product is chosen so that every operand is
+//    a 16-byte shared-memory vector: no shuffles, no transposes.  tcgen05 would
+//    take 8 heads as 128 rows; at 4 * group FLOPs a value the tensor pipe is not
+//    what bounds this kernel.  One or two heads are cheaper as plain FMAs of FP32
+//    (a lane has a part of a key's dims, so only scores are added up across four
+//    lanes).
 //
 // Device time of a launch on a B200 (floor: the cached values at the 6.53 TB/s
 // of a copy); 32 heads on 8 of 128, bf16, unless it says otherwise:
