@@ -35,13 +35,16 @@ CACHE_TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float1
 class PagePool:
     """Which pages of a cache belong to which sequence (host side).  table is
     the int32 [batch, max_pages] that the operators read; `reserve` gives a
-    sequence the pages for `tokens` tokens, `release` takes them back."""
+    sequence the pages for `tokens` tokens, `release` takes them back.  A row
+    names the pages that its sequence owns and is -1 past them, which the
+    operators take for no place: a token too many gives NaN there and does not
+    reach another sequence's pages."""
 
     def __init__(self, pages: int, page_size: int, batch: int, max_pages: int, device):
         self.page_size, self.max_pages = page_size, max_pages
         self.free = list(range(pages - 1, -1, -1))
         self.owned: list[list[int]] = [[] for _ in range(batch)]
-        self.table = torch.zeros(batch, max_pages, dtype=torch.int32, device=device)
+        self.table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=device)
 
     def reserve(self, seq: int, tokens: int) -> None:
         have, need = self.owned[seq], -(-tokens // self.page_size)
@@ -58,6 +61,7 @@ class PagePool:
     def release(self, seq: int) -> None:
         self.free.extend(reversed(self.owned[seq]))
         self.owned[seq] = []
+        self.table[seq] = -1
 
 
 class Generator:
