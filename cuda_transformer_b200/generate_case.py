@@ -65,7 +65,9 @@ class PagePool:
 
 
 class Generator:
-    """Generates from a GPT for `batch` sequences of up to `max_len` tokens."""
+    """Generates from a GPT for `batch` sequences of up to `max_len` tokens.
+    `prompt` begins a sequence, `release` ends it; in between every `step` feeds
+    it a token.  Sequences that have not begun or have ended take no part."""
 
     def __init__(self, model: GPT, batch: int, max_len: int, page_size: int = 16,
                  cache: torch.dtype = torch.float32, rotary: bool = False):
@@ -87,6 +89,8 @@ class Generator:
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)  # tokens in the history
         self.prompt_lens = torch.zeros_like(self.lens)
         self.rows = torch.arange(batch, device=device)
+        self.live = torch.zeros(batch, dtype=torch.bool, device=device)  # takes part in steps
+        self.counts = [0] * batch  # the host's count of the tokens; 0: none begun
 
     def _embed(self, idx, positions):
         x = self.model.tok(idx)
@@ -109,12 +113,23 @@ class Generator:
         w = m.tok.weight.t() if m.tied else m.lm_head_weights
         return CudaLinearLayer.apply(m.ln(x), w, m.lm_head_bias)[0]
 
+    def release(self, seq: int) -> None:
+        """Ends a sequence and gives its pages back."""
+        self.pool.release(seq)
+        self.live[seq] = False
+        self.lens[seq] = self.prompt_lens[seq] = 0
+        self.counts[seq] = 0
+
     @torch.no_grad()
     def prompt(self, seq: int, tokens: torch.Tensor, room: int = 0) -> torch.Tensor:
         """Runs a prompt (int64 [n], n > 0) as sequence `seq` and returns the
         logits after it [vocab]; `room`: tokens to reserve pages for."""
         n = tokens.numel()
-        self.pool.release(seq)
+        if n == 0:
+            raise ValueError("a prompt has at least one token")
+        if max(n, room) > self.max_len:
+            raise ValueError(f"{max(n, room)} tokens are more than max_len, {self.max_len}")
+        self.release(seq)
         self.pool.reserve(seq, max(n, room))
         device = self.history.device
         positions = torch.arange(n, dtype=torch.int32, device=device)
@@ -132,26 +147,43 @@ class Generator:
 
         x = self._blocks(self._embed(tokens.to(device), positions).unsqueeze(0), attend)
         self.history[seq, :n] = tokens.to(device)
-        self.lens[seq] = self.prompt_lens[seq] = n
+        self.lens[seq] = self.prompt_lens[seq] = self.counts[seq] = n
+        self.live[seq] = True
         return self._logits(x[:, -1:])[0]
 
-    @torch.no_grad()
     def step(self, idx: torch.Tensor) -> torch.Tensor:
         """Feeds one token a sequence (int64 [batch]; their places are the
-        current lengths) and returns the logits after them [batch, vocab].
-        No host synchronisation."""
-        positions = self.lens.clone()
-        self.history[self.rows, positions.long()] = idx
-        self.lens += 1
+        current lengths) and returns the logits after them [batch, vocab]
+        (those of sequences that take no part mean nothing).  No host
+        synchronisation.  A sequence without room for it is a ValueError."""
+        self._take_room()
+        return self._step(idx)
+
+    def _take_room(self) -> None:
+        for seq, n in enumerate(self.counts):
+            if n and n >= min(self.max_len, len(self.pool.owned[seq]) * self.pool.page_size):
+                raise ValueError(f"sequence {seq} has no room for a token after its {n}")
+        self.counts = [n + 1 if n else 0 for n in self.counts]
+
+    @torch.no_grad()
+    def _step(self, idx: torch.Tensor) -> torch.Tensor:
+        """The device's part of a step."""
+        live = self.live & (self.lens < self.max_len)
+        positions = torch.where(live, self.lens, -1)  # -1: padding
+        at = positions.clamp(min=0)
+        self.history[self.rows, at.long()] = torch.where(
+            live, idx, self.history[self.rows, at.long()])
+        self.lens += live
+        lens = torch.where(live, self.lens, 0)
 
         def attend(layer, q, k, v):
             q2, _ = ops.kv_append_(*self.caches[layer], k, v, self.pool.table, positions,
                                    q=q if self.rotary else None, cos=self.cos, sin=self.sin)
             o, _ = ops.paged_attention(q2 if self.rotary else q, *self.caches[layer],
-                                       self.pool.table, self.lens, workspace=self.workspace)
+                                       self.pool.table, lens, workspace=self.workspace)
             return o
 
-        return self._logits(self._blocks(self._embed(idx, positions).unsqueeze(0), attend))
+        return self._logits(self._blocks(self._embed(idx, at).unsqueeze(0), attend))
 
     @torch.no_grad()
     def choose(self, logits: torch.Tensor, temperature: float = 0.0, uniform=None,
@@ -172,6 +204,8 @@ class Generator:
                  graph: bool = False, **processing):
         """`new` tokens after each prompt; returns them [batch, new] and the
         unprocessed logits that each was chosen from [new, batch, vocab]."""
+        if len(prompts) != self.batch:
+            raise ValueError(f"{len(prompts)} prompts for {self.batch} sequences")
         g = torch.Generator(device=self.history.device).manual_seed(seed)
         uniform = torch.rand(new, self.batch, generator=g, device=self.history.device)
         logits = torch.stack([self.prompt(b, t, t.numel() + new) for b, t in enumerate(prompts)])
@@ -180,7 +214,7 @@ class Generator:
 
         def advance():
             idx = self.choose(state["logits"], temperature, draw, **processing)
-            return idx, self.step(idx)
+            return idx, self._step(idx)
 
         replay = None
         if graph:
@@ -203,6 +237,7 @@ class Generator:
         for t in range(new):
             draw.copy_(uniform[t])
             seen.append(state["logits"].clone())
+            self._take_room()
             if replay is not None:
                 replay.replay()
                 tokens.append(held.clone())
