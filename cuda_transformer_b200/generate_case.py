@@ -197,8 +197,13 @@ class Generator:
             return logits.argmax(-1)
         probs = ops.cuda_softmax((logits / temperature).unsqueeze(0))[0]
         upto = probs.cumsum(-1)
-        drawn = torch.searchsorted(upto, (uniform * upto[:, -1])[:, None], right=True)[:, 0]
-        return drawn.clamp_(max=logits.shape[1] - 1)
+        # the first token whose running sum passes the number; a scan's sums can
+        # step up by a rounding at a token of probability 0, so that is asked for
+        # too; the last such token where no sum passes
+        some = probs > 0
+        hit = some & (upto > (uniform * upto[:, -1])[:, None])
+        last = probs.shape[1] - 1 - some.int().flip(1).argmax(-1)
+        return torch.where(hit.any(-1), hit.int().argmax(-1), last)
 
     def generate(self, prompts, new: int, temperature: float = 0.0, seed: int = 0,
                  graph: bool = False, **processing):

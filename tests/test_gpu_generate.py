@@ -71,3 +71,29 @@ def test_sequences_can_be_replaced(cuda_device):
     want = gen.generate(prompts[::-1], 10)[0]
     _, _, fresh = setup()
     assert torch.equal(want, fresh.generate(prompts[::-1], 10)[0])
+
+
+def test_a_drawn_token_has_a_probability(cuda_device):
+    """The running sums of a parallel scan can step up by a rounding at a token of
+    probability 0; numbers that fall into such a step must not draw it."""
+    from cuda_transformer_b200.generate_case import Generator
+    from cuda_transformer_b200.gpt_case import GPT
+
+    vocab = 60000
+    gen = Generator(GPT(1, 64, 2, 8, vocab).cuda(), 1, 8)
+    gen.prompt(0, torch.zeros(1, dtype=torch.int64, device="cuda"), 8)
+    g, steps = torch.Generator(device="cuda").manual_seed(1), 0
+    from cuda_transformer import ops
+    for _ in range(20):
+        logits = 3 * torch.randn(1, vocab, generator=g, device="cuda")
+        mask = torch.randint(-2 ** 31, 2 ** 31, (1, vocab // 32), generator=g, device="cuda").int()
+        masked = ops.logits_process(logits, mask=mask)
+        probs = ops.cuda_softmax(masked.unsqueeze(0))[0]
+        upto = probs.cumsum(-1)[0]
+        rises = ((probs[0, 1:] == 0) & (upto[1:] > upto[:-1])).nonzero()[:8, 0] + 1
+        for i in rises.tolist():
+            uniform = (upto[i - 1] / upto[-1])[None].clamp(max=1 - 2.0 ** -24)
+            idx = gen.choose(logits, 1.0, uniform, mask=mask)
+            assert probs[0, idx] > 0
+            steps += 1
+    print("steps at tokens of probability 0:", steps)
