@@ -195,7 +195,9 @@ class Generator:
                                     prompt_lens=self.prompt_lens, **processing)
         if temperature == 0.0:
             return logits.argmax(-1)
-        probs = ops.cuda_softmax((logits / temperature).unsqueeze(0))[0]
+        # (bounded: +inf, as a bias can make it, takes all of the softmax)
+        top = torch.finfo(torch.float32).max
+        probs = ops.cuda_softmax((logits / temperature).clamp_(max=top).unsqueeze(0))[0]
         upto = probs.cumsum(-1)
         # the first token whose running sum passes the number; a scan's sums can
         # step up by a rounding at a token of probability 0, so that is asked for

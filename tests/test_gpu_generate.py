@@ -97,3 +97,12 @@ def test_a_drawn_token_has_a_probability(cuda_device):
             assert probs[0, idx] > 0
             steps += 1
     print("steps at tokens of probability 0:", steps)
+
+
+def test_infinite_bias_decides(cuda_device):
+    for temperature in (0.0, 0.9):
+        model, prompts, gen = setup()
+        tokens, _ = gen.generate(prompts, 4, temperature=temperature,
+                                 bias_ids=torch.full((3, 1), 11, device="cuda"),
+                                 bias_values=torch.full((3, 1), float("inf"), device="cuda"))
+        assert (tokens == 11).all()
