@@ -154,7 +154,8 @@ class Generator:
     def step(self, idx: torch.Tensor) -> torch.Tensor:
         """Feeds one token a sequence (int64 [batch]; their places are the
         current lengths) and returns the logits after them [batch, vocab]
-        (those of sequences that take no part mean nothing).  No host
+        (those of sequences that take no part mean nothing).  A negative token
+        ends its sequence; its pages stay until `release`.  No host
         synchronisation.  A sequence without room for it is a ValueError."""
         self._take_room()
         return self._step(idx)
@@ -168,6 +169,7 @@ class Generator:
     @torch.no_grad()
     def _step(self, idx: torch.Tensor) -> torch.Tensor:
         """The device's part of a step."""
+        self.live &= idx >= 0
         live = self.live & (self.lens < self.max_len)
         positions = torch.where(live, self.lens, -1)  # -1: padding
         at = positions.clamp(min=0)
@@ -183,18 +185,22 @@ class Generator:
                                        self.pool.table, lens, workspace=self.workspace)
             return o
 
-        return self._logits(self._blocks(self._embed(idx, at).unsqueeze(0), attend))
+        x = self._embed(idx.clamp(min=0), at).unsqueeze(0)
+        return self._logits(self._blocks(x, attend))
 
     @torch.no_grad()
     def choose(self, logits: torch.Tensor, temperature: float = 0.0, uniform=None,
                **processing) -> torch.Tensor:
         """The next token of each row: the best one, or with a temperature the
-        one that `uniform` ([batch] numbers in [0, 1)) draws.  processing:
-        logits_process's repetition, frequency, presence, biases and mask."""
+        one that `uniform` ([batch] numbers in [0, 1)) draws; -1 for rows without
+        one: the mask leaves nothing, the logits are NaN, the sequence takes no
+        part.  processing: logits_process's repetition, frequency, presence,
+        biases and mask."""
         logits = ops.logits_process(logits, tokens=self.history, lens=self.lens,
                                     prompt_lens=self.prompt_lens, **processing)
         if temperature == 0.0:
-            return logits.argmax(-1)
+            there = logits.amax(-1) > float("-inf")  # (false for NaN too)
+            return torch.where(there & self.live, logits.argmax(-1), -1)
         # (bounded: +inf, as a bias can make it, takes all of the softmax)
         top = torch.finfo(torch.float32).max
         probs = ops.cuda_softmax((logits / temperature).clamp_(max=top).unsqueeze(0))[0]
@@ -205,12 +211,14 @@ class Generator:
         some = probs > 0
         hit = some & (upto > (uniform * upto[:, -1])[:, None])
         last = probs.shape[1] - 1 - some.int().flip(1).argmax(-1)
-        return torch.where(hit.any(-1), hit.int().argmax(-1), last)
+        drawn = torch.where(hit.any(-1), hit.int().argmax(-1), last)
+        return torch.where(some.any(-1) & self.live, drawn, -1)
 
     def generate(self, prompts, new: int, temperature: float = 0.0, seed: int = 0,
                  graph: bool = False, **processing):
         """`new` tokens after each prompt; returns them [batch, new] and the
-        unprocessed logits that each was chosen from [new, batch, vocab]."""
+        unprocessed logits that each was chosen from [new, batch, vocab].  A
+        sequence that has no next token ends: -1 from there on."""
         if len(prompts) != self.batch:
             raise ValueError(f"{len(prompts)} prompts for {self.batch} sequences")
         g = torch.Generator(device=self.history.device).manual_seed(seed)
@@ -227,7 +235,7 @@ class Generator:
         if graph:
             # warm up on a side stream (lazy initialisation), then capture; the
             # lengths go back to the prompts' and every step overwrites its slots
-            keep = self.lens.clone()
+            keep, live = self.lens.clone(), self.live.clone()
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
@@ -235,6 +243,7 @@ class Generator:
                 advance()
             torch.cuda.current_stream().wait_stream(side)
             self.lens.copy_(keep)
+            self.live.copy_(live)
             replay = torch.cuda.CUDAGraph()
             with torch.cuda.graph(replay):
                 held, after = advance()

@@ -111,3 +111,15 @@ def test_what_a_step_passes_to_the_operators(monkeypatch):
     gen.live[0] = True
     gen.step(torch.tensor([3, 4]))
     assert seen == [[3, -1], [4, 0]]
+
+
+def test_a_negative_token_ends_its_sequence():
+    gen = generator()
+    for seq in range(2):
+        gen.prompt(seq, torch.arange(2), 8)
+    for idx in ([5, -1], [6, 7], [4, 4]):
+        gen.step(torch.tensor(idx))
+    assert gen.lens.tolist() == [5, 2] and gen.history[1].tolist() == [0, 1] + [0] * 6
+    gen.prompt(1, torch.arange(3), 8)
+    gen.step(torch.tensor([1, 2]))
+    assert gen.lens.tolist() == [6, 4] and gen.history[1, :4].tolist() == [0, 1, 2, 2]

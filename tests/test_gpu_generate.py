@@ -73,6 +73,36 @@ def test_sequences_can_be_replaced(cuda_device):
     assert torch.equal(want, fresh.generate(prompts[::-1], 10)[0])
 
 
+def test_no_token_left(cuda_device):
+    """A row whose mask leaves nothing, or whose logits are NaN, has no next token: -1, with
+    and without a temperature, and it has ended: nothing more is fed to it."""
+    for temperature in (0.0, 0.7):
+        model, prompts, gen = setup()
+        mask = torch.full((3, 3), -1, dtype=torch.int32, device="cuda")
+        mask[1] = 0
+        tokens, logits = gen.generate(prompts, 6, temperature=temperature, mask=mask)
+        assert (tokens[1] == -1).all() and (tokens[[0, 2]] >= 0).all()
+        assert gen.lens.tolist() == [p.numel() + n for p, n in zip(prompts, (6, 0, 6))]
+        _, _, other = setup()
+        want, ref = other.generate(prompts, 6, temperature=temperature)
+        assert torch.equal(tokens[[0, 2]], want[[0, 2]])
+        assert torch.equal(logits[:, [0, 2]], ref[:, [0, 2]])
+        bad = ref[0].clone()
+        bad[2] = float("nan")
+        uniform = torch.full((3,), 0.5, device="cuda")
+        got = other.choose(bad, temperature, uniform)
+        assert got[2] == -1 and got[0] >= 0
+
+
+def test_infinite_bias_decides(cuda_device):
+    for temperature in (0.0, 0.9):
+        model, prompts, gen = setup()
+        tokens, _ = gen.generate(prompts, 4, temperature=temperature,
+                                 bias_ids=torch.full((3, 1), 11, device="cuda"),
+                                 bias_values=torch.full((3, 1), float("inf"), device="cuda"))
+        assert (tokens == 11).all()
+
+
 def test_a_drawn_token_has_a_probability(cuda_device):
     """The running sums of a parallel scan can step up by a rounding at a token of
     probability 0; numbers that fall into such a step must not draw it."""
@@ -97,12 +127,3 @@ def test_a_drawn_token_has_a_probability(cuda_device):
             assert probs[0, idx] > 0
             steps += 1
     print("steps at tokens of probability 0:", steps)
-
-
-def test_infinite_bias_decides(cuda_device):
-    for temperature in (0.0, 0.9):
-        model, prompts, gen = setup()
-        tokens, _ = gen.generate(prompts, 4, temperature=temperature,
-                                 bias_ids=torch.full((3, 1), 11, device="cuda"),
-                                 bias_values=torch.full((3, 1), float("inf"), device="cuda"))
-        assert (tokens == 11).all()
