@@ -275,17 +275,16 @@ __global__ void __launch_bounds__(kMendThreads, 2)
   if (dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (n > 0) {
-    const float rep = p.repetition ? p.repetition[r] : 1.0f, inverse = 1.0f / rep;
+    const float rep = p.repetition ? p.repetition[r] : 1.0f;
     const float freq = p.frequency ? p.frequency[r] : 0.0f;
     const float pres = p.presence ? p.presence[r] : 0.0f;
     using Mark = std::conditional_t<WIDE, uint32_t, uint16_t>;
     Mark* const mark_of = reinterpret_cast<Mark*>(marks);
     auto mended = [&](float x, uint32_t mark) {
       const uint32_t count = mark >> 1;
-      // (x / rep to 1 ulp more: the reciprocal is rounded first)
       // (the roundings are spelled out: a row's result does not depend on
       // which of the two places mends it)
-      const float y = __fmul_rn(x, x > 0.0f ? inverse : rep);
+      const float y = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
       return count ? __fsub_rn(y, fmaf(freq, (float)count, pres)) : y;
     };
     const int in_list = listed < kListed ? listed : kListed;

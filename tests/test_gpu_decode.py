@@ -640,3 +640,19 @@ def test_refusals(cuda_device, ops):
         ops.logits_process(x.double())
     with pytest.raises(RuntimeError):
         ops.logits_process(x[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab,hist", [(3, 5000, 4000), (2, 60000, 40000)])
+def test_logits_penalty_is_a_division(cuda_device, ops, dtype, rows, vocab, hist):
+    """x / r and x * r, each rounded once: the same bits as torch's.  (The longer histories
+    exceed the list of tokens, so that both places that mend are met.)"""
+    g = gen(vocab)
+    x = (3 * torch.randn(rows, vocab, generator=g, device="cuda")).to(dtype)
+    tokens = torch.randint(0, vocab, (rows, hist), generator=g, device="cuda")
+    rep = 1.0 + torch.rand(rows, generator=g, device="cuda")
+    rep[0] = 1e-39                       # its reciprocal is beyond FP32
+    seen = torch.zeros(rows, vocab, dtype=torch.bool, device="cuda").scatter_(1, tokens, True)
+    r, y = rep[:, None], x.float()
+    want = torch.where(seen, torch.where(y > 0, y / r, y * r), y)
+    assert torch.equal(ops.logits_process(x, tokens, repetition=rep), want)
