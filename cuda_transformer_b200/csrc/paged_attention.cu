@@ -43,6 +43,8 @@
 // tile is worked on, 1 us at the end of an item and about 3 us (write, fence,
 // counter, read) for each level of joining, two of them from 9 parts on.  Where
 // a choice below names a figure, both sides were measured on the code of its day.
+#include <cfloat>
+
 #include "decode_common.cuh"
 
 namespace ct {
@@ -102,7 +104,8 @@ struct Cfg {
   static constexpr int kVVec = kVec < D / 8 ? kVec : D / 8;  // V elements a lane reads at once
   static constexpr int kVIter = D / (8 * kVVec);
   static constexpr int kOTiles = D / 8;
-  // Terms q and the probabilities are split into.  With 16-bit activations q
+  // Terms q and the probabilities are split into (pairs share a product, a term
+  // in rows 0-7 and a term in rows 8-15).  With 16-bit activations q
   // is exact as it is, and two terms of p leave an error (2^-16 in bf16) far
   // below the output's own rounding; FP32 activations take as many as hold 22
   // bits or more.
@@ -191,10 +194,15 @@ __device__ __forceinline__ uint32_t low_tf32(uint32_t x) {
   return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u));
 }
 // The next 16-bit term of x and y (x in the low half); x and y keep the rest.
-template <class C>
+template <class C, bool CUT = false>
 __device__ __forceinline__ uint32_t take_term(float& x, float& y) {
   uint32_t w;
-  if constexpr (std::is_same<C, __nv_bfloat16>::value) {
+  if constexpr (CUT) {  // cut off instead of rounded: the rest has x's sign
+    static_assert(std::is_same<C, __nv_bfloat16>::value, "");
+    w = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    x -= __uint_as_float(w << 16);
+    y -= __uint_as_float(w & 0xffff0000u);
+  } else if constexpr (std::is_same<C, __nv_bfloat16>::value) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     w = *reinterpret_cast<const uint32_t*>(&h);
     x -= __uint_as_float(w << 16);
@@ -207,6 +215,22 @@ __device__ __forceinline__ uint32_t take_term(float& x, float& y) {
     y -= f.y;
   }
   return w;
+}
+
+// Infinite cached values.  The product of the first terms alone has the right
+// infinity, or NaN; the others' are 0 * inf or of either sign.  So a result is
+// the first terms' sum where that is not finite, and their rows or accumulators
+// hold nothing of the others that could be NaN.
+__device__ __forceinline__ float with_rest(float first, float rest) {
+  return fabsf(first) < INFINITY ? first + rest : first;
+}
+// The low part of a cached V, whose products join the first terms': some finite
+// number (and no sum over KEYS keys overflows) where inf - inf made it NaN.
+// (It is below 2^116, and so kept, of values below 2^126.  A NaN is one by its
+// high mantissa bits here, which every NaN that arithmetic makes has set.)
+template <int KEYS>
+__device__ __forceinline__ uint32_t finite_low_tf32(uint32_t x) {
+  return __float_as_uint(fminf(__uint_as_float(low_tf32(x)), 0x1p121f / KEYS));
 }
 
 // Element e of a 16-byte chunk.
@@ -894,7 +918,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
             } else {
 #pragma unroll
               for (int k = 0; k < F::kQOps; ++k)
-                mma<C>(s_acc[n][(e + k) & 1], q_regs[s][k], kw[n][2 * e], kw[n][2 * e + 1]);
+                mma<C>(s_acc[n][F::kQOps == 2 ? k : e], q_regs[s][k], kw[n][2 * e], kw[n][2 * e + 1]);
             }
           }
         }
@@ -910,7 +934,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float(&x)[2][4] = s_acc[n];
-            v[n][e] = ((x[0][e] + x[1][e]) + (x[0][e + 2] + x[1][e + 2])) * s_mul[0];
+            if constexpr (F::kQTerms == 1)
+              v[n][e] = (x[0][e] + x[1][e]) * s_mul[0];
+            else if constexpr (F::kF32)
+              v[n][e] = with_rest(x[0][e], x[1][e] + (x[0][e + 2] + x[1][e + 2])) * s_mul[0];
+            else if constexpr (F::kQTerms == 2)
+              v[n][e] = with_rest(x[0][e] + x[1][e], x[0][e + 2] + x[1][e + 2]) * s_mul[0];
+            else
+              v[n][e] = with_rest(x[0][e], x[1][e] + x[0][e + 2]) * s_mul[0];
             if (first_key + n * 8 + 2 * t + e >= end_key) v[n][e] = -INFINITY;
             top = fmaxf(top, v[n][e]);
           }
@@ -935,10 +966,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
             split_tf32(x, pa[n][0][0], pa[n][0][1]);
             split_tf32(y, pa[n][0][2], pa[n][0][3]);
           } else {
+            constexpr bool kCut = F::kPTerms == 3;
 #pragma unroll
-            for (int k = 0; k < F::kPTerms; ++k)
-              pa[n / 2][k / 2][k % 2 + 2 * (n % 2)] = take_term<C>(x, y);
-            if (F::kPTerms % 2) pa[n / 2][F::kPTerms / 2][1 + 2 * (n % 2)] = 0u;
+            for (int k = 0; k < 2; ++k)
+              pa[n / 2][0][k + 2 * (n % 2)] = take_term<C, kCut>(x, y);
+            if constexpr (kCut) {
+              // it shares rows with the first term: positive, so that infinite
+              // values times it have their own sign
+              x = fmaxf(x, FLT_MIN);
+              y = fmaxf(y, FLT_MIN);
+              pa[n / 2][1][2 * (n % 2)] = take_term<C>(x, y);
+              pa[n / 2][1][1 + 2 * (n % 2)] = 0u;
+            }
           }
         }
       }
@@ -973,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
           for (int e = 0; e < F::kVVec; ++e) {
             if constexpr (F::kF32) {
               const uint32_t x = vw[0][e], y = vw[1][e];
-              mma<C>(c[e], pa[ks][0], low_tf32(x), low_tf32(y));
+              mma<C>(c[e], pa[ks][0], finite_low_tf32<F::kKeys>(x), finite_low_tf32<F::kKeys>(y));
               mma<C>(c[e], pa[ks][0], x, y);
             } else {
               // element e of keys 2 t and 2 t + 1 (and 8 further) in one word
@@ -1064,7 +1103,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const float(&o)[4] = o_acc[i * F::kVVec + e + k];
-                xs[k] = (o[cc] + o[cc + 2]) * f;
+                xs[k] = with_rest(o[cc], o[cc + 2]) * f;
               }
               put((2 * t + cc + 8 * i) * F::kVVec + e, x);
             }

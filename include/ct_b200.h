@@ -361,7 +361,8 @@ enum { CT_DTYPE_F32 = 0, CT_DTYPE_BF16 = 1, CT_DTYPE_F16 = 2 };
  * activations' type; they may not overlap the inputs.  A token with a negative position is
  * padding: nothing is appended and its q_out and k_out rows are zero.  A token
  * with no place (sequence, page table entry or angle row out of range) is not
- * appended and its q_out and k_out rows are NaN.  Two tokens with the same place leave either's values
+ * appended and its q_out and k_out rows are NaN.  Values beyond an f16 cache's
+ * range become infinite in it (ct_paged_attention says what follows).  Two tokens with the same place leave either's values
  * there.  No reference counterpart (the reference keeps no cache). */
 int ct_kv_append(const void* q, const int64_t q_stride[3],
                  const void* k, const int64_t k_stride[3],
@@ -388,7 +389,12 @@ size_t ct_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int6
  * out is dense [batch, q_heads, head_dim] of q's type; lse (may be NULL) dense
  * [batch, q_heads].  A length of zero or below gives O = 0 and LSE = -inf; one
  * beyond max_pages * page_size, or a page out of range, gives NaN.  Slots past
- * the length are not read.  The cache's base and strides must be multiples of
+ * the length are not read.  Cached values that are not finite follow the
+ * formula: a key with a score of -inf has no weight, a score of +inf or NaN makes
+ * its head NaN, an infinite value with a weight makes its element of O infinite,
+ * one without NaN.  (Weights below 2^-120 of the largest count as none, and
+ * with more than one head a key/value head of an f16 cache those below 2^-30;
+ * there, elements of an FP32 q below 2^-38 of their head's largest count as 0.)  The cache's base and strides must be multiples of
  * 16 bytes (CT_ERR_UNSUPPORTED_LAYOUT otherwise).
  * The first CT_PAGED_ATTENTION_COUNTER_BYTES of the workspace must be zero
  * before its first use; every call leaves them so, ready for the next call of

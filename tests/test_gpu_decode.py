@@ -656,3 +656,73 @@ def test_logits_penalty_is_a_division(cuda_device, ops, dtype, rows, vocab, hist
     r, y = rep[:, None], x.float()
     want = torch.where(seen, torch.where(y > 0, y / r, y * r), y)
     assert torch.equal(ops.logits_process(x, tokens, repetition=rep), want)
+
+
+# ------------------------------------------------------- non-finite cached values
+GROUPS = [(F32, F32, 1), (F32, F32, 2), (F32, F32, 5), (F32, BF16, 1), (F32, BF16, 2),
+          (F32, BF16, 8), (F32, F16, 1), (F32, F16, 2), (F32, F16, 3), (BF16, BF16, 1),
+          (BF16, BF16, 4), (F16, F16, 1), (F16, F16, 8), (F32, F32, 20), (BF16, BF16, 12)]
+
+
+def infinite_case(act, cache, group, dim, seed):
+    """Two key/value heads, sequences of one tile, of several and of several CTAs'
+    shares; q is positive in dim 3, so that an infinite key there decides the sign."""
+    lens, page, g = [9, 100, 3000], 16, gen(seed)
+    k, v, table = make_cache(lens, 2, dim, page, cache, "token", g)
+    q = torch.randn(3, 2 * group, dim, generator=g, device="cuda")
+    q[:, :, 3] = q[:, :, 3].abs() + 0.1
+    return lens, page, k, v, table, q.to(act)
+
+
+def slot(table, b, j, page=16):
+    return int(table[b, j // page]), slice(None), j % page
+
+
+@pytest.mark.parametrize("act,cache,group", GROUPS)
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_attention_infinite_keys(cuda_device, ops, act, cache, group, dim):
+    """A key whose score is -inf has no weight, wherever it lies; one whose score is +inf
+    leaves no number."""
+    lens, page, k, v, table, q = infinite_case(act, cache, group, dim, 40 + dim + group)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    clean_k, keep = k.clone(), [torch.ones(m, dtype=torch.bool) for m in lens]
+    for b, m in enumerate(lens):
+        for j in (0, m // 2, m - 1):
+            k[slot(table, b, j)][..., 3] = -math.inf
+            keep[b][j] = False
+    got = ops.paged_attention(q, k, v, table, n)
+    # the same without those keys
+    k2, v2, table2 = make_cache([int(x.sum()) for x in keep], 2, dim, page, cache, "head", gen(1))
+    for b, x in enumerate(keep):
+        for i, j in enumerate(x.nonzero()[:, 0].tolist()):
+            for new, old in ((k2, clean_k), (v2, v)):
+                new[slot(table2, b, i)] = old[slot(table, b, j)]
+    check_attention(q, k2, v2, table2, [int(x.sum()) for x in keep], page, got, dim ** -0.5)
+    k[slot(table, 1, 50)][..., 3] = math.inf
+    out, lse = ops.paged_attention(q, k, v, table, n)
+    assert out[1].isnan().all()
+    assert torch.equal(out[[0, 2]], got[0][[0, 2]]) and torch.equal(lse[[0, 2]], got[1][[0, 2]])
+
+
+@pytest.mark.parametrize("act,cache,group", GROUPS)
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_attention_infinite_values(cuda_device, ops, act, cache, group, dim):
+    """An infinite value with a weight makes its dim of the result infinite, two of opposite
+    signs NaN; the other dims are untouched.  Scores are kept within a few units, so that
+    every weight is a normal number of each type."""
+    lens, page, k, v, table, q = infinite_case(act, cache, group, dim, 80 + dim + group)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    clean = v.clone()
+    want = ops.paged_attention(q, k, v, table, n)
+    for b, m in enumerate(lens):
+        v[slot(table, b, 0)][..., 5] = math.inf
+        v[slot(table, b, m - 1)][..., dim - 2] = -math.inf
+        v[slot(table, b, m // 2)][..., dim // 2] = math.inf
+        v[slot(table, b, m // 3)][..., dim // 2] = -math.inf
+    out, lse = ops.paged_attention(q, k, v, table, n)
+    assert torch.equal(lse, want[1])
+    assert (out[..., 5] == math.inf).all() and (out[..., dim - 2] == -math.inf).all()
+    assert out[..., dim // 2].isnan().all()
+    rest = [d for d in range(dim) if d not in (5, dim - 2, dim // 2)]
+    assert torch.equal(out[..., rest], want[0][..., rest])
+    check_attention(q, k, clean, table, lens, page, want, dim ** -0.5)
