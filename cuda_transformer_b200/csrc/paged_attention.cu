@@ -333,81 +333,63 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // Reference point of a maximum: sums that have seen no key are 0 to any.
 __device__ __forceinline__ float finite(float top) { return top == -INFINITY ? 0.0f : top; }
 
-// Joins the partials k0, k0 + step, .. (n of them) of the item that CTA c0
-// starts, in that order, 8 or 16 at a time: into partial k0 or the output.
+// Joins the partials k0, k0 + step, .. (n of them, kFan at most) of the item
+// that CTA c0 starts, in that order: into partial k0 or the output.
 template <int HEADS, int D>
 __device__ __forceinline__ void join_partials(const Launch& a, int c0, int k0, int step, int n,
                                               bool to_partial, int64_t row, int heads) {
   constexpr int64_t kSize = partial_floats(HEADS, D);
-  constexpr int kItems = HEADS * D / 4;  // float4s, one or two to a thread at a time
-  constexpr int kPart = kItems > kThreads ? 2 : 1, kBatch = 16 / kPart;
+  constexpr int kItems = HEADS * D / 4;  // float4s, one or two to a thread
+  constexpr int kPart = kItems > kThreads ? 2 : 1;
+  static_assert(kItems <= kPart * kThreads, "");
   auto at = [&](int k) { return a.partials + (k == 0 ? 2 * c0 + 1 : 2 * (c0 + k)) * kSize; };
-#pragma unroll 1
-  for (int base = 0; base < kItems; base += kPart * kThreads) {
-    float m[kPart], l[kPart];
-    float4 x[kPart];
+  float km[kPart][kFan], kl[kPart][kFan];
+  float4 y[kPart][kFan];
+#pragma unroll
+  for (int j = 0; j < kFan; ++j) {
+    if (j >= n) continue;
+    const float* s = at(k0 + j * step);
 #pragma unroll
     for (int i = 0; i < kPart; ++i) {
-      m[i] = -INFINITY;
-      l[i] = 0.0f;
-      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll 1
-    for (int b = 0; b < n; b += kBatch) {
-      float km[kPart][kBatch], kl[kPart][kBatch];
-      float4 y[kPart][kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (b + j >= n) continue;
-        const float* s = at(k0 + (b + j) * step);
-#pragma unroll
-        for (int i = 0; i < kPart; ++i) {
-          const int id = base + threadIdx.x + i * kThreads;
-          if (id >= kItems) continue;
-          km[i][j] = __ldcg(s + HEADS * D + id / (D / 4));
-          kl[i][j] = __ldcg(s + HEADS * D + HEADS + id / (D / 4));
-          y[i][j] = __ldcg(reinterpret_cast<const float4*>(s + id * 4));
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kPart; ++i) {
-        float top = m[i];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (b + j < n) top = fmaxf(top, km[i][j]);
-        const float ref = finite(top), f0 = exp2_fast(m[i] - ref);
-        m[i] = top;
-        l[i] *= f0;
-        x[i] = make_float4(x[i].x * f0, x[i].y * f0, x[i].z * f0, x[i].w * f0);
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          if (b + j >= n) continue;
-          const float f = exp2_fast(km[i][j] - ref);
-          x[i].x = fmaf(y[i][j].x, f, x[i].x);
-          x[i].y = fmaf(y[i][j].y, f, x[i].y);
-          x[i].z = fmaf(y[i][j].z, f, x[i].z);
-          x[i].w = fmaf(y[i][j].w, f, x[i].w);
-          l[i] = fmaf(kl[i][j], f, l[i]);
-        }
-      }
-    }
-    // a head's maxima and sums are read by the lanes of one warp; partial k0 is
-    // overwritten after they have them
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kPart; ++i) {
-      const int id = base + threadIdx.x + i * kThreads, h = id / (D / 4), d = id % (D / 4) * 4;
+      const int id = threadIdx.x + i * kThreads;
       if (id >= kItems) continue;
-      if (to_partial) {
-        float* s = at(k0);
-        *reinterpret_cast<float4*>(s + id * 4) = x[i];
-        if (d == 0) {
-          s[HEADS * D + h] = m[i];
-          s[HEADS * D + HEADS + h] = l[i];
-        }
-      } else if (h < heads) {
-        write_out(a.p, row + h, d, D, x[i], m[i], l[i]);
+      km[i][j] = __ldcg(s + HEADS * D + id / (D / 4));
+      kl[i][j] = __ldcg(s + HEADS * D + HEADS + id / (D / 4));
+      y[i][j] = __ldcg(reinterpret_cast<const float4*>(s + id * 4));
+    }
+  }
+  // a head's maxima and sums are read by the lanes of one warp; partial k0 is
+  // overwritten after they have them
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kPart; ++i) {
+    const int id = threadIdx.x + i * kThreads, h = id / (D / 4), d = id % (D / 4) * 4;
+    if (id >= kItems) continue;
+    float m = -INFINITY, l = 0.0f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < kFan; ++j)
+      if (j < n) m = fmaxf(m, km[i][j]);
+    const float ref = finite(m);
+#pragma unroll
+    for (int j = 0; j < kFan; ++j) {
+      if (j >= n) continue;
+      const float f = exp2_fast(km[i][j] - ref);
+      x.x = fmaf(y[i][j].x, f, x.x);
+      x.y = fmaf(y[i][j].y, f, x.y);
+      x.z = fmaf(y[i][j].z, f, x.z);
+      x.w = fmaf(y[i][j].w, f, x.w);
+      l = fmaf(kl[i][j], f, l);
+    }
+    if (to_partial) {
+      float* s = at(k0);
+      *reinterpret_cast<float4*>(s + id * 4) = x;
+      if (d == 0) {
+        s[HEADS * D + h] = m;
+        s[HEADS * D + HEADS + h] = l;
       }
+    } else if (h < heads) {
+      write_out(a.p, row + h, d, D, x, m, l);
     }
   }
 }
