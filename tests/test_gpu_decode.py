@@ -726,3 +726,76 @@ def test_attention_infinite_values(cuda_device, ops, act, cache, group, dim):
     rest = [d for d in range(dim) if d not in (5, dim - 2, dim // 2)]
     assert torch.equal(out[..., rest], want[0][..., rest])
     check_attention(q, k, clean, table, lens, page, want, dim ** -0.5)
+
+
+# ---------------------------------------------------------------- forms seldom met
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(3, 3, 64), (4, 2, 32), (5, 1, 128), (12, 1, 64),
+                                          (16, 2, 64)])
+def test_attention_query_layouts(cuda_device, ops, act, cache, heads, kv, dim):
+    """q that is not made of 16-byte vectors (a last stride other than one, an odd offset, an odd
+    row stride) is read element by element: the same bits as its dense copy."""
+    lens, g = [40, 0, 700, 3], gen(heads + dim)
+    k, v, table = make_cache(lens, kv, dim, 16, cache, "token", g)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    flat = torch.randn(4 * (heads + 1) * (2 * dim + 3) + 5, generator=g, device="cuda").to(act)
+    views = (torch.as_strided(flat, (4, heads, dim), (heads * 2 * dim, 2 * dim, 2), 1),
+             torch.as_strided(flat, (4, heads, dim), (heads * dim, dim, 1), 1),
+             torch.as_strided(flat, (4, heads, dim), (heads * (dim + 3), dim + 3, 1), 0),
+             torch.as_strided(flat, (4, heads, dim), (heads * dim, 1, heads), 0),
+             torch.as_strided(flat, (4, heads, dim), (0, dim, 1), 3))
+    for q in views:
+        got = ops.paged_attention(q, k, v, table, n)
+        want = ops.paged_attention(q.contiguous(), k, v, table, n)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        check_attention(q, k, v, table, lens, 16, got, dim ** -0.5)
+
+
+# rows of 128 parts that a token's heads make (FP32: four elements a part's vector, 16-bit: eight,
+# or one), and the parts a thread that follow: 2, 3, 4, 3 with a partly filled block of y
+@pytest.mark.parametrize("act,cache,heads,kv,dim,rot,interleaved,vec,rows", [
+    (F32, BF16, 16, 8, 64, 64, False, 4, 2), (F32, F32, 32, 8, 64, 32, True, 4, 3),
+    (F32, F16, 48, 8, 64, 64, False, 4, 4), (F32, BF16, 50, 10, 64, 64, False, 4, 5),
+    (BF16, BF16, 100, 6, 128, 128, False, 8, 7), (F16, F16, 28, 2, 128, 64, True, 8, 2),
+    (F32, F16, 32, 4, 32, 6, False, 1, 5), (F16, F16, 12, 2, 32, 10, True, 1, 2),
+    (BF16, BF16, 18, 3, 64, 2, False, 1, 6), (F32, F32, 40, 12, 32, 2, True, 1, 8)])
+@pytest.mark.parametrize("layout", ["head", "token"])
+def test_append_many_tokens(cuda_device, ops, act, cache, heads, kv, dim, rot, interleaved, vec,
+                            rows, layout):
+    """Prompts long enough that a thread has several parts of a token's heads."""
+    assert -(-(heads + 2 * kv) * (dim // (2 * vec)) // 128) == rows
+    sms, page, g = torch.cuda.get_device_properties(0).multi_processor_count, 13, gen(rows + dim)
+    tokens = -(-128 * sms // rows) + 5
+    lens = [tokens // 3, tokens - tokens // 3]
+    need = [-(-n // page) for n in lens]
+    table = torch.full((2, max(need)), -1, dtype=torch.int32, device="cuda")
+    perm = torch.randperm(sum(need) + 2, generator=g, device="cuda").int()
+    table[0, :need[0]], table[1, :need[1]] = perm[:need[0]], perm[need[0]:sum(need)]
+    shape = (sum(need) + 2, kv, page, dim)
+    if layout == "token":
+        shape = (shape[0], page, kv, dim)
+    k_cache, v_cache = (torch.full(shape, 7.0, dtype=cache, device="cuda") for _ in range(2))
+    if layout == "token":
+        k_cache, v_cache = k_cache.transpose(1, 2), v_cache.transpose(1, 2)
+    ids = torch.cat([torch.full((n,), b) for b, n in enumerate(lens)]).int().cuda()
+    pos = torch.cat([torch.arange(n) for n in lens]).int().cuda()
+    pos[5], pos[tokens - 2] = -1, -1           # padding
+    there = pos >= 0
+    qkv = torch.randn(tokens, heads + 2 * kv, dim, generator=g, device="cuda").to(act)
+    q, k, v = qkv.split([heads, kv, kv], 1)
+    cos, sin = ops.rotary_tables(max(lens), rot, device="cuda")
+    want_k, want_v = k_cache.double(), v_cache.clone()
+    q_out, k_out = ops.kv_append_(k_cache, v_cache, k, v, table, pos, seq_ids=ids, q=q, cos=cos,
+                                  sin=sin, interleaved=interleaved, want_k=True)
+    assert torch.count_nonzero(q_out[~there]) == torch.count_nonzero(k_out[~there]) == 0
+    ids, pos, qd, kd, vd = (t[there] for t in (ids, pos, q, k, v))
+    qr, qb = rotate(qd, pos, cos, sin, interleaved)
+    kr, kb = rotate(kd, pos, cos, sin, interleaved)
+    for got, ref, bound in ((q_out[there], qr, qb), (k_out[there], kr, kb)):
+        assert bool(((got.double() - ref).abs() <= bound + ROUND[act] * ref.abs() + 2.0 ** -25).all())
+    where = (table[ids.long(), pos.long() // page].long(), slice(None), pos.long() % page)
+    want_k[where], want_v[where] = kr, vd.to(cache)
+    bound = torch.zeros_like(want_k)
+    bound[where] = kb + ROUND[cache] * kr.abs() + 2.0 ** -25
+    assert bool(((k_cache.double() - want_k).abs() <= bound).all())
+    assert torch.equal(v_cache, want_v)
