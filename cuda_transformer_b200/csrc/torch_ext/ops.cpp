@@ -527,17 +527,18 @@ std::tuple<Tensor, Tensor> kv_append_(Tensor k_cache, Tensor v_cache, Tensor k0,
   const int32_t* seq = vector_of<int32_t>(seq_ids0, tokens, k, at::kInt, "seq_ids", &keep_seq);
   int64_t q_heads = 0, rot = 0, max_positions = 0;
   int64_t qs[3] = {0, 0, 1}, ks[3], vs[3], kcs[4], vcs[4];
-  Tensor q_out = empty_like_of({0}, k.scalar_type(), k), k_out = q_out;
   if (q0.has_value()) {
     check_on(*q0, k, k.scalar_type(), "q");
     TORCH_CHECK(q0->dim() == 3 && q0->size(0) == tokens && q0->size(2) == c.dim,
                 "q must be [tokens, nh, hs]");
     q = unit_last(*q0);
     q_heads = q.size(1);
-    q_out = empty_like_of({tokens, q_heads, c.dim}, k.scalar_type(), k);
     strides3(q, qs);
   }
-  if (want_k) k_out = empty_like_of({tokens, c.heads, c.dim}, k.scalar_type(), k);
+  Tensor q_out = q0.has_value() ? empty_like_of({tokens, q_heads, c.dim}, k.scalar_type(), k)
+                                : empty_like_of({0}, k.scalar_type(), k);
+  Tensor k_out = want_k ? empty_like_of({tokens, c.heads, c.dim}, k.scalar_type(), k)
+                        : empty_like_of({0}, k.scalar_type(), k);
   TORCH_CHECK(cos0.has_value() == sin0.has_value(), "cos and sin go together");
   if (cos0.has_value()) {
     check_on(*cos0, k, at::kFloat, "cos");

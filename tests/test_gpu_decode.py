@@ -799,3 +799,26 @@ def test_append_many_tokens(cuda_device, ops, act, cache, heads, kv, dim, rot, i
     bound[where] = kb + ROUND[cache] * kr.abs() + 2.0 ** -25
     assert bool(((k_cache.double() - want_k).abs() <= bound).all())
     assert torch.equal(v_cache, want_v)
+
+
+def test_operators_keep_their_schemas(cuda_device, ops):
+    """Outputs are tensors of their own, only what the schema names is written, and the fake
+    kernels give the shapes and types of the real ones."""
+    g = gen(31)
+    k, v = (torch.randn(4, 2, 8, 64, generator=g, device="cuda") for _ in range(2))
+    table = torch.tensor([[0, 1], [2, 3], [1, 0]], dtype=torch.int32, device="cuda")
+    n = torch.tensor([3, 9, 0], dtype=torch.int32, device="cuda")
+    q, kn = (torch.randn(3, h, 64, generator=g, device="cuda") for h in (4, 2))
+    cos, sin = ops.rotary_tables(16, 64, device="cuda")
+    x = torch.randn(3, 50, generator=g, device="cuda").half()
+    tokens = torch.randint(0, 50, (3, 7), generator=g, device="cuda")
+    ct = torch.ops.cuda_transformer
+    ws = ops.paged_attention_workspace(4, 2, 64)
+    for op, args in ((ct.kv_append_, (k, v, kn, kn, table, n, None, None, None, None, False, False)),
+                     (ct.kv_append_, (k, v, kn, kn, table, n, None, q, cos, sin, False, True)),
+                     (ct.paged_attention, (q, k, v, table, n, 0.125, ws)),
+                     (ct.paged_attention, (q, k, v, table, n, 0.125, None)),
+                     (ct.logits_process, (x, tokens, n, None, None, None, None, None, None, None))):
+        torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
+    a, b = ops.kv_append_(k, v, kn, kn, table, n)
+    assert a is not b
