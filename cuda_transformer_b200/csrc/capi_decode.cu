@@ -10,6 +10,10 @@ constexpr int64_t kLim = 1ll << 31;
 // longest sequence: the tiles of 32 are counted in 32 bits
 constexpr int64_t kMaxTokens = (1ll << 30) - 256;
 
+// tiles (of 8 keys at least) of all items, with 16 for each item's ends: times
+// the CTAs, fewer than 2^9, they stay below 2^62
+constexpr int64_t kMaxTiles = 1ll << 52;
+
 bool in_range(int64_t v, int64_t low) { return v >= low && v < kLim; }
 
 bool valid_types(int act, int cache) {
@@ -17,8 +21,7 @@ bool valid_types(int act, int cache) {
          (act == cache || act == CT_DTYPE_F32);
 }
 
-// Sizes of a paged cache (status, no CUDA call); every product that is formed
-// later stays below 2^62.
+// Sizes of a paged cache (status, no CUDA call).
 int check_cache(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
                 int64_t page_size, int64_t max_pages, int act, int cache) {
   if (!in_range(batch, 0) || !in_range(q_heads, 0) || !in_range(kv_heads, 1) ||
@@ -124,7 +127,9 @@ int ct_paged_attention(const void* q, const int64_t q_stride[3], const void* k_c
   int rc = check_cache(batch, q_heads, kv_heads, head_dim, pages, page_size, max_pages, act_dtype,
                        cache_dtype);
   if (rc != CT_OK) return rc;
-  if (q_heads % kv_heads != 0 || batch * q_heads >= kLim) return CT_ERR_INVALID_ARGUMENT;
+  if (q_heads % kv_heads != 0 || batch * q_heads >= kLim ||
+      batch * q_heads * (max_pages * page_size / 8 + 16) >= kMaxTiles)
+    return CT_ERR_INVALID_ARGUMENT;
   if (batch * q_heads == 0) return CT_OK;
   if (!q || !q_stride || !seq_lens || !out || !aligned16(out)) return CT_ERR_INVALID_ARGUMENT;
   PagedAttention p{};

@@ -385,14 +385,15 @@ size_t ct_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int6
  *   O = sum_j softmax_j(scale q . k_j) v_j,  LSE = ln sum_j exp(scale q . k_j)
  * over the first seq_lens[b] cached tokens of sequence b.  q is indexed
  * [batch, q_head, head_dim] through its strides; q_heads is a multiple of
- * kv_heads and query head h reads key/value head h / (q_heads / kv_heads).
+ * kv_heads and query head h reads key/value head h / (q_heads / kv_heads);
+ * batch * q_heads < 2^31, and times (max_pages * page_size / 8 + 16) < 2^52.
  * out is dense [batch, q_heads, head_dim] of q's type; lse (may be NULL) dense
  * [batch, q_heads].  A length of zero or below gives O = 0 and LSE = -inf; one
  * beyond max_pages * page_size, or a page out of range, gives NaN.  Slots past
  * the length are not read.  Cached values that are not finite follow the
  * formula: a key with a score of -inf has no weight, a score of +inf or NaN makes
- * its head NaN, an infinite value with a weight makes its element of O infinite,
- * one without NaN.  (Weights below 2^-120 of the largest count as none, and
+ * its head NaN, an infinite value makes its element of O infinite, or NaN where
+ * its key has no weight.  (Weights below 2^-120 of the largest count as none, and
  * with more than one head a key/value head of an f16 cache those below 2^-30;
  * there, elements of an FP32 q below 2^-38 of their head's largest count as 0.)  The cache's base and strides must be multiples of
  * 16 bytes (CT_ERR_UNSUPPORTED_LAYOUT otherwise).

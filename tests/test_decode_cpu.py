@@ -139,3 +139,16 @@ def test_page_pool():
     pool.release(0)
     pool.reserve(1, 16)
     assert len(pool.free) == 2 and pool.table[1].tolist() == pool.owned[1]
+
+
+def test_attention_size_bound():
+    """Shares are products of the tiles of all items and the CTAs, in 64 bits: sizes whose
+    products could pass them are refused before any device call."""
+    bad = cb.CT_ERR_INVALID_ARGUMENT
+    big = dict(heads=1 << 10, kv=1, width=1 << 20, page=1 << 9)      # 2^26 tiles of 8 keys
+    assert attention(batch=1 << 20, **big) == bad                    # 2^30 heads
+    assert attention(batch=1 << 17, **big) == bad
+    for ok in (dict(big, batch=1 << 15), dict(batch=(1 << 20) - 1, heads=1 << 11, kv=1, width=1,
+                                              page=128)):
+        # (accepted up to the workspace)
+        assert attention(wsb=0, **ok) == cb.CT_ERR_WORKSPACE_TOO_SMALL
