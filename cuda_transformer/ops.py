@@ -298,6 +298,7 @@ def rotary_tables(positions: int, rot: int, base: float = 10000.0, device=None):
     """cos and sin of position * base^(-2i/rot), i < rot/2, for kv_append_:
     FP32 [positions, rot/2], formed in FP64 (an FP32 angle loses its low bits
     as the position grows)."""
+    torch._check(rot >= 0 and rot % 2 == 0, lambda: f"rot must be even, not {rot}")
     inv = base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv
     return angle.cos().float(), angle.sin().float()

@@ -152,3 +152,10 @@ def test_attention_size_bound():
                                               page=128)):
         # (accepted up to the workspace)
         assert attention(wsb=0, **ok) == cb.CT_ERR_WORKSPACE_TOO_SMALL
+
+
+def test_rotary_tables_of_an_odd_part_are_refused():
+    from cuda_transformer import ops
+    for rot in (7, -2):
+        with pytest.raises(RuntimeError):
+            ops.rotary_tables(4, rot)
