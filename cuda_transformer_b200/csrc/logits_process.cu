@@ -5,8 +5,8 @@
 //   seen(i) = i is in h[0 .. n),  count(i) = occurrences of i in h[m .. n)
 //   x = logit(i);  if seen(i): x = x > 0 ? x / r : x * r
 //   x -= frequency * count(i) + presence * (count(i) > 0)
-//   x += sum of the row's biases for i;  x = -inf where i's mask bit is 0
-// in FP32.  Biases listed twice for a token are summed in their order.
+//   x += each of the row's biases for i;  x = -inf where i's mask bit is 0
+// in FP32.  Biases listed twice for a token are added in their order.
 //
 // Bound by HBM: a logit is read once and written once; all but the mask
 // concerns a few thousand tokens of a row.  So one kernel streams the rows
@@ -155,7 +155,7 @@ constexpr int kMendThreads = 768;
 constexpr int kMendShared = 108 * 1024;  // most of a CTA: two an SM
 constexpr int kListed = 4096;           // tokens that the list holds
 constexpr int kMends = 4;               // tokens of a thread that are on the way at once
-constexpr int kBiases = 512;            // of a CTA that are kept in shared memory
+constexpr int kBiases = 512;            // of a CTA that are in shared memory at a time
 constexpr int kMostEntries = 65536;     // (the list holds 16 bits)
 
 constexpr int kReads = 4;               // of the history, of a thread, likewise
@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(kMendThreads, 2)
   __shared__ alignas(16) uint32_t bias_id[kBiases];
   __shared__ float bias_value[kBiases];
   __shared__ int listed, biases;
+  __shared__ int64_t bias_next;
   const int64_t r = blockIdx.x >> shift;
   const uint32_t part = blockIdx.x & ((1u << shift) - 1);
   const uint32_t vocab = (uint32_t)p.vocab;
@@ -202,17 +203,18 @@ __global__ void __launch_bounds__(kMendThreads, 2)
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
 
-  // ---- the biases of these tokens in their order, by one warp
+  // ---- the biases of these tokens in their order: from entry j0 on, as many as
+  // surely fit, by the last warp
   const int64_t* ids = p.bias_ids + r * p.bias_ld;
   const float* values = p.bias_values + r * p.bias_values_ld;
-  if (p.bias_n > 0 && threadIdx.x >= kMendThreads - 32) {
+  auto gather = [&](int64_t j0) {
     int found = 0;
-    for (int64_t j0 = lane; j0 - lane < p.bias_n; j0 += 32 * kReads) {
+    for (; j0 < p.bias_n && found + 32 * kReads <= kBiases; j0 += 32 * kReads) {
       uint32_t id[kReads];
       float value[kReads];
 #pragma unroll
       for (int k = 0; k < kReads; ++k) {
-        const int64_t j = j0 + k * 32;
+        const int64_t j = j0 + lane + k * 32;
         id[k] = j < p.bias_n ? known(ids[j]) : kNoToken;
         value[k] = j < p.bias_n ? values[j] : 0.0f;
       }
@@ -220,16 +222,21 @@ __global__ void __launch_bounds__(kMendThreads, 2)
       for (int k = 0; k < kReads; ++k) {
         const bool mine = is_mine(id[k]);
         const uint32_t vote = __ballot_sync(0xffffffffu, mine);
-        const int at = found + __popc(vote & ((1u << lane) - 1));
-        if (mine && at < kBiases) {
+        if (mine) {
+          const int at = found + __popc(vote & ((1u << lane) - 1));
           bias_id[at] = id[k];
           bias_value[at] = value[k];
         }
         found += __popc(vote);
       }
     }
-    if (lane == 0) biases = found;
-  }
+    if (lane == 0) {
+      biases = found;
+      bias_next = j0;
+    }
+  };
+  const bool gathers = threadIdx.x >= kMendThreads - 32;
+  if (p.bias_n > 0 && gathers) gather(0);
   // ---- the history
   const int64_t* history = p.tokens + r * p.tokens_ld;
   for (int64_t j0 = threadIdx.x; j0 - threadIdx.x < n; j0 += kReads * kMendThreads) {
@@ -260,18 +267,21 @@ __global__ void __launch_bounds__(kMendThreads, 2)
     }
   }
   __syncthreads();
-  // the first entry of a biased token holds the sum of all of its entries
-  const int kept = p.bias_n > 0 ? biases : 0;
-  float sum = 0.0f;
-  bool sums = kept <= kBiases && (int)threadIdx.x < kept;
-  if (sums) {
+  // the first of a token's gathered entries adds them all to its output, in their
+  // order (so that it does not matter how many are gathered at a time)
+  bool leads = false, repeats = false;
+  auto look_around = [&]() {
+    leads = (int)threadIdx.x < biases;
+    repeats = false;
+    if (!leads) return;
     const uint32_t id = bias_id[threadIdx.x];
-    for (int i = 0; i < kept; ++i)
+    for (int i = 0; i < biases; ++i)
       if (bias_id[i] == id) {
-        if (i < (int)threadIdx.x) sums = false;
-        sum += bias_value[i];
+        if (i < (int)threadIdx.x) leads = false;
+        if (i > (int)threadIdx.x) repeats = true;
       }
-  }
+  };
+  if (p.bias_n > 0) look_around();
   if (dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (n > 0) {
@@ -316,22 +326,22 @@ __global__ void __launch_bounds__(kMendThreads, 2)
     }
   }
   if (p.bias_n == 0) return;
-  __syncthreads();
-  if (kept <= kBiases) {
-    if (sums && allowed(bias_id[threadIdx.x])) dst[bias_id[threadIdx.x]] += sum;
-    return;
-  }
-  for (int64_t j = threadIdx.x; j < p.bias_n; j += kMendThreads) {
-    const int64_t id = ids[j];
-    if (!is_mine(known(id)) || !allowed((uint32_t)id)) continue;
-    float total = 0.0f;
-    bool earlier = false;
-    for (int64_t i = 0; i < p.bias_n && !earlier; ++i)
-      if (ids[i] == id) {
-        earlier = i < j;
-        total += values[i];
-      }
-    if (!earlier) dst[id] += total;
+  while (true) {
+    __syncthreads();
+    if (leads && allowed(bias_id[threadIdx.x])) {
+      const uint32_t id = bias_id[threadIdx.x];
+      float x = dst[id] + bias_value[threadIdx.x];
+      if (repeats)
+        for (int i = threadIdx.x + 1; i < biases; ++i)
+          if (bias_id[i] == id) x += bias_value[i];
+      dst[id] = x;
+    }
+    const int64_t next = bias_next;
+    if (next >= p.bias_n) return;
+    __syncthreads();
+    if (gathers) gather(next);
+    __syncthreads();
+    look_around();
   }
 }
 
