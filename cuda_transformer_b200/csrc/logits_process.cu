@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kMendThreads, 2)
   uint16_t* const list = reinterpret_cast<uint16_t*>(marks + words);
   __shared__ alignas(16) uint32_t bias_id[kBiases];
   __shared__ float bias_value[kBiases];
+  __shared__ int16_t bias_link[kBiases];  // the token's next entry, -1: none
   __shared__ int listed, biases;
   __shared__ int64_t bias_next;
   const int64_t r = blockIdx.x >> shift;
@@ -230,6 +231,7 @@ __global__ void __launch_bounds__(kMendThreads, 2)
         found += __popc(vote);
       }
     }
+    if (found + lane < (found + 3) / 4 * 4) bias_id[found + lane] = kNoToken;  // (read in fours)
     if (lane == 0) {
       biases = found;
       bias_next = j0;
@@ -269,17 +271,27 @@ __global__ void __launch_bounds__(kMendThreads, 2)
   __syncthreads();
   // the first of a token's gathered entries adds them all to its output, in their
   // order (so that it does not matter how many are gathered at a time)
-  bool leads = false, repeats = false;
+  bool leads = false;
   auto look_around = [&]() {
-    leads = (int)threadIdx.x < biases;
-    repeats = false;
+    const int kept = biases, mine = threadIdx.x;
+    leads = mine < kept;
     if (!leads) return;
-    const uint32_t id = bias_id[threadIdx.x];
-    for (int i = 0; i < biases; ++i)
-      if (bias_id[i] == id) {
-        if (i < (int)threadIdx.x) leads = false;
-        if (i > (int)threadIdx.x) repeats = true;
+    const uint32_t id = bias_id[mine];
+    int link = -1;
+    for (int i = (kept + 3) / 4 * 4 - 4; i >= 0; i -= 4) {
+      const uint4 four = *reinterpret_cast<const uint4*>(bias_id + i);
+      if (four.x != id && four.y != id && four.z != id && four.w != id) continue;
+      const uint32_t each[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+      for (int e = 3; e >= 0; --e) {
+        if (each[e] != id || i + e == mine) continue;
+        if (i + e > mine)
+          link = i + e;
+        else
+          leads = false;
       }
+    }
+    bias_link[mine] = (int16_t)link;
   };
   if (p.bias_n > 0) look_around();
   if (dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -330,10 +342,8 @@ __global__ void __launch_bounds__(kMendThreads, 2)
     __syncthreads();
     if (leads && allowed(bias_id[threadIdx.x])) {
       const uint32_t id = bias_id[threadIdx.x];
-      float x = dst[id] + bias_value[threadIdx.x];
-      if (repeats)
-        for (int i = threadIdx.x + 1; i < biases; ++i)
-          if (bias_id[i] == id) x += bias_value[i];
+      float x = dst[id];
+      for (int i = threadIdx.x; i >= 0; i = bias_link[i]) x += bias_value[i];
       dst[id] = x;
     }
     const int64_t next = bias_next;
