@@ -85,10 +85,11 @@ class Generator:
         self.workspace = ops.paged_attention_workspace(heads, heads, hs, device)
         self.cos, self.sin = (ops.rotary_tables(max_len, hs, device=device) if rotary
                               else (None, None))
-        self.history = torch.zeros(batch, max_len, dtype=torch.int64, device=device)
+        # one column more than is read: where tokens without a place are written
+        self._columns = torch.zeros(batch, max_len + 1, dtype=torch.int64, device=device)
+        self.history = self._columns[:, :max_len]
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)  # tokens in the history
         self.prompt_lens = torch.zeros_like(self.lens)
-        self.rows = torch.arange(batch, device=device)
         self.live = torch.zeros(batch, dtype=torch.bool, device=device)  # takes part in steps
         self.counts = [0] * batch  # the host's count of the tokens; 0: none begun
 
@@ -170,13 +171,13 @@ class Generator:
     def _step(self, idx: torch.Tensor) -> torch.Tensor:
         """The device's part of a step."""
         self.live &= idx >= 0
-        live = self.live & (self.lens < self.max_len)
-        positions = torch.where(live, self.lens, -1)  # -1: padding
-        at = positions.clamp(min=0)
-        self.history[self.rows, at.long()] = torch.where(
-            live, idx, self.history[self.rows, at.long()])
-        self.lens += live
-        lens = torch.where(live, self.lens, 0)
+        positions = torch.where(self.live, self.lens, -1)  # -1: padding
+        at = self.lens.clamp(max=self.max_len - 1)
+        column = positions.remainder(self.max_len + 1).long()
+        self._columns.scatter_(1, column[:, None], idx[:, None])
+        self.lens += self.live
+        self.lens.clamp_(max=self.max_len)
+        lens = positions + 1
 
         def attend(layer, q, k, v):
             q2, _ = ops.kv_append_(*self.caches[layer], k, v, self.pool.table, positions,
@@ -199,20 +200,19 @@ class Generator:
         logits = ops.logits_process(logits, tokens=self.history, lens=self.lens,
                                     prompt_lens=self.prompt_lens, **processing)
         if temperature == 0.0:
-            there = logits.amax(-1) > float("-inf")  # (false for NaN too)
-            return torch.where(there & self.live, logits.argmax(-1), -1)
-        # (bounded: +inf, as a bias can make it, takes all of the softmax)
-        top = torch.finfo(torch.float32).max
-        probs = ops.cuda_softmax((logits / temperature).clamp_(max=top).unsqueeze(0))[0]
-        upto = probs.cumsum(-1)
-        # the first token whose running sum passes the number; a scan's sums can
-        # step up by a rounding at a token of probability 0, so that is asked for
-        # too; the last such token where no sum passes
-        some = probs > 0
-        hit = some & (upto > (uniform * upto[:, -1])[:, None])
-        last = probs.shape[1] - 1 - some.int().flip(1).argmax(-1)
-        drawn = torch.where(hit.any(-1), hit.int().argmax(-1), last)
-        return torch.where(some.any(-1) & self.live, drawn, -1)
+            best, idx = logits.max(-1)
+            there = best > float("-inf")  # (false for NaN too)
+        else:
+            # (bounded: +inf, as a bias can make it, takes all of the softmax)
+            top = torch.finfo(torch.float32).max
+            probs = ops.cuda_softmax((logits / temperature).clamp_(max=top).unsqueeze(0))[0]
+            # the first token whose running sum passes the number; a scan's sums can
+            # step up by a rounding at a token of probability 0, which has no say
+            upto = torch.where(probs > 0, probs.cumsum(-1), 0.0)
+            total = upto.amax(-1)
+            idx = (upto > (uniform * total)[:, None]).int().argmax(-1)
+            there = total > 0
+        return torch.where(there & self.live, idx, -1)
 
     def generate(self, prompts, new: int, temperature: float = 0.0, seed: int = 0,
                  graph: bool = False, **processing):
