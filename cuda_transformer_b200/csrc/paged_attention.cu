@@ -965,8 +965,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
       }
 
       // ---- O += P V.  The tensor cores cut sums off instead of rounding
-      // them, which adds up over a long sequence; with FP32 outputs each
-      // tile's product is therefore formed by itself and added in FP32.
+      // them, which adds up over a long sequence (f16, 450 sequences of 524288
+      // tokens, values about 1: 9.6e-4 of O, against 2.4e-4 at most of the output's
+      // rounding), so each tile's product is formed by itself and added in FP32.
       const uint8_t* vt = tile + F::kKeys * F::kRowBytes;
 #pragma unroll
       for (int i = 0; i < F::kVIter; ++i) {
@@ -975,7 +976,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
         for (int e = 0; e < F::kVVec; ++e)
 #pragma unroll
           for (int x = 0; x < 4; ++x)  // (the low part's sum may be cut off)
-            c[e][x] = !F32ACT || x >= 2 ? o_acc[i * F::kVVec + e][x] : 0.0f;
+            c[e][x] = x >= 2 ? o_acc[i * F::kVVec + e][x] : 0.0f;
 #pragma unroll
         for (int ks = 0; ks < kKSteps; ++ks) {
           constexpr int kV = F::kF32 ? 2 : 4;  // of the lane's keys in a product
@@ -1011,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, F32ACT, D, M>::kCtas)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             float& o = o_acc[i * F::kVVec + e][x];
-            o = F32ACT && x < 2 ? o + c[e][x] : c[e][x];
+            o = x < 2 ? o + c[e][x] : c[e][x];
           }
       }
       }

@@ -864,3 +864,23 @@ def test_logits_time_of_many_biases(cuda_device, ops):
         end.record()
     torch.cuda.synchronize()
     assert start.elapsed_time(end) < 200.0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_sums_of_long_sequences(cuda_device, ops, dim):
+    """Half a million keys in one block's hands (as many sequences as that takes, on the same
+    pages), values about 1: sums that were cut off a little at each of some 8000 steps a warp
+    would be short by 2^-10.  f16 rounds by 2^-11 of the result at most; 8192 roundings of
+    2^-24 that point either way add 2^-17.5, of which 2^-15 is a sixfold."""
+    n, page, g = 1 << 19, 128, gen(dim)
+    batch = 3 * torch.cuda.get_device_properties(0).multi_processor_count + 6
+    k = (0.05 * torch.randn(n // page, 1, page, dim, generator=g, device="cuda")).to(F16)
+    v = (1 + 0.01 * torch.randn(k.shape, generator=g, device="cuda")).to(F16)
+    table = torch.arange(n // page, device="cuda").int().expand(batch, -1)
+    q = torch.randn(batch, 8, dim, generator=g, device="cuda").to(F16)
+    lens = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out, _ = ops.paged_attention(q, k, v, table, lens)
+    kk, vv = (t[:, 0].flatten(0, 1).double() for t in (k, v))
+    for b in (0, batch // 2, batch - 1):
+        ref = (q[b].double() @ kk.T * dim ** -0.5).softmax(-1) @ vv
+        assert bool(((out[b].double() - ref).abs() <= (2.0 ** -11 + 2.0 ** -15) * ref.abs()).all())
