@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kStreamThreads, 5)
 // (256 x 100256, histories of 64 to 8192: 53.3 us; 512 threads and 8 reads 54.6,
 // 1024 threads 57 to 59)
 constexpr int kMendThreads = 768;
-constexpr int kMendShared = 108 * 1024;  // most of a CTA: two an SM
+constexpr int kMendShared = 108 * 1024 - 64;  // most of a CTA beside its 5 KB of biases: two an SM
 constexpr int kListed = 4096;           // tokens that the list holds
 constexpr int kMends = 4;               // tokens of a thread that are on the way at once
 constexpr int kBiases = 512;            // of a CTA that are in shared memory at a time
