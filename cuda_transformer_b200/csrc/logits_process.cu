@@ -21,9 +21,11 @@
 // Device time on a B200 (floor: bytes at the 6.53 TB/s of a copy):
 //   256 x 100256 FP32, mask                     33.4 us   floor 31.9 (95 %)
 //   the same, histories of 64 / 64 .. 8192 / 8192 tokens, 64 biases
-//                            41.5 / 53.5 / 73     floor 32 to 34
-//   33 x 50257 bf16, histories up to 2048, mask 7.6       1.6
-//   1 x 100256, history of 256, 16 biases       4.9       0.1
+//                            41 / 53 / 72         floor 32 to 34
+//   256 x 100256, 300 / 500 biases              42.7 / 47.0
+//   33 x 50257 bf16, histories up to 2048, mask 7.7       1.6
+//   1 x 100256, history of 256, 16 biases       4.8       0.1
+//   1 x 100256, 100256 biases (a row's are gathered 512 at a time) 296
 // The mending alone takes 8 / 23 / 52 us: a history of 8192 is counted in 8,
 // and its few thousand outputs are single sectors, read and written.  The
 // overlap saves 3 (256 x 100256: 54.5 us against 57.7).  What else was tried

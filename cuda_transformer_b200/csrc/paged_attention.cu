@@ -18,26 +18,32 @@
 //  * Each warp streams q and its keys and values through a private cp.async
 //    ring (16-byte copies gather pages of any size and layout) that runs ahead
 //    across items; a block barrier comes only where a long item ends.
-//  * Products run on mma.sync with FP32 accuracy: 16-bit cache values go in as
-//    they are, q and the probabilities as two or three 16-bit terms; FP32
-//    caches take three TF32 products.  8 heads put two terms into the 16 rows of
-//    one product (high and low sums of a head then sit in the same lane).  The
-//    order of keys and dims inside a product is chosen so that every operand is
-//    a 16-byte shared-memory vector: no shuffles, no transposes.  tcgen05 would
-//    take 8 heads as 128 rows; at 4 * group FLOPs a value the tensor pipe is not
-//    what bounds this kernel.  One or two heads are cheaper as plain FMAs of FP32
-//    (a lane has a part of a key's dims, so only scores are added up across four
-//    lanes).
+//  * Products run on mma.sync: 16-bit cache values go in as they are, FP32 q and
+//    the probabilities as two or three 16-bit terms (16 bits and more for 16-bit
+//    outputs, 22 and more for FP32 ones); of FP32 caches both sides are two TF32
+//    terms (21 bits and more), all four products of which are formed by two
+//    instructions.  8 heads put two terms into the 16 rows of one product (high and
+//    low sums of a head then sit in the same lane).  The order of keys and dims
+//    inside a product is chosen so that every operand is a 16-byte shared-memory
+//    vector: no shuffles, no transposes.  On tcgen05 keys or dims would be the 128
+//    rows and the heads the 8 or 16 columns; up to 8 heads the tensor pipe is not
+//    what bounds this kernel (15 % active with 4), beyond them that form has not
+//    been built.  One or two heads are cheaper as plain FMAs of FP32 (a lane has a
+//    part of a key's dims, so only scores are added up across four lanes).
+//    Relative error of O against 64 bits, 8 x 100..3000 tokens, FP32 q: one head
+//    1.6e-7 to 1.8e-7, 16-bit caches with 4 or 8 heads 1.8e-7 to 2.6e-7, FP32 caches
+//    4.0e-7 to 5.6e-7 (FP32 throughout in PyTorch: 1.9e-7 to 4.5e-7).
 //
 // Device time of a launch on a B200 (floor: the cached values at the 6.53 TB/s
 // of a copy); 32 heads on 8 of 128, bf16, unless it says otherwise:
-//   64 sequences of 4096 tokens            175 us         floor 164
-//   one of 131072                          92.5           82.2
-//   32 on 32 of 64, FP32 q, 16 x 3500..4096 81.9          76.0
-//   64 of 16 .. 4096                       43.9           30.4
-//   FP32, 8 on 8 of 128, 5 x 777..4097     25.0           13.2
-//   f16, 16 on 1 of 64, 128 x 1..16384     28.2           8.7
-//   one of 8192 / 1024 / 64         18.1 / 13.5 / 6.6     5.1 / 0.6 / 0.04
+//   64 sequences of 4096 tokens            174 us         floor 164
+//   one of 131072                          91.5           82.2
+//   32 on 32 of 64, FP32 q, 16 x 3500..4096 82.8          76.0
+//   64 of 16 .. 4096                       44.4           30.4
+//   FP32, 8 on 8 of 128, 5 x 777..4097     24.7           13.2
+//   FP32, 32 on 8 of 64 / 128, 16 / 8 x 4096 60.6 / 60.8  41.1
+//   f16, 16 on 1 of 64, 128 x 1..16384     28.6           8.7
+//   one of 8192 / 1024 / 64         17.9 / 13.0 / 6.5     5.1 / 0.6 / 0.04
 // Long batches run at the copy's rate.  The rest is a fixed chain of latencies:
 // 2 us to start, 2 us for the lengths and the table, 2 to 3 us until the first
 // tile is worked on, 1 us at the end of an item and about 3 us (write, fence,
@@ -134,9 +140,11 @@ struct Cfg {
   // Three CTAs an SM of 168 registers a thread, with two stages of 8 KB or as
   // many smaller ones; two CTAs with three stages where q and O of several heads
   // of 128 dims leave too few registers.  (32 heads on 8 of 128: FP32 q on f16,
-  // 16 x 4096 tokens, 55 us instead of 72, which spilled; bf16, 64 x 16..4096
-  // 43.9 instead of 45.5, 64 x 64 9.7 instead of 11.9, 64 x 4096 174.9 instead of
-  // 173.  Two CTAs at 64 dims: FP32, 32 on 8, 16 x 4096 61.4 instead of 59.4.)
+  // 16 x 4096 tokens, 55 us instead of 72; bf16, 64 x 16..4096 43.9 instead of 45.5,
+  // 64 x 64 9.7 instead of 11.9, 64 x 4096 174.9 instead of 173.  Two CTAs at 64
+  // dims: FP32, 32 on 8, 16 x 4096 61.4 instead of 59.4.)  FP32 q of several heads
+  // still spills a little: 44 (f16), 146 (bf16) and 172 (FP32) bytes a thread at 128
+  // dims with 255 registers, 4 to 74 below, 8 with 16-bit q at 64.
   static constexpr int kCtas = D == 128 && M > 1 ? 2 : 3;
   static constexpr int kRing = kCtas == 3 ? 16384 : 24576;
   static constexpr int kStages = kRing / kStageBytes > 6 ? 6 : kRing / kStageBytes;

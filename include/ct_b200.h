@@ -362,8 +362,9 @@ enum { CT_DTYPE_F32 = 0, CT_DTYPE_BF16 = 1, CT_DTYPE_F16 = 2 };
  * padding: nothing is appended and its q_out and k_out rows are zero.  A token
  * with no place (sequence, page table entry or angle row out of range) is not
  * appended and its q_out and k_out rows are NaN.  Values beyond an f16 cache's
- * range become infinite in it (ct_paged_attention says what follows).  Two tokens with the same place leave either's values
- * there.  No reference counterpart (the reference keeps no cache). */
+ * range become infinite in it (ct_paged_attention says what follows).  Two
+ * tokens with the same place leave a mix of both there.  No reference counterpart
+ * (the reference keeps no cache). */
 int ct_kv_append(const void* q, const int64_t q_stride[3],
                  const void* k, const int64_t k_stride[3],
                  const void* v, const int64_t v_stride[3],
@@ -420,7 +421,7 @@ int ct_paged_attention(const void* q, const int64_t q_stride[3],
  * and count(i) the occurrences of token i in the rest of h:
  *   x = logit(i);  where i occurs in h: x = x > 0 ? x / repetition : x * repetition
  *   x -= frequency * count(i) + presence * (count(i) > 0)
- *   x += bias_values of the row's entries with bias_ids == i
+ *   x += bias_values of the row's entries with bias_ids == i, one by one
  *   x = -inf where bit i % 32 of mask[r][i / 32] is 0
  * tokens NULL: no penalties; repetition, frequency and presence are FP32
  * [rows], NULL: 1, 0 and 0; bias_n entries a row (0: none); mask NULL: none.
