@@ -32,18 +32,23 @@ int check_cache(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_d
   return CT_OK;
 }
 
+// The stride of a dimension of `size` elements: that of a single one says
+// nothing (imported tensors have any value there).
+int64_t stride_of(int64_t size, int64_t stride) { return size > 1 ? stride : 0; }
+
 int fill_cache(PagedKv* kv, const void* k, const int64_t* ks, const void* v, const int64_t* vs,
-               const int32_t* table, int64_t table_s, int64_t pages, int64_t page_size,
-               int64_t max_pages, int dtype) {
-  if (!ks || !vs || (pages > 0 && (!k || !v)) || (max_pages > 0 && !table))
+               const int32_t* table, int64_t table_s, int64_t batch, int64_t kv_heads,
+               int64_t pages, int64_t page_size, int64_t max_pages, int dtype) {
+  if (!ks || !vs || (pages > 0 && (!k || !v)) || (batch > 0 && max_pages > 0 && !table))
     return CT_ERR_INVALID_ARGUMENT;
   if (ks[3] != 1 || vs[3] != 1) return CT_ERR_UNSUPPORTED_LAYOUT;
+  const int64_t sizes[3] = {pages, kv_heads, page_size};
   kv->k = const_cast<void*>(k);
   kv->v = const_cast<void*>(v);
   for (int i = 0; i < 3; ++i) {
-    if (ks[i] < 0 || vs[i] < 0) return CT_ERR_UNSUPPORTED_LAYOUT;
-    kv->ks[i] = ks[i];
-    kv->vs[i] = vs[i];
+    kv->ks[i] = stride_of(sizes[i], ks[i]);
+    kv->vs[i] = stride_of(sizes[i], vs[i]);
+    if (kv->ks[i] < 0 || kv->vs[i] < 0) return CT_ERR_UNSUPPORTED_LAYOUT;
   }
   kv->table = table;
   kv->table_s = table_s;
@@ -79,16 +84,17 @@ int ct_kv_append(const void* q, const int64_t q_stride[3], const void* k, const 
       (rot_dim > 0 && max_positions > 0 && (!cos || !sin)))
     return CT_ERR_INVALID_ARGUMENT;
   KvAppend p{};
-  rc = fill_cache(&p.kv, k_cache, kc_stride, v_cache, vc_stride, block_table, table_stride, pages,
-                  page_size, max_pages, cache_dtype);
+  rc = fill_cache(&p.kv, k_cache, kc_stride, v_cache, vc_stride, block_table, table_stride, batch,
+                  kv_heads, pages, page_size, max_pages, cache_dtype);
   if (rc != CT_OK) return rc;
   p.q = q;
   p.k = k;
   p.v = v;
   for (int i = 0; i < 3; ++i) {
-    p.qs[i] = q_heads > 0 ? q_stride[i] : 0;
-    p.ks[i] = k_stride[i];
-    p.vs[i] = v_stride[i];
+    const int64_t size = i == 0 ? tokens : i == 1 ? kv_heads : head_dim;
+    p.qs[i] = q_heads > 0 ? stride_of(i == 1 ? q_heads : size, q_stride[i]) : 0;
+    p.ks[i] = stride_of(size, k_stride[i]);
+    p.vs[i] = stride_of(size, v_stride[i]);
   }
   if ((q_heads > 0 && p.qs[2] != 1) || p.ks[2] != 1 || p.vs[2] != 1)
     return CT_ERR_UNSUPPORTED_LAYOUT;
@@ -133,19 +139,21 @@ int ct_paged_attention(const void* q, const int64_t q_stride[3], const void* k_c
   if (batch * q_heads == 0) return CT_OK;
   if (!q || !q_stride || !seq_lens || !out || !aligned16(out)) return CT_ERR_INVALID_ARGUMENT;
   PagedAttention p{};
-  rc = fill_cache(&p.kv, k_cache, kc_stride, v_cache, vc_stride, block_table, table_stride, pages,
-                  page_size, max_pages, cache_dtype);
+  rc = fill_cache(&p.kv, k_cache, kc_stride, v_cache, vc_stride, block_table, table_stride, batch,
+                  kv_heads, pages, page_size, max_pages, cache_dtype);
   if (rc != CT_OK) return rc;
   const int64_t align = 16 / dtype_bytes(cache_dtype);
   bool ok = aligned16(k_cache) && aligned16(v_cache);
-  for (int i = 0; i < 3; ++i) ok = ok && kc_stride[i] % align == 0 && vc_stride[i] % align == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && p.kv.ks[i] % align == 0 && p.kv.vs[i] % align == 0;
   if (!ok) return CT_ERR_UNSUPPORTED_LAYOUT;
   if (workspace_bytes < paged_attention_workspace(head_dim) ||
       (workspace_bytes > 0 && !workspace))
     return CT_ERR_WORKSPACE_TOO_SMALL;
   if (!aligned16(workspace)) return CT_ERR_INVALID_ARGUMENT;
   p.q = q;
-  for (int i = 0; i < 3; ++i) p.qs[i] = q_stride[i];
+  p.qs[0] = stride_of(batch, q_stride[0]);
+  p.qs[1] = stride_of(q_heads, q_stride[1]);
+  p.qs[2] = q_stride[2];
   p.seq_lens = seq_lens;
   p.out = out;
   p.lse = lse;

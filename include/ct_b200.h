@@ -343,7 +343,8 @@ enum { CT_DTYPE_F32 = 0, CT_DTYPE_BF16 = 1, CT_DTYPE_F16 = 2 };
 /* A paged cache is a pool of `pages` pages of `page_size` token slots:
  * k_cache and v_cache are indexed [page, kv_head, slot, head_dim] through
  * their element strides (any order of the first three; unit stride along
- * head_dim, no negative strides).  Row s of block_table ([batch, max_pages]
+ * head_dim, no negative strides; those of dimensions of one element are not
+ * looked at).  Row s of block_table ([batch, max_pages]
  * int32, row stride table_stride) lists the pages of sequence s in order:
  * its token j lives in page block_table[s][j / page_size], slot
  * j % page_size.  head_dim in {32, 64, 128};

@@ -159,3 +159,19 @@ def test_rotary_tables_of_an_odd_part_are_refused():
     for rot in (7, -2):
         with pytest.raises(RuntimeError):
             ops.rotary_tables(4, rot)
+
+
+def test_strides_of_single_elements_do_not_matter():
+    """A dimension of one element may have any stride (imported tensors have 1 there), also
+    where others must be multiples of 16 bytes or not negative; a table without rows has no
+    address.  (Accepted up to the workspace, or the device.)"""
+    odd = (ctypes.c_int64 * 4)(1, -3, 64, 1)
+    assert attention(ks=odd, vs=odd, pages=1, kv=1, wsb=0) == cb.CT_ERR_WORKSPACE_TOO_SMALL
+    one = (ctypes.c_int64 * 4)(128, 64, 7, 1)
+    assert attention(ks=one, vs=one, page=1, wsb=0) == cb.CT_ERR_WORKSPACE_TOO_SMALL
+    assert attention(ks=one, vs=one, wsb=0) == cb.CT_ERR_UNSUPPORTED_LAYOUT
+    refused = (cb.CT_ERR_INVALID_ARGUMENT, cb.CT_ERR_UNSUPPORTED_LAYOUT)
+    assert attention(ks=odd, vs=odd, pages=1, kv=2, wsb=0) in refused
+    if not torch.cuda.is_available():   # (the addresses are made up)
+        assert append(kcs=odd, vcs=odd, pages=1, kv=1) not in refused
+        assert append(batch=0, table=None) not in refused

@@ -884,3 +884,34 @@ def test_attention_sums_of_long_sequences(cuda_device, ops, dim):
     for b in (0, batch // 2, batch - 1):
         ref = (q[b].double() @ kk.T * dim ** -0.5).softmax(-1) @ vv
         assert bool(((out[b].double() - ref).abs() <= (2.0 ** -11 + 2.0 ** -15) * ref.abs()).all())
+
+
+def test_strides_of_single_elements(cuda_device, ops):
+    """One page, one key/value head, slots of one, one token, one sequence: their strides say
+    nothing, and the results are those of dense tensors."""
+    g = gen(61)
+    lens = torch.tensor([9], dtype=torch.int32, device="cuda")
+    cos, sin = ops.rotary_tables(16, 64, device="cuda")
+    for pages, kv, page in ((1, 1, 16), (16, 1, 1), (1, 2, 16)):
+        for cache in (F32, BF16):
+            k, v = (torch.randn(pages, kv, page, 64, generator=g, device="cuda").to(cache)
+                    for _ in range(2))
+            table = torch.arange(16 if page == 1 else 1, device="cuda").int()[None]
+            q = torch.randn(1, 4 * kv, 64, generator=g, device="cuda")
+            kn, vn = (torch.randn(1, kv, 64, generator=g, device="cuda") for _ in range(2))
+
+            def odd(t):
+                s = [3 + 2 * i if n == 1 else st for i, (n, st) in enumerate(zip(t.shape, t.stride()))]
+                return torch.as_strided(t, t.shape, s)
+
+            want = ops.paged_attention(q, k, v, table, lens)
+            got = ops.paged_attention(odd(q), odd(k), odd(v), table, lens)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            k2, v2 = k.clone(), v.clone()
+            a = ops.kv_append_(k, v, kn, vn, table, lens, q=q, cos=cos, sin=sin, want_k=True)
+            b = ops.kv_append_(odd(k2), odd(v2), odd(kn), odd(vn), table, lens, q=odd(q), cos=cos,
+                               sin=sin, want_k=True)
+            assert all(torch.equal(x, y) for x, y in zip((*a, k, v), (*b, k2, v2)))
+    q_out, k_out = ops.kv_append_(k, v, kn, vn, torch.zeros(0, 3, dtype=torch.int32, device="cuda"),
+                                  lens, want_k=True)
+    assert k_out.isnan().all()
