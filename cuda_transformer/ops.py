@@ -1,8 +1,10 @@
 """Python wrappers over ``torch.ops.cuda_transformer`` with fake (meta)
 implementations -- the same ten functions, names and argument meaning as the
 reference's ``cuda_transformer/ops.py:4-139``, plus this implementation's
-LayerNorm and precision-explicit variants and the token-generation operators
-(paged key/value cache, one-token attention, logits processing).
+LayerNorm and precision-explicit variants, the token-generation operators
+(paged key/value cache, one-token attention, logits processing) and those of
+speculative decoding (attention of drafted tokens, their verification, moving
+and copying what the cache holds).
 
 ``precision`` (the ``*_ex`` functions): 0 = 3xTF32 (FP32-accurate, the default
 of the plain functions), 1 = TF32, 2 = FP32 on the CUDA cores.  The plain
@@ -22,6 +24,7 @@ __all__ = [
     "linear_fused", "linear_accumulate_", "cross_entropy_fwd_bwd_",
     "kv_append_", "rotary_tables", "paged_attention", "paged_attention_workspace",
     "logits_process",
+    "tree_attention", "verify_drafts", "kv_compact_", "kv_copy_pages_",
 ]
 
 PRECISION_3XTF32 = 0
@@ -307,7 +310,8 @@ def rotary_tables(positions: int, rot: int, base: float = 10000.0, device=None):
 def kv_append_(k_cache: Tensor, v_cache: Tensor, k: Tensor, v: Tensor, block_table: Tensor,
                positions: Tensor, seq_ids: Tensor | None = None, q: Tensor | None = None,
                cos: Tensor | None = None, sin: Tensor | None = None, interleaved: bool = False,
-               want_k: bool = False) -> tuple[Tensor, Tensor]:
+               want_k: bool = False,
+               rotary_positions: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """Appends k, v [tokens, kv_heads, hs] to a paged cache, turning k (and q
     [tokens, nh, hs]) by the rotary angles of their positions on the way.
 
@@ -319,14 +323,17 @@ def kv_append_(k_cache: Tensor, v_cache: Tensor, k: Tensor, v: Tensor, block_tab
     [positions, rot/2] (rotary_tables); element i pairs with i + rot/2, or 2i
     with 2i + 1 when interleaved; None: no rotation.  A negative position is
     padding (nothing appended, zero outputs); a token that has no place in the
-    cache gives NaN outputs.  Returns (turned q, turned k if want_k); unused
+    cache gives NaN outputs.  rotary_positions (int32 [tokens]): the positions
+    that the angles are taken of, where they are not the slots' (a drafted
+    token's depth in its tree).  Returns (turned q, turned k if want_k); unused
     ones are empty."""
     return _kv_append(k_cache, v_cache, k, v, block_table, positions, seq_ids, q, cos, sin,
-                      interleaved, want_k)
+                      interleaved, want_k, rotary_positions)
 
 
 @torch.library.register_fake("cuda_transformer::kv_append_")
-def _(k_cache, v_cache, k, v, block_table, positions, seq_ids, q, cos, sin, interleaved, want_k):
+def _(k_cache, v_cache, k, v, block_table, positions, seq_ids, q, cos, sin, interleaved, want_k,
+      rotary_positions=None):
     _same_device(k, v, k_cache, v_cache, block_table, positions)
     torch._check(k.dtype == v.dtype and k_cache.dtype == v_cache.dtype)
     q_out = q.new_empty(q.shape) if q is not None else k.new_empty(0)
@@ -385,3 +392,100 @@ def logits_process(logits: Tensor, tokens: Tensor | None = None, lens: Tensor | 
 def _(logits, tokens, lens, prompt_lens, repetition, frequency, presence, bias_ids, bias_values,
       mask):
     return logits.new_empty(logits.shape, dtype=torch.float32)
+
+
+# -------------------------------------------------------- speculative decoding
+_tree_attention = torch.ops.cuda_transformer.tree_attention.default
+_verify_drafts = torch.ops.cuda_transformer.verify_drafts.default
+_kv_compact = torch.ops.cuda_transformer.kv_compact_.default
+_kv_copy_pages = torch.ops.cuda_transformer.kv_copy_pages_.default
+
+
+def tree_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
+                   context_lens: Tensor, draft_lens: Tensor | None = None,
+                   mask: Tensor | None = None,
+                   scale: float | None = None) -> tuple[Tensor, Tensor]:
+    """Attention of several new tokens per sequence, q [batch, drafts, nh, hs],
+    over a paged cache (kv_append_'s layout; nh a multiple of kv_heads; cache
+    rows 16-byte aligned).
+
+    context_lens (int32 [batch]): tokens before the new ones; new token i is in
+    the cache at position context_lens[b] + i.  draft_lens (int32 [batch]): how
+    many there are (default: all).  mask (int32 [batch, drafts, ceil(drafts /
+    32)]): new token i sees new token j where bit j % 32 of word j / 32 of its
+    row is set, as a tree's node sees its ancestors and itself; default: all
+    up to itself (a chain, or a piece of a prompt).  The tokens before the new
+    ones are seen by all.  Returns O [batch, drafts, nh, hs] and L = logsumexp
+    [batch, drafts, nh]; rows that are not there or see nothing, and sequences
+    with a negative context_lens, give O = 0, L = -inf; lengths that the table
+    cannot hold give NaN.  scale: hs^-0.5 by default."""
+    s = q.shape[-1] ** -0.5 if scale is None else scale
+    return _tree_attention(q, k_cache, v_cache, block_table, context_lens, draft_lens, mask, s)
+
+
+@torch.library.register_fake("cuda_transformer::tree_attention")
+def _(q, k_cache, v_cache, block_table, context_lens, draft_lens, mask, scale):
+    _same_device(q, k_cache, v_cache, block_table, context_lens)
+    return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+
+def verify_drafts(target: Tensor, tokens: Tensor, parents: Tensor | None = None,
+                  draft_lens: Tensor | None = None, draft_probs: Tensor | None = None,
+                  uniform: Tensor | None = None) -> tuple[Tensor, Tensor, Tensor]:
+    """Which drafted tokens are kept, and the token after them, so that the
+    result is distributed as the target's own tokens.
+
+    A sequence's draft is a tree: node 0 is its last certain token, node i > 0
+    proposes tokens[b, i] (int64 [batch, drafts]) after node parents[b, i] < i
+    (int32 [batch, drafts]; default: i - 1).  draft_lens (int32 [batch]): its
+    nodes (default: all; 0: it takes no part).  target [batch, drafts, vocab]
+    (float32, bfloat16 or float16): the target's probabilities after each node.
+    draft_probs (target's type and shape): the drafter's, which the proposals
+    were drawn from one by one; None: proposals that were certain to be made
+    (looked up, or the drafter's best).  uniform (float32 [batch, drafts]):
+    numbers in [0, 1); those of the nodes decide over them, the one of node 0
+    draws the token after the path.  uniform None: target holds scores (logits)
+    and the best token is kept at each place.
+
+    Returns (new_tokens int64 [batch, drafts], path int32 [batch, drafts],
+    counts int32 [batch]): the path's nodes from node 0 on, counts[b] of them,
+    and the token after each; -1 behind them, and where there is no next token
+    (a row without probabilities, of -inf, with a NaN).  kv_compact_ takes path
+    and counts."""
+    return _verify_drafts(target, tokens, parents, draft_lens, draft_probs, uniform)
+
+
+@torch.library.register_fake("cuda_transformer::verify_drafts")
+def _(target, tokens, parents, draft_lens, draft_probs, uniform):
+    _same_device(target, tokens)
+    return (tokens.new_empty(tokens.shape), tokens.new_empty(tokens.shape, dtype=torch.int32),
+            tokens.new_empty(tokens.shape[:1], dtype=torch.int32))
+
+
+def kv_compact_(caches: list[Tensor], block_table: Tensor, context_lens: Tensor, keep: Tensor,
+                counts: Tensor) -> None:
+    """Moves the kept ones of the last tokens up, in all of `caches` (keys and
+    values of any layers, of one shape and type, kv_append_'s layout): what is
+    at position context_lens[b] + keep[b, j] goes to context_lens[b] + j, for
+    j < counts[b].  keep (int32 [batch, n]) ascends along a row; context_lens,
+    counts: int32 [batch].  verify_drafts gives path and counts to pass here;
+    any other choice of tokens to keep is made the same way.  A move without a
+    place in the cache is left out."""
+    _kv_compact(caches, block_table, context_lens, keep, counts)
+
+
+@torch.library.register_fake("cuda_transformer::kv_compact_")
+def _(caches, block_table, context_lens, keep, counts):
+    return None
+
+
+def kv_copy_pages_(caches: list[Tensor], src: Tensor, dst: Tensor) -> None:
+    """Copies page src[i] to page dst[i] (int32 [n]) in all of `caches` (of one
+    shape and type, kv_append_'s layout).  No dst may be among src or twice.  A
+    pair with a page out of range is left out."""
+    _kv_copy_pages(caches, src, dst)
+
+
+@torch.library.register_fake("cuda_transformer::kv_copy_pages_")
+def _(caches, src, dst):
+    return None

@@ -35,6 +35,8 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
 CT_FA2_BWD_NOALLOC_MAX_ROWS = 2097152  # batch * heads * seq_len limit of ct_fa2_bwd_noalloc
+CT_TREE_ATTENTION_MAX_DRAFTS = 16384
+CT_VERIFY_DRAFTS_MAX = 1024
 CT_DEVSTAT_TIMEOUT = 1  # watchdog word bit: a bounded device-side wait ran out
 CT_WAIT_LIMIT_MIN_NS = 100000
 CT_WAIT_LIMIT_MAX_NS = 60000000000
@@ -85,12 +87,25 @@ SIGNATURES = {
     "ct_kv_append": ([_fp, _i64p, _fp, _i64p, _fp, _i64p, _fp, _fp, _fp, _fp, _fp, _i64p, _fp,
                       _i64p, _fp, _i64, _fp, _fp, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64,
                       _i64, _i64, _i64, _int, _int, _fp], _int),
+    "ct_kv_append_ex": ([_fp, _i64p, _fp, _i64p, _fp, _i64p, _fp, _fp, _fp, _fp, _fp, _i64p, _fp,
+                         _i64p, _fp, _i64, _fp, _fp, _fp, _i64, _i64, _i64, _i64, _i64, _int, _i64,
+                         _i64, _i64, _i64, _i64, _int, _int, _fp], _int),
     "ct_paged_attention_workspace_size": ([_i64, _i64, _i64], _sz),
     "ct_paged_attention": ([_fp, _i64p, _fp, _i64p, _fp, _i64p, _fp, _i64, _fp, _fp, _fp, _i64,
                             _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _int, _int, _fp,
                             _sz, _fp], _int),
     "ct_logits_process": ([_fp, _i64, _int, _fp, _i64, _i64, _i64, _fp, _i64, _i64, _fp, _fp, _fp,
                            _fp, _fp, _fp, _i64, _fp, _i64, _i64, _fp, _i64, _fp], _int),
+    "ct_tree_attention_workspace_size": ([_i64, _i64, _i64, _i64], _sz),
+    "ct_tree_attention": ([_fp, _i64p, _fp, _i64p, _fp, _i64p, _fp, _i64, _fp, _fp, _fp, _i64p,
+                           _fp, _fp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                           ctypes.c_float, _int, _int, _fp, _sz, _fp], _int),
+    "ct_verify_drafts": ([_fp, _i64p, _fp, _i64p, _int, _fp, _i64, _fp, _i64, _fp, _fp, _i64, _fp,
+                          _fp, _fp, _i64, _i64, _i64, _fp], _int),
+    "ct_kv_compact": ([ctypes.POINTER(_fp), _i64p, _i64, _fp, _i64, _fp, _fp, _i64, _fp, _i64,
+                       _i64, _i64, _i64, _i64, _i64, _i64, _int, _fp], _int),
+    "ct_kv_copy_pages": ([ctypes.POINTER(_fp), _i64p, _i64, _fp, _fp, _i64, _i64, _i64, _i64, _i64,
+                          _int, _fp], _int),
     "ct_set_wait_limit_ns": ([_int, ctypes.c_ulonglong], _int),
     "ct_get_wait_limit_ns": ([_int, ctypes.POINTER(ctypes.c_ulonglong)], _int),
     "ct_watchdog_selftest": ([_fp], _int),

@@ -197,6 +197,7 @@ struct KvAppend {
   const float *cos, *sin;
   PagedKv kv;
   const int32_t *seq_ids, *positions;
+  const int32_t* rotary_positions;  // nullptr: positions
   int64_t tokens, q_heads, kv_heads, batch, max_positions;
   int head_dim, rot_dim, act_dtype;
   bool interleaved;
@@ -232,6 +233,66 @@ struct LogitsProcess {
   int dtype;
 };
 int launch_logits_process(const LogitsProcess& p, const DeviceInfo& dev, cudaStream_t st);
+
+// ------------------------------------- speculative decoding (drafted tokens)
+struct TreeAttention {
+  const void* q;
+  int64_t qs[4];  // sequence, drafted token, head, dim
+  PagedKv kv;
+  const int32_t *context_lens, *draft_lens;
+  const uint32_t* mask;
+  int64_t ms[2];  // sequence, drafted token
+  void* out;
+  float* lse;
+  int64_t batch, drafts, q_heads, kv_heads;
+  int head_dim, act_dtype;
+  float scale;
+  void* ws;
+};
+size_t tree_attention_workspace(int64_t drafts, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim);
+int launch_tree_attention(const TreeAttention& p, const DeviceInfo& dev, cudaStream_t st);
+struct VerifyDrafts {
+  const void *target, *draft_probs;
+  int64_t ts[2], ds[2];  // sequence, node
+  const int64_t* tokens;
+  int64_t tokens_ld;
+  const int32_t* parents;
+  int64_t parents_ld;
+  const int32_t* draft_lens;
+  const float* uniform;
+  int64_t uniform_ld;
+  int64_t* new_tokens;
+  int32_t *path, *counts;
+  int64_t batch, drafts, vocab;
+  int dtype;
+};
+constexpr int64_t kMostDrafts = 1024;  // nodes of a tree that verify_drafts takes
+int launch_verify_drafts(const VerifyDrafts& p, const DeviceInfo& dev, cudaStream_t st);
+// Several caches of one shape, [page, kv_head, slot, head_dim]; the most that
+// one launch takes.
+constexpr int kMostCaches = 64;
+struct CacheList {
+  int n;
+  void* base[kMostCaches];
+  int64_t s[kMostCaches][3];  // page, head, slot strides (elements)
+};
+struct KvCompact {
+  CacheList caches;
+  const int32_t* table;
+  int64_t table_s, batch, kv_heads, pages, max_pages, drafts;
+  const int32_t *context_lens, *keep, *counts;
+  int64_t keep_ld;
+  int page_size, head_dim, dtype;
+};
+int launch_kv_compact(const KvCompact& p, const DeviceInfo& dev, cudaStream_t st);
+struct KvCopyPages {
+  CacheList caches;
+  const int32_t *src, *dst;
+  int64_t count, kv_heads, pages;
+  int page_size, head_dim, dtype;
+};
+int launch_kv_copy_pages(const KvCopyPages& p, const DeviceInfo& dev, cudaStream_t st);
 
 // ------------------------------------------------------------ watchdog
 // One CTA whose waits on a barrier phase that nothing completes run out after

@@ -140,12 +140,14 @@ __global__ void __launch_bounds__(kThreads, 6)
   // a negative position marks a padding token; one that has no place in the
   // cache (or no row in the table of angles) gives NaN
   const bool pad = pos < 0;
-  bool bad = !pad && (seq < 0 || seq >= p.batch || pos >= p.max_positions);
+  // (a drafted token's angles are those of its depth in the tree, not of its slot)
+  const int angle = p.rotary_positions ? p.rotary_positions[t] : pos;
+  bool bad = !pad && (seq < 0 || seq >= p.batch || angle < 0 || angle >= p.max_positions);
   const bool angles = !pad && !bad && turns;
   Pack<float, VEC> cs{}, sn{};
   if (angles) {
-    cs = pack<VEC>(p.cos + (int64_t)pos * hr + first);
-    sn = pack<VEC>(p.sin + (int64_t)pos * hr + first);
+    cs = pack<VEC>(p.cos + (int64_t)angle * hr + first);
+    sn = pack<VEC>(p.sin + (int64_t)angle * hr + first);
   }
   int page = 0, slot = 0;
   if (!pad && !bad) {

@@ -1,0 +1,226 @@
+// kv_pages.cu -- what a cache holds, moved about inside it: the kept ones of a
+// sequence's last tokens move up (kv_compact), pages are copied (kv_copy_pages).
+// Both work on all caches of a list (keys and values of every layer) at once.
+//
+// Bound by HBM: every moved value is read once and written once.  A thread
+// moves 16 bytes at a time of one cache, head and place in the row (a column);
+// where rows are not aligned to that, one element.
+#include "decode_common.cuh"
+
+namespace ct {
+namespace {
+
+constexpr int kThreads = 256;
+// Moves of a thread that are on the way at once.
+constexpr int kMoves = 8;
+
+struct Columns {
+  int row_units;   // of a head's row
+  uint32_t count;  // units of a token: caches * heads * row_units
+  uint32_t blocks;  // CTAs for them
+};
+
+// A column's base address and strides in units of T.
+template <class T>
+struct Column {
+  T* base;
+  int64_t page, slot;
+};
+template <class T>
+__device__ __forceinline__ Column<T> column(const CacheList& caches, int heads, int row_units,
+                                            int bytes, uint32_t c) {
+  const uint32_t unit = c % (uint32_t)row_units, row = c / (uint32_t)row_units;
+  const uint32_t head = row % (uint32_t)heads, t = row / (uint32_t)heads;
+  char* base = (char*)caches.base[t] + head * caches.s[t][1] * bytes;
+  return {(T*)base + unit, caches.s[t][0] * bytes / (int64_t)sizeof(T),
+          caches.s[t][2] * bytes / (int64_t)sizeof(T)};
+}
+
+struct Place {
+  int page, slot;  // page < 0: none
+};
+__device__ __forceinline__ Place place_of(const KvCompact& p, int64_t b, int64_t position) {
+  Place at{-1, 0};
+  if (position < 0 || position >= p.max_pages * p.page_size) return at;
+  const int index = (int)position / p.page_size;
+  const int page = p.table[b * p.table_s + index];
+  if (page >= 0 && page < p.pages) at = {page, (int)position - index * p.page_size};
+  return at;
+}
+
+// Drafts of at most this many tokens: a thread makes all moves of its column,
+// kMoves at a time in their order, which is safe as the kept ones ascend (what a
+// later move reads lies behind what the earlier ones wrote).
+constexpr int kShortDraft = 64;
+
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+    compact_short_kernel(const __grid_constant__ KvCompact p, const Columns cols, const int bytes) {
+  __shared__ Place from[kShortDraft], to[kShortDraft];
+  __shared__ int listed;
+  const int64_t b = blockIdx.x / cols.blocks;
+  const int base = p.context_lens[b];
+  int n = p.counts[b];
+  n = n > p.drafts ? (int)p.drafts : n;
+  if (base < 0 || n <= 0) return;
+  if (threadIdx.x < 32) {  // the moves that there are, in their order
+    int found = 0;
+    for (int j0 = 0; j0 < n; j0 += 32) {
+      const int j = j0 + threadIdx.x, k = j < n ? p.keep[b * p.keep_ld + j] : 0;
+      Place src{-1, 0}, dst{-1, 0};
+      if (j < n && k > j) {
+        src = place_of(p, b, (int64_t)base + k);
+        dst = place_of(p, b, (int64_t)base + j);
+      }
+      const bool moves = src.page >= 0 && dst.page >= 0;
+      const uint32_t vote = __ballot_sync(0xffffffffu, moves);
+      if (moves) {
+        const int at = found + __popc(vote & ((1u << threadIdx.x) - 1));
+        from[at] = src;
+        to[at] = dst;
+      }
+      found += __popc(vote);
+    }
+    if (threadIdx.x == 0) listed = found;
+  }
+  __syncthreads();
+  const uint32_t c = blockIdx.x % cols.blocks * kThreads + threadIdx.x;
+  if (c >= cols.count) return;
+  const Column<T> col = column<T>(p.caches, (int)p.kv_heads, cols.row_units, bytes, c);
+  const int moves = listed;
+  for (int j0 = 0; j0 < moves; j0 += kMoves) {
+    T x[kMoves];
+#pragma unroll
+    for (int k = 0; k < kMoves; ++k)
+      if (j0 + k < moves) x[k] = col.base[from[j0 + k].page * col.page + from[j0 + k].slot * col.slot];
+#pragma unroll
+    for (int k = 0; k < kMoves; ++k)
+      if (j0 + k < moves) col.base[to[j0 + k].page * col.page + to[j0 + k].slot * col.slot] = x[k];
+  }
+}
+
+// Longer drafts: place x takes the value of place keep[x], which then takes that
+// of keep[keep[x]], and so on up to a place that nothing moves to.  Such chains
+// have no place in common (keep ascends, so no place is kept twice), and each
+// begins at a place that is not kept itself.  So the chains run in parallel, a
+// thread following one of them for its column.  keep[x] > x along a chain
+// whatever keep holds, so each of them ends.
+constexpr int kPlaces = 64;  // of a CTA
+
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+    compact_long_kernel(const __grid_constant__ KvCompact p, const Columns cols, const int bytes,
+                        const uint32_t pieces) {
+  __shared__ int starts[kPlaces], listed;
+  const uint32_t piece = blockIdx.x / cols.blocks;
+  const int64_t b = piece / pieces;
+  const int base = p.context_lens[b];
+  const int n = p.counts[b] > p.drafts ? (int)p.drafts : p.counts[b];
+  const int x0 = (int)(piece - b * pieces) * kPlaces;
+  if (base < 0 || x0 >= n) return;
+  const int32_t* keep = p.keep + b * p.keep_ld;
+  if (threadIdx.x == 0) listed = 0;
+  __syncthreads();
+  if (threadIdx.x < kPlaces && x0 + (int)threadIdx.x < n) {
+    const int x = x0 + threadIdx.x;
+    int low = 0, high = x;  // keep[j] >= j: x is kept as one of the first x + 1, if at all
+    while (low < high) {
+      const int mid = (low + high) / 2;
+      if (keep[mid] < x) low = mid + 1; else high = mid;
+    }
+    if (keep[low] != x && keep[x] > x) starts[atomicAdd(&listed, 1)] = x;
+  }
+  __syncthreads();
+  const uint32_t c = blockIdx.x % cols.blocks * kThreads + threadIdx.x;
+  if (c >= cols.count) return;
+  const Column<T> col = column<T>(p.caches, (int)p.kv_heads, cols.row_units, bytes, c);
+  const int chains = listed;
+  for (int s = 0; s < chains; ++s) {
+    int x = starts[s];
+    Place to = place_of(p, b, (int64_t)base + x);
+    while (x < n) {
+      const int k = keep[x];
+      if (k <= x) break;
+      const Place from = place_of(p, b, (int64_t)base + k);
+      if (to.page >= 0 && from.page >= 0)
+        col.base[to.page * col.page + to.slot * col.slot] =
+            col.base[from.page * col.page + from.slot * col.slot];
+      to = from;
+      x = k;
+    }
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+    copy_pages_kernel(const __grid_constant__ KvCopyPages p, const Columns cols, const int bytes) {
+  const int64_t i = blockIdx.x / cols.blocks;
+  const int src = p.src[i], dst = p.dst[i];
+  if (src < 0 || src >= p.pages || dst < 0 || dst >= p.pages) return;
+  const uint32_t c = blockIdx.x % cols.blocks * kThreads + threadIdx.x;
+  if (c >= cols.count) return;
+  const Column<T> col = column<T>(p.caches, (int)p.kv_heads, cols.row_units, bytes, c);
+  for (int64_t slot = 0; slot < p.page_size; ++slot)
+    col.base[dst * col.page + slot * col.slot] = col.base[src * col.page + slot * col.slot];
+}
+
+// Whether the rows of all caches are whole 16-byte vectors.
+bool rows_of_vectors(const CacheList& caches, int head_dim, int bytes) {
+  bool ok = head_dim * bytes % 16 == 0;
+  for (int t = 0; t < caches.n; ++t) {
+    ok = ok && aligned16(caches.base[t]);
+    for (int i = 0; i < 3; ++i) ok = ok && caches.s[t][i] * bytes % 16 == 0;
+  }
+  return ok;
+}
+
+// f with the type of a unit (16 bytes, or an element) and the columns.
+template <class P, class F>
+int with_units(const P& p, F&& f) {
+  const int bytes = dtype_bytes(p.dtype);
+  const bool vectors = rows_of_vectors(p.caches, p.head_dim, bytes);
+  Columns cols;
+  cols.row_units = vectors ? p.head_dim * bytes / 16 : p.head_dim;
+  const int64_t count = p.caches.n * p.kv_heads * cols.row_units;
+  if (count >= 1ll << 32) return CT_ERR_INVALID_ARGUMENT;
+  cols.count = (uint32_t)count;
+  cols.blocks = (uint32_t)((count + kThreads - 1) / kThreads);
+  if (vectors) return f(uint4{}, cols, bytes);
+  if (bytes == 4) return f(uint32_t{}, cols, bytes);
+  return f(uint16_t{}, cols, bytes);
+}
+
+// The CTAs of `n` pieces of work, `each` a piece (0: more than a grid has).
+unsigned grid_of(int64_t n, int64_t each) {
+  return n * each < 1ll << 31 ? (unsigned)(n * each) : 0u;
+}
+
+}  // namespace
+
+int launch_kv_compact(const KvCompact& p, const DeviceInfo&, cudaStream_t st) {
+  return with_units(p, [&](auto unit, const Columns& cols, int bytes) {
+    using T = decltype(unit);
+    const bool is_short = p.drafts <= kShortDraft;
+    const int64_t pieces = is_short ? 1 : (p.drafts + kPlaces - 1) / kPlaces;
+    if (p.batch * pieces >= 1ll << 31) return (int)CT_ERR_INVALID_ARGUMENT;
+    const unsigned grid = grid_of(p.batch * pieces, cols.blocks);
+    if (grid == 0) return (int)CT_ERR_INVALID_ARGUMENT;
+    if (is_short)
+      compact_short_kernel<T><<<grid, kThreads, 0, st>>>(p, cols, bytes);
+    else
+      compact_long_kernel<T><<<grid, kThreads, 0, st>>>(p, cols, bytes, (uint32_t)pieces);
+    return check_launch();
+  });
+}
+
+int launch_kv_copy_pages(const KvCopyPages& p, const DeviceInfo&, cudaStream_t st) {
+  return with_units(p, [&](auto unit, const Columns& cols, int bytes) {
+    using T = decltype(unit);
+    const unsigned grid = grid_of(p.count, cols.blocks);
+    if (grid == 0) return (int)CT_ERR_INVALID_ARGUMENT;
+    copy_pages_kernel<T><<<grid, kThreads, 0, st>>>(p, cols, bytes);
+    return check_launch();
+  });
+}
+
+}  // namespace ct

@@ -25,6 +25,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "ct_b200.h"
 
@@ -511,7 +512,8 @@ std::tuple<Tensor, Tensor> kv_append_(Tensor k_cache, Tensor v_cache, Tensor k0,
                                       Tensor table0, Tensor positions,
                                       std::optional<Tensor> seq_ids0, std::optional<Tensor> q0,
                                       std::optional<Tensor> cos0, std::optional<Tensor> sin0,
-                                      bool interleaved, bool want_k) {
+                                      bool interleaved, bool want_k,
+                                      std::optional<Tensor> rotary_positions0) {
   const CacheArgs c = check_cache(k_cache, v_cache, table0, k0);
   const int act = dtype_code(k0, "k");
   check_on(v0, k0, k0.scalar_type(), "v");
@@ -522,9 +524,11 @@ std::tuple<Tensor, Tensor> kv_append_(Tensor k_cache, Tensor v_cache, Tensor k0,
   c10::cuda::CUDAGuard guard(k0.device());
   const int64_t tokens = k0.size(0);
   const Tensor k = unit_last(k0), v = unit_last(v0);
-  Tensor keep_pos, keep_seq, q, cos, sin;
+  Tensor keep_pos, keep_seq, keep_rotary, q, cos, sin;
   const int32_t* pos = vector_of<int32_t>(positions, tokens, k, at::kInt, "positions", &keep_pos);
   const int32_t* seq = vector_of<int32_t>(seq_ids0, tokens, k, at::kInt, "seq_ids", &keep_seq);
+  const int32_t* rotary = vector_of<int32_t>(rotary_positions0, tokens, k, at::kInt,
+                                             "rotary_positions", &keep_rotary);
   int64_t q_heads = 0, rot = 0, max_positions = 0;
   int64_t qs[3] = {0, 0, 1}, ks[3], vs[3], kcs[4], vcs[4];
   if (q0.has_value()) {
@@ -554,13 +558,13 @@ std::tuple<Tensor, Tensor> kv_append_(Tensor k_cache, Tensor v_cache, Tensor k0,
   strides3(v, vs);
   strides4(k_cache, kcs);
   strides4(v_cache, vcs);
-  check_rc(ct_kv_append(q_heads ? q.const_data_ptr() : nullptr, qs, k.const_data_ptr(), ks,
+  check_rc(ct_kv_append_ex(q_heads ? q.const_data_ptr() : nullptr, qs, k.const_data_ptr(), ks,
                         v.const_data_ptr(), vs, q_heads ? q_out.data_ptr() : nullptr,
                         want_k ? k_out.data_ptr() : nullptr,
                         rot ? cos.const_data_ptr<float>() : nullptr,
                         rot ? sin.const_data_ptr<float>() : nullptr, k_cache.data_ptr(), kcs,
                         v_cache.data_ptr(), vcs, c.table.const_data_ptr<int32_t>(),
-                        c.table.stride(0), seq, pos, tokens, q_heads, c.heads, c.dim, rot,
+                        c.table.stride(0), seq, pos, rotary, tokens, q_heads, c.heads, c.dim, rot,
                         interleaved ? 1 : 0, max_positions, c.batch, c.pages, c.page_size,
                         c.max_pages, act, c.dtype, cur_stream()),
            "kv_append_");
@@ -661,6 +665,170 @@ Tensor logits_process(Tensor logits0, std::optional<Tensor> tokens0, std::option
   return out;
 }
 
+// ------------------------------------------------------ speculative decoding
+std::tuple<Tensor, Tensor> tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor table,
+                                          Tensor context_lens0, std::optional<Tensor> draft_lens0,
+                                          std::optional<Tensor> mask0, double scale) {
+  const CacheArgs c = check_cache(k_cache, v_cache, table, q);
+  const int act = dtype_code(q, "q");
+  TORCH_CHECK(act == c.dtype || act == CT_DTYPE_F32, "q must be float32 or of the cache's type");
+  TORCH_CHECK(q.dim() == 4 && q.size(3) == c.dim, "q must be [batch, drafts, nh, hs]");
+  TORCH_CHECK(q.size(0) == c.batch, "block_table must have a row for each sequence of q");
+  c10::cuda::CUDAGuard guard(q.device());
+  const int64_t batch = q.size(0), drafts = q.size(1), heads = q.size(2);
+  Tensor keep_context, keep_drafts, mask;
+  const int32_t* context =
+      vector_of<int32_t>(context_lens0, batch, q, at::kInt, "context_lens", &keep_context);
+  const int32_t* lens =
+      vector_of<int32_t>(draft_lens0, batch, q, at::kInt, "draft_lens", &keep_drafts);
+  int64_t ms[2] = {0, 0};
+  if (mask0.has_value()) {
+    mask = *mask0;
+    check_on(mask, q, at::kInt, "mask");
+    TORCH_CHECK(mask.dim() == 3 && mask.size(0) == batch && mask.size(1) == drafts &&
+                    mask.size(2) >= (drafts + 31) / 32,
+                "mask must be [batch, drafts, ceil(drafts / 32)]");
+    if (mask.stride(2) != 1 && mask.size(2) > 1) mask = mask.contiguous();
+    ms[0] = mask.stride(0);
+    ms[1] = mask.stride(1);
+  }
+  const int64_t need = ct_tree_attention_workspace_size(drafts, heads, c.heads, c.dim);
+  // (no counters in it: nothing to clear, and a captured call has its own)
+  Tensor ws = empty_like_of({need}, at::kByte, q);
+  Tensor out = empty_like_of({batch, drafts, heads, c.dim}, q.scalar_type(), q);
+  Tensor lse = empty_like_of({batch, drafts, heads}, at::kFloat, q);
+  int64_t qs[4], kcs[4], vcs[4];
+  strides4(q, qs);
+  strides4(k_cache, kcs);
+  strides4(v_cache, vcs);
+  check_rc(ct_tree_attention(q.const_data_ptr(), qs, k_cache.const_data_ptr(), kcs,
+                             v_cache.const_data_ptr(), vcs, c.table.const_data_ptr<int32_t>(),
+                             c.table.stride(0), context, lens,
+                             mask.defined() ? mask.const_data_ptr<int32_t>() : nullptr, ms,
+                             out.data_ptr(), lse.data_ptr<float>(), batch, drafts, heads, c.heads,
+                             c.dim, c.pages, c.page_size, c.max_pages, (float)scale, act, c.dtype,
+                             ws.data_ptr(), (size_t)need, cur_stream()),
+           "tree_attention");
+  return {out, lse};
+}
+
+// [batch, nodes, vocab] with unit stride along the last (copied once otherwise).
+Tensor node_rows(const Tensor& t, const Tensor& first, at::ScalarType type, const char* name) {
+  check_on(t, first, type, name);
+  TORCH_CHECK(t.dim() == 3 && t.sizes() == first.sizes(), name,
+              " must be [batch, drafts, vocab], as target");
+  return t.stride(2) == 1 || t.size(2) <= 1 ? t : t.contiguous();
+}
+
+std::tuple<Tensor, Tensor, Tensor> verify_drafts(Tensor target0, Tensor tokens0,
+                                                 std::optional<Tensor> parents0,
+                                                 std::optional<Tensor> draft_lens0,
+                                                 std::optional<Tensor> draft_probs0,
+                                                 std::optional<Tensor> uniform0) {
+  TORCH_CHECK(target0.is_cuda(), "target must be a CUDA tensor");
+  const int dtype = dtype_code(target0, "target");
+  const Tensor target = node_rows(target0, target0, target0.scalar_type(), "target");
+  c10::cuda::CUDAGuard guard(target.device());
+  const int64_t batch = target.size(0), drafts = target.size(1), vocab = target.size(2);
+  TORCH_CHECK(!draft_probs0.has_value() || uniform0.has_value(), "draft_probs needs uniform");
+  auto of_nodes = [&](const Tensor& t, at::ScalarType type, const char* name) {
+    Tensor m = matrix_of(t, batch, target, type, name);
+    TORCH_CHECK(m.size(1) == drafts, name, " must be [batch, drafts]");
+    return m;
+  };
+  const Tensor tokens = of_nodes(tokens0, at::kLong, "tokens");
+  Tensor parents, uniform, draft_probs, keep_lens;
+  if (parents0.has_value()) parents = of_nodes(*parents0, at::kInt, "parents");
+  if (uniform0.has_value()) uniform = of_nodes(*uniform0, at::kFloat, "uniform");
+  if (draft_probs0.has_value())
+    draft_probs = node_rows(*draft_probs0, target, target.scalar_type(), "draft_probs");
+  const int32_t* lens =
+      vector_of<int32_t>(draft_lens0, batch, target, at::kInt, "draft_lens", &keep_lens);
+  Tensor new_tokens = empty_like_of({batch, drafts}, at::kLong, target);
+  Tensor path = empty_like_of({batch, drafts}, at::kInt, target);
+  Tensor counts = empty_like_of({batch}, at::kInt, target);
+  const int64_t ts[2] = {target.stride(0), target.stride(1)};
+  int64_t ds[2] = {0, 0};
+  if (draft_probs.defined()) {
+    ds[0] = draft_probs.stride(0);
+    ds[1] = draft_probs.stride(1);
+  }
+  check_rc(ct_verify_drafts(target.const_data_ptr(), ts,
+                            draft_probs.defined() ? draft_probs.const_data_ptr() : nullptr, ds,
+                            dtype, tokens.const_data_ptr<int64_t>(), tokens.stride(0),
+                            parents.defined() ? parents.const_data_ptr<int32_t>() : nullptr,
+                            parents.defined() ? parents.stride(0) : 0, lens,
+                            uniform.defined() ? uniform.const_data_ptr<float>() : nullptr,
+                            uniform.defined() ? uniform.stride(0) : 0,
+                            new_tokens.data_ptr<int64_t>(), path.data_ptr<int32_t>(),
+                            counts.data_ptr<int32_t>(), batch, drafts, vocab, cur_stream()),
+           "verify_drafts");
+  return {new_tokens, path, counts};
+}
+
+// A list of caches of one shape and type, as the C ABI takes it.
+struct CacheTensors {
+  std::vector<void*> base;
+  std::vector<int64_t> strides;
+  int64_t pages = 0, heads = 1, page_size = 1, dim = 1;
+  int dtype = CT_DTYPE_F32;
+};
+
+CacheTensors cache_tensors(at::TensorList caches) {
+  CacheTensors c;
+  for (const Tensor& t : caches) {
+    TORCH_CHECK(t.is_cuda(), "caches must be CUDA tensors");
+    check_on(t, caches[0], caches[0].scalar_type(), "caches");
+    TORCH_CHECK(t.dim() == 4 && t.sizes() == caches[0].sizes(),
+                "caches must be [pages, kv_heads, page_size, hs] of equal shape");
+    TORCH_CHECK(t.stride(3) == 1, "caches must have unit stride along hs");
+    c.base.push_back(t.data_ptr());
+    for (int i = 0; i < 4; ++i) c.strides.push_back(t.stride(i));
+  }
+  if (!caches.empty()) {
+    c.pages = caches[0].size(0);
+    c.heads = caches[0].size(1);
+    c.page_size = caches[0].size(2);
+    c.dim = caches[0].size(3);
+    c.dtype = dtype_code(caches[0], "caches");
+  }
+  return c;
+}
+
+void kv_compact_(at::TensorList caches, Tensor table0, Tensor context_lens0, Tensor keep0,
+                 Tensor counts0) {
+  TORCH_CHECK(!caches.empty(), "caches must not be an empty list");
+  const CacheTensors c = cache_tensors(caches);
+  c10::cuda::CUDAGuard guard(caches[0].device());
+  const int64_t batch = table0.size(0);
+  const Tensor table = matrix_of(table0, batch, caches[0], at::kInt, "block_table");
+  const Tensor keep = matrix_of(keep0, batch, caches[0], at::kInt, "keep");
+  Tensor keep_context, keep_counts;
+  const int32_t* context = vector_of<int32_t>(context_lens0, batch, caches[0], at::kInt,
+                                              "context_lens", &keep_context);
+  const int32_t* counts =
+      vector_of<int32_t>(counts0, batch, caches[0], at::kInt, "counts", &keep_counts);
+  check_rc(ct_kv_compact(c.base.data(), c.strides.data(), (int64_t)c.base.size(),
+                         table.const_data_ptr<int32_t>(), table.stride(0), context,
+                         keep.const_data_ptr<int32_t>(), keep.stride(0), counts, batch,
+                         keep.size(1), c.heads, c.dim, c.pages, c.page_size, table.size(1),
+                         c.dtype, cur_stream()),
+           "kv_compact_");
+}
+
+void kv_copy_pages_(at::TensorList caches, Tensor src0, Tensor dst0) {
+  TORCH_CHECK(!caches.empty(), "caches must not be an empty list");
+  const CacheTensors c = cache_tensors(caches);
+  c10::cuda::CUDAGuard guard(caches[0].device());
+  const int64_t n = src0.numel();
+  Tensor keep_src, keep_dst;
+  const int32_t* src = vector_of<int32_t>(src0, n, caches[0], at::kInt, "src", &keep_src);
+  const int32_t* dst = vector_of<int32_t>(dst0, n, caches[0], at::kInt, "dst", &keep_dst);
+  check_rc(ct_kv_copy_pages(c.base.data(), c.strides.data(), (int64_t)c.base.size(), src, dst, n,
+                            c.heads, c.dim, c.pages, c.page_size, c.dtype, cur_stream()),
+           "kv_copy_pages_");
+}
+
 // ------------------------------------------- materialised (naive) attention
 // Kept registered so cuda_autograd_fns imports; composed from this library's
 // own GEMM and softmax kernels.  qkv: (B, T, 3C) contiguous.
@@ -735,10 +903,14 @@ TORCH_LIBRARY(cuda_transformer, m) {
   m.def("linear_fused(Tensor x, Tensor weights, Tensor bias, int precision, int epilogue, Tensor? act_in, bool want_colsum) -> (Tensor, Tensor, Tensor)");
   m.def("linear_accumulate_(Tensor(a!) out, Tensor(b!)? colsum, Tensor x, Tensor weights, Tensor bias, int precision) -> ()");
   m.def("cross_entropy_fwd_bwd_(Tensor(a!) logits, Tensor targets, int ignore_index) -> Tensor");
-  m.def("kv_append_(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor k, Tensor v, Tensor block_table, Tensor positions, Tensor? seq_ids, Tensor? q, Tensor? cos, Tensor? sin, bool interleaved, bool want_k) -> (Tensor, Tensor)");
+  m.def("kv_append_(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor k, Tensor v, Tensor block_table, Tensor positions, Tensor? seq_ids, Tensor? q, Tensor? cos, Tensor? sin, bool interleaved, bool want_k, Tensor? rotary_positions=None) -> (Tensor, Tensor)");
   m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, float scale, Tensor(a!)? workspace) -> (Tensor, Tensor)");
   m.def("paged_attention_workspace_size(int nh, int kv_heads, int hs) -> int", &paged_attention_workspace_size);
   m.def("logits_process(Tensor logits, Tensor? tokens, Tensor? lens, Tensor? prompt_lens, Tensor? repetition, Tensor? frequency, Tensor? presence, Tensor? bias_ids, Tensor? bias_values, Tensor? mask) -> Tensor");
+  m.def("tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor context_lens, Tensor? draft_lens, Tensor? mask, float scale) -> (Tensor, Tensor)");
+  m.def("verify_drafts(Tensor target, Tensor tokens, Tensor? parents, Tensor? draft_lens, Tensor? draft_probs, Tensor? uniform) -> (Tensor, Tensor, Tensor)");
+  m.def("kv_compact_(Tensor(a!)[] caches, Tensor block_table, Tensor context_lens, Tensor keep, Tensor counts) -> ()");
+  m.def("kv_copy_pages_(Tensor(a!)[] caches, Tensor src, Tensor dst) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(cuda_transformer, CUDA, m) {
@@ -763,6 +935,10 @@ TORCH_LIBRARY_IMPL(cuda_transformer, CUDA, m) {
   m.impl("kv_append_", &kv_append_);
   m.impl("paged_attention", &paged_attention);
   m.impl("logits_process", &logits_process);
+  m.impl("tree_attention", &tree_attention);
+  m.impl("verify_drafts", &verify_drafts);
+  m.impl("kv_compact_", &kv_compact_);
+  m.impl("kv_copy_pages_", &kv_copy_pages_);
 }
 
 }  // namespace cuda_transformer

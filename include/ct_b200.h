@@ -379,6 +379,25 @@ int ct_kv_append(const void* q, const int64_t q_stride[3],
                  int64_t batch, int64_t pages, int64_t page_size, int64_t max_pages,
                  int act_dtype, int cache_dtype, void* stream);
 
+/* ct_kv_append with the angles of other positions than the slots': token t is
+ * turned by the angles of rotary_positions[t] (NULL: positions[t]) and still
+ * written to positions[t].  A drafted token of a tree has the angles of its
+ * depth and the slot of its number.  One without a row in the tables of angles
+ * has no place, unless it is padding by positions[t].  No reference counterpart. */
+int ct_kv_append_ex(const void* q, const int64_t q_stride[3],
+                    const void* k, const int64_t k_stride[3],
+                    const void* v, const int64_t v_stride[3],
+                    void* q_out, void* k_out, const float* cos, const float* sin,
+                    void* k_cache, const int64_t kc_stride[4],
+                    void* v_cache, const int64_t vc_stride[4],
+                    const int32_t* block_table, int64_t table_stride,
+                    const int32_t* seq_ids, const int32_t* positions,
+                    const int32_t* rotary_positions,
+                    int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                    int64_t rot_dim, int interleaved, int64_t max_positions,
+                    int64_t batch, int64_t pages, int64_t page_size, int64_t max_pages,
+                    int act_dtype, int cache_dtype, void* stream);
+
 /* Bytes of workspace ct_paged_attention needs; they do not depend on the batch
  * or the lengths. */
 size_t ct_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim);
@@ -438,6 +457,110 @@ int ct_logits_process(const void* logits, int64_t ld, int dtype, float* out, int
                       const int64_t* bias_ids, int64_t bias_ids_ld,
                       const float* bias_values, int64_t bias_values_ld, int64_t bias_n,
                       const int32_t* mask, int64_t mask_ld, void* stream);
+
+/* ======================================================================== */
+/* Speculative decoding: drafted tokens over the paged cache                  */
+/* ======================================================================== */
+
+/* Bytes of workspace ct_tree_attention needs; they do not depend on the batch
+ * or the lengths (0: arguments out of range). */
+size_t ct_tree_attention_workspace_size(int64_t drafts, int64_t q_heads, int64_t kv_heads,
+                                        int64_t head_dim);
+
+/* Attention of up to `drafts` new tokens per sequence over the paged cache.
+ * Sequence b has context_lens[b] tokens before them; its draft_lens[b] new ones
+ * (NULL: `drafts`; clamped to [0, drafts]) are in the cache behind those, token i
+ * at position context_lens[b] + i.  New token i sees the tokens before the draft
+ * and the new tokens j whose bit j % 32 of the word mask[b][i][j / 32] is set
+ * (mask strides in words, unit stride along the last; bits from draft_lens[b] on
+ * are not looked at), or those with j <= i when mask is NULL:
+ *   O = sum_j softmax_j(scale q_i . k_j) v_j,  LSE = ln sum_j exp(scale q_i . k_j)
+ * q is indexed [batch, draft, q_head, head_dim] through its strides; heads are
+ * shared and the cache is laid out as in ct_paged_attention, with its limits on
+ * layout and types; drafts <= CT_TREE_ATTENTION_MAX_DRAFTS, batch * drafts *
+ * q_heads < 2^31, and times (max_pages * page_size / 8 + 16) < 2^52.  out is dense
+ * [batch, drafts, q_heads, head_dim] of q's type; lse (may be NULL) dense [batch,
+ * drafts, q_heads].  Rows from draft_lens[b] on, rows that see nothing, and all
+ * rows of a sequence with a negative context_lens[b] (it takes no part) give O = 0
+ * and LSE = -inf; a length beyond max_pages * page_size, or a page out of range,
+ * gives NaN in the rows that are there.  Slots past the last new token are not
+ * read.  A cached value that is not finite reaches the rows that see its token:
+ * a key with a score of -inf has no weight, scores of +inf or NaN make their row
+ * NaN, and values that are not finite make their element of O infinite or NaN.
+ * The workspace (16-byte aligned) needs no clearing and must not be used by
+ * another call that can run concurrently.  Deterministic.  No reference
+ * counterpart (the reference keeps no cache). */
+#define CT_TREE_ATTENTION_MAX_DRAFTS 16384
+int ct_tree_attention(const void* q, const int64_t q_stride[4],
+                      const void* k_cache, const int64_t kc_stride[4],
+                      const void* v_cache, const int64_t vc_stride[4],
+                      const int32_t* block_table, int64_t table_stride,
+                      const int32_t* context_lens, const int32_t* draft_lens,
+                      const int32_t* mask, const int64_t mask_stride[2],
+                      void* out, float* lse,
+                      int64_t batch, int64_t drafts, int64_t q_heads, int64_t kv_heads,
+                      int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages,
+                      float scale, int act_dtype, int cache_dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which drafted tokens are kept, and the token after them.  The draft of a
+ * sequence is a tree of draft_lens[b] nodes (NULL: `drafts`; clamped to [0,
+ * drafts]; 1 <= drafts <= CT_VERIFY_DRAFTS_MAX; vocab < 2^30): node 0 is the last token that is
+ * certain, node i > 0 proposes tokens[b][i] after its parent parents[b][i] < i
+ * (parents NULL: i - 1).  target ([batch, node, vocab] through its strides, unit
+ * along vocab, of type `dtype`) holds the target's probabilities of the token after
+ * each node; draft_probs (NULL: proposals are certain, each the only one that its
+ * drafter could make) those that the proposals after each node were drawn from, one
+ * by one; uniform[b][i] are numbers in [0, 1).
+ * From node 0 on, the children of the last kept node are tried in the order of
+ * their numbers.  With r the target's row of that node, q the drafter's and Z = 1:
+ *   child i with token x is kept when uniform[b][i] q(x) Z < r(x)
+ *   else r <- max(r / Z - q, 0), Z <- sum r        (when that sum is positive)
+ * and for certain proposals q(x) counts as 1, r(x) <- 0 and Z <- Z - r(x).  When no
+ * child is kept, the token after the path is the first t with
+ *   sum_{s <= t} r(s) > uniform[b][0] sum_s r(s)
+ * (-1 when the sum is not positive), so that the tokens are distributed as the
+ * target's own.  uniform NULL (draft_probs NULL too): target holds scores, a child
+ * is kept when it is the best token (the lowest of equal ones), which is also the
+ * token after the path; -1 for a row of -inf or with a NaN.  A child whose token is
+ * outside the vocabulary is not tried.
+ * counts[b]: nodes of the path, node 0 among them (0 without nodes); path
+ * ([batch, drafts], dense): their numbers, then -1; new_tokens (likewise): the
+ * tokens after each node of the path, then -1.  Sums and products are formed in
+ * 64 bits.  Deterministic.  The reference's GPT.generate draws one token a step
+ * (gpt/gpt.py:177-190). */
+#define CT_VERIFY_DRAFTS_MAX 1024
+int ct_verify_drafts(const void* target, const int64_t target_stride[2],
+                     const void* draft_probs, const int64_t draft_stride[2], int dtype,
+                     const int64_t* tokens, int64_t tokens_ld,
+                     const int32_t* parents, int64_t parents_ld, const int32_t* draft_lens,
+                     const float* uniform, int64_t uniform_ld,
+                     int64_t* new_tokens, int32_t* path, int32_t* counts,
+                     int64_t batch, int64_t drafts, int64_t vocab, void* stream);
+
+/* The kept ones of the last tokens move up: in each of caches_n caches (of one
+ * shape and type, [page, kv_head, slot, head_dim] with 4 strides each in
+ * cache_strides; keys and values of all layers, any head_dim up to 65536) the
+ * values at position context_lens[b] + keep[b][j] of sequence b go to position
+ * context_lens[b] + j, for j < counts[b] (clamped to [0, drafts]).  keep[b][0] <
+ * keep[b][1] < ... (ct_verify_drafts' path); a move is left out when its page is
+ * out of range, and when keep[b][j] <= j (it is in its place).  Where they do not
+ * ascend, the moved rows' values mean nothing.  Two sequences must not share the
+ * pages that are written.  No reference counterpart. */
+int ct_kv_compact(void* const* caches, const int64_t* cache_strides, int64_t caches_n,
+                  const int32_t* block_table, int64_t table_stride,
+                  const int32_t* context_lens, const int32_t* keep, int64_t keep_ld,
+                  const int32_t* counts, int64_t batch, int64_t drafts,
+                  int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size,
+                  int64_t max_pages, int cache_dtype, void* stream);
+
+/* Copies page src[i] to page dst[i], i < count, in each of caches_n caches (as
+ * in ct_kv_compact).  A pair with a page out of range is left out.  No dst may
+ * be a src or another dst.  No reference counterpart. */
+int ct_kv_copy_pages(void* const* caches, const int64_t* cache_strides, int64_t caches_n,
+                     const int32_t* src, const int32_t* dst, int64_t count,
+                     int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size,
+                     int cache_dtype, void* stream);
 
 #ifdef __cplusplus
 }
