@@ -105,6 +105,32 @@ int make_tmap_f32(CUtensorMap* map, const void* base, int rank, const uint64_t* 
   return r == CUDA_SUCCESS ? CT_OK : CT_ERR_UNSUPPORTED_LAYOUT;
 }
 
+int make_tmap_pages(CUtensorMap* map, const void* base, int dtype, int64_t pages, int64_t heads,
+                    int64_t page_size, int64_t head_dim, const int64_t strides[3], int rows) {
+  std::call_once(g_encode_once, load_encode);
+  if (!g_encode) return CT_ERR_CUDA;
+  const int64_t bytes = dtype == CT_DTYPE_F32 ? 4 : 2, row = head_dim * bytes;
+  const cuuint64_t gd[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)heads,
+                            (cuuint64_t)pages};
+  const cuuint32_t bd[4] = {(cuuint32_t)((row < 128 ? row : 128) / bytes), (cuuint32_t)rows, 1, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  cuuint64_t gs[3];
+  for (int i = 0; i < 3; ++i) {  // slot, head, page
+    const int64_t s = gd[i + 1] > 1 ? strides[2 - i] * bytes : row;
+    if (s <= 0 || s % 16 != 0 || s >= 1ll << 40) return CT_ERR_UNSUPPORTED_LAYOUT;
+    gs[i] = (cuuint64_t)s;
+  }
+  const CUtensorMapDataType type = dtype == CT_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == CT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = g_encode(map, type, 4, const_cast<void*>(base), gd, gs, bd, es,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              row < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CT_OK : CT_ERR_UNSUPPORTED_LAYOUT;
+}
+
 bool fa2_shape_ok(int64_t B, int64_t H, int64_t T, int64_t D) {
   constexpr int64_t kLim = 1ll << 31;
   return B >= 0 && H >= 0 && T >= 0 && D > 0 && T < kLim && B < kLim && H < kLim &&

@@ -3,75 +3,1113 @@
 //   s_ij = scale q_i . k_j over the tokens j before the draft and the drafted
 //   ones that i's mask names,  O_i = sum_j softmax(s_i)_j v_j,
 //   L_i = ln sum_j exp(s_ij);  O = 0 and L = -inf for rows that see nothing.
-// A warp works on one row, a lane on every 32nd dim.
+// The rows of a (sequence, key/value head) are its drafted tokens times the
+// query heads that share the head.
+#include <cfloat>
+
 #include "decode_common.cuh"
+#include "tc_ptx.cuh"
 
 namespace ct {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxCtas = 448;  // partial slots (two each) and records in the workspace
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// The base of the exponents is raised only when a score passes it by this much
+// (in powers of two): most tiles skip the rescaling of O.
+constexpr float kMaxSlack = 6.0f;
+#ifndef CT_COST
+#define CT_COST 6
+#endif
+// C: the cache's type; F32ACT: q and out are FP32, else of type C; MT: 16-row tiles
+// of a warp; WR: warps along the rows, a group.  The groups take turns at the tiles.
+template <class C_, bool F32ACT_, int D_, int MT_, int WR_>
+struct Cfg {
+  using C = C_;
+  static constexpr bool F32ACT = F32ACT_;
+  static constexpr int D = D_, MT = MT_, WR = WR_;
+  using A = std::conditional_t<F32ACT, float, C>;
+  static constexpr bool kF32 = sizeof(C) == 4;
+  static constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
+  static constexpr int kRows = 16 * MT * WR;
+  static constexpr int WK = kWarps / WR;  // groups
+  static constexpr int kRowBytes = D * (int)sizeof(C);
+  static constexpr int kChunks = kRowBytes / 16;
+  // Keys of a tile: 8 KB of K and as many of V (4 KB where four groups have a ring
+  // each), 128 at most.
+  static constexpr int kHalf = WK == 4 ? 4096 : 8192;
+  static constexpr int kKeys = kHalf / kRowBytes < 128 ? kHalf / kRowBytes : 128;
+  // Keys that a warp's scores are formed of at a time.
+  static constexpr int kMost = F32ACT && D == 128 ? 16 : 32;
+  static constexpr int kBlock = kKeys < kMost ? kKeys : kMost;
+  static constexpr int NT = kBlock / 8;
+  static constexpr int kTileBytes = kKeys * kRowBytes;  // K or V
+  // 16-bit terms of q and of the weights (FP32 activations: 22 bits and more).
+  static constexpr int kTerms = kF32 || !F32ACT ? 1 : kBf16 ? 3 : 2;
+  static constexpr int kQBytes = kTerms * kRows * kRowBytes;
+  static constexpr int kJoinDims = 32;
+  static constexpr int kJoinBytes = WK > 1 ? (WK - 1) * kRows * kJoinDims * 4 : 0;
+  static constexpr int kStatBytes = WK > 1 ? 2 * WK * kRows * 4 : 0;
+  static constexpr int kHeadBytes =
+      ((kQBytes > kJoinBytes + kStatBytes ? kQBytes : kJoinBytes + kStatBytes) + 1023) / 1024 * 1024;
+  // Stages of a group's ring: two CTAs an SM (228 KB, of which each takes 1 KB and
+  // the static 1 KB; 1 KB more to begin at a whole one).
+  static constexpr int kFit = (110 * 1024 - kHeadBytes) / (2 * kTileBytes) / WK;
+  static constexpr int kStages = kFit > 6 ? 6 : kFit;
+  static_assert(kStages >= 1 && kStages * WK >= 3, "tiles on the way");
+  static constexpr int kSmem = 1024 + kHeadBytes + WK * kStages * 2 * kTileBytes;
+  // What an item (a sequence and a key/value head) costs beside its tiles (q, the
+  // end), in tiles; units of a share at least.
+  static constexpr int kItemCost = 16384 / kHalf * CT_COST;
+  static constexpr int kMinShare = kItemCost + 2 * WK;
+  // f16 weights reach up to 2^14 instead of 1, clear of the subnormals.
+  static constexpr float kBelow = !kF32 && !kBf16 ? 8.0f : 0.0f;
+};
 
-template <class A, class C, int D>
-__global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_constant__ TreeAttention p) {
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (row >= p.batch * p.drafts * p.q_heads) return;
-  const int h = (int)(row % p.q_heads);
-  const int64_t i = row / p.q_heads % p.drafts, b = row / p.q_heads / p.drafts;
-  const int64_t kh = h / (p.q_heads / p.kv_heads);
-  constexpr int N = D / 32;
-  float q[N], o[N] = {};
-  for (int e = 0; e < N; ++e)
-    q[e] = to_f32(((const A*)p.q)[b * p.qs[0] + i * p.qs[1] + h * p.qs[2] + (lane + 32 * e) * p.qs[3]]) * p.scale;
-  int64_t n = p.draft_lens ? p.draft_lens[b] : p.drafts;
-  n = n < 0 ? 0 : n > p.drafts ? p.drafts : n;
-  const int64_t context = p.context_lens[b];
-  bool bad = context + n > p.kv.max_pages * p.kv.page_size;
-  float m = -INFINITY, l = 0.0f;
-  if (context >= 0 && i < n && !bad) {
-    for (int64_t j = 0; j < context + n; ++j) {
-      const int page = p.kv.table[b * p.kv.table_s + j / p.kv.page_size];
-      if (page < 0 || page >= p.kv.pages) {
-        bad = true;
-        break;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+// Arrives on `bar` when this thread's copies so far are done.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// c += A B for one tile: 16 x 8 x 8 in TF32, 16 x 8 x 16 in the 16-bit types.
+template <class C>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(C) == 4)
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else if constexpr (std::is_same<C, __nv_bfloat16>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// c = A B.
+template <class C>
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (sizeof(C) == 4)
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  else if constexpr (std::is_same<C, __nv_bfloat16>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+template <class C>
+__device__ __forceinline__ void mma_next(bool first, float (&c)[4], const uint32_t (&a)[4],
+                                         uint32_t b0, uint32_t b1) {
+  if (first) mma_first<C>(c, a, b0, b1); else mma<C>(c, a, b0, b1);
+}
+// What is left of x beside the TF32 value that the tensor core makes of it (it
+// drops the 13 low bits).
+__device__ __forceinline__ uint32_t low_tf32(uint32_t x) {
+  return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u));
+}
+// The next 16-bit term of x and y (x in the low half); x and y keep the rest.
+template <class C>
+__device__ __forceinline__ uint32_t take_term(float& x, float& y) {
+  uint32_t w;
+  if constexpr (std::is_same<C, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    w = *reinterpret_cast<const uint32_t*>(&h);
+    x -= __uint_as_float(w << 16);
+    y -= __uint_as_float(w & 0xffff0000u);
+  } else {
+    const __half2 h = __floats2half2_rn(x, y);
+    w = *reinterpret_cast<const uint32_t*>(&h);
+    const float2 f = __half22float2(h);
+    x -= f.x;
+    y -= f.y;
+  }
+  return w;
+}
+template <class C>
+__device__ __forceinline__ float half_value(uint32_t w, int e) {
+  if constexpr (std::is_same<C, __nv_bfloat16>::value)
+    return __uint_as_float(e ? w & 0xffff0000u : w << 16);
+  else
+    return e ? __high2float(*reinterpret_cast<const __half2*>(&w))
+             : __low2float(*reinterpret_cast<const __half2*>(&w));
+}
+// A word of V (one FP32 or two 16-bit values) with what is not finite as 0.
+template <class C>
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) {
+  if constexpr (sizeof(C) == 4) return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+  constexpr uint32_t kExp = std::is_same<C, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  if ((w & kExp) == kExp) w &= 0xffff0000u;
+  if ((w >> 16 & kExp) == kExp) w &= 0xffffu;
+  return w;
+}
+
+// Byte position of 16-byte chunk c of row r in a tile of `ROWS` rows: parts of 128
+// bytes of all rows one behind the other, chunks permuted so that eight rows' meet
+// different banks (as TMA writes them with a swizzle of 128 bytes, of 64 for
+// shorter rows).
+template <int ROW_BYTES, int ROWS>
+__device__ __forceinline__ uint32_t chunk_pos(int r, int c) {
+  if constexpr (ROW_BYTES >= 128)
+    return (uint32_t)((c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+  return (uint32_t)(r * ROW_BYTES + ((c ^ (r >> 1 & 3)) << 4));  // 64-byte rows
+}
+
+struct Launch {
+  TreeAttention p;
+  int group, blocks;    // query heads of a key/value head; row blocks of an item
+  int shares;
+  bool whole;           // an item a CTA: none is split
+  bool q_vectors;       // q's rows are 16-byte vectors
+  int page_shift;       // log2 of page_size, -1 when it is no power of two
+  float c2;             // |scale| log2 e
+  bool negative;        // scale: q's sign turns
+  int box;              // slots of a TMA box; 0: copies of single chunks
+  uint32_t* status;
+  int4* records;        // of each CTA: the split item that begins in it
+  float* partials;
+};
+
+struct Sequence {
+  int context, drafts, tiles;
+  bool there, bad;
+};
+template <class K>
+__device__ __forceinline__ Sequence sequence(const TreeAttention& p, int64_t b) {
+  Sequence s;
+  s.context = p.context_lens[b];
+  const int n = p.draft_lens ? p.draft_lens[b] : (int)p.drafts;
+  s.drafts = n < 0 ? 0 : n > p.drafts ? (int)p.drafts : n;
+  s.there = s.context >= 0 && s.drafts > 0;
+  const int64_t len = (int64_t)s.context + s.drafts;
+  s.bad = s.there && len > p.kv.max_pages * p.kv.page_size;
+  s.tiles = s.there && !s.bad ? (int)((len + K::kKeys - 1) / K::kKeys) : 0;
+  return s;
+}
+
+template <class K>
+__device__ __forceinline__ int64_t units_of(const Launch& a, int tiles) {
+  return tiles > 0 ? (int64_t)(tiles + K::kItemCost) * a.p.kv_heads : 0;
+}
+
+// A place in the list of tiles.
+struct Cursor {
+  int64_t b;
+  int head, tile, stop, tiles;  // stop: end of this share's part of the item
+  int context, drafts;
+  int64_t left;                 // units of the share from this item's part on
+};
+
+// The item at (c.b, c.head), `within` units into it, or the next one there is.
+template <class K>
+__device__ __forceinline__ bool enter(const Launch& a, Cursor& c, int64_t within) {
+  while (c.left > 0 && c.b < a.p.batch) {
+    const Sequence s = sequence<K>(a.p, c.b);
+    if (s.tiles == 0 || c.head == (int)a.p.kv_heads) {
+      ++c.b;
+      c.head = 0;
+      within = 0;
+      continue;
+    }
+    const int64_t units = s.tiles + K::kItemCost;
+    const int64_t end = within + c.left < units ? within + c.left : units;
+    c.left -= end - within;
+    c.tile = within > K::kItemCost ? (int)(within - K::kItemCost) : 0;
+    c.stop = end > K::kItemCost ? (int)(end - K::kItemCost) : 0;
+    c.tiles = s.tiles;
+    c.context = s.context;
+    c.drafts = s.drafts;
+    within = 0;
+    if (c.tile < c.stop) return true;
+    ++c.head;
+  }
+  return false;
+}
+template <class A>
+__device__ __forceinline__ void store2(void* out, int64_t i, float x, float y) {
+  if constexpr (sizeof(A) == 4) {
+    *reinterpret_cast<float2*>((float*)out + i) = make_float2(x, y);
+  } else if constexpr (std::is_same<A, __nv_bfloat16>::value) {
+    *reinterpret_cast<__nv_bfloat162*>((A*)out + i) = __floats2bfloat162_rn(x, y);
+  } else {
+    *reinterpret_cast<__half2*>((A*)out + i) = __floats2half2_rn(x, y);
+  }
+}
+
+// Bytes of workspace of a partial: O [rows][D], then the exponents' base and the
+// sum of each row.
+constexpr int64_t partial_floats(int rows, int D) { return (int64_t)rows * (D + 4); }
+
+template <class K>
+__global__ void __launch_bounds__(kThreads, 2)
+    tree_attention_kernel(const __grid_constant__ Launch a, const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map) {
+  using C = typename K::C;
+  using A = typename K::A;
+  constexpr int D = K::D, MT = K::MT, NT = K::NT;
+  extern __shared__ char shared_base[];
+  char* const shared = shared_base + (-smem_u32(shared_base) & 1023u);
+  // (the join's buffers lie where q was)
+  float(*const stat)[K::WK][K::kRows] =
+      reinterpret_cast<float(*)[K::WK][K::kRows]>(shared + K::kJoinBytes);
+  __shared__ int64_t scan[kWarps];
+  __shared__ int64_t found_b, found_x;
+  __shared__ alignas(8) uint64_t full[K::WK][K::kStages], empty[K::WK][K::kStages];
+  __shared__ int stage_bad[K::WK][K::kStages];
+  __shared__ CtaCtl ctl;
+  __shared__ bool raised;
+  const TreeAttention& p = a.p;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int wr = warp % K::WR, wk = warp / K::WR;  // row part, group
+  const int share = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks;
+  const uint32_t q_smem = smem_u32(shared);
+  const uint32_t ring = q_smem + K::kHeadBytes + wk * (K::kStages * 2 * K::kTileBytes);
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (a.box && warp == 0) {
+    if (lane == 0) tma_prefetch_desc(&k_map);
+    if (lane == 1) tma_prefetch_desc(&v_map);
+  }
+  if (tid == 0) {
+    raised = *reinterpret_cast<const volatile uint32_t*>(a.status) != 0u;
+    ctl.abort = 0u;
+    for (int g = 0; g < K::WK; ++g)
+      for (int s = 0; s < K::kStages; ++s) {
+        mbar_init(smem_u32(&full[g][s]), a.box ? 1 : 33);
+        mbar_init(smem_u32(&empty[g][s]), K::WR);
       }
-      const int64_t d = j - context;
-      if (d >= 0 && !(p.mask ? p.mask[b * p.ms[0] + i * p.ms[1] + d / 32] >> (d % 32) & 1u : d <= i)) continue;
-      const int64_t slot = j % p.kv.page_size;
-      const C* k = (const C*)p.kv.k + page * p.kv.ks[0] + kh * p.kv.ks[1] + slot * p.kv.ks[2];
-      const C* v = (const C*)p.kv.v + page * p.kv.vs[0] + kh * p.kv.vs[1] + slot * p.kv.vs[2];
-      float s = 0.0f;
-      for (int e = 0; e < N; ++e) s += q[e] * to_f32(k[lane + 32 * e]);
-      for (int w = 16; w; w /= 2) s += __shfl_xor_sync(0xffffffffu, s, w);
-      if (s == -INFINITY) continue;
-      const float top = fmaxf(m, s), f = m == -INFINITY ? 0.0f : expf(m - top), w = expf(s - top);
-      l = l * f + w;
-      for (int e = 0; e < N; ++e) o[e] = o[e] * f + w * to_f32(v[lane + 32 * e]);
-      m = top;
+    fence_barrier_init();
+    if (!a.whole) a.records[blockIdx.x] = make_int4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  if (raised) return;
+
+  // ---- this CTA's share of the units
+  Cursor next;
+  int64_t share_units = 0, within = 0;
+  next.head = 0;
+  if (a.whole) {
+    next.b = share / (int)p.kv_heads;
+    next.head = share % (int)p.kv_heads;
+    const int tiles = sequence<K>(p, next.b).tiles;
+    next.left = tiles > 0 ? tiles + K::kItemCost : 0;
+  } else {
+    const int64_t each = (p.batch + kThreads - 1) / kThreads;
+    const int64_t b0 = tid * each, b1 = b0 + each < p.batch ? b0 + each : p.batch;
+    int64_t mine = 0;
+    for (int64_t b = b0; b < b1; ++b) mine += units_of<K>(a, sequence<K>(p, b).tiles);
+    int64_t run = mine;
+    for (int w = 1; w < 32; w *= 2) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, run, w);
+      if (lane >= w) run += y;
+    }
+    if (lane == 31) scan[warp] = run;
+    if (tid == 0) found_b = p.batch;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    before += run - mine;
+    share_units = (total + a.shares - 1) / a.shares;
+    if (share_units < K::kMinShare) share_units = K::kMinShare;
+    const int64_t begin = share * share_units;
+    if (mine > 0 && begin >= before && begin < before + mine) {
+      int64_t b = b0;
+      for (; b < b1; ++b) {
+        const int64_t u = units_of<K>(a, sequence<K>(p, b).tiles);
+        if (begin < before + u) break;
+        before += u;
+      }
+      found_b = b;
+      found_x = begin - before;
+    }
+    __syncthreads();
+    next.b = found_b;
+    next.left = total - begin < share_units ? total - begin : share_units;
+    if (next.b >= p.batch) next.left = 0;
+    if (next.left > 0) {
+      const int64_t units = sequence<K>(p, next.b).tiles + K::kItemCost;
+      next.head = (int)(found_x / units);
+      within = found_x - next.head * units;
     }
   }
-  const bool there = context >= 0 && i < n;
-  for (int e = 0; e < N; ++e)
-    ((A*)p.out)[row * D + lane + 32 * e] = from_f32<A>(there && bad ? NAN : l == 0.0f ? 0.0f : o[e] / l);
-  if (lane == 0 && p.lse) p.lse[row] = there && bad ? NAN : l == 0.0f ? -INFINITY : m + logf(l);
+  // the first part that has rows in this block
+  auto settle = [&](Cursor& c, bool ok) {
+    while (ok && block * K::kRows >= c.drafts * a.group) {
+      ++c.head;
+      ok = enter<K>(a, c, 0);
+    }
+    return ok;
+  };
+  bool more = settle(next, enter<K>(a, next, within));
+  Cursor cur = next;
+
+  // ---- copies: the group's first warp fetches the tiles that are its group's, as
+  // many ahead as there are stages
+  const bool leader = wr == 0;
+  int page_next = -1;  // of lane's box of `next`'s tile
+  uint32_t in_count = 0, out_count = 0;
+  auto page_of = [&](int position, int& slot) {
+    const int index = a.page_shift >= 0 ? position >> a.page_shift : position / p.kv.page_size;
+    slot = position - index * p.kv.page_size;
+    return index;
+  };
+  auto look_up = [&]() {
+    const int len = next.context + next.drafts, from = next.tile * K::kKeys, row = lane * a.box;
+    int slot;
+    page_next = row < K::kKeys && from + row < len
+                    ? p.kv.table[next.b * p.kv.table_s + page_of(from + row, slot)] : -1;
+  };
+  // `next` goes to the group's tile at or behind it
+  bool more_in = more;
+  auto to_own_tile = [&]() {
+    while (more_in && next.tile >= next.stop) {
+      ++next.head;
+      more_in = settle(next, enter<K>(a, next, 0));
+      next.tile += wk;
+    }
+    if (more_in && a.box) look_up();
+  };
+  auto copy_in = [&]() {
+    const int stage = in_count % K::kStages;
+    if (K::WR > 1 && in_count >= K::kStages)
+      mbar_wait(smem_u32(&empty[wk][stage]), (in_count / K::kStages - 1) & 1, &ctl, a.status);
+    __syncwarp();
+    const int len = next.context + next.drafts, from = next.tile * K::kKeys;
+    const uint32_t k_tile = ring + stage * 2 * K::kTileBytes, v_tile = k_tile + K::kTileBytes;
+    const uint32_t bar = smem_u32(&full[wk][stage]);
+    if (a.box) {
+      const int row = lane * a.box;
+      const bool in = row < K::kKeys && from + row < len;
+      const bool fine = in && page_next >= 0 && page_next < p.kv.pages;
+      const uint32_t vote = __ballot_sync(0xffffffffu, fine);
+      const bool bad = __any_sync(0xffffffffu, in && !fine);
+      if (lane == 0) {
+        stage_bad[wk][stage] = bad;
+        mbar_arrive_expect_tx(bar, __popc(vote) * a.box * 2 * K::kRowBytes);
+      }
+      __syncwarp();
+      if (fine) {
+        int slot;
+        page_of(from + row, slot);
+        constexpr int kPart = K::kRowBytes < 128 ? K::kRowBytes : 128;
+#pragma unroll
+        for (int h = 0; h < K::kRowBytes / kPart; ++h) {
+          const uint32_t at = h * (K::kKeys * kPart) + row * kPart;
+          const int dim = h * (kPart / (int)sizeof(C));
+          tma_load_4d(k_tile + at, &k_map, bar, dim, slot, next.head, page_next);
+          tma_load_4d(v_tile + at, &v_map, bar, dim, slot, next.head, page_next);
+        }
+      }
+    } else {
+      const int chunk = lane % K::kChunks;
+      const C* kh = (const C*)p.kv.k + next.head * p.kv.ks[1] + chunk * (16 / (int)sizeof(C));
+      const C* vh = (const C*)p.kv.v + next.head * p.kv.vs[1] + chunk * (16 / (int)sizeof(C));
+      bool bad = false;
+#pragma unroll 4
+      for (int i = 0; i < K::kKeys * K::kChunks / 32; ++i) {
+        const int row = i * (32 / K::kChunks) + lane / K::kChunks;
+        int slot;
+        const int index = page_of(from + row, slot);
+        const bool in = from + row < len;
+        const int64_t page = in ? p.kv.table[next.b * p.kv.table_s + index] : -1;
+        const bool fine = in && page >= 0 && page < p.kv.pages;
+        bad = bad || (in && !fine);
+        const uint32_t at = chunk_pos<K::kRowBytes, K::kKeys>(row, chunk);
+        // (nothing is read where there is no page)
+        const void* k = fine ? (const void*)(kh + page * p.kv.ks[0] + slot * p.kv.ks[2]) : p.out;
+        const void* v = fine ? (const void*)(vh + page * p.kv.vs[0] + slot * p.kv.vs[2]) : p.out;
+        cp_async16(k_tile + at, k, fine ? 16 : 0);
+        cp_async16(v_tile + at, v, fine ? 16 : 0);
+      }
+      bad = __any_sync(0xffffffffu, bad);
+      if (lane == 0) {
+        stage_bad[wk][stage] = bad;
+        mbar_arrive(bar);
+      }
+      cp_async_arrive(bar);
+    }
+    ++in_count;
+    next.tile += K::WK;
+    to_own_tile();
+  };
+  // q: rows of 16-byte chunks as the cache's type, or its terms one behind the other
+  constexpr int kEight = D / 8;
+  auto load_q = [&](int64_t b, int head, int drafts) {
+    const int row0 = block * K::kRows;
+    for (int e = tid; e < K::kRows * kEight; e += kThreads) {
+      const int r = e / kEight, d = e % kEight * 8;
+      const int i = (row0 + r) / a.group, h = head * a.group + (row0 + r) % a.group;
+      const A* src = (const A*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+      if constexpr (sizeof(A) == 2) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (i < drafts) {
+          if (a.q_vectors) {
+            w = *reinterpret_cast<const uint4*>(src + d);
+          } else {
+            alignas(16) A x[8];
+            for (int j = 0; j < 8; ++j) x[j] = src[(d + j) * p.qs[3]];
+            w = *reinterpret_cast<const uint4*>(x);
+          }
+        }
+        const uint32_t sign = a.negative ? 0x80008000u : 0u;
+        *reinterpret_cast<uint4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 8)) =
+            make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
+      } else {
+        float x[8];
+        if (i < drafts && a.q_vectors) {
+          *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src + d);
+          *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(src + d + 4);
+        } else {
+          for (int j = 0; j < 8; ++j) x[j] = i < drafts ? src[(d + j) * p.qs[3]] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = a.negative ? -x[j] : x[j];
+        if constexpr (K::kF32) {
+          *reinterpret_cast<float4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 4)) =
+              *reinterpret_cast<float4*>(x);
+          *reinterpret_cast<float4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 4 + 1)) =
+              *reinterpret_cast<float4*>(x + 4);
+        } else {
+#pragma unroll
+          for (int t = 0; t < K::kTerms; ++t) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = take_term<C>(x[2 * j], x[2 * j + 1]);
+            *reinterpret_cast<uint4*>(shared + t * K::kRows * K::kRowBytes +
+                                      chunk_pos<K::kRowBytes, K::kRows>(r, d / 8)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  };
+  if (leader) {
+    next.tile += wk;
+    to_own_tile();
+  }
+  if (more) load_q(cur.b, cur.head, cur.drafts);
+  if (leader) {
+#pragma unroll 1
+    for (int s = 0; s < K::kStages && more_in; ++s) copy_in();
+  }
+
+  // ---- the parts of items
+  const float c2 = a.c2;
+  while (more) {
+    const int context = cur.context, drafts = cur.drafts;
+    const int64_t b = cur.b;
+    const int head = cur.head, part0 = cur.tile, part1 = cur.stop, tiles = cur.tiles;
+    const int row0 = block * K::kRows;  // row r: token (row0 + r) / group, head (row0 + r) % group
+    __syncthreads();  // q has been written
+
+    float o[MT][D / 8][4], base[MT][2], sum[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.0f;
+      base[m][0] = base[m][1] = -INFINITY;
+      sum[m][0] = sum[m][1] = 0.0f;
+    }
+    // a thread's rows: warp_row + 16 m + lane / 4, and 8 below
+    const int warp_row = wr * 16 * MT;
+    // which of the 32 tokens from `position` on row r (of the block) sees, as bits
+    auto seen_from = [&](int r, int position) -> uint32_t {
+      const int d = position - context, i = (row0 + r) / a.group;
+      if (d <= -32) return ~0u;
+      if (i >= drafts || d >= drafts) return d < 0 ? (1u << -d) - 1u : 0u;
+      uint32_t w;
+      if (p.mask) {
+        const uint32_t* words = p.mask + b * p.ms[0] + i * p.ms[1];
+        const int at = d < 0 ? 0 : d >> 5, last = (drafts - 1) >> 5;
+        const uint32_t low = words[at], high = at < last ? words[at + 1] : 0u;
+        w = d < 0 ? low << -d | ((1u << -d) - 1u) : __funnelshift_r(low, high, d & 31);
+      } else {
+        w = i < d ? 0u : i - d >= 31 ? ~0u : (2u << (i - d)) - 1u;
+      }
+      return drafts - d >= 32 ? w : w & ((1u << (drafts - d)) - 1u);
+    };
+
+#pragma unroll 1
+    for (int tile = part0 + wk; tile < part1; tile += K::WK) {
+      const int stage = out_count % K::kStages;
+      mbar_wait(smem_u32(&full[wk][stage]), out_count / K::kStages & 1, &ctl, a.status);
+      const char* const k_at = shared + K::kHeadBytes + (wk * K::kStages + stage) * 2 * K::kTileBytes;
+      const char* const v_at = k_at + K::kTileBytes;
+      const uint32_t k_tile = ring + stage * 2 * K::kTileBytes, v_tile = k_tile + K::kTileBytes;
+      const bool masked = (tile + 1) * K::kKeys > context;
+      if (stage_bad[wk][stage]) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) sum[m][0] = sum[m][1] = NAN;
+      }
+
+#pragma unroll 1
+      for (int k0 = 0; k0 < K::kKeys; k0 += K::kBlock) {
+        const int position0 = tile * K::kKeys + k0;
+        if (masked && position0 >= context + drafts) break;
+        // ---- scores; of several terms the first one's product apart, which alone
+        // has the right infinity or NaN
+        float s[MT][NT][4], rest[K::F32ACT ? MT : 1][NT][4];
+        if constexpr (K::kF32) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t k[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              ldsm4(k[n], k_tile + chunk_pos<K::kRowBytes, K::kKeys>(k0 + 8 * n + lane % 8,
+                                                                    4 * kk + lane / 8));
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                uint32_t qa[4], ql[4];
+                ldsm4(qa, q_smem + chunk_pos<K::kRowBytes, K::kRows>(warp_row + 16 * m + lane % 16,
+                                                                    4 * kk + 2 * j + lane / 16));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ql[e] = low_tf32(qa[e]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  const uint32_t b0 = k[n][2 * j], b1 = k[n][2 * j + 1];
+                  mma_next<C>(kk + j == 0, s[m][n], qa, b0, b1);
+                  mma_next<C>(kk + j == 0, rest[m][n], ql, b0, b1);
+                  mma<C>(rest[m][n], qa, low_tf32(b0), low_tf32(b1));
+                }
+              }
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t k[NT / 2][4];
+#pragma unroll
+            for (int n = 0; n < NT / 2; ++n)
+              ldsm4(k[n], k_tile + chunk_pos<K::kRowBytes, K::kKeys>(
+                                       k0 + 16 * n + lane / 16 * 8 + lane % 8, 2 * ks + lane / 8 % 2));
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int t = 0; t < K::kTerms; ++t) {
+                uint32_t qa[4];
+                ldsm4(qa, q_smem + t * K::kRows * K::kRowBytes +
+                              chunk_pos<K::kRowBytes, K::kRows>(warp_row + 16 * m + lane % 16,
+                                                                2 * ks + lane / 16));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  const uint32_t b0 = k[n / 2][n % 2 * 2], b1 = k[n / 2][n % 2 * 2 + 1];
+                  if constexpr (K::F32ACT) {
+                    if (t > 0) {
+                      mma_next<C>(ks == 0 && t == 1, rest[m][n], qa, b0, b1);
+                      continue;
+                    }
+                  }
+                  mma_next<C>(ks == 0, s[m][n], qa, b0, b1);
+                }
+              }
+          }
+        }
+        if constexpr (K::F32ACT) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = s[m][n][e] + rest[m][n][e];
+                s[m][n][e] = x == x ? x : s[m][n][e];
+              }
+        }
+        bool dirty = false;
+        uint32_t seen[MT][2];
+        if (masked) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              seen[m][h] = seen_from(warp_row + 16 * m + lane / 4 + 8 * h, position0);
+              const uint32_t bits = seen[m][h] >> (lane % 4 * 2);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (!(bits >> (8 * n + e) & 1u)) s[m][n][2 * h + e] = -INFINITY;
+            }
+          // what lies behind the last token counts as zero (a weight of 0 would leave
+          // its NaN)
+          const int rows = context + drafts - position0;
+          if (rows < K::kBlock) {
+            for (int e = rows * K::kChunks + lane; e < K::kBlock * K::kChunks; e += 32)
+              *reinterpret_cast<uint4*>(
+                  shared + (v_tile - q_smem) +
+                  chunk_pos<K::kRowBytes, K::kKeys>(k0 + e / K::kChunks, e % K::kChunks)) =
+                  make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();  // (before a TMA copy writes there)
+            __syncwarp();
+          }
+          // values that are not finite, where not all rows see them
+          for (int e = lane; e < K::kBlock * K::kChunks; e += 32) {
+            const uint4 w = *reinterpret_cast<const uint4*>(
+                v_at + chunk_pos<K::kRowBytes, K::kKeys>(k0 + e / K::kChunks, e % K::kChunks));
+            dirty = dirty || only_finite<C>(w.x) != w.x || only_finite<C>(w.y) != w.y ||
+                    only_finite<C>(w.z) != w.z || only_finite<C>(w.w) != w.w;
+          }
+          dirty = __any_sync(0xffffffffu, dirty);
+        }
+
+        // ---- the exponents' base, weights
+        bool raise = false;
+        float top[MT][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float t = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[m][n][2 * h], s[m][n][2 * h + 1]));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            top[m][h] = t * c2 - K::kBelow;
+            raise = raise || top[m][h] > base[m][h] + kMaxSlack;
+          }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float old = base[m][h];
+              base[m][h] = fmaxf(old, top[m][h]);
+              const float f = old == -INFINITY ? 0.0f : ex2(old - base[m][h]);
+              sum[m][h] = old == -INFINITY ? sum[m][h] : sum[m][h] * f;
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) {
+                o[m][n][2 * h] *= f;
+                o[m][n][2 * h + 1] *= f;
+              }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float from = base[m][h] == -INFINITY ? 0.0f : base[m][h];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                s[m][n][e] = ex2(__fmaf_rn(s[m][n][e], c2, -from));
+                sum[m][h] += s[m][n][e];
+              }
+          }
+
+        // ---- O += weights V, a block's products apart (the tensor core cuts its
+        // sums off: a whole sequence's would be too small)
+        if constexpr (K::kF32) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            float acc[MT][4];
+#pragma unroll
+            for (int ks = 0; ks < NT; ++ks) {
+              // the product's keys k and k + 4 are 2 k and 2 k + 1 of the eight
+              const int key = k0 + 8 * ks + lane % 4 * 2, dim = 8 * n + lane / 4;
+              uint32_t v[2], vl[2];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                v[j] = *reinterpret_cast<const uint32_t*>(
+                    v_at + chunk_pos<K::kRowBytes, K::kKeys>(key + j, dim / 4) + dim % 4 * 4);
+                if (dirty) v[j] = only_finite<C>(v[j]);
+                vl[j] = low_tf32(v[j]);
+              }
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const uint32_t w[4] = {__float_as_uint(s[m][ks][0]), __float_as_uint(s[m][ks][2]),
+                                       __float_as_uint(s[m][ks][1]), __float_as_uint(s[m][ks][3])};
+                const uint32_t wl[4] = {low_tf32(w[0]), low_tf32(w[1]), low_tf32(w[2]), low_tf32(w[3])};
+                mma_next<C>(ks == 0, acc[m], w, v[0], v[1]);
+                mma<C>(acc[m], wl, v[0], v[1]);
+                mma<C>(acc[m], w, vl[0], vl[1]);
+              }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[m][n][e] += acc[m][e];
+          }
+        } else {
+          uint32_t w[MT][NT / 2][K::kTerms][4];
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int ks = 0; ks < NT / 2; ++ks)
+#pragma unroll
+              for (int t = 0; t < K::kTerms; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  w[m][ks][t][j] = take_term<C>(s[m][2 * ks + j / 2][j % 2 * 2],
+                                                s[m][2 * ks + j / 2][j % 2 * 2 + 1]);
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            float acc[MT][2][4];
+#pragma unroll
+            for (int ks = 0; ks < NT / 2; ++ks) {
+              uint32_t v[4];
+              ldsm4_trans(v, v_tile + chunk_pos<K::kRowBytes, K::kKeys>(k0 + 16 * ks + lane % 16,
+                                                                       2 * n + lane / 16));
+              if (dirty) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = only_finite<C>(v[j]);
+              }
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int t = 0; t < K::kTerms; ++t) {
+                  mma_next<C>(ks + t == 0, acc[m][0], w[m][ks][t], v[0], v[1]);
+                  mma_next<C>(ks + t == 0, acc[m][1], w[m][ks][t], v[2], v[3]);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[m][2 * n + j][e] += acc[m][j][e];
+          }
+        }
+        if (dirty) {  // infinities and NaN, for the rows that see their token
+#pragma unroll 1
+          for (int k = 0; k < K::kBlock; ++k) {
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int dim = 8 * n + lane % 4 * 2 + j;
+                const C* v = (const C*)(v_at + chunk_pos<K::kRowBytes, K::kKeys>(
+                                                   k0 + k, dim * (int)sizeof(C) / 16));
+                const float x = to_f32(v[dim % (16 / (int)sizeof(C))]);
+                if (!(fabsf(x) < INFINITY)) {
+#pragma unroll
+                  for (int m = 0; m < MT; ++m) {
+                    if (seen[m][0] >> k & 1u) o[m][n][j] += x;
+                    if (seen[m][1] >> k & 1u) o[m][n][2 + j] += x;
+                  }
+                }
+              }
+          }
+        }
+      }
+      __syncwarp();
+      if (K::WR > 1 && lane == 0) mbar_arrive(smem_u32(&empty[wk][stage]));
+      ++out_count;
+      if (leader && more_in) copy_in();
+    }
+
+    // ---- the part's end: the four lanes of a row, then the warps that divided
+    // the keys, meet
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
+        sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 2);
+      }
+    __syncthreads();  // (q has been read)
+    if constexpr (K::WK > 1) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (lane % 4 == 0) {
+            stat[0][wk][warp_row + 16 * m + lane / 4 + 8 * h] = base[m][h];
+            stat[1][wk][warp_row + 16 * m + lane / 4 + 8 * h] = sum[m][h];
+          }
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = warp_row + 16 * m + lane / 4 + 8 * h;
+          float top = -INFINITY, all = 0.0f;
+#pragma unroll
+          for (int w = 0; w < K::WK; ++w) top = fmaxf(top, stat[0][w][r]);
+#pragma unroll
+          for (int w = 0; w < K::WK; ++w) {
+            const float t = stat[0][w][r];
+            // (a base of -inf has a sum of 0, or NaN from a page out of range)
+            all += t == -INFINITY ? stat[1][w][r] : stat[1][w][r] * ex2(t - top);
+          }
+          const float f = base[m][h] == -INFINITY ? 1.0f : ex2(base[m][h] - top);
+          base[m][h] = top;
+          sum[m][h] = all;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[m][n][2 * h] *= f;
+            o[m][n][2 * h + 1] *= f;
+          }
+        }
+      float* const join = reinterpret_cast<float*>(shared);
+#pragma unroll
+      for (int d0 = 0; d0 < D; d0 += K::kJoinDims) {
+        if (d0 > 0) __syncthreads();
+        if (wk > 0) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < K::kJoinDims / 8; ++n)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<float2*>(
+                    join + (((wk - 1) * K::kRows + warp_row + 16 * m + lane / 4 + 8 * h) *
+                                K::kJoinDims + (8 * n ^ (lane / 4 % 4 * 8)) + lane % 4 * 2)) =
+                    make_float2(o[m][d0 / 8 + n][2 * h], o[m][d0 / 8 + n][2 * h + 1]);
+        }
+        __syncthreads();
+        if (wk == 0) {
+#pragma unroll
+          for (int w = 1; w < K::WK; ++w)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int n = 0; n < K::kJoinDims / 8; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const float2 x = *reinterpret_cast<const float2*>(
+                      join + (((w - 1) * K::kRows + warp_row + 16 * m + lane / 4 + 8 * h) *
+                                  K::kJoinDims + (8 * n ^ (lane / 4 % 4 * 8)) + lane % 4 * 2));
+                  o[m][d0 / 8 + n][2 * h] += x.x;
+                  o[m][d0 / 8 + n][2 * h + 1] += x.y;
+                }
+        }
+      }
+    }
+    const bool whole = part0 == 0 && part1 == tiles;
+    if (wk == 0) {
+      float* const slot = a.partials + ((int64_t)blockIdx.x * 2 + (part0 == 0 ? 1 : 0)) *
+                                           partial_floats(K::kRows, D);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = warp_row + 16 * m + lane / 4 + 8 * h, i = (row0 + r) / a.group;
+          if (i >= drafts) continue;
+          if (whole) {
+            const float f = sum[m][h] == 0.0f ? 0.0f : 1.0f / sum[m][h];
+            const int64_t row = (b * p.drafts + i) * p.q_heads + head * a.group + (row0 + r) % a.group;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+              store2<A>(p.out, row * D + 8 * n + lane % 4 * 2, o[m][n][2 * h] * f,
+                        o[m][n][2 * h + 1] * f);
+            if (lane % 4 == 0 && p.lse)
+              p.lse[row] = sum[m][h] == 0.0f ? -INFINITY : (base[m][h] + log2f(sum[m][h])) * kLn2;
+          } else {
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+              *reinterpret_cast<float2*>(slot + r * D + 8 * n + lane % 4 * 2) =
+                  make_float2(o[m][n][2 * h], o[m][n][2 * h + 1]);
+            if (lane % 4 == 0)
+              *reinterpret_cast<float2*>(slot + K::kRows * D + 2 * r) =
+                  make_float2(base[m][h], sum[m][h]);
+          }
+        }
+    }
+    if (!whole && part0 == 0 && tid == 0) {
+      // the item ends in the share that has its last unit
+      const int64_t end = (int64_t)(share + 1) * share_units + (tiles - part1);
+      a.records[blockIdx.x] = make_int4((int)((end - 1) / share_units) - share + 1, (int)b, head, drafts);
+    }
+    __syncthreads();  // (the join has been read, q may be written)
+    ++cur.head;
+    more = settle(cur, enter<K>(a, cur, 0));
+    if (more) load_q(cur.b, cur.head, cur.drafts);
+  }
+  // ---- rows that are not there: zero, NaN where a length is out of range
+  for (int64_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    const Sequence s = sequence<K>(p, b);
+    const int first = s.there && !s.bad ? s.drafts : 0;
+    const int64_t row0 = b * p.drafts * p.q_heads;
+    for (int64_t e = (int64_t)first * p.q_heads * D + 2 * tid; e < p.drafts * p.q_heads * D;
+         e += 2 * kThreads) {
+      const int64_t row = e / D;
+      const bool nan = s.bad && row < (int64_t)s.drafts * p.q_heads;
+      store2<A>(p.out, row0 * D + e, nan ? NAN : 0.0f, nan ? NAN : 0.0f);
+      if (e % D == 0 && p.lse) p.lse[row0 + row] = nan ? NAN : -INFINITY;
+    }
+  }
+
+  // after a wait that ran out: copies still on the way end before the memory is
+  // given back
+  if (ctl.abort && leader)
+    for (uint32_t n = in_count > K::kStages ? in_count - K::kStages : 0; n < in_count; ++n)
+      for (int i = 0; i < 1 << 20; ++i)
+        if (mbar_test_wait(smem_u32(&full[wk][n % K::kStages]), n / K::kStages & 1)) break;
+}
+
+// The partials of the split item that begins in CTA `cta`, kJoinRows rows of it.
+constexpr int kJoinRows = 8;
+
+template <class A, int D>
+__global__ void __launch_bounds__(kJoinRows * 32)
+    tree_join_kernel(const __grid_constant__ Launch a, const int rows) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (*reinterpret_cast<const volatile uint32_t*>(a.status) != 0u) return;
+  const int cta = blockIdx.x, block = cta % a.blocks;
+  const int4 rec = a.records[cta];
+  if (rec.x == 0) return;
+  const int r = blockIdx.y * kJoinRows + threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int i = (block * rows + r) / a.group;
+  if (i >= rec.w) return;
+  const int64_t each = partial_floats(rows, D);
+  // the first part ends its CTA's share, the others begin theirs
+  auto part = [&](int k) {
+    return a.partials + ((int64_t)(cta + k * a.blocks) * 2 + (k == 0)) * each;
+  };
+  constexpr int N = D / 32;
+  float top = -INFINITY, sum = 0.0f, o[N] = {};
+  for (int k = lane; k < rec.x; k += 32)
+    top = fmaxf(top, part(k)[rows * D + 2 * r]);
+  for (int w = 16; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+#pragma unroll 4
+  for (int k = 0; k < rec.x; ++k) {
+    const float2 ml = *reinterpret_cast<const float2*>(part(k) + rows * D + 2 * r);
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+    sum += ml.x == -INFINITY ? ml.y : ml.y * f;
+    const float* src = part(k) + r * D + lane * N;
+    float x[N];
+    if constexpr (N == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
+    else if constexpr (N == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
+    else x[0] = *src;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] += ml.x == -INFINITY ? 0.0f : x[e] * f;
+  }
+  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int64_t row = ((int64_t)rec.y * a.p.drafts + i) * a.p.q_heads + rec.z * a.group +
+                      (block * rows + r) % a.group;
+#pragma unroll
+  for (int e = 0; e < N; ++e) ((A*)a.p.out)[row * D + lane * N + e] = from_f32<A>(o[e] * f);
+  if (lane == 0 && a.p.lse) a.p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// Contexts of at most so many tokens (as the table holds) are not split: an item a
+// CTA, and no join.
+constexpr int64_t kWholeTokens = 512;
+
+template <class K>
+int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
+  const TreeAttention& p = a.p;
+  int rc = allow_shared<tree_attention_kernel<K>>(K::kSmem, dev);
+  if (rc != CT_OK) return rc;
+  a.blocks = (int)((p.drafts * a.group + K::kRows - 1) / K::kRows);
+  const int64_t items = p.batch * p.kv_heads;
+  int ctas = 2 * dev.sm_count;
+  if (ctas > kMaxCtas) ctas = kMaxCtas;
+  a.whole = p.kv.max_pages * p.kv.page_size <= kWholeTokens || a.blocks > ctas / 2;
+  int64_t shares = a.whole ? items : ctas / a.blocks;
+  if (shares * a.blocks >= 1ll << 31) return CT_ERR_INVALID_ARGUMENT;
+  a.shares = (int)shares;
+  a.records = reinterpret_cast<int4*>(p.ws);
+  a.partials = reinterpret_cast<float*>(a.records + kMaxCtas);
+  a.status = dev.status;
+  // (not 0, so that scores of -inf, which mark what is not seen, stay so)
+  a.c2 = fabsf(p.scale) * kLog2e;
+  if (a.c2 < FLT_MIN) a.c2 = FLT_MIN;
+  a.negative = p.scale < 0.0f;
+  // Boxes of the largest power of two of slots that fills pages and tiles, of 8 at
+  // least (the swizzle's period); pages without one are copied chunk by chunk.
+  CUtensorMap k_map{}, v_map{};
+  a.box = 1;
+  while (p.kv.page_size % (2 * a.box) == 0 && 2 * a.box <= K::kKeys) a.box *= 2;
+  if (a.box < 8 || p.kv.pages == 0 ||
+      make_tmap_pages(&k_map, p.kv.k, p.kv.dtype, p.kv.pages, p.kv_heads, p.kv.page_size, K::D,
+                      p.kv.ks, a.box) != CT_OK ||
+      make_tmap_pages(&v_map, p.kv.v, p.kv.dtype, p.kv.pages, p.kv_heads, p.kv.page_size, K::D,
+                      p.kv.vs, a.box) != CT_OK)
+    a.box = 0;
+  const unsigned grid = (unsigned)(shares * a.blocks);
+  tree_attention_kernel<K><<<grid, kThreads, K::kSmem, st>>>(a, k_map, v_map);
+  rc = check_launch();
+  if (rc != CT_OK || a.whole) return rc;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid, K::kRows / kJoinRows);
+  config.blockDim = dim3(kJoinRows * 32);
+  config.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, tree_join_kernel<typename K::A, K::D>, a, (int)K::kRows) != cudaSuccess) {
+    cudaGetLastError();
+    return CT_ERR_LAUNCH_FAILED;
+  }
+  return CT_OK;
+}
+
+template <class C, bool F32ACT, int D>
+int launch_rows(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
+  const int64_t rows = a.p.drafts * a.group;
+  constexpr int MT = F32ACT ? 1 : 2;
+  if (rows <= 16) return launch<Cfg<C, F32ACT, D, 1, 1>>(a, dev, st);
+  if (rows <= 32) return launch<Cfg<C, F32ACT, D, MT, 2 / MT>>(a, dev, st);
+  return launch<Cfg<C, F32ACT, D, MT, 4 / MT>>(a, dev, st);
 }
 
 }  // namespace
 
-size_t tree_attention_workspace(int64_t, int64_t, int64_t, int64_t) { return 0; }
+size_t tree_attention_workspace(int64_t drafts, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim) {
+  const int64_t rows = drafts * (q_heads / kv_heads);
+  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  return kMaxCtas * (sizeof(int4) + 2 * (size_t)partial_floats(tile, (int)head_dim) * sizeof(float));
+}
 
-int launch_tree_attention(const TreeAttention& p, const DeviceInfo&, cudaStream_t st) {
-  return with_dtype(p.act_dtype, [&](auto a) {
-    return with_dtype(p.kv.dtype, [&](auto c) {
-      using A = decltype(a);
-      using C = decltype(c);
+int launch_tree_attention(const TreeAttention& p, const DeviceInfo& dev, cudaStream_t st) {
+  Launch a{};
+  a.p = p;
+  a.group = (int)(p.q_heads / p.kv_heads);
+  const int64_t align = 16 / dtype_bytes(p.act_dtype);
+  a.q_vectors = aligned16(p.q) && p.qs[0] % align == 0 && p.qs[1] % align == 0 &&
+                p.qs[2] % align == 0 && p.qs[3] == 1;
+  a.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (p.kv.page_size == 1 << s) a.page_shift = s;
+  return with_dtype(p.act_dtype, [&](auto act) {
+    return with_dtype(p.kv.dtype, [&](auto cache) {
+      using A = decltype(act);
+      using C = decltype(cache);
       if constexpr (std::is_same<A, C>::value || std::is_same<A, float>::value) {
-        const int64_t rows = p.batch * p.drafts * p.q_heads;
-        const unsigned grid = (unsigned)((rows + kThreads / 32 - 1) / (kThreads / 32));
-        if (p.head_dim == 32) tree_attention_kernel<A, C, 32><<<grid, kThreads, 0, st>>>(p);
-        else if (p.head_dim == 64) tree_attention_kernel<A, C, 64><<<grid, kThreads, 0, st>>>(p);
-        else tree_attention_kernel<A, C, 128><<<grid, kThreads, 0, st>>>(p);
-        return check_launch();
+        constexpr bool kF32Act = std::is_same<A, float>::value;
+        if (p.head_dim == 32) return launch_rows<C, kF32Act, 32>(a, dev, st);
+        if (p.head_dim == 64) return launch_rows<C, kF32Act, 64>(a, dev, st);
+        return launch_rows<C, kF32Act, 128>(a, dev, st);
       } else {
         return (int)CT_ERR_INVALID_ARGUMENT;
       }
