@@ -7,23 +7,16 @@
 // query heads that share the head.
 #include <cfloat>
 
-#include "decode_common.cuh"
-#include "tc_ptx.cuh"
+#include "tree_attention.cuh"
 
 namespace ct {
+
+using namespace tree;
+
 namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxCtas = 448;  // partial slots (two each) and records in the workspace
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-// The base of the exponents is raised only when a score passes it by this much
-// (in powers of two): most tiles skip the rescaling of O.
-constexpr float kMaxSlack = 6.0f;
-#ifndef CT_COST
-#define CT_COST 6
-#endif
 // C: the cache's type; F32ACT: q and out are FP32, else of type C; MT: 16-row tiles
 // of a warp; WR: warps along the rows, a group.  The groups take turns at the tiles.
 template <class C_, bool F32ACT_, int D_, int MT_, int WR_>
@@ -63,7 +56,7 @@ struct Cfg {
   static constexpr int kSmem = 1024 + kHeadBytes + WK * kStages * 2 * kTileBytes;
   // What an item (a sequence and a key/value head) costs beside its tiles (q, the
   // end), in tiles; units of a share at least.
-  static constexpr int kItemCost = 16384 / kHalf * CT_COST;
+  static constexpr int kItemCost = 16384 / kHalf * 6;
   static constexpr int kMinShare = kItemCost + 2 * WK;
   // f16 weights reach up to 2^14 instead of 1, clear of the subnormals.
   static constexpr float kBelow = !kF32 && !kBf16 ? 8.0f : 0.0f;
@@ -76,11 +69,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
 // Arrives on `bar` when this thread's copies so far are done.
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -186,91 +174,6 @@ __device__ __forceinline__ uint32_t chunk_pos(int r, int c) {
   return (uint32_t)(r * ROW_BYTES + ((c ^ (r >> 1 & 3)) << 4));  // 64-byte rows
 }
 
-struct Launch {
-  TreeAttention p;
-  int group, blocks;    // query heads of a key/value head; row blocks of an item
-  int shares;
-  bool whole;           // an item a CTA: none is split
-  bool q_vectors;       // q's rows are 16-byte vectors
-  int page_shift;       // log2 of page_size, -1 when it is no power of two
-  float c2;             // |scale| log2 e
-  bool negative;        // scale: q's sign turns
-  int box;              // slots of a TMA box; 0: copies of single chunks
-  uint32_t* status;
-  int4* records;        // of each CTA: the split item that begins in it
-  float* partials;
-};
-
-struct Sequence {
-  int context, drafts, tiles;
-  bool there, bad;
-};
-template <class K>
-__device__ __forceinline__ Sequence sequence(const TreeAttention& p, int64_t b) {
-  Sequence s;
-  s.context = p.context_lens[b];
-  const int n = p.draft_lens ? p.draft_lens[b] : (int)p.drafts;
-  s.drafts = n < 0 ? 0 : n > p.drafts ? (int)p.drafts : n;
-  s.there = s.context >= 0 && s.drafts > 0;
-  const int64_t len = (int64_t)s.context + s.drafts;
-  s.bad = s.there && len > p.kv.max_pages * p.kv.page_size;
-  s.tiles = s.there && !s.bad ? (int)((len + K::kKeys - 1) / K::kKeys) : 0;
-  return s;
-}
-
-template <class K>
-__device__ __forceinline__ int64_t units_of(const Launch& a, int tiles) {
-  return tiles > 0 ? (int64_t)(tiles + K::kItemCost) * a.p.kv_heads : 0;
-}
-
-// A place in the list of tiles.
-struct Cursor {
-  int64_t b;
-  int head, tile, stop, tiles;  // stop: end of this share's part of the item
-  int context, drafts;
-  int64_t left;                 // units of the share from this item's part on
-};
-
-// The item at (c.b, c.head), `within` units into it, or the next one there is.
-template <class K>
-__device__ __forceinline__ bool enter(const Launch& a, Cursor& c, int64_t within) {
-  while (c.left > 0 && c.b < a.p.batch) {
-    const Sequence s = sequence<K>(a.p, c.b);
-    if (s.tiles == 0 || c.head == (int)a.p.kv_heads) {
-      ++c.b;
-      c.head = 0;
-      within = 0;
-      continue;
-    }
-    const int64_t units = s.tiles + K::kItemCost;
-    const int64_t end = within + c.left < units ? within + c.left : units;
-    c.left -= end - within;
-    c.tile = within > K::kItemCost ? (int)(within - K::kItemCost) : 0;
-    c.stop = end > K::kItemCost ? (int)(end - K::kItemCost) : 0;
-    c.tiles = s.tiles;
-    c.context = s.context;
-    c.drafts = s.drafts;
-    within = 0;
-    if (c.tile < c.stop) return true;
-    ++c.head;
-  }
-  return false;
-}
-template <class A>
-__device__ __forceinline__ void store2(void* out, int64_t i, float x, float y) {
-  if constexpr (sizeof(A) == 4) {
-    *reinterpret_cast<float2*>((float*)out + i) = make_float2(x, y);
-  } else if constexpr (std::is_same<A, __nv_bfloat16>::value) {
-    *reinterpret_cast<__nv_bfloat162*>((A*)out + i) = __floats2bfloat162_rn(x, y);
-  } else {
-    *reinterpret_cast<__half2*>((A*)out + i) = __floats2half2_rn(x, y);
-  }
-}
-
-// Bytes of workspace of a partial: O [rows][D], then the exponents' base and the
-// sum of each row.
-constexpr int64_t partial_floats(int rows, int D) { return (int64_t)rows * (D + 4); }
-
 template <class K>
 __global__ void __launch_bounds__(kThreads, 2)
     tree_attention_kernel(const __grid_constant__ Launch a, const __grid_constant__ CUtensorMap k_map,
@@ -283,8 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   // (the join's buffers lie where q was)
   float(*const stat)[K::WK][K::kRows] =
       reinterpret_cast<float(*)[K::WK][K::kRows]>(shared + K::kJoinBytes);
-  __shared__ int64_t scan[kWarps];
-  __shared__ int64_t found_b, found_x;
+  __shared__ Finder finder;
   __shared__ alignas(8) uint64_t full[K::WK][K::kStages], empty[K::WK][K::kStages];
   __shared__ int stage_bad[K::WK][K::kStages];
   __shared__ CtaCtl ctl;
@@ -315,56 +217,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (raised) return;
 
   // ---- this CTA's share of the units
-  Cursor next;
-  int64_t share_units = 0, within = 0;
-  next.head = 0;
-  if (a.whole) {
-    next.b = share / (int)p.kv_heads;
-    next.head = share % (int)p.kv_heads;
-    const int tiles = sequence<K>(p, next.b).tiles;
-    next.left = tiles > 0 ? tiles + K::kItemCost : 0;
-  } else {
-    const int64_t each = (p.batch + kThreads - 1) / kThreads;
-    const int64_t b0 = tid * each, b1 = b0 + each < p.batch ? b0 + each : p.batch;
-    int64_t mine = 0;
-    for (int64_t b = b0; b < b1; ++b) mine += units_of<K>(a, sequence<K>(p, b).tiles);
-    int64_t run = mine;
-    for (int w = 1; w < 32; w *= 2) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, run, w);
-      if (lane >= w) run += y;
-    }
-    if (lane == 31) scan[warp] = run;
-    if (tid == 0) found_b = p.batch;
-    __syncthreads();
-    int64_t before = 0, total = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
-    }
-    before += run - mine;
-    share_units = (total + a.shares - 1) / a.shares;
-    if (share_units < K::kMinShare) share_units = K::kMinShare;
-    const int64_t begin = share * share_units;
-    if (mine > 0 && begin >= before && begin < before + mine) {
-      int64_t b = b0;
-      for (; b < b1; ++b) {
-        const int64_t u = units_of<K>(a, sequence<K>(p, b).tiles);
-        if (begin < before + u) break;
-        before += u;
-      }
-      found_b = b;
-      found_x = begin - before;
-    }
-    __syncthreads();
-    next.b = found_b;
-    next.left = total - begin < share_units ? total - begin : share_units;
-    if (next.b >= p.batch) next.left = 0;
-    if (next.left > 0) {
-      const int64_t units = sequence<K>(p, next.b).tiles + K::kItemCost;
-      next.head = (int)(found_x / units);
-      within = found_x - next.head * units;
-    }
-  }
+  int64_t share_units, within;
+  Cursor next = first_place<K>(a, share, finder, share_units, within);
   // the first part that has rows in this block
   auto settle = [&](Cursor& c, bool ok) {
     while (ok && block * K::kRows >= c.drafts * a.group) {
@@ -546,21 +400,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     // a thread's rows: warp_row + 16 m + lane / 4, and 8 below
     const int warp_row = wr * 16 * MT;
-    // which of the 32 tokens from `position` on row r (of the block) sees, as bits
-    auto seen_from = [&](int r, int position) -> uint32_t {
-      const int d = position - context, i = (row0 + r) / a.group;
-      if (d <= -32) return ~0u;
-      if (i >= drafts || d >= drafts) return d < 0 ? (1u << -d) - 1u : 0u;
-      uint32_t w;
-      if (p.mask) {
-        const uint32_t* words = p.mask + b * p.ms[0] + i * p.ms[1];
-        const int at = d < 0 ? 0 : d >> 5, last = (drafts - 1) >> 5;
-        const uint32_t low = words[at], high = at < last ? words[at + 1] : 0u;
-        w = d < 0 ? low << -d | ((1u << -d) - 1u) : __funnelshift_r(low, high, d & 31);
-      } else {
-        w = i < d ? 0u : i - d >= 31 ? ~0u : (2u << (i - d)) - 1u;
-      }
-      return drafts - d >= 32 ? w : w & ((1u << (drafts - d)) - 1u);
+    auto seen = [&](int r, int position) {
+      return seen_from(p, b, (row0 + r) / a.group, position - context, drafts);
     };
 
 #pragma unroll 1
@@ -651,14 +492,14 @@ __global__ void __launch_bounds__(kThreads, 2)
               }
         }
         bool dirty = false;
-        uint32_t seen[MT][2];
+        uint32_t sees[MT][2];
         if (masked) {
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              seen[m][h] = seen_from(warp_row + 16 * m + lane / 4 + 8 * h, position0);
-              const uint32_t bits = seen[m][h] >> (lane % 4 * 2);
+              sees[m][h] = seen(warp_row + 16 * m + lane / 4 + 8 * h, position0);
+              const uint32_t bits = sees[m][h] >> (lane % 4 * 2);
 #pragma unroll
               for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -708,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float old = base[m][h];
-              base[m][h] = fmaxf(old, top[m][h]);
+              base[m][h] = top[m][h] > old + kMaxSlack ? top[m][h] : old;
               const float f = old == -INFINITY ? 0.0f : ex2(old - base[m][h]);
               sum[m][h] = old == -INFINITY ? sum[m][h] : sum[m][h] * f;
 #pragma unroll
@@ -819,8 +660,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (!(fabsf(x) < INFINITY)) {
 #pragma unroll
                   for (int m = 0; m < MT; ++m) {
-                    if (seen[m][0] >> k & 1u) o[m][n][j] += x;
-                    if (seen[m][1] >> k & 1u) o[m][n][2 + j] += x;
+                    if (sees[m][0] >> k & 1u) o[m][n][j] += x;
+                    if (sees[m][1] >> k & 1u) o[m][n][2 + j] += x;
                   }
                 }
               }
@@ -951,20 +792,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     more = settle(cur, enter<K>(a, cur, 0));
     if (more) load_q(cur.b, cur.head, cur.drafts);
   }
-  // ---- rows that are not there: zero, NaN where a length is out of range
-  for (int64_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    const Sequence s = sequence<K>(p, b);
-    const int first = s.there && !s.bad ? s.drafts : 0;
-    const int64_t row0 = b * p.drafts * p.q_heads;
-    for (int64_t e = (int64_t)first * p.q_heads * D + 2 * tid; e < p.drafts * p.q_heads * D;
-         e += 2 * kThreads) {
-      const int64_t row = e / D;
-      const bool nan = s.bad && row < (int64_t)s.drafts * p.q_heads;
-      store2<A>(p.out, row0 * D + e, nan ? NAN : 0.0f, nan ? NAN : 0.0f);
-      if (e % D == 0 && p.lse) p.lse[row0 + row] = nan ? NAN : -INFINITY;
-    }
-  }
-
+  write_rows_not_there<K>(p);
   // after a wait that ran out: copies still on the way end before the memory is
   // given back
   if (ctl.abort && leader)
@@ -972,55 +800,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i = 0; i < 1 << 20; ++i)
         if (mbar_test_wait(smem_u32(&full[wk][n % K::kStages]), n / K::kStages & 1)) break;
 }
-
-// The partials of the split item that begins in CTA `cta`, kJoinRows rows of it.
-constexpr int kJoinRows = 8;
-
-template <class A, int D>
-__global__ void __launch_bounds__(kJoinRows * 32)
-    tree_join_kernel(const __grid_constant__ Launch a, const int rows) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (*reinterpret_cast<const volatile uint32_t*>(a.status) != 0u) return;
-  const int cta = blockIdx.x, block = cta % a.blocks;
-  const int4 rec = a.records[cta];
-  if (rec.x == 0) return;
-  const int r = blockIdx.y * kJoinRows + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int i = (block * rows + r) / a.group;
-  if (i >= rec.w) return;
-  const int64_t each = partial_floats(rows, D);
-  // the first part ends its CTA's share, the others begin theirs
-  auto part = [&](int k) {
-    return a.partials + ((int64_t)(cta + k * a.blocks) * 2 + (k == 0)) * each;
-  };
-  constexpr int N = D / 32;
-  float top = -INFINITY, sum = 0.0f, o[N] = {};
-  for (int k = lane; k < rec.x; k += 32)
-    top = fmaxf(top, part(k)[rows * D + 2 * r]);
-  for (int w = 16; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-#pragma unroll 4
-  for (int k = 0; k < rec.x; ++k) {
-    const float2 ml = *reinterpret_cast<const float2*>(part(k) + rows * D + 2 * r);
-    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-    sum += ml.x == -INFINITY ? ml.y : ml.y * f;
-    const float* src = part(k) + r * D + lane * N;
-    float x[N];
-    if constexpr (N == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
-    else if constexpr (N == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
-    else x[0] = *src;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] += ml.x == -INFINITY ? 0.0f : x[e] * f;
-  }
-  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t row = ((int64_t)rec.y * a.p.drafts + i) * a.p.q_heads + rec.z * a.group +
-                      (block * rows + r) % a.group;
-#pragma unroll
-  for (int e = 0; e < N; ++e) ((A*)a.p.out)[row * D + lane * N + e] = from_f32<A>(o[e] * f);
-  if (lane == 0 && a.p.lse) a.p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-}
-
-// Contexts of at most so many tokens (as the table holds) are not split: an item a
-// CTA, and no join.
-constexpr int64_t kWholeTokens = 512;
 
 template <class K>
 int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
@@ -1035,42 +814,13 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
   int64_t shares = a.whole ? items : ctas / a.blocks;
   if (shares * a.blocks >= 1ll << 31) return CT_ERR_INVALID_ARGUMENT;
   a.shares = (int)shares;
-  a.records = reinterpret_cast<int4*>(p.ws);
-  a.partials = reinterpret_cast<float*>(a.records + kMaxCtas);
-  a.status = dev.status;
-  // (not 0, so that scores of -inf, which mark what is not seen, stay so)
-  a.c2 = fabsf(p.scale) * kLog2e;
-  if (a.c2 < FLT_MIN) a.c2 = FLT_MIN;
-  a.negative = p.scale < 0.0f;
-  // Boxes of the largest power of two of slots that fills pages and tiles, of 8 at
-  // least (the swizzle's period); pages without one are copied chunk by chunk.
   CUtensorMap k_map{}, v_map{};
-  a.box = 1;
-  while (p.kv.page_size % (2 * a.box) == 0 && 2 * a.box <= K::kKeys) a.box *= 2;
-  if (a.box < 8 || p.kv.pages == 0 ||
-      make_tmap_pages(&k_map, p.kv.k, p.kv.dtype, p.kv.pages, p.kv_heads, p.kv.page_size, K::D,
-                      p.kv.ks, a.box) != CT_OK ||
-      make_tmap_pages(&v_map, p.kv.v, p.kv.dtype, p.kv.pages, p.kv_heads, p.kv.page_size, K::D,
-                      p.kv.vs, a.box) != CT_OK)
-    a.box = 0;
+  make_maps(a, &k_map, &v_map, K::kKeys);
   const unsigned grid = (unsigned)(shares * a.blocks);
   tree_attention_kernel<K><<<grid, kThreads, K::kSmem, st>>>(a, k_map, v_map);
   rc = check_launch();
   if (rc != CT_OK || a.whole) return rc;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(grid, K::kRows / kJoinRows);
-  config.blockDim = dim3(kJoinRows * 32);
-  config.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  if (cudaLaunchKernelEx(&config, tree_join_kernel<typename K::A, K::D>, a, (int)K::kRows) != cudaSuccess) {
-    cudaGetLastError();
-    return CT_ERR_LAUNCH_FAILED;
-  }
-  return CT_OK;
+  return launch_join<typename K::A, K::D>(a, grid, K::kRows, st);
 }
 
 template <class C, bool F32ACT, int D>
@@ -1087,20 +837,15 @@ int launch_rows(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
 size_t tree_attention_workspace(int64_t drafts, int64_t q_heads, int64_t kv_heads,
                                 int64_t head_dim) {
   const int64_t rows = drafts * (q_heads / kv_heads);
-  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  // (rows of a slot: a block's of this kernel, or up to 128 on tcgen05)
+  const int tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows >= 128 ? 128 : (int)(rows + 15) / 16 * 16;
   return kMaxCtas * (sizeof(int4) + 2 * (size_t)partial_floats(tile, (int)head_dim) * sizeof(float));
 }
 
 int launch_tree_attention(const TreeAttention& p, const DeviceInfo& dev, cudaStream_t st) {
-  Launch a{};
-  a.p = p;
-  a.group = (int)(p.q_heads / p.kv_heads);
-  const int64_t align = 16 / dtype_bytes(p.act_dtype);
-  a.q_vectors = aligned16(p.q) && p.qs[0] % align == 0 && p.qs[1] % align == 0 &&
-                p.qs[2] % align == 0 && p.qs[3] == 1;
-  a.page_shift = -1;
-  for (int s = 0; s < 31; ++s)
-    if (p.kv.page_size == 1 << s) a.page_shift = s;
+  const int rc = launch_tc(p, dev, st);
+  if (rc != kNoTc) return rc;
+  const Launch a = begin_launch(p, dev);
   return with_dtype(p.act_dtype, [&](auto act) {
     return with_dtype(p.kv.dtype, [&](auto cache) {
       using A = decltype(act);

@@ -1,0 +1,330 @@
+// tree_attention.cuh -- what the two kernels of tree_attention share: how the
+// work is divided, which tokens a row sees, the joining of split items.
+//
+// Work is cut into tiles of keys of one item (a sequence and a key/value head),
+// and every CTA takes an equal share of the tiles, counted on the device from
+// the lengths (the host knows none).  Rows that do not fit one CTA are blocks,
+// whose CTAs take the same share side by side and meet its keys in L2.  A share
+// that starts or ends inside an item leaves a partial (base of the exponents, sum,
+// O) in the workspace, and a second kernel joins the partials in their order: the
+// results do not depend on timing and nothing has to be cleared.
+#pragma once
+
+#include <cfloat>
+
+#include "decode_common.cuh"
+#include "tc_ptx.cuh"
+
+namespace ct {
+namespace tree {
+namespace {
+
+constexpr int kMaxCtas = 448;  // partial slots (two each) and records in the workspace
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// The base of the exponents is raised only when a score passes it by this much
+// (in powers of two): most tiles skip the rescaling of O.
+constexpr float kMaxSlack = 6.0f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Launch {
+  TreeAttention p;
+  int group, blocks;    // query heads of a key/value head; row blocks of an item
+  int shares;
+  bool whole;           // an item a CTA: none is split
+  bool q_vectors;       // q's rows are 16-byte vectors
+  int page_shift;       // log2 of page_size, -1 when it is no power of two
+  float c2;             // |scale| log2 e
+  bool negative;        // scale: q's sign turns
+  int box;              // slots of a TMA box; 0: copies of single chunks
+  uint32_t* status;
+  int4* records;        // of each CTA: the split item that begins in it
+  float* partials;
+};
+
+struct Sequence {
+  int context, drafts, tiles;
+  bool there, bad;
+};
+template <class K>
+__device__ __forceinline__ Sequence sequence(const TreeAttention& p, int64_t b) {
+  Sequence s;
+  s.context = p.context_lens[b];
+  const int n = p.draft_lens ? p.draft_lens[b] : (int)p.drafts;
+  s.drafts = n < 0 ? 0 : n > p.drafts ? (int)p.drafts : n;
+  s.there = s.context >= 0 && s.drafts > 0;
+  const int64_t len = (int64_t)s.context + s.drafts;
+  s.bad = s.there && len > p.kv.max_pages * p.kv.page_size;
+  s.tiles = s.there && !s.bad ? (int)((len + K::kKeys - 1) / K::kKeys) : 0;
+  return s;
+}
+
+template <class K>
+__device__ __forceinline__ int64_t units_of(const Launch& a, int tiles) {
+  return tiles > 0 ? (int64_t)(tiles + K::kItemCost) * a.p.kv_heads : 0;
+}
+
+// A place in the list of tiles.
+struct Cursor {
+  int64_t b;
+  int head, tile, stop, tiles;  // stop: end of this share's part of the item
+  int context, drafts;
+  int64_t left;                 // units of the share from this item's part on
+};
+
+// The item at (c.b, c.head), `within` units into it, or the next one there is.
+template <class K>
+__device__ __forceinline__ bool enter(const Launch& a, Cursor& c, int64_t within) {
+  while (c.left > 0 && c.b < a.p.batch) {
+    const Sequence s = sequence<K>(a.p, c.b);
+    if (s.tiles == 0 || c.head == (int)a.p.kv_heads) {
+      ++c.b;
+      c.head = 0;
+      within = 0;
+      continue;
+    }
+    const int64_t units = s.tiles + K::kItemCost;
+    const int64_t end = within + c.left < units ? within + c.left : units;
+    c.left -= end - within;
+    c.tile = within > K::kItemCost ? (int)(within - K::kItemCost) : 0;
+    c.stop = end > K::kItemCost ? (int)(end - K::kItemCost) : 0;
+    c.tiles = s.tiles;
+    c.context = s.context;
+    c.drafts = s.drafts;
+    within = 0;
+    if (c.tile < c.stop) return true;
+    ++c.head;
+  }
+  return false;
+}
+
+struct Finder {
+  int64_t scan[32];
+  int64_t b, x;
+};
+
+// Where share `share` of the units begins (all threads of the CTA; the first barrier
+// of theirs): `within` units into an item, which `enter` takes.
+template <class K>
+__device__ __forceinline__ Cursor first_place(const Launch& a, int share, Finder& f,
+                                              int64_t& share_units, int64_t& within) {
+  const TreeAttention& p = a.p;
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid % 32;
+  Cursor c;
+  c.head = 0;
+  share_units = within = 0;
+  if (a.whole) {
+    c.b = share / (int)p.kv_heads;
+    c.head = share % (int)p.kv_heads;
+    const int tiles = sequence<K>(p, c.b).tiles;
+    c.left = tiles > 0 ? tiles + K::kItemCost : 0;
+    return c;
+  }
+  const int64_t each = (p.batch + threads - 1) / threads;
+  const int64_t b0 = tid * each, b1 = b0 + each < p.batch ? b0 + each : p.batch;
+  int64_t mine = 0;
+  for (int64_t b = b0; b < b1; ++b) mine += units_of<K>(a, sequence<K>(p, b).tiles);
+  int64_t run = mine;
+  for (int w = 1; w < 32; w *= 2) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, run, w);
+    if (lane >= w) run += y;
+  }
+  if (lane == 31) f.scan[tid / 32] = run;
+  if (tid == 0) f.b = p.batch;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+  for (int w = 0; w < threads / 32; ++w) {
+    if (w < tid / 32) before += f.scan[w];
+    total += f.scan[w];
+  }
+  before += run - mine;
+  share_units = (total + a.shares - 1) / a.shares;
+  if (share_units < K::kMinShare) share_units = K::kMinShare;
+  const int64_t begin = share * share_units;
+  if (mine > 0 && begin >= before && begin < before + mine) {
+    int64_t b = b0;
+    for (; b < b1; ++b) {
+      const int64_t u = units_of<K>(a, sequence<K>(p, b).tiles);
+      if (begin < before + u) break;
+      before += u;
+    }
+    f.b = b;
+    f.x = begin - before;
+  }
+  __syncthreads();
+  c.b = f.b;
+  c.left = c.b >= p.batch ? 0 : total - begin < share_units ? total - begin : share_units;
+  if (c.left > 0) {
+    const int64_t units = sequence<K>(p, c.b).tiles + K::kItemCost;
+    c.head = (int)(f.x / units);
+    within = f.x - c.head * units;
+  }
+  return c;
+}
+
+// Which of the 32 drafted tokens from number d on (d < 0: some before the draft) the
+// drafted token i of sequence b sees, as bits.
+__device__ __forceinline__ uint32_t seen_from(const TreeAttention& p, int64_t b, int i, int d,
+                                              int drafts) {
+  if (d <= -32) return ~0u;
+  if (i >= drafts || d >= drafts) return d < 0 ? (1u << -d) - 1u : 0u;
+  uint32_t w;
+  if (p.mask) {
+    const uint32_t* words = p.mask + b * p.ms[0] + i * p.ms[1];
+    const int at = d < 0 ? 0 : d >> 5, last = (drafts - 1) >> 5;
+    const uint32_t low = words[at], high = at < last ? words[at + 1] : 0u;
+    w = d < 0 ? low << -d | ((1u << -d) - 1u) : __funnelshift_r(low, high, d & 31);
+  } else {
+    w = i < d ? 0u : i - d >= 31 ? ~0u : (2u << (i - d)) - 1u;
+  }
+  return drafts - d >= 32 ? w : w & ((1u << (drafts - d)) - 1u);
+}
+
+template <class A>
+__device__ __forceinline__ void store2(void* out, int64_t i, float x, float y) {
+  if constexpr (sizeof(A) == 4) {
+    *reinterpret_cast<float2*>((float*)out + i) = make_float2(x, y);
+  } else if constexpr (std::is_same<A, __nv_bfloat16>::value) {
+    *reinterpret_cast<__nv_bfloat162*>((A*)out + i) = __floats2bfloat162_rn(x, y);
+  } else {
+    *reinterpret_cast<__half2*>((A*)out + i) = __floats2half2_rn(x, y);
+  }
+}
+
+// Bytes of workspace of a partial: O [rows][D], then the exponents' base and the
+// sum of each row.
+constexpr int64_t partial_floats(int rows, int D) { return (int64_t)rows * (D + 4); }
+
+// Rows that are not there: zero; all of a sequence whose length is out of range: NaN.
+template <class K>
+__device__ __forceinline__ void write_rows_not_there(const TreeAttention& p) {
+  using A = typename K::A;
+  constexpr int D = K::D;
+  for (int64_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    const Sequence s = sequence<K>(p, b);
+    const int first = s.there && !s.bad ? s.drafts : 0;
+    const int64_t row0 = b * p.drafts * p.q_heads;
+    for (int64_t e = (int64_t)first * p.q_heads * D + 2 * threadIdx.x; e < p.drafts * p.q_heads * D;
+         e += 2 * blockDim.x) {
+      const int64_t row = e / D;
+      const bool nan = s.bad && row < (int64_t)s.drafts * p.q_heads;
+      store2<A>(p.out, row0 * D + e, nan ? NAN : 0.0f, nan ? NAN : 0.0f);
+      if (e % D == 0 && p.lse) p.lse[row0 + row] = nan ? NAN : -INFINITY;
+    }
+  }
+}
+
+// The partials of the split item that begins in CTA `cta`, kJoinRows rows of it.
+constexpr int kJoinRows = 8;
+
+template <class A, int D>
+__global__ void __launch_bounds__(kJoinRows * 32)
+    tree_join_kernel(const __grid_constant__ Launch a, const int rows) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (*reinterpret_cast<const volatile uint32_t*>(a.status) != 0u) return;
+  const int cta = blockIdx.x, block = cta % a.blocks;
+  const int4 rec = a.records[cta];
+  if (rec.x == 0) return;
+  const int r = blockIdx.y * kJoinRows + threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int i = (block * rows + r) / a.group;
+  if (i >= rec.w) return;
+  const int64_t each = partial_floats(rows, D);
+  // the first part ends its CTA's share, the others begin theirs
+  auto part = [&](int k) {
+    return a.partials + ((int64_t)(cta + k * a.blocks) * 2 + (k == 0)) * each;
+  };
+  constexpr int N = D / 32;
+  float top = -INFINITY, sum = 0.0f, o[N] = {};
+  for (int k = lane; k < rec.x; k += 32)
+    top = fmaxf(top, part(k)[rows * D + 2 * r]);
+  for (int w = 16; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+#pragma unroll 4
+  for (int k = 0; k < rec.x; ++k) {
+    const float2 ml = *reinterpret_cast<const float2*>(part(k) + rows * D + 2 * r);
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+    sum += ml.x == -INFINITY ? ml.y : ml.y * f;
+    const float* src = part(k) + r * D + lane * N;
+    float x[N];
+    if constexpr (N == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
+    else if constexpr (N == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
+    else x[0] = *src;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] += ml.x == -INFINITY ? 0.0f : x[e] * f;
+  }
+  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int64_t row = ((int64_t)rec.y * a.p.drafts + i) * a.p.q_heads + rec.z * a.group +
+                      (block * rows + r) % a.group;
+#pragma unroll
+  for (int e = 0; e < N; ++e) ((A*)a.p.out)[row * D + lane * N + e] = from_f32<A>(o[e] * f);
+  if (lane == 0 && a.p.lse) a.p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+template <class A, int D>
+int launch_join(const Launch& a, unsigned grid, int rows, cudaStream_t st) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid, rows / kJoinRows);
+  config.blockDim = dim3(kJoinRows * 32);
+  config.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, tree_join_kernel<A, D>, a, rows) != cudaSuccess) {
+    cudaGetLastError();
+    return CT_ERR_LAUNCH_FAILED;
+  }
+  return CT_OK;
+}
+
+// Contexts of at most so many tokens (as the table holds) are not split: an item a
+// CTA, and no join.
+constexpr int64_t kWholeTokens = 512;
+
+inline Launch begin_launch(const TreeAttention& p, const DeviceInfo& dev) {
+  Launch a{};
+  a.p = p;
+  a.status = dev.status;
+  // (not 0, so that scores of -inf, which mark what is not seen, stay so)
+  a.c2 = fabsf(p.scale) * kLog2e;
+  if (a.c2 < FLT_MIN) a.c2 = FLT_MIN;
+  a.negative = p.scale < 0.0f;
+  a.group = (int)(p.q_heads / p.kv_heads);
+  const int64_t align = 16 / dtype_bytes(p.act_dtype);
+  a.q_vectors = aligned16(p.q) && p.qs[0] % align == 0 && p.qs[1] % align == 0 &&
+                p.qs[2] % align == 0 && p.qs[3] == 1;
+  a.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (p.kv.page_size == 1 << s) a.page_shift = s;
+  a.records = reinterpret_cast<int4*>(p.ws);
+  a.partials = reinterpret_cast<float*>(a.records + kMaxCtas);
+  return a;
+}
+
+// Boxes of the largest power of two of slots that fills pages and tiles, of 8 at
+// least (the swizzle's period); a.box is 0 for pages without one.
+inline void make_maps(Launch& a, CUtensorMap* k_map, CUtensorMap* v_map, int keys) {
+  const PagedKv& kv = a.p.kv;
+  a.box = 1;
+  while (kv.page_size % (2 * a.box) == 0 && 2 * a.box <= keys) a.box *= 2;
+  if (a.box < 8 || kv.pages == 0 ||
+      make_tmap_pages(k_map, kv.k, kv.dtype, kv.pages, a.p.kv_heads, kv.page_size, a.p.head_dim,
+                      kv.ks, a.box) != CT_OK ||
+      make_tmap_pages(v_map, kv.v, kv.dtype, kv.pages, a.p.kv_heads, kv.page_size, a.p.head_dim,
+                      kv.vs, a.box) != CT_OK)
+    a.box = 0;
+}
+
+}  // namespace
+
+// The call on tcgen05 (tree_attention_tc.cu); kNoTc where that does not take it.
+constexpr int kNoTc = -1;
+int launch_tc(const TreeAttention& p, const DeviceInfo& dev, cudaStream_t st);
+
+}  // namespace tree
+}  // namespace ct

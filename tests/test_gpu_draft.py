@@ -139,6 +139,22 @@ def test_attention_lengths(cuda_device, ops, context, kv, group, n, cache):
     check(q, k, v, table, context, [n] * len(context), bits, 32, got, 0.125)
 
 
+@pytest.mark.parametrize("kind,dim,n", [(F16, 64, 3), (F16, 64, 40), (BF16, 128, 33), (F32, 64, 2)])
+def test_attention_long_shares(cuda_device, ops, kind, dim, n):
+    """So many keys that every CTA goes through thousands of them in one piece: many
+    sequences over the same pages.  All weights near 1: a sum that loses its low bits
+    on the way shows."""
+    batch, context, g = 56, 60000, gen(n)
+    k, v, table = make_cache([context + n], 1, dim, 64, kind, "head", g)
+    v += 1
+    table = table.expand(batch, table.shape[1])
+    q = (0.1 * torch.randn(batch, n, 1, dim, generator=g, device="cuda")).to(kind)
+    out, lse = ops.tree_attention(q, k, v, table, ints([context] * batch))
+    for b in (0, 17, batch - 1):
+        one = slice(b, b + 1)
+        check(q[one], k, v, table[one], [context], [n], None, 64, (out[one], lse[one]), dim ** -0.5)
+
+
 @pytest.mark.parametrize("act,cache", TYPES)
 def test_attention_masks(cuda_device, ops, act, cache):
     """Rows that see nothing of the draft, and without a context nothing at all;
