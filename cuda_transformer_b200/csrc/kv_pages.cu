@@ -102,16 +102,28 @@ __global__ void __launch_bounds__(kThreads)
 // Longer drafts: place x takes the value of place keep[x], which then takes that
 // of keep[keep[x]], and so on up to a place that nothing moves to.  Such chains
 // have no place in common (keep ascends, so no place is kept twice), and each
-// begins at a place that is not kept itself.  So the chains run in parallel, a
-// thread following one of them for its column.  keep[x] > x along a chain
-// whatever keep holds, so each of them ends.
-constexpr int kPlaces = 64;  // of a CTA
+// begins at a place that is not kept itself.  So the chains run in parallel: a CTA
+// has those that begin in kPlaces places, for the columns of its threads.  It lists
+// the next moves of each, then makes them, kMoves at a time: what a batch reads is
+// read before the batch writes.  keep[x] > x along a chain whatever keep holds, so
+// each of them ends.
+constexpr int kPlaces = 64;
+constexpr int kListed = 256;
+static_assert(kListed == kThreads, "a thread an entry");
+
+struct Move {
+  Place from, to;  // from.page < 0: none
+};
 
 template <class T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
     compact_long_kernel(const __grid_constant__ KvCompact p, const Columns cols, const int bytes,
                         const uint32_t pieces) {
-  __shared__ int starts[kPlaces], listed;
+  __shared__ alignas(16) Move list[kListed];
+  __shared__ int at[kPlaces], chains;  // where the chains are
+  __shared__ bool kept[kPlaces];
+  __shared__ int found[kThreads / 32];
+  __shared__ uint8_t order[kListed];
   const uint32_t piece = blockIdx.x / cols.blocks;
   const int64_t b = piece / pieces;
   const int base = p.context_lens[b];
@@ -119,35 +131,85 @@ __global__ void __launch_bounds__(kThreads)
   const int x0 = (int)(piece - b * pieces) * kPlaces;
   if (base < 0 || x0 >= n) return;
   const int32_t* keep = p.keep + b * p.keep_ld;
-  if (threadIdx.x == 0) listed = 0;
-  __syncthreads();
-  if (threadIdx.x < kPlaces && x0 + (int)threadIdx.x < n) {
-    const int x = x0 + threadIdx.x;
-    int low = 0, high = x;  // keep[j] >= j: x is kept as one of the first x + 1, if at all
-    while (low < high) {
-      const int mid = (low + high) / 2;
-      if (keep[mid] < x) low = mid + 1; else high = mid;
-    }
-    if (keep[low] != x && keep[x] > x) starts[atomicAdd(&listed, 1)] = x;
+  const int tid = threadIdx.x;
+  if (tid == 0) chains = 0;
+  if (tid < kPlaces) kept[tid] = false;
+  // the first kept one that is not before x0 (kThreads of them looked at at a time)
+  int low = 0, high = x0 < n ? x0 : n;  // (keep[j] >= j)
+  while (high > low) {
+    const int step = (high - low + kThreads - 1) / kThreads, j = low + tid * step;
+    const int before = __syncthreads_count(j < high && keep[j] < x0);
+    if (before == 0) break;
+    const int from = low + (before - 1) * step;  // keep[from] < x0
+    high = from + step < high ? from + step : high;
+    low = from + 1;
   }
   __syncthreads();
-  const uint32_t c = blockIdx.x % cols.blocks * kThreads + threadIdx.x;
-  if (c >= cols.count) return;
-  const Column<T> col = column<T>(p.caches, (int)p.kv_heads, cols.row_units, bytes, c);
-  const int chains = listed;
-  for (int s = 0; s < chains; ++s) {
-    int x = starts[s];
-    Place to = place_of(p, b, (int64_t)base + x);
-    while (x < n) {
-      const int k = keep[x];
-      if (k <= x) break;
-      const Place from = place_of(p, b, (int64_t)base + k);
-      if (to.page >= 0 && from.page >= 0)
-        col.base[to.page * col.page + to.slot * col.slot] =
-            col.base[from.page * col.page + from.slot * col.slot];
-      to = from;
-      x = k;
+  if (tid < kPlaces && low + tid < n) {
+    const int x = keep[low + tid] - x0;
+    if (x >= 0 && x < kPlaces) kept[x] = true;
+  }
+  __syncthreads();
+  if (tid < kPlaces && x0 + tid < n && !kept[tid] && keep[x0 + tid] > x0 + tid)
+    at[atomicAdd(&chains, 1)] = x0 + tid;
+  __syncthreads();
+  const uint32_t c = blockIdx.x % cols.blocks * kThreads + tid;
+  const bool mine = c < cols.count;
+  const Column<T> col = column<T>(p.caches, (int)p.kv_heads, cols.row_units, bytes, mine ? c : 0);
+  while (chains > 0) {
+    const int active = chains, steps = kListed / active;
+    // the next moves of each chain, in their order
+    int x = tid < active ? at[tid] : n;
+    if (tid < active) {
+      Place to = place_of(p, b, (int64_t)base + x);
+      for (int k = 0; k < steps; ++k) {
+        Move m{{-1, 0}, {-1, 0}};
+        const int y = x < n ? keep[x] : -1;
+        if (x < n && y > x) {
+          const Place from = place_of(p, b, (int64_t)base + y);
+          if (to.page >= 0 && from.page >= 0) m = {from, to};
+          to = from;
+          x = y;
+        } else {
+          x = n;
+        }
+        list[tid * steps + k] = m;
+      }
     }
+    __syncthreads();
+    if (tid == 0) chains = 0;
+    // those that there are, close together, in their order
+    const bool is_move = tid < active * steps && list[tid].from.page >= 0;
+    const uint32_t vote = __ballot_sync(0xffffffffu, is_move);
+    if (tid % 32 == 0) found[tid / 32] = __popc(vote);
+    __syncthreads();
+    int moves = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < tid / 32) before += found[w];
+      moves += found[w];
+    }
+    if (is_move) order[before + __popc(vote & ((1u << tid % 32) - 1))] = (uint8_t)tid;
+    __syncthreads();
+    if (mine)
+      for (int j0 = 0; j0 < moves; j0 += kMoves) {
+        T value[kMoves];
+#pragma unroll
+        for (int k = 0; k < kMoves; ++k)
+          if (j0 + k < moves) {
+            const Place from = list[order[j0 + k]].from;
+            value[k] = col.base[from.page * col.page + from.slot * col.slot];
+          }
+#pragma unroll
+        for (int k = 0; k < kMoves; ++k)
+          if (j0 + k < moves) {
+            const Place to = list[order[j0 + k]].to;
+            col.base[to.page * col.page + to.slot * col.slot] = value[k];
+          }
+      }
+    __syncthreads();
+    if (x < n) at[atomicAdd(&chains, 1)] = x;
+    __syncthreads();
   }
 }
 

@@ -27,7 +27,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kCtasSm = 4;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostCtas = 8;  // of a cluster
 
@@ -50,7 +51,7 @@ struct Node {
 };
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyDrafts p) {
+__global__ void __launch_bounds__(kThreads, kCtasSm) verify_kernel(const __grid_constant__ VerifyDrafts p) {
   extern __shared__ __align__(16) char shared[];
   Node* const node = reinterpret_cast<Node*>(shared);
   __shared__ double warp_sum[kWarps], cta_sum[2][kMostCtas];
@@ -80,13 +81,29 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
   }
   cluster.sync();  // (all of its CTAs run before one writes into another's memory)
 
-  // this CTA's part of the vocabulary, and this warp's of that
+  // This warp's part of a row: whole 16-byte vectors, evenly; the elements before the
+  // first of them are the first warp's, those behind the last one the last warp's.
   const int vocab = (int)p.vocab;
-  const int per_cta = (vocab + ctas - 1) / ctas;
-  const int per_warp = (per_cta + kWarps - 1) / kWarps;
-  const int cta_end = min(vocab, (rank + 1) * per_cta);
-  const int begin = min(cta_end, rank * per_cta + warp * per_warp);
-  const int end = min(cta_end, begin + per_warp);
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int part = rank * kWarps + warp, parts = ctas * kWarps;
+  struct Vec {
+    T v[VEC];
+  };
+  int head, first, last, tail;  // elements before the vectors; this warp's vectors
+  const T *p_row, *q_row;
+  auto set_row = [&](int at) {
+    p_row = target + at * p.ts[1];
+    q_row = drafter ? drafter + at * p.ds[1] : nullptr;
+    head = (int)((16 - reinterpret_cast<uintptr_t>(p_row) % 16) % 16 / sizeof(T));
+    // (rows that are aligned differently are read element by element)
+    const bool alike = !drafter || (reinterpret_cast<uintptr_t>(p_row) -
+                                    reinterpret_cast<uintptr_t>(q_row)) % 16 == 0;
+    const int vectors = !alike || head > vocab ? 0 : (vocab - head) / VEC;
+    if (vectors == 0) head = 0;
+    first = (int)((int64_t)vectors * part / parts);
+    last = (int)((int64_t)vectors * (part + 1) / parts);
+    tail = head + vectors * VEC;
+  };
   int parity = 0;
 
   int current = 0, last_refused = 0, refused = 0;
@@ -104,13 +121,54 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     return (double)pt;
   };
   auto mass_at = [&](int t) -> double {
-    return mass(t, to_f32(target[current * p.ts[1] + t]),
-                drafter ? to_f32(drafter[current * p.ds[1] + t]) : 0.0f);
+    return mass(t, to_f32(p_row[t]), drafter ? to_f32(q_row[t]) : 0.0f);
   };
+  // single elements of this warp: [0, head) before its vectors, [tail, vocab) behind
+  // them.  Without vectors a warp's elements are a part of [0, vocab).
+  auto singles = [&](bool behind, int& from, int& to) {
+    if (tail == 0) {
+      from = behind ? 0 : (int)((int64_t)vocab * part / parts);
+      to = behind ? 0 : (int)((int64_t)vocab * (part + 1) / parts);
+    } else if (behind) {
+      from = part == parts - 1 ? tail : vocab;
+      to = vocab;
+    } else {
+      from = 0;
+      to = part == 0 ? head : 0;
+    }
+  };
+  constexpr int kLoads = 4;  // vectors of a lane that are on the way at once
   // the sum of r; the parts of warps and CTAs stay in shared memory
   auto sum_row = [&]() -> double {
+    set_row(current);
     double sum = 0.0;
-    for (int t = begin + lane; t < end; t += 32) sum += mass_at(t);
+    for (int side = 0; side < 2; ++side) {
+      int from, to;
+      singles(side == 1, from, to);
+      for (int t = from + lane; t < to; t += 32) sum += mass_at(t);
+    }
+    for (int i = first + lane; i < last; i += 32 * kLoads) {
+      Vec pv[kLoads], qv[kLoads];
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+        if (i + 32 * k < last) {
+          *reinterpret_cast<uint4*>(&pv[k]) =
+              *reinterpret_cast<const uint4*>(p_row + head + (int64_t)(i + 32 * k) * VEC);
+          if (drafter)
+            *reinterpret_cast<uint4*>(&qv[k]) =
+                *reinterpret_cast<const uint4*>(q_row + head + (int64_t)(i + 32 * k) * VEC);
+        }
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+        if (i + 32 * k < last) {
+          double each = 0.0;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            each += mass(head + (i + 32 * k) * VEC + e, to_f32(pv[k].v[e]),
+                         drafter ? to_f32(qv[k].v[e]) : 0.0f);
+          sum += each;
+        }
+    }
     for (int w = 16; w; w /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
     __syncthreads();  // (the last pass's sums have been read)
     if (lane == 0) warp_sum[warp] = sum;
@@ -127,11 +185,38 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     return all;
   };
   auto best_of_row = [&]() -> Best {
-    Best best{0.0f, -1};
-    for (int t = begin + lane; t < end; t += 32) {
-      const float x = to_f32(target[current * p.ts[1] + t]);
-      best = better(best, x != x ? Best{0.0f, -2} : x == -INFINITY ? Best{0.0f, -1} : Best{x, t});
+    set_row(current);
+    // the largest value of a lane, its place (the lowest, as they come in order), NaN
+    float top = -INFINITY;
+    int where = -1;
+    bool nan = false;
+    auto take = [&](int t, float x) {
+      nan = nan || x != x;
+      if (x > top) {
+        top = x;
+        where = t;
+      }
+    };
+    int from, to;
+    singles(false, from, to);
+    for (int t = from + lane; t < to; t += 32) take(t, to_f32(p_row[t]));
+    for (int i = first + lane; i < last; i += 32 * kLoads) {
+      Vec pv[kLoads];
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+        if (i + 32 * k < last)
+          *reinterpret_cast<uint4*>(&pv[k]) =
+              *reinterpret_cast<const uint4*>(p_row + head + (int64_t)(i + 32 * k) * VEC);
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+        if (i + 32 * k < last) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) take(head + (i + 32 * k) * VEC + e, to_f32(pv[k].v[e]));
+        }
     }
+    singles(true, from, to);
+    for (int t = from + lane; t < to; t += 32) take(t, to_f32(p_row[t]));
+    Best best{top, nan ? -2 : where};
     for (int w = 16; w; w /= 2)
       best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.value, w),
                                __shfl_xor_sync(0xffffffffu, best.index, w)});
@@ -234,22 +319,49 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
         upto += warp_sum[w];
       }
       if (mine == warp) {
-        int found = -1, last = -1;
-        for (int t0 = begin; t0 < end && found < 0; t0 += 32) {
-          const double x = t0 + lane < end ? mass_at(t0 + lane) : 0.0;
-          double run = x;
+        int found = -1, last_one = -1;
+        // the next elements in their order, N of each lane from t0 + lane N on
+        auto look = [&](int t0, int end, auto count) {
+          constexpr int N = decltype(count)::value;
+          double x[N], run = 0.0;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const int t = t0 + lane * N + e;
+            x[e] = t < end ? mass_at(t) : 0.0;
+            run += x[e];
+          }
+          const double own = run;
           for (int w = 1; w < 32; w *= 2) {
             const double y = __shfl_up_sync(0xffffffffu, run, w);
             if (lane >= w) run += y;
           }
-          const uint32_t hit = __ballot_sync(0xffffffffu, x > 0.0 && before + run > mark);
-          const uint32_t any = __ballot_sync(0xffffffffu, x > 0.0);
-          if (hit) found = t0 + __ffs(hit) - 1;
-          if (any) last = t0 + 31 - __clz(any);
+          int hit = -1, any = -1;
+          double upto_here = before + (run - own);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            upto_here += x[e];
+            if (x[e] > 0.0) {
+              any = t0 + lane * N + e;
+              if (hit < 0 && upto_here > mark) hit = any;
+            }
+          }
+          const uint32_t hits = __ballot_sync(0xffffffffu, hit >= 0);
+          const uint32_t some = __ballot_sync(0xffffffffu, any >= 0);
+          if (hits) found = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+          if (some) last_one = __shfl_sync(0xffffffffu, any, 31 - __clz(some));
           before += __shfl_sync(0xffffffffu, run, 31);
-        }
+        };
+        int from, to;
+        singles(false, from, to);
+        for (int t = from; t < to && found < 0; t += 32)
+          look(t, to, std::integral_constant<int, 1>{});
+        for (int i = first; i < last && found < 0; i += 32)
+          look(head + i * VEC, head + last * VEC, std::integral_constant<int, VEC>{});
+        singles(true, from, to);
+        for (int t = from; t < to && found < 0; t += 32)
+          look(t, to, std::integral_constant<int, 1>{});
         // (roundings can leave the mark behind the last of them)
-        if (lane == 0) new_tokens[count - 1] = found >= 0 ? found : last;
+        if (lane == 0) new_tokens[count - 1] = found >= 0 ? found : last_one;
       }
     }
   }
@@ -263,9 +375,9 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
 }
 
 template <class T>
-int launch(const VerifyDrafts& p, cudaStream_t st) {
+int launch(const VerifyDrafts& p, const DeviceInfo& dev, cudaStream_t st) {
   int ctas = kMostCtas;
-  while (ctas > 1 && p.vocab < ctas * 2048) ctas /= 2;
+  while (ctas > 1 && (p.vocab < ctas * 2048 || p.batch * ctas > kCtasSm * dev.sm_count)) ctas /= 2;
   if (p.batch * ctas >= 1ll << 31) return CT_ERR_INVALID_ARGUMENT;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)(p.batch * ctas));
@@ -287,8 +399,8 @@ int launch(const VerifyDrafts& p, cudaStream_t st) {
 
 }  // namespace
 
-int launch_verify_drafts(const VerifyDrafts& p, const DeviceInfo&, cudaStream_t st) {
-  return with_dtype(p.dtype, [&](auto t) { return launch<decltype(t)>(p, st); });
+int launch_verify_drafts(const VerifyDrafts& p, const DeviceInfo& dev, cudaStream_t st) {
+  return with_dtype(p.dtype, [&](auto t) { return launch<decltype(t)>(p, dev, st); });
 }
 
 }  // namespace ct
