@@ -106,13 +106,15 @@ int make_tmap_f32(CUtensorMap* map, const void* base, int rank, const uint64_t* 
 }
 
 int make_tmap_pages(CUtensorMap* map, const void* base, int dtype, int64_t pages, int64_t heads,
-                    int64_t page_size, int64_t head_dim, const int64_t strides[3], int rows) {
+                    int64_t page_size, int64_t head_dim, const int64_t strides[3], int rows,
+                    int box_heads) {
   std::call_once(g_encode_once, load_encode);
   if (!g_encode) return CT_ERR_CUDA;
   const int64_t bytes = dtype == CT_DTYPE_F32 ? 4 : 2, row = head_dim * bytes;
   const cuuint64_t gd[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)heads,
                             (cuuint64_t)pages};
-  const cuuint32_t bd[4] = {(cuuint32_t)((row < 128 ? row : 128) / bytes), (cuuint32_t)rows, 1, 1};
+  const cuuint32_t bd[4] = {(cuuint32_t)((row < 128 ? row : 128) / bytes), (cuuint32_t)rows,
+                            (cuuint32_t)box_heads, 1};
   const cuuint32_t es[4] = {1, 1, 1, 1};
   cuuint64_t gs[3];
   for (int i = 0; i < 3; ++i) {  // slot, head, page

@@ -34,10 +34,11 @@ int make_tmap_f32(CUtensorMap* map, const void* base, int rank, const uint64_t* 
 
 // Encodes a TMA descriptor for the pages of a cache: [page, kv_head, slot, dim]
 // of a CT_DTYPE_*, read in boxes of 128 bytes of a row (64 of a shorter row)
-// times `rows` slots of one page and head, swizzled over that many bytes.
-// strides are in elements; those of single-element dimensions are not looked at.
+// times `rows` slots times `box_heads` heads of one page, swizzled over that many
+// bytes.  strides are in elements; those of single-element dimensions are not looked at.
 int make_tmap_pages(CUtensorMap* map, const void* base, int dtype, int64_t pages, int64_t heads,
-                    int64_t page_size, int64_t head_dim, const int64_t strides[3], int rows);
+                    int64_t page_size, int64_t head_dim, const int64_t strides[3], int rows,
+                    int box_heads = 1);
 
 // True when a float tensor with these element strides (innermost first
 // omitted) can be described by a TMA map: unit inner stride, 16-byte aligned

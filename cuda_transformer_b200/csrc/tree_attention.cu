@@ -174,6 +174,114 @@ __device__ __forceinline__ uint32_t chunk_pos(int r, int c) {
   return (uint32_t)(r * ROW_BYTES + ((c ^ (r >> 1 & 3)) << 4));  // 64-byte rows
 }
 
+// A part's q into shared memory: rows of 16-byte chunks as the cache's type, or its
+// terms one behind the other; and the rows' first mask words.
+template <class K>
+__device__ __forceinline__ void load_rows(const Launch& a, const Cursor& c, int row0, char* shared,
+                                       uint2* mask_words) {
+  using C = typename K::C;
+  using A = typename K::A;
+  constexpr int D = K::D, kEight = D / 8;
+  const TreeAttention& p = a.p;
+  const int tid = threadIdx.x, head = c.head, drafts = c.drafts;
+  const int64_t b = c.b;
+  for (int r = tid; r < K::kRows; r += kThreads) {
+    const int i = token_of(a, row0 + r);
+    mask_words[r] = make_uint2(mask_word(p, b, i, 0), mask_word(p, b, i, 1));
+  }
+  constexpr int kPieces = K::kRows * kEight;
+  constexpr int kBatch = kPieces / kThreads < 1 ? 1 : kPieces / kThreads < 4 ? kPieces / kThreads : 4;
+  constexpr int kWords = sizeof(A) == 2 ? 1 : 2;
+  for (int e0 = tid; e0 < kPieces; e0 += kBatch * kThreads) {
+    uint4 in[kBatch][kWords];  // 8 elements
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int r = (e0 + k * kThreads) / kEight, d = (e0 + k * kThreads) % kEight * 8;
+      const int i = token_of(a, row0 + r), h = head * a.group + (row0 + r) - i * a.group;
+      const A* src = (const A*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        in[k][w] = make_uint4(0u, 0u, 0u, 0u);
+        if (i < drafts) {
+          if (a.q_vectors) {
+            in[k][w] = reinterpret_cast<const uint4*>(src + d)[w];
+          } else {
+            in[k][w] = gather8(src + (d + w * 4) * p.qs[3], p.qs[3]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int r = (e0 + k * kThreads) / kEight, d = (e0 + k * kThreads) % kEight * 8;
+      if constexpr (sizeof(A) == 2) {
+        const uint32_t sign = a.negative ? 0x80008000u : 0u;
+        const uint4 w = in[k][0];
+        *reinterpret_cast<uint4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 8)) =
+            make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
+      } else {
+        float x[8];
+        *reinterpret_cast<uint4*>(x) = in[k][0];
+        *reinterpret_cast<uint4*>(x + 4) = in[k][kWords - 1];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) x[y] = a.negative ? -x[y] : x[y];
+        if constexpr (K::kF32) {
+          *reinterpret_cast<float4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 4)) =
+              *reinterpret_cast<float4*>(x);
+          *reinterpret_cast<float4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 4 + 1)) =
+              *reinterpret_cast<float4*>(x + 4);
+        } else {
+#pragma unroll
+          for (int t = 0; t < K::kTerms; ++t) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = take_term<C>(x[2 * j], x[2 * j + 1]);
+            *reinterpret_cast<uint4*>(shared + t * K::kRows * K::kRowBytes +
+                                      chunk_pos<K::kRowBytes, K::kRows>(r, d / 8)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// A tile, chunk by chunk (pages that TMA boxes do not fit); whether a page of this
+// lane's is out of range.
+template <class K>
+__device__ __forceinline__ bool copy_chunks(const Launch& a, const Cursor& next, uint32_t k_tile) {
+  using C = typename K::C;
+  const TreeAttention& p = a.p;
+  const int lane = threadIdx.x % 32, len = next.context + next.drafts, from = next.tile * K::kKeys;
+  const uint32_t v_tile = k_tile + K::kTileBytes;
+  auto page_of = [&](int position, int& slot) {
+    const int index = a.page_shift >= 0 ? position >> a.page_shift : position / p.kv.page_size;
+    slot = position - index * p.kv.page_size;
+    return index;
+  };
+  const int chunk = lane % K::kChunks;
+  const C* kh = (const C*)p.kv.k + next.head * p.kv.ks[1] + chunk * (16 / (int)sizeof(C));
+  const C* vh = (const C*)p.kv.v + next.head * p.kv.vs[1] + chunk * (16 / (int)sizeof(C));
+  bool bad = false;
+#pragma unroll 4
+  for (int i = 0; i < K::kKeys * K::kChunks / 32; ++i) {
+    const int row = i * (32 / K::kChunks) + lane / K::kChunks;
+    int slot;
+    const int index = page_of(from + row, slot);
+    const bool in = from + row < len;
+    const int64_t page = in ? p.kv.table[next.b * p.kv.table_s + index] : -1;
+    const bool fine = in && page >= 0 && page < p.kv.pages;
+    bad = bad || (in && !fine);
+    const uint32_t at = chunk_pos<K::kRowBytes, K::kKeys>(row, chunk);
+    // (nothing is read where there is no page)
+    const void* k = fine ? (const void*)(kh + page * p.kv.ks[0] + slot * p.kv.ks[2]) : p.out;
+    const void* v = fine ? (const void*)(vh + page * p.kv.vs[0] + slot * p.kv.vs[2]) : p.out;
+    cp_async16(k_tile + at, k, fine ? 16 : 0);
+    cp_async16(v_tile + at, v, fine ? 16 : 0);
+  }
+  return bad;
+}
+
 template <class K>
 __global__ void __launch_bounds__(kThreads, 2)
     tree_attention_kernel(const __grid_constant__ Launch a, const __grid_constant__ CUtensorMap k_map,
@@ -187,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   float(*const stat)[K::WK][K::kRows] =
       reinterpret_cast<float(*)[K::WK][K::kRows]>(shared + K::kJoinBytes);
   __shared__ Finder finder;
+  __shared__ uint2 mask_words[K::kRows];
   __shared__ alignas(8) uint64_t full[K::WK][K::kStages], empty[K::WK][K::kStages];
   __shared__ int stage_bad[K::WK][K::kStages];
   __shared__ CtaCtl ctl;
@@ -219,15 +328,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   // ---- this CTA's share of the units
   int64_t share_units, within;
   Cursor next = first_place<K>(a, share, finder, share_units, within);
-  // the first part that has rows in this block
-  auto settle = [&](Cursor& c, bool ok) {
-    while (ok && block * K::kRows >= c.drafts * a.group) {
-      ++c.head;
-      ok = enter<K>(a, c, 0);
-    }
-    return ok;
-  };
-  bool more = settle(next, enter<K>(a, next, within));
+  const int row0 = block * K::kRows;  // row r: token (row0 + r) / group, head (row0 + r) % group
+  bool more = enter<K>(a, next, within, row0);
   Cursor cur = next;
 
   // ---- copies: the group's first warp fetches the tiles that are its group's, as
@@ -251,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto to_own_tile = [&]() {
     while (more_in && next.tile >= next.stop) {
       ++next.head;
-      more_in = settle(next, enter<K>(a, next, 0));
+      more_in = enter<K>(a, next, 0, row0);
       next.tile += wk;
     }
     if (more_in && a.box) look_up();
@@ -288,27 +390,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     } else {
-      const int chunk = lane % K::kChunks;
-      const C* kh = (const C*)p.kv.k + next.head * p.kv.ks[1] + chunk * (16 / (int)sizeof(C));
-      const C* vh = (const C*)p.kv.v + next.head * p.kv.vs[1] + chunk * (16 / (int)sizeof(C));
-      bool bad = false;
-#pragma unroll 4
-      for (int i = 0; i < K::kKeys * K::kChunks / 32; ++i) {
-        const int row = i * (32 / K::kChunks) + lane / K::kChunks;
-        int slot;
-        const int index = page_of(from + row, slot);
-        const bool in = from + row < len;
-        const int64_t page = in ? p.kv.table[next.b * p.kv.table_s + index] : -1;
-        const bool fine = in && page >= 0 && page < p.kv.pages;
-        bad = bad || (in && !fine);
-        const uint32_t at = chunk_pos<K::kRowBytes, K::kKeys>(row, chunk);
-        // (nothing is read where there is no page)
-        const void* k = fine ? (const void*)(kh + page * p.kv.ks[0] + slot * p.kv.ks[2]) : p.out;
-        const void* v = fine ? (const void*)(vh + page * p.kv.vs[0] + slot * p.kv.vs[2]) : p.out;
-        cp_async16(k_tile + at, k, fine ? 16 : 0);
-        cp_async16(v_tile + at, v, fine ? 16 : 0);
-      }
-      bad = __any_sync(0xffffffffu, bad);
+      const bool bad = __any_sync(0xffffffffu, copy_chunks<K>(a, next, k_tile));
       if (lane == 0) {
         stage_bad[wk][stage] = bad;
         mbar_arrive(bar);
@@ -319,62 +401,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     next.tile += K::WK;
     to_own_tile();
   };
-  // q: rows of 16-byte chunks as the cache's type, or its terms one behind the other
-  constexpr int kEight = D / 8;
-  auto load_q = [&](int64_t b, int head, int drafts) {
-    const int row0 = block * K::kRows;
-    for (int e = tid; e < K::kRows * kEight; e += kThreads) {
-      const int r = e / kEight, d = e % kEight * 8;
-      const int i = (row0 + r) / a.group, h = head * a.group + (row0 + r) % a.group;
-      const A* src = (const A*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
-      if constexpr (sizeof(A) == 2) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (i < drafts) {
-          if (a.q_vectors) {
-            w = *reinterpret_cast<const uint4*>(src + d);
-          } else {
-            alignas(16) A x[8];
-            for (int j = 0; j < 8; ++j) x[j] = src[(d + j) * p.qs[3]];
-            w = *reinterpret_cast<const uint4*>(x);
-          }
-        }
-        const uint32_t sign = a.negative ? 0x80008000u : 0u;
-        *reinterpret_cast<uint4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 8)) =
-            make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
-      } else {
-        float x[8];
-        if (i < drafts && a.q_vectors) {
-          *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src + d);
-          *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(src + d + 4);
-        } else {
-          for (int j = 0; j < 8; ++j) x[j] = i < drafts ? src[(d + j) * p.qs[3]] : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = a.negative ? -x[j] : x[j];
-        if constexpr (K::kF32) {
-          *reinterpret_cast<float4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 4)) =
-              *reinterpret_cast<float4*>(x);
-          *reinterpret_cast<float4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 4 + 1)) =
-              *reinterpret_cast<float4*>(x + 4);
-        } else {
-#pragma unroll
-          for (int t = 0; t < K::kTerms; ++t) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = take_term<C>(x[2 * j], x[2 * j + 1]);
-            *reinterpret_cast<uint4*>(shared + t * K::kRows * K::kRowBytes +
-                                      chunk_pos<K::kRowBytes, K::kRows>(r, d / 8)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-    }
-  };
   if (leader) {
     next.tile += wk;
     to_own_tile();
   }
-  if (more) load_q(cur.b, cur.head, cur.drafts);
+  if (more) load_rows<K>(a, cur, row0, shared, mask_words);
   if (leader) {
 #pragma unroll 1
     for (int s = 0; s < K::kStages && more_in; ++s) copy_in();
@@ -386,7 +417,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int context = cur.context, drafts = cur.drafts;
     const int64_t b = cur.b;
     const int head = cur.head, part0 = cur.tile, part1 = cur.stop, tiles = cur.tiles;
-    const int row0 = block * K::kRows;  // row r: token (row0 + r) / group, head (row0 + r) % group
     __syncthreads();  // q has been written
 
     float o[MT][D / 8][4], base[MT][2], sum[MT][2];
@@ -401,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // a thread's rows: warp_row + 16 m + lane / 4, and 8 below
     const int warp_row = wr * 16 * MT;
     auto seen = [&](int r, int position) {
-      return seen_from(p, b, (row0 + r) / a.group, position - context, drafts);
+      return seen_from(p, mask_words[r], b, token_of(a, row0 + r), position - context, drafts);
     };
 
 #pragma unroll 1
@@ -519,7 +549,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             __syncwarp();
           }
           // values that are not finite, where not all rows see them
-          for (int e = lane; e < K::kBlock * K::kChunks; e += 32) {
+          const int scanned = rows < K::kBlock ? rows : K::kBlock;
+          for (int e = max(0, context - position0) * K::kChunks + lane; e < scanned * K::kChunks; e += 32) {
             const uint4 w = *reinterpret_cast<const uint4*>(
                 v_at + chunk_pos<K::kRowBytes, K::kKeys>(k0 + e / K::kChunks, e % K::kChunks));
             dirty = dirty || only_finite<C>(w.x) != w.x || only_finite<C>(w.y) != w.y ||
@@ -760,11 +791,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int r = warp_row + 16 * m + lane / 4 + 8 * h, i = (row0 + r) / a.group;
+          const int r = warp_row + 16 * m + lane / 4 + 8 * h, i = token_of(a, row0 + r);
           if (i >= drafts) continue;
           if (whole) {
             const float f = sum[m][h] == 0.0f ? 0.0f : 1.0f / sum[m][h];
-            const int64_t row = (b * p.drafts + i) * p.q_heads + head * a.group + (row0 + r) % a.group;
+            const int64_t row = (b * p.drafts + i) * p.q_heads + head * a.group + (row0 + r) - i * a.group;
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
               store2<A>(p.out, row * D + 8 * n + lane % 4 * 2, o[m][n][2 * h] * f,
@@ -789,8 +820,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncthreads();  // (the join has been read, q may be written)
     ++cur.head;
-    more = settle(cur, enter<K>(a, cur, 0));
-    if (more) load_q(cur.b, cur.head, cur.drafts);
+    more = enter<K>(a, cur, 0, row0);
+    if (more) load_rows<K>(a, cur, row0, shared, mask_words);
   }
   write_rows_not_there<K>(p);
   // after a wait that ran out: copies still on the way end before the memory is

@@ -35,6 +35,7 @@ __device__ __forceinline__ float ex2(float x) {
 struct Launch {
   TreeAttention p;
   int group, blocks;    // query heads of a key/value head; row blocks of an item
+  int group_shift;      // log2 of group, -1 when it is no power of two
   int shares;
   bool whole;           // an item a CTA: none is split
   bool q_vectors;       // q's rows are 16-byte vectors
@@ -46,6 +47,11 @@ struct Launch {
   int4* records;        // of each CTA: the split item that begins in it
   float* partials;
 };
+
+// The drafted token of an item's row.
+__device__ __forceinline__ int token_of(const Launch& a, int row) {
+  return a.group_shift >= 0 ? row >> a.group_shift : row / a.group;
+}
 
 struct Sequence {
   int context, drafts, tiles;
@@ -77,9 +83,10 @@ struct Cursor {
   int64_t left;                 // units of the share from this item's part on
 };
 
-// The item at (c.b, c.head), `within` units into it, or the next one there is.
+// The item at (c.b, c.head), `within` units into it, or the next one there is that
+// has rows behind row0.
 template <class K>
-__device__ __forceinline__ bool enter(const Launch& a, Cursor& c, int64_t within) {
+__device__ __forceinline__ bool enter(const Launch& a, Cursor& c, int64_t within, int row0) {
   while (c.left > 0 && c.b < a.p.batch) {
     const Sequence s = sequence<K>(a.p, c.b);
     if (s.tiles == 0 || c.head == (int)a.p.kv_heads) {
@@ -97,7 +104,7 @@ __device__ __forceinline__ bool enter(const Launch& a, Cursor& c, int64_t within
     c.context = s.context;
     c.drafts = s.drafts;
     within = 0;
-    if (c.tile < c.stop) return true;
+    if (c.tile < c.stop && row0 < c.drafts * a.group) return true;
     ++c.head;
   }
   return false;
@@ -167,22 +174,44 @@ __device__ __forceinline__ Cursor first_place(const Launch& a, int share, Finder
   return c;
 }
 
+// The first two words of a row's mask; both rows' and words' ends are looked at where
+// they are used.
+constexpr int kKeptWords = 2;
+__device__ __forceinline__ uint32_t mask_word(const TreeAttention& p, int64_t b, int i, int word) {
+  return p.mask && i < p.drafts && word * 32 < p.drafts ? p.mask[b * p.ms[0] + i * p.ms[1] + word] : 0u;
+}
+
 // Which of the 32 drafted tokens from number d on (d < 0: some before the draft) the
-// drafted token i of sequence b sees, as bits.
-__device__ __forceinline__ uint32_t seen_from(const TreeAttention& p, int64_t b, int i, int d,
-                                              int drafts) {
+// drafted token i of sequence b sees, as bits; kept: its first words.
+__device__ __forceinline__ uint32_t seen_from(const TreeAttention& p, uint2 kept, int64_t b, int i, int d,
+                                           int drafts) {
   if (d <= -32) return ~0u;
   if (i >= drafts || d >= drafts) return d < 0 ? (1u << -d) - 1u : 0u;
   uint32_t w;
   if (p.mask) {
-    const uint32_t* words = p.mask + b * p.ms[0] + i * p.ms[1];
     const int at = d < 0 ? 0 : d >> 5, last = (drafts - 1) >> 5;
-    const uint32_t low = words[at], high = at < last ? words[at + 1] : 0u;
+    uint32_t low, high;
+    if (last < kKeptWords) {
+      low = at == 0 ? kept.x : kept.y;
+      high = at < last ? kept.y : 0u;
+    } else {
+      const uint32_t* words = p.mask + b * p.ms[0] + i * p.ms[1];
+      low = words[at];
+      high = at < last ? words[at + 1] : 0u;
+    }
     w = d < 0 ? low << -d | ((1u << -d) - 1u) : __funnelshift_r(low, high, d & 31);
   } else {
     w = i < d ? 0u : i - d >= 31 ? ~0u : (2u << (i - d)) - 1u;
   }
   return drafts - d >= 32 ? w : w & ((1u << (drafts - d)) - 1u);
+}
+
+// Eight 16-bit (four 32-bit) elements that lie `stride` apart.
+template <class A>
+__device__ __noinline__ uint4 gather8(const A* src, int64_t stride) {
+  alignas(16) A x[16 / sizeof(A)];
+  for (int e = 0; e < 16 / (int)sizeof(A); ++e) x[e] = src[e * stride];
+  return *reinterpret_cast<const uint4*>(x);
 }
 
 template <class A>
@@ -231,7 +260,7 @@ __global__ void __launch_bounds__(kJoinRows * 32)
   const int4 rec = a.records[cta];
   if (rec.x == 0) return;
   const int r = blockIdx.y * kJoinRows + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int i = (block * rows + r) / a.group;
+  const int i = token_of(a, block * rows + r);
   if (i >= rec.w) return;
   const int64_t each = partial_floats(rows, D);
   // the first part ends its CTA's share, the others begin theirs
@@ -258,7 +287,7 @@ __global__ void __launch_bounds__(kJoinRows * 32)
   }
   const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
   const int64_t row = ((int64_t)rec.y * a.p.drafts + i) * a.p.q_heads + rec.z * a.group +
-                      (block * rows + r) % a.group;
+                      (block * rows + r) - i * a.group;
 #pragma unroll
   for (int e = 0; e < N; ++e) ((A*)a.p.out)[row * D + lane * N + e] = from_f32<A>(o[e] * f);
   if (lane == 0 && a.p.lse) a.p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
@@ -298,9 +327,12 @@ inline Launch begin_launch(const TreeAttention& p, const DeviceInfo& dev) {
   const int64_t align = 16 / dtype_bytes(p.act_dtype);
   a.q_vectors = aligned16(p.q) && p.qs[0] % align == 0 && p.qs[1] % align == 0 &&
                 p.qs[2] % align == 0 && p.qs[3] == 1;
+  a.group_shift = -1;
   a.page_shift = -1;
-  for (int s = 0; s < 31; ++s)
-    if (p.kv.page_size == 1 << s) a.page_shift = s;
+  for (int s = 0; s < 31; ++s) {
+      if (p.kv.page_size == 1 << s) a.page_shift = s;
+      if (a.group == 1 << s) a.group_shift = s;
+    }
   a.records = reinterpret_cast<int4*>(p.ws);
   a.partials = reinterpret_cast<float*>(a.records + kMaxCtas);
   return a;

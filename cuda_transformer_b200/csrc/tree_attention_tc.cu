@@ -51,7 +51,7 @@ struct Bars {
   // of a buffer: S is there, the weights are, their product is in O (the rows' threads
   // may be two products behind: one barrier's parity would not tell them apart)
   uint64_t s_full[2], p_ready[2], pv_done[2];
-  uint64_t q_ready, last;
+  uint64_t q_ready, q_free, last;  // q is there; its last product is done
   CtaCtl ctl;
   int bad[kBad];   // of a tile: a page out of range
   int skip[2];     // of a buffer: O has been formed by the rows' threads
@@ -112,11 +112,60 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (uint32_t)((c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// O += weights V of one tile without the tensor core, for the tokens that a row sees
+// (fresh: O = ...).  All threads of a warp.
+template <class K>
+__device__ __noinline__ void add_tile(uint32_t lanes, const float* each, uint32_t sees0,
+                                      uint32_t sees1, const char* v, int rows, bool fresh) {
+  using C = typename K::C;
+#pragma unroll 1
+  for (int d = 0; d < K::D; d += 16) {
+    float o[16];
+    if (fresh) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+    } else {
+      tmem_ld16(lanes + d, o);
+    }
+#pragma unroll 1
+    for (int k = 0; k < rows; ++k) {
+      if (!((k < 32 ? sees0 : sees1) >> (k & 31) & 1u)) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        o[e] += each[k] * to_f32(((const C*)(v + chunk_at<K::kKeys>(k, (d + e) / 8)))[e % 8]);
+    }
+    __syncwarp();
+    tmem_st16(lanes + d, o);
+  }
+}
+
+// The rows' q into shared memory by threads 0 .. 127, where TMA does not do it (odd
+// groups, strides that are no vectors, a negative scale).
+template <class K>
+__device__ __forceinline__ void load_rows(const Launch& a, const Cursor& c, int row0, char* shared) {
+  using C = typename K::C;
+  const TreeAttention& p = a.p;
+  const int rows = min(K::kRows, c.drafts * a.group - row0);
+  const uint32_t sign = a.negative ? 0x80008000u : 0u;
+#pragma unroll 1
+  for (int e = threadIdx.x; e < rows * K::kChunks; e += 128) {
+    const int r = e / K::kChunks, d = e % K::kChunks * 8;
+    const int i = token_of(a, row0 + r), h = c.head * a.group + (row0 + r) - i * a.group;
+    const C* src = (const C*)p.q + c.b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+    const uint4 w = a.q_vectors ? *reinterpret_cast<const uint4*>(src + d)
+                                : gather8(src + d * p.qs[3], p.qs[3]);
+    *reinterpret_cast<uint4*>(shared + chunk_at<K::kRows>(r, d / 8)) =
+        make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
+  }
+}
+
 template <class K>
 __global__ void __launch_bounds__(kThreads, 2)
     tree_attention_tc_kernel(const __grid_constant__ Launch a,
                              const __grid_constant__ CUtensorMap k_map,
-                             const __grid_constant__ CUtensorMap v_map, const int slot_rows) {
+                             const __grid_constant__ CUtensorMap v_map,
+                             const __grid_constant__ CUtensorMap q_map, const int slot_rows,
+                             const int q_rows) {
   using C = typename K::C;
   constexpr int D = K::D;
   extern __shared__ __align__(1024) char shared[];
@@ -133,6 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     bars.raised = *reinterpret_cast<const volatile uint32_t*>(a.status) != 0u;
     tma_prefetch_desc(&k_map);
     tma_prefetch_desc(&v_map);
+    if (q_rows > 0) tma_prefetch_desc(&q_map);
     for (int u = 0; u < K::kUnits; ++u) {
       mbar_init(B(bars.full[u]), 1);
       mbar_init(B(bars.empty[u]), 1);
@@ -142,7 +192,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(B(bars.p_ready[i]), 4);
       mbar_init(B(bars.pv_done[i]), 1);
     }
-    mbar_init(B(bars.q_ready), 4);
+    mbar_init(B(bars.q_ready), q_rows > 0 ? 1 : 4);
+    mbar_init(B(bars.q_free), 1);
     mbar_init(B(bars.last), 1);
     ctl->abort = 0u;
     fence_barrier_init();
@@ -158,17 +209,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem_base;
-  auto settle = [&](Cursor& c, bool ok) {
-    while (ok && row0 >= c.drafts * a.group) {
-      ++c.head;
-      ok = enter<K>(a, c, 0);
-    }
-    return ok;
-  };
-  bool more = !bars.raised && settle(cur, enter<K>(a, cur, within));
+  bool more = !bars.raised && enter<K>(a, cur, within, row0);
   auto next_part = [&]() {
     ++cur.head;
-    more = settle(cur, enter<K>(a, cur, 0));
+    more = enter<K>(a, cur, 0, row0);
   };
   auto wait = [&](const uint64_t& bar, uint32_t parity) {
     return mbar_wait(smem_u32(&bar), parity, ctl, a.status);
@@ -183,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 4) {
     // ------------------------------------------------------------ producer
-    uint32_t unit = 0, tile_count = 0;
+    uint32_t unit = 0, tile_count = 0, part = 0;
     const int row = lane * a.box;  // lane's box of a tile
     bool ok = true;
     auto page_of = [&](int position, int& slot) {
@@ -226,6 +270,16 @@ __global__ void __launch_bounds__(kThreads, 2)
         ++unit;
       };
       int now = look_up(0), next = look_up(1);
+      if (q_rows > 0) {  // q_rows rows of whole tokens, as rows (token, head) of the box
+        if (part > 0) ok = ok && warp_wait(bars.q_free, (part - 1) & 1);
+        if (ok && lane == 0) {
+          mbar_arrive_expect_tx(B(bars.q_ready), q_rows * K::kRowBytes);
+          for (int h = 0; h < K::kParts; ++h)
+            tma_load_4d(q_smem + h * (K::kRows * 128), &q_map, B(bars.q_ready), 64 * h,
+                        cur.head * a.group, token_of(a, row0), (int)cur.b);
+        }
+        ++part;
+      }
       fetch(0, now, true);
       for (int t = 0; t < T && ok; ++t) {
         const int after = look_up(t + 2);
@@ -263,6 +317,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                         sdesc_kmajor(k + s / 4 * (K::kKeys * 128) + s % 4 * 32), kIdescS, s > 0);
           umma_commit(B(bars.empty[u]));
           umma_commit(B(bars.s_full[buf]));
+          if (t == T - 1) umma_commit(B(bars.q_free));
         };
         ok = ok && wait(bars.q_ready, part & 1);
         issue_s(0);
@@ -305,24 +360,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar));
     };
+    uint2 kept = make_uint2(0u, 0u);  // the row's mask
     auto load_q = [&]() {
-      const int rows = min(K::kRows, cur.drafts * a.group - row0);
-      for (int e = tid; e < rows * K::kChunks; e += 128) {
-        const int r = e / K::kChunks, d = e % K::kChunks * 8;
-        const int i = (row0 + r) / a.group, h = cur.head * a.group + (row0 + r) % a.group;
-        const C* src = (const C*)p.q + cur.b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
-        uint4 w;
-        if (a.q_vectors) {
-          w = *reinterpret_cast<const uint4*>(src + d);
-        } else {
-          alignas(16) C x[8];
-          for (int k = 0; k < 8; ++k) x[k] = src[(d + k) * p.qs[3]];
-          w = *reinterpret_cast<const uint4*>(x);
-        }
-        const uint32_t sign = a.negative ? 0x80008000u : 0u;
-        *reinterpret_cast<uint4*>(shared + chunk_at<K::kRows>(r, d / 8)) =
-            make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
-      }
+      const int i = token_of(a, row0 + tid);
+      kept = make_uint2(mask_word(p, cur.b, i, 0), mask_word(p, cur.b, i, 1));
+      if (q_rows > 0) return;  // TMA does it
+      load_rows<K>(a, cur, row0, shared);
       fence_proxy_async_smem();
       arrive(bars.q_ready);
     };
@@ -331,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int64_t b = cur.b;
       const int head = cur.head, context = cur.context, drafts = cur.drafts;
       const int part0 = cur.tile, tiles = cur.tiles, T = cur.stop - cur.tile;
-      const int r = row0 + tid, i = r / a.group;
+      const int r = row0 + tid, i = token_of(a, r);
       const bool active = row0 + 32 * warp < drafts * a.group, there = i < drafts;
       float* const slot = a.partials + ((int64_t)blockIdx.x * 2 + (part0 == 0 ? 1 : 0)) *
                                            partial_floats(slot_rows, D);
@@ -356,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (masked) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            sees[h] = seen_from(p, b, i, position + 32 * h - context, drafts);
+            sees[h] = seen_from(p, kept, b, i, position + 32 * h - context, drafts);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!(sees[h] >> e & 1u)) s[h][e] = -INFINITY;
@@ -406,10 +449,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (!(ok = warp_wait(bars.full[u], n / K::kUnits & 1))) break;
           char* const v = shared + K::kQBytes + u * K::kUnit;
           const int rows = min(K::kKeys, context + drafts - position);
-          for (int e = rows * K::kChunks + lane; e < K::kKeys * K::kChunks; e += 32)
+          const int zeroers = min(4, (drafts * a.group - row0 + 31) / 32);  // active warps
+          for (int e = rows * K::kChunks + tid; e < K::kKeys * K::kChunks; e += 32 * zeroers)
             *reinterpret_cast<uint4*>(v + chunk_at<K::kKeys>(e / K::kChunks, e % K::kChunks)) =
                 make_uint4(0u, 0u, 0u, 0u);
-          for (int e = lane; e < rows * K::kChunks; e += 32) {
+          for (int e = max(0, context - position) * K::kChunks + lane; e < rows * K::kChunks; e += 32) {
             const uint4 x = *reinterpret_cast<const uint4*>(
                 v + chunk_at<K::kKeys>(e / K::kChunks, e % K::kChunks));
             dirty = dirty || not_finite<C>(x.x) || not_finite<C>(x.y) || not_finite<C>(x.z) ||
@@ -423,27 +467,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             float each[K::kKeys];
 #pragma unroll
             for (int e = 0; e < K::kKeys; ++e) each[e] = s[e / 32][e % 32];
-#pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-              float o[32];
-              if (fresh) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-              } else {
-                tmem_ld32(lanes + d, o);
-              }
-#pragma unroll 1
-              for (int k = 0; k < rows; ++k) {
-                if (!((k < 32 ? sees[0] : sees[1]) >> (k & 31) & 1u)) continue;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const C* x = (const C*)(v + chunk_at<K::kKeys>(k, (d + e) / 8));
-                  o[e] += each[k] * to_f32(x[(d + e) % 8]);
-                }
-              }
-              __syncwarp();
-              tmem_st32(lanes + d, o);
-            }
+            add_tile<K>(lanes, each, sees[0], sees[1], v, rows, fresh);
           }
         }
         if (lane == 0) *(volatile int*)&bars.skip[buf] = dirty;
@@ -488,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (active) {
         const float f = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
         const float g = has_flushed && flushed > -INFINITY ? ex2(flushed - base) : 0.0f;
-        const int64_t row = (b * p.drafts + i) * p.q_heads + head * a.group + r % a.group;
+        const int64_t row = (b * p.drafts + i) * p.q_heads + head * a.group + r - i * a.group;
 #pragma unroll 1
         for (int d = 0; d < D; d += 32) {
           float o[32];
@@ -559,9 +583,17 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
   CUtensorMap k_map{}, v_map{};
   make_maps(a, &k_map, &v_map, K::kKeys);
   if (a.box == 0) return kNoTc;
+  // q by TMA where a block's rows are whole tokens
+  CUtensorMap q_map{};
+  int q_rows = a.blocks == 1 ? (int)rows : K::kRows % a.group == 0 ? K::kRows : 0;
+  if (!a.q_vectors || a.negative || q_rows == 0 ||
+      make_tmap_pages(&q_map, p.q, p.act_dtype, p.batch, p.drafts, p.q_heads, K::D, p.qs, a.group,
+                      q_rows / a.group) != CT_OK)
+    q_rows = 0;
   const int slot_rows = rows >= K::kRows ? K::kRows : (int)(rows + 15) / 16 * 16;
   const unsigned grid = (unsigned)(shares * a.blocks);
-  tree_attention_tc_kernel<K><<<grid, kThreads, smem_bytes<K>(), st>>>(a, k_map, v_map, slot_rows);
+  tree_attention_tc_kernel<K><<<grid, kThreads, smem_bytes<K>(), st>>>(a, k_map, v_map, q_map, slot_rows,
+                                                                      q_rows);
   rc = check_launch();
   if (rc != CT_OK || a.whole) return rc;
   return launch_join<typename K::A, K::D>(a, grid, slot_rows, st);
