@@ -18,16 +18,21 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 // C: the cache's type; F32ACT: q and out are FP32, else of type C; MT: 16-row tiles
-// of a warp; WR: warps along the rows, a group.  The groups take turns at the tiles.
+// of a warp, 0 for 8 rows; WR: warps along the rows, a group.  The groups take turns
+// at the tiles.  With 8 rows two terms of q and of the weights share a product, in
+// rows 0-7 and 8-15, whose sums then sit in the same lane.
 template <class C_, bool F32ACT_, int D_, int MT_, int WR_>
 struct Cfg {
+  static constexpr bool kPack = MT_ == 0;
   using C = C_;
   static constexpr bool F32ACT = F32ACT_;
-  static constexpr int D = D_, MT = MT_, WR = WR_;
+  static constexpr int D = D_, MT = kPack ? 1 : MT_, WR = WR_;
+  static constexpr int kH = kPack ? 1 : 2;  // rows of a lane in a 16-row tile
   using A = std::conditional_t<F32ACT, float, C>;
   static constexpr bool kF32 = sizeof(C) == 4;
   static constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
-  static constexpr int kRows = 16 * MT * WR;
+  static constexpr int kRows = kPack ? 8 : 16 * MT * WR;
+  static constexpr int kCtas = kPack ? 3 : 2;  // of an SM
   static constexpr int WK = kWarps / WR;  // groups
   static constexpr int kRowBytes = D * (int)sizeof(C);
   static constexpr int kChunks = kRowBytes / 16;
@@ -42,15 +47,18 @@ struct Cfg {
   static constexpr int kTileBytes = kKeys * kRowBytes;  // K or V
   // 16-bit terms of q and of the weights (FP32 activations: 22 bits and more).
   static constexpr int kTerms = kF32 || !F32ACT ? 1 : kBf16 ? 3 : 2;
-  static constexpr int kQBytes = kTerms * kRows * kRowBytes;
+  // (packed: pairs of terms, 16 rows each)
+  static constexpr int kQTiles = kPack ? (kTerms + 1) / 2 : kTerms;
+  static constexpr int kQRows = kPack && !kF32 ? 16 : kRows;
+  static constexpr int kQBytes = kQTiles * kQRows * kRowBytes;
   static constexpr int kJoinDims = 32;
   static constexpr int kJoinBytes = WK > 1 ? (WK - 1) * kRows * kJoinDims * 4 : 0;
   static constexpr int kStatBytes = WK > 1 ? 2 * WK * kRows * 4 : 0;
   static constexpr int kHeadBytes =
       ((kQBytes > kJoinBytes + kStatBytes ? kQBytes : kJoinBytes + kStatBytes) + 1023) / 1024 * 1024;
-  // Stages of a group's ring: two CTAs an SM (228 KB, of which each takes 1 KB and
+  // Stages of a group's ring: kCtas CTAs an SM (228 KB, of which each takes 1 KB and
   // the static 1 KB; 1 KB more to begin at a whole one).
-  static constexpr int kFit = (110 * 1024 - kHeadBytes) / (2 * kTileBytes) / WK;
+  static constexpr int kFit = ((kPack ? 72 : 110) * 1024 - kHeadBytes) / (2 * kTileBytes) / WK;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static_assert(kStages >= 1 && kStages * WK >= 3, "tiles on the way");
   static constexpr int kSmem = 1024 + kHeadBytes + WK * kStages * 2 * kTileBytes;
@@ -217,7 +225,7 @@ __device__ __forceinline__ void load_rows(const Launch& a, const Cursor& c, int 
       if constexpr (sizeof(A) == 2) {
         const uint32_t sign = a.negative ? 0x80008000u : 0u;
         const uint4 w = in[k][0];
-        *reinterpret_cast<uint4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 8)) =
+        *reinterpret_cast<uint4*>(shared + chunk_pos<K::kRowBytes, K::kQRows>(r, d / 8)) =
             make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
       } else {
         float x[8];
@@ -236,8 +244,9 @@ __device__ __forceinline__ void load_rows(const Launch& a, const Cursor& c, int 
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = take_term<C>(x[2 * j], x[2 * j + 1]);
-            *reinterpret_cast<uint4*>(shared + t * K::kRows * K::kRowBytes +
-                                      chunk_pos<K::kRowBytes, K::kRows>(r, d / 8)) =
+            *reinterpret_cast<uint4*>(
+                shared + (K::kPack ? t / 2 : t) * K::kQRows * K::kRowBytes +
+                chunk_pos<K::kRowBytes, K::kQRows>(K::kPack ? r + t % 2 * 8 : r, d / 8)) =
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
@@ -283,7 +292,7 @@ __device__ __forceinline__ bool copy_chunks(const Launch& a, const Cursor& next,
 }
 
 template <class K>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, K::kCtas)
     tree_attention_kernel(const __grid_constant__ Launch a, const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map) {
   using C = typename K::C;
@@ -419,14 +428,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int head = cur.head, part0 = cur.tile, part1 = cur.stop, tiles = cur.tiles;
     __syncthreads();  // q has been written
 
-    float o[MT][D / 8][4], base[MT][2], sum[MT][2];
+    constexpr int H = K::kH;
+    float o[MT][D / 8][2 * H], base[MT][H], sum[MT][H];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.0f;
-      base[m][0] = base[m][1] = -INFINITY;
-      sum[m][0] = sum[m][1] = 0.0f;
+      for (int h = 0; h < H; ++h) {
+        base[m][h] = -INFINITY;
+        sum[m][h] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[m][n][2 * h] = o[m][n][2 * h + 1] = 0.0f;
+      }
     }
     // a thread's rows: warp_row + 16 m + lane / 4, and 8 below
     const int warp_row = wr * 16 * MT;
@@ -444,7 +456,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       const bool masked = (tile + 1) * K::kKeys > context;
       if (stage_bad[wk][stage]) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) sum[m][0] = sum[m][1] = NAN;
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < H; ++h) sum[m][h] = NAN;
       }
 
 #pragma unroll 1
@@ -462,6 +476,22 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int n = 0; n < NT; ++n)
               ldsm4(k[n], k_tile + chunk_pos<K::kRowBytes, K::kKeys>(k0 + 8 * n + lane % 8,
                                                                     4 * kk + lane / 8));
+            if constexpr (K::kPack) {  // q in rows 0-7, what TF32 leaves of it in 8-15
+              uint32_t q4[4];
+              ldsm4(q4, q_smem + chunk_pos<K::kRowBytes, K::kRows>(lane % 8, 4 * kk + lane / 8));
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint32_t qa[4] = {q4[2 * j], low_tf32(q4[2 * j]), q4[2 * j + 1],
+                                        low_tf32(q4[2 * j + 1])};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  const uint32_t b0 = k[n][2 * j], b1 = k[n][2 * j + 1];
+                  mma_next<C>(kk + j == 0, s[0][n], qa, b0, b1);
+                  mma_next<C>(kk + j == 0, rest[0][n], qa, low_tf32(b0), low_tf32(b1));
+                }
+              }
+              continue;
+            }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -491,10 +521,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-              for (int t = 0; t < K::kTerms; ++t) {
+              for (int t = 0; t < K::kQTiles; ++t) {
                 uint32_t qa[4];
-                ldsm4(qa, q_smem + t * K::kRows * K::kRowBytes +
-                              chunk_pos<K::kRowBytes, K::kRows>(warp_row + 16 * m + lane % 16,
+                ldsm4(qa, q_smem + t * K::kQRows * K::kRowBytes +
+                              chunk_pos<K::kRowBytes, K::kQRows>(warp_row + 16 * m + lane % 16,
                                                                 2 * ks + lane / 16));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -516,18 +546,22 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = s[m][n][e] + rest[m][n][e];
+              for (int e = 0; e < 2 * H; ++e) {
+                float others;
+                if constexpr (!K::kPack) others = rest[m][n][e];
+                else if constexpr (K::kF32) others = s[m][n][2 + e] + (rest[m][n][e] + rest[m][n][2 + e]);
+                else others = K::kTerms > 2 ? s[m][n][2 + e] + rest[m][n][e] : s[m][n][2 + e];
+                const float x = s[m][n][e] + others;
                 s[m][n][e] = x == x ? x : s[m][n][e];
               }
         }
         bool dirty = false;
-        uint32_t sees[MT][2];
+        uint32_t sees[MT][H];
         if (masked) {
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < H; ++h) {
               sees[m][h] = seen(warp_row + 16 * m + lane / 4 + 8 * h, position0);
               const uint32_t bits = sees[m][h] >> (lane % 4 * 2);
 #pragma unroll
@@ -561,11 +595,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 
         // ---- the exponents' base, weights
         bool raise = false;
-        float top[MT][2];
+        float top[MT][H];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < H; ++h) {
             float t = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[m][n][2 * h], s[m][n][2 * h + 1]));
@@ -578,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < H; ++h) {
               const float old = base[m][h];
               base[m][h] = top[m][h] > old + kMaxSlack ? top[m][h] : old;
               const float f = old == -INFINITY ? 0.0f : ex2(old - base[m][h]);
@@ -593,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < H; ++h) {
             const float from = base[m][h] == -INFINITY ? 0.0f : base[m][h];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -624,6 +658,13 @@ __global__ void __launch_bounds__(kThreads, 2)
               }
 #pragma unroll
               for (int m = 0; m < MT; ++m) {
+                if constexpr (K::kPack) {
+                  const uint32_t w0 = __float_as_uint(s[m][ks][0]), w1 = __float_as_uint(s[m][ks][1]);
+                  const uint32_t w[4] = {w0, low_tf32(w0), w1, low_tf32(w1)};
+                  mma_next<C>(ks == 0, acc[m], w, v[0], v[1]);
+                  mma<C>(acc[m], w, vl[0], vl[1]);
+                  continue;
+                }
                 const uint32_t w[4] = {__float_as_uint(s[m][ks][0]), __float_as_uint(s[m][ks][2]),
                                        __float_as_uint(s[m][ks][1]), __float_as_uint(s[m][ks][3])};
                 const uint32_t wl[4] = {low_tf32(w[0]), low_tf32(w[1]), low_tf32(w[2]), low_tf32(w[3])};
@@ -635,20 +676,28 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[m][n][e] += acc[m][e];
+              for (int e = 0; e < 2 * H; ++e)
+                o[m][n][e] += K::kPack ? acc[m][e] + acc[m][2 + e] : acc[m][e];
           }
         } else {
-          uint32_t w[MT][NT / 2][K::kTerms][4];
+          uint32_t w[MT][NT / 2][K::kQTiles][4];
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int ks = 0; ks < NT / 2; ++ks)
 #pragma unroll
-              for (int t = 0; t < K::kTerms; ++t)
+              for (int t = 0; t < K::kQTiles; ++t)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  w[m][ks][t][j] = take_term<C>(s[m][2 * ks + j / 2][j % 2 * 2],
-                                                s[m][2 * ks + j / 2][j % 2 * 2 + 1]);
+                for (int j = 0; j < 4; ++j) {
+                  if constexpr (K::kPack) {  // rows 0-7 and 8-15: two terms
+                    w[m][ks][t][j] = 2 * t + j % 2 >= K::kTerms
+                                         ? 0u
+                                         : take_term<C>(s[m][2 * ks + j / 2][0], s[m][2 * ks + j / 2][1]);
+                  } else {
+                    w[m][ks][t][j] = take_term<C>(s[m][2 * ks + j / 2][j % 2 * 2],
+                                                  s[m][2 * ks + j / 2][j % 2 * 2 + 1]);
+                  }
+                }
 #pragma unroll
           for (int n = 0; n < D / 16; ++n) {
             float acc[MT][2][4];
@@ -664,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
               for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int t = 0; t < K::kTerms; ++t) {
+                for (int t = 0; t < K::kQTiles; ++t) {
                   mma_next<C>(ks + t == 0, acc[m][0], w[m][ks][t], v[0], v[1]);
                   mma_next<C>(ks + t == 0, acc[m][1], w[m][ks][t], v[2], v[3]);
                 }
@@ -674,7 +723,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
               for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[m][2 * n + j][e] += acc[m][j][e];
+                for (int e = 0; e < 2 * H; ++e)
+                  o[m][2 * n + j][e] += K::kPack ? acc[m][j][e] + acc[m][j][2 + e] : acc[m][j][e];
           }
         }
         if (dirty) {  // infinities and NaN, for the rows that see their token
@@ -691,8 +741,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (!(fabsf(x) < INFINITY)) {
 #pragma unroll
                   for (int m = 0; m < MT; ++m) {
-                    if (sees[m][0] >> k & 1u) o[m][n][j] += x;
-                    if (sees[m][1] >> k & 1u) o[m][n][2 + j] += x;
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+                      if (sees[m][h] >> k & 1u) o[m][n][2 * h + j] += x;
                   }
                 }
               }
@@ -710,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < H; ++h) {
         sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
         sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 2);
       }
@@ -719,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < H; ++h)
           if (lane % 4 == 0) {
             stat[0][wk][warp_row + 16 * m + lane / 4 + 8 * h] = base[m][h];
             stat[1][wk][warp_row + 16 * m + lane / 4 + 8 * h] = sum[m][h];
@@ -728,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
           const int r = warp_row + 16 * m + lane / 4 + 8 * h;
           float top = -INFINITY, all = 0.0f;
 #pragma unroll
@@ -758,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int n = 0; n < K::kJoinDims / 8; ++n)
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
+              for (int h = 0; h < H; ++h)
                 *reinterpret_cast<float2*>(
                     join + (((wk - 1) * K::kRows + warp_row + 16 * m + lane / 4 + 8 * h) *
                                 K::kJoinDims + (8 * n ^ (lane / 4 % 4 * 8)) + lane % 4 * 2)) =
@@ -773,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
               for (int n = 0; n < K::kJoinDims / 8; ++n)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < H; ++h) {
                   const float2 x = *reinterpret_cast<const float2*>(
                       join + (((w - 1) * K::kRows + warp_row + 16 * m + lane / 4 + 8 * h) *
                                   K::kJoinDims + (8 * n ^ (lane / 4 % 4 * 8)) + lane % 4 * 2));
@@ -790,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
           const int r = warp_row + 16 * m + lane / 4 + 8 * h, i = token_of(a, row0 + r);
           if (i >= drafts) continue;
           if (whole) {
@@ -839,7 +890,7 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
   if (rc != CT_OK) return rc;
   a.blocks = (int)((p.drafts * a.group + K::kRows - 1) / K::kRows);
   const int64_t items = p.batch * p.kv_heads;
-  int ctas = 2 * dev.sm_count;
+  int ctas = K::kCtas * dev.sm_count;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   a.whole = p.kv.max_pages * p.kv.page_size <= kWholeTokens || a.blocks > ctas / 2;
   int64_t shares = a.whole ? items : ctas / a.blocks;
@@ -858,6 +909,7 @@ template <class C, bool F32ACT, int D>
 int launch_rows(const Launch& a, const DeviceInfo& dev, cudaStream_t st) {
   const int64_t rows = a.p.drafts * a.group;
   constexpr int MT = F32ACT ? 1 : 2;
+  if (rows <= 8) return launch<Cfg<C, F32ACT, D, 0, 1>>(a, dev, st);
   if (rows <= 16) return launch<Cfg<C, F32ACT, D, 1, 1>>(a, dev, st);
   if (rows <= 32) return launch<Cfg<C, F32ACT, D, MT, 2 / MT>>(a, dev, st);
   return launch<Cfg<C, F32ACT, D, MT, 4 / MT>>(a, dev, st);
