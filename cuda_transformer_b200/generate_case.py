@@ -11,8 +11,16 @@ of their own.  With --rotary the learned position table gives way to rotary
 embeddings.  The steps can run from a CUDA graph: nothing in a step depends on
 a value that the host would have to read.
 
+Prompts that are given several times run once and are forked: kv_copy_pages_
+copies the page that is not full, the others are shared.  With --drafts a step
+feeds a small tree of tokens instead of one: what followed the last token
+where it came up before.  tree_attention looks at all of them, verify_drafts
+keeps a path, kv_compact_ moves its keys and values to where the next step
+expects them.
+
   python -m cuda_transformer_b200.generate_case [--batch 8 --new 128 --graph]
       [--cache bf16] [--rotary] [--temperature 0.8 --repetition 1.1] [--check]
+      [--samples 4] [--drafts 4 --branches 2]
 
 --check generates the same tokens again by running every whole sequence through
 the model at each step, and compares the logits.  Prints one JSON line.
@@ -35,15 +43,16 @@ CACHE_TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float1
 class PagePool:
     """Which pages of a cache belong to which sequence (host side).  table is
     the int32 [batch, max_pages] that the operators read; `reserve` gives a
-    sequence the pages for `tokens` tokens, `release` takes them back.  A row
-    names the pages that its sequence owns and is -1 past them, which the
-    operators take for no place: a token too many gives NaN there and does not
-    reach another sequence's pages."""
+    sequence the pages for `tokens` tokens, `release` takes them back, `fork`
+    lets one begin with another's.  A row names the pages that its sequence
+    owns and is -1 past them, which the operators take for no place: a token
+    too many gives NaN there and does not reach another sequence's pages."""
 
     def __init__(self, pages: int, page_size: int, batch: int, max_pages: int, device):
         self.page_size, self.max_pages = page_size, max_pages
         self.free = list(range(pages - 1, -1, -1))
         self.owned: list[list[int]] = [[] for _ in range(batch)]
+        self.users = [0] * pages  # sequences that have a page
         self.table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=device)
 
     def reserve(self, seq: int, tokens: int) -> None:
@@ -56,12 +65,37 @@ class PagePool:
             new = [self.free.pop() for _ in range(need - len(have))]
             at = len(have)
             have.extend(new)
+            for page in new:
+                self.users[page] += 1
             self.table[seq, at:need] = torch.tensor(new, dtype=torch.int32)
 
     def release(self, seq: int) -> None:
-        self.free.extend(reversed(self.owned[seq]))
+        for page in reversed(self.owned[seq]):
+            self.users[page] -= 1
+            if self.users[page] == 0:
+                self.free.append(page)
         self.owned[seq] = []
         self.table[seq] = -1
+
+    def fork(self, src: int, dst: int, tokens: int) -> list[tuple[int, int]]:
+        """Sequence dst, which has no pages, begins with the first `tokens`
+        tokens of src: it shares the pages that those fill and gets one of its
+        own for the rest.  Returns the (from, to) pages to copy: that one."""
+        if self.owned[dst]:
+            raise ValueError(f"sequence {dst} has pages")
+        full, need = tokens // self.page_size, -(-tokens // self.page_size)
+        if need > len(self.owned[src]):
+            raise ValueError(f"sequence {src} has no {tokens} tokens")
+        if need > full and not self.free:
+            raise RuntimeError("out of pages: 1 needed, 0 free")
+        shared = self.owned[src][:full]
+        for page in shared:
+            self.users[page] += 1
+        self.owned[dst] = list(shared)
+        if full:
+            self.table[dst, :full] = self.table[src, :full]
+        self.reserve(dst, tokens)
+        return [(self.owned[src][full], self.owned[dst][full])] if need > full else []
 
 
 class Generator:
@@ -152,6 +186,24 @@ class Generator:
         self.live[seq] = True
         return self._logits(x[:, -1:])[0]
 
+    def fork(self, src: int, dst: int, room: int = 0) -> None:
+        """Sequence dst begins as src is now (its tokens and their cached keys
+        and values); `room`: tokens to reserve pages for."""
+        n = self.counts[src]
+        if n == 0 or src == dst:
+            raise ValueError(f"sequence {src} cannot be forked into {dst}")
+        if max(n, room) > self.max_len:
+            raise ValueError(f"{max(n, room)} tokens are more than max_len, {self.max_len}")
+        self.release(dst)
+        pairs = self.pool.fork(src, dst, n)
+        self.pool.reserve(dst, max(n, room))
+        if pairs:
+            pages = torch.tensor(pairs, dtype=torch.int32, device=self.history.device)
+            ops.kv_copy_pages_([c for pair in self.caches for c in pair], pages[:, 0], pages[:, 1])
+        for t in (self.history, self.lens, self.prompt_lens, self.live):
+            t[dst] = t[src]
+        self.counts[dst] = n
+
     def step(self, idx: torch.Tensor) -> torch.Tensor:
         """Feeds one token a sequence (int64 [batch]; their places are the
         current lengths) and returns the logits after them [batch, vocab]
@@ -214,16 +266,150 @@ class Generator:
             there = total > 0
         return torch.where(there & self.live, idx, -1)
 
+    def _prompts(self, prompts, room: int) -> torch.Tensor:
+        """Begins all sequences, with pages for `room` tokens after their
+        prompts; the logits after them [batch, vocab]."""
+        logits: list[torch.Tensor] = []
+        for b, t in enumerate(prompts):
+            same = next((i for i in range(b) if prompts[i] is t), None)
+            if same is None:
+                logits.append(self.prompt(b, t, t.numel() + room))
+            else:
+                self.fork(same, b, t.numel() + room)
+                logits.append(logits[same])
+        return torch.stack(logits)
+
+    def look_up_drafts(self, root: torch.Tensor, depth: int, branches: int) -> torch.Tensor:
+        """Drafts for the tokens after `root` (int64 [batch], which the history
+        does not hold yet): `depth` tokens of what followed it at the last
+        `branches` places where it came up before, those first where the token
+        before it is the same too.  int64 [batch, 1 + branches * depth]: root,
+        then the branches; -1: no token."""
+        at = torch.arange(self.max_len, device=root.device)
+        lens = self.lens[:, None].long()
+        known = at < lens
+        there = known & (self.history == root[:, None])
+        last = self.history.gather(1, (lens - 1).clamp(min=0))
+        alike = torch.zeros_like(there)
+        alike[:, 1:] = there[:, 1:] & (self.history[:, :-1] == last)
+        rank = torch.where(alike, at + self.max_len, torch.where(there, at, -1))
+        best = rank.topk(min(branches, self.max_len), dim=1).values
+        places = best.remainder(self.max_len)[:, :, None] + torch.arange(1, depth + 1, device=root.device)
+        tokens = self.history.gather(1, places.flatten(1).clamp(max=self.max_len - 1))
+        fine = (best >= 0)[:, :, None] & (places < lens[:, :, None])
+        return torch.cat([root[:, None], torch.where(fine.flatten(1), tokens, -1)], 1)
+
+    @torch.no_grad()
+    def step_drafts(self, tokens: torch.Tensor, parents: torch.Tensor, mask: torch.Tensor,
+                    depths: torch.Tensor) -> torch.Tensor:
+        """Feeds every sequence the nodes of a tree (tokens int64 [batch, n],
+        node 0 its next token; the tree as verify_drafts and tree_attention
+        take it, depths int32 [n] its nodes' distances from node 0) and returns
+        the logits after each [batch, n, vocab].  The nodes' keys and values
+        are in the cache behind the sequence, in their order; `keep_path` says
+        which of them stay.  The sequences' pages must have room for n tokens."""
+        batch, n = tokens.shape
+        at = torch.arange(n, dtype=torch.int32, device=tokens.device)
+        live = (self.live & (tokens[:, 0] >= 0))[:, None]
+        context = torch.where(live[:, 0], self.lens, -1)
+        slots = torch.where(live, self.lens[:, None] + at, -1).flatten()
+        places = (self.lens[:, None] + depths).clamp(max=self.max_len - 1).flatten()
+        ids = torch.arange(batch, dtype=torch.int32, device=tokens.device).repeat_interleave(n)
+
+        def attend(layer, q, k, v):
+            q2, _ = ops.kv_append_(*self.caches[layer], k, v, self.pool.table, slots, seq_ids=ids,
+                                   q=q if self.rotary else None, cos=self.cos, sin=self.sin,
+                                   rotary_positions=places if self.rotary else None)
+            q = (q2 if self.rotary else q).unflatten(0, (batch, n))
+            o, _ = ops.tree_attention(q, *self.caches[layer], self.pool.table, context, mask=mask)
+            return o.flatten(0, 1)
+
+        x = self._embed(tokens.flatten().clamp(min=0), places).unsqueeze(0)
+        return self._logits(self._blocks(x, attend)).unflatten(0, (batch, n))
+
+    @torch.no_grad()
+    def keep_path(self, tokens: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> None:
+        """The nodes of `path` (verify_drafts') join their sequences, in the
+        cache and in the history."""
+        counts = torch.where(self.live, counts, 0)
+        ops.kv_compact_([c for pair in self.caches for c in pair], self.pool.table, self.lens, path,
+                        counts)
+        at = torch.arange(path.shape[1], device=path.device)
+        kept = at < counts[:, None]
+        column = torch.where(kept, self.lens[:, None] + at, self.max_len)
+        self._columns.scatter_(1, column.long(), tokens.gather(1, path.clamp(min=0).long()))
+        self.lens += counts
+
+    def generate_drafted(self, prompts, new: int, depth: int = 4, branches: int = 1,
+                         temperature: float = 0.0, seed: int = 0):
+        """`new` tokens after each prompt [batch, new], as generate gives them
+        without processing (with a temperature: distributed alike), and the
+        number of steps that it took.  Each step feeds a tree of looked-up
+        tokens; max_len has to hold branches * depth tokens more than the
+        prompts and the new ones.  A sequence that has no next token ends: -1."""
+        if len(prompts) != self.batch:
+            raise ValueError(f"{len(prompts)} prompts for {self.batch} sequences")
+        device = self.history.device
+        n = 1 + branches * depth
+        node = torch.arange(n, dtype=torch.int32, device=device)
+        first = (node - 1) % depth == 0
+        parents = torch.where(node == 0, -1, torch.where(first, 0, node - 1))
+        depths = torch.where(node == 0, 0, (node - 1) % depth + 1).int()
+        # a node sees the root and its branch up to itself
+        alike = (node[:, None] - 1) // depth == (node - 1) // depth
+        sees = (node == 0) | (alike & (node <= node[:, None]) & (node[:, None] > 0))
+        words = torch.nn.functional.pad(sees, (0, -n % 32)).unflatten(1, (-1, 32)).long()
+        words = (words << torch.arange(32, device=device)).sum(-1)
+        mask = torch.where(words >= 2 ** 31, words - 2 ** 32, words).int()
+        mask = mask.expand(self.batch, n, mask.shape[1])
+        parents = parents.int().expand(self.batch, n)
+        g = torch.Generator(device=device).manual_seed(seed)
+
+        def uniform():
+            return torch.rand(self.batch, n, generator=g, device=device) if temperature else None
+
+        def scores(logits):  # what verify_drafts takes: scores, or probabilities
+            return logits if temperature == 0.0 else ops.cuda_softmax(logits / temperature)
+
+        logits = self._prompts(prompts, new + n)
+        # the first token: a tree of its root alone
+        u = uniform()
+        root = ops.verify_drafts(scores(logits[:, None]), torch.zeros_like(self.lens)[:, None].long(),
+                                 uniform=None if u is None else u[:, :1])[0][:, 0]
+        made = [[] for _ in prompts]
+        steps, roots = 0, root.tolist()
+        for seq, token in enumerate(roots):
+            made[seq].append(token)
+        while True:
+            ended = [len(m) >= new or m[-1] < 0 for m in made]
+            if all(ended):
+                break
+            self.live &= ~torch.tensor(ended, device=device)
+            tokens = self.look_up_drafts(root, depth, branches)
+            logits = self.step_drafts(tokens, parents, mask, depths)
+            found, path, counts = ops.verify_drafts(scores(logits), tokens, parents,
+                                                    uniform=uniform())
+            self.keep_path(tokens, path, counts)
+            root = found.gather(1, (counts - 1).clamp(min=0).long()[:, None])[:, 0]
+            steps += 1
+            for seq, (row, count) in enumerate(zip(found.tolist(), counts.tolist())):
+                if not ended[seq]:
+                    self.counts[seq] += count
+                    made[seq].extend(row[:count])
+        filled = [(m + [-1] * new)[:new] for m in made]
+        return torch.tensor(filled, device=device), steps
+
     def generate(self, prompts, new: int, temperature: float = 0.0, seed: int = 0,
                  graph: bool = False, **processing):
         """`new` tokens after each prompt; returns them [batch, new] and the
         unprocessed logits that each was chosen from [new, batch, vocab].  A
-        sequence that has no next token ends: -1 from there on."""
+        sequence that has no next token ends: -1 from there on.  A prompt that
+        is in the list several times (one tensor) runs once and is forked."""
         if len(prompts) != self.batch:
             raise ValueError(f"{len(prompts)} prompts for {self.batch} sequences")
         g = torch.Generator(device=self.history.device).manual_seed(seed)
         uniform = torch.rand(new, self.batch, generator=g, device=self.history.device)
-        logits = torch.stack([self.prompt(b, t, t.numel() + new) for b, t in enumerate(prompts)])
+        logits = self._prompts(prompts, new)
         draw = torch.empty(self.batch, device=uniform.device)
         state = {"logits": logits}
 
@@ -307,6 +493,9 @@ def main() -> None:
     ap.add_argument("--repetition", type=float, default=1.0)
     ap.add_argument("--frequency", type=float, default=0.0)
     ap.add_argument("--presence", type=float, default=0.0)
+    ap.add_argument("--samples", type=int, default=1, help="answers to each prompt (forked)")
+    ap.add_argument("--drafts", type=int, default=0, help="looked-up tokens a branch and step")
+    ap.add_argument("--branches", type=int, default=1)
     ap.add_argument("--check", action="store_true")
     a = ap.parse_args()
     dev = torch.device("cuda", 0)
@@ -314,17 +503,29 @@ def main() -> None:
     torch.manual_seed(1234)
     model = GPT(a.layers, a.d, a.heads, a.ctx, a.vocab).to(dev)
     g = torch.Generator().manual_seed(7)
-    most = a.ctx - a.new
+    nodes = 1 + a.drafts * a.branches if a.drafts else 0
+    most = a.ctx - a.new - nodes
+    if a.drafts and (a.graph or a.repetition != 1.0 or a.frequency or a.presence):
+        ap.error("--drafts goes without --graph and without penalties")
+    if most < 1 or a.batch % a.samples:
+        ap.error("--ctx must hold a prompt and the new tokens, --batch whole groups of --samples")
     prompts = [torch.randint(0, a.vocab, (int(n),), generator=g).to(dev)
-               for n in torch.randint(1, most + 1, (a.batch,), generator=g)]
+               for n in torch.randint(1, most + 1, (a.batch // a.samples,), generator=g)]
+    prompts = [p for p in prompts for _ in range(a.samples)]
     gen = Generator(model, a.batch, a.ctx, a.page, CACHE_TYPES[a.cache], a.rotary)
     full = lambda x: torch.full((a.batch,), x, device=dev)  # noqa: E731
     args = dict(temperature=a.temperature, graph=a.graph, repetition=full(a.repetition),
                 frequency=full(a.frequency), presence=full(a.presence))
-    gen.generate(prompts, min(a.new, 4), **args)  # warm-up
+
+    def run(new):
+        if a.drafts:
+            return gen.generate_drafted(prompts, new, a.drafts, a.branches, a.temperature)
+        return gen.generate(prompts, new, **args)
+
+    run(min(a.new, 4))  # warm-up
     torch.cuda.synchronize()
     t0 = time.perf_counter()
-    tokens, logits = gen.generate(prompts, a.new, **args)
+    tokens, logits = run(a.new)
     torch.cuda.synchronize()
     took = time.perf_counter() - t0
     line = {"metric": "GPT generation tokens/s", "value": a.batch * a.new / took,
@@ -333,7 +534,19 @@ def main() -> None:
             "config": {"layers": a.layers, "d_model": a.d, "heads": a.heads, "vocab": a.vocab,
                        "page": a.page, "cache": a.cache, "rotary": a.rotary, "graph": a.graph},
             "data": "random prompts and weights; prompts included in the time"}
-    if a.check:
+    if a.drafts:
+        steps, logits = logits, None
+        line["steps"] = steps
+        line["config"] |= {"drafts": a.drafts, "branches": a.branches}
+    if a.check and a.drafts:  # how far below the best one a chosen token's logit is
+        worst = 0.0
+        for b, p in enumerate(prompts):
+            seq = torch.cat([p, tokens[b]])
+            for t in range(a.new):
+                ref = whole_sequence_logits(model, seq[:p.numel() + t], a.rotary)
+                worst = max(worst, (ref.max() - ref[tokens[b, t]]).item())
+        line["below_best_logit"] = worst
+    elif a.check:
         worst = 0.0
         for b, p in enumerate(prompts):
             seq = torch.cat([p, tokens[b]])
