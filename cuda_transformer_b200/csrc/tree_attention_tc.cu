@@ -98,6 +98,32 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
+// Two FP32 operations an instruction.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ float2 parts(uint64_t p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Whether one of the two 16-bit values of w is not finite.
 template <class C>
 __device__ __forceinline__ bool not_finite(uint32_t w) {
@@ -405,9 +431,10 @@ __global__ void __launch_bounds__(kThreads, 2)
               if (!(sees[h] >> e & 1u)) s[h][e] = -INFINITY;
           }
         }
-        float top = -INFINITY;
+        float tops[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
-        for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
+        for (int e = 0; e < 32; ++e) tops[e % 4] = max3(tops[e % 4], s[0][e], s[1][e]);
+        float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
         top = top * c2 - K::kBelow;
         if (__any_sync(0xffffffffu, top > base + kMaxSlack)) {
           const float old = base;
@@ -429,17 +456,20 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
         const float from = base == -INFINITY ? 0.0f : base;
-        float w[32], part_sum[4] = {};
+        float w[32];
+        const uint64_t factor = pair(c2, c2), shift = pair(-from, -from);
+        uint64_t part_sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float x = ex2(__fmaf_rn(s[e / 16][e % 16 * 2], c2, -from));
-          const float y = ex2(__fmaf_rn(s[e / 16][e % 16 * 2 + 1], c2, -from));
-          part_sum[e % 4] += x + y;
+          const float2 z = parts(fma2(pair(s[e / 16][e % 16 * 2], s[e / 16][e % 16 * 2 + 1]), factor, shift));
+          const float x = ex2(z.x), y = ex2(z.y);
+          part_sum[e % 4] = add2(part_sum[e % 4], pair(x, y));
           s[e / 16][e % 16 * 2] = x;
           s[e / 16][e % 16 * 2 + 1] = y;
           w[e] = __uint_as_float(pack2<C>(x, y));
         }
-        sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+        const float2 both = parts(add2(add2(part_sum[0], part_sum[1]), add2(part_sum[2], part_sum[3])));
+        sum += both.x + both.y;
         tmem_st32(lanes + K::kS + K::kKeys * buf, w);
         bool dirty = false;
         if (masked) {
