@@ -902,7 +902,7 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
   tree_attention_kernel<K><<<grid, kThreads, K::kSmem, st>>>(a, k_map, v_map);
   rc = check_launch();
   if (rc != CT_OK || a.whole) return rc;
-  return launch_join<typename K::A, K::D>(a, grid, K::kRows, st);
+  return launch_join<typename K::A, K::D>(a, grid, K::kRows, dev, st);
 }
 
 template <class C, bool F32ACT, int D>

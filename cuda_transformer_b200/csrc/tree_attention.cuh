@@ -248,63 +248,120 @@ __device__ __forceinline__ void write_rows_not_there(const TreeAttention& p) {
   }
 }
 
-// The partials of the split item that begins in CTA `cta`, kJoinRows rows of it.
-constexpr int kJoinRows = 8;
+// Joins the partials of split items.  Every CTA collects the records (most CTAs of the
+// first kernel leave one where sequences are short, few where one is long), so that
+// the rows there are can be dealt out evenly: a row a warp while that keeps all rows
+// on the way at once, four rows a warp when there are many.
+constexpr int kJoinThreads = 512;
 
-template <class A, int D>
-__global__ void __launch_bounds__(kJoinRows * 32)
-    tree_join_kernel(const __grid_constant__ Launch a, const int rows) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (*reinterpret_cast<const volatile uint32_t*>(a.status) != 0u) return;
-  const int cta = blockIdx.x, block = cta % a.blocks;
-  const int4 rec = a.records[cta];
-  if (rec.x == 0) return;
-  const int r = blockIdx.y * kJoinRows + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int i = token_of(a, block * rows + r);
-  if (i >= rec.w) return;
+// Rows at, at + step, ... of the split items, LANES lanes a row.
+template <class A, int D, int LANES>
+__device__ __forceinline__ void join_rows(const Launch& a, const int4* record, const int* first_cta,
+                                          int all, int rows, int at, int step) {
+  constexpr int N = D / LANES;  // dims of a lane
+  const int lane = threadIdx.x % LANES;
   const int64_t each = partial_floats(rows, D);
-  // the first part ends its CTA's share, the others begin theirs
-  auto part = [&](int k) {
-    return a.partials + ((int64_t)(cta + k * a.blocks) * 2 + (k == 0)) * each;
-  };
-  constexpr int N = D / 32;
-  float top = -INFINITY, sum = 0.0f, o[N] = {};
-  for (int k = lane; k < rec.x; k += 32)
-    top = fmaxf(top, part(k)[rows * D + 2 * r]);
-  for (int w = 16; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-#pragma unroll 4
-  for (int k = 0; k < rec.x; ++k) {
-    const float2 ml = *reinterpret_cast<const float2*>(part(k) + rows * D + 2 * r);
-    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-    sum += ml.x == -INFINITY ? ml.y : ml.y * f;
-    const float* src = part(k) + r * D + lane * N;
-    float x[N];
-    if constexpr (N == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
-    else if constexpr (N == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
-    else x[0] = *src;
+  // (all rows of a warp go through the same number of steps)
+  for (; at - (int)(threadIdx.x % 32) / LANES < all; at += step) {
+    const bool in = at < all;
+    const int4 rec = record[in ? at / rows : 0];
+    const int cta = first_cta[in ? at / rows : 0], block = cta % a.blocks, r = at % rows;
+    const int i = token_of(a, block * rows + r);
+    const int n = in && i < rec.w ? rec.x : 0;
+    // the first part ends its CTA's share, the others begin theirs
+    auto part = [&](int k) {
+      return a.partials + ((int64_t)(cta + k * a.blocks) * 2 + (k == 0)) * each;
+    };
+    float top = -INFINITY, sum = 0.0f, o[N] = {};
+    for (int k = lane; k < n; k += LANES) top = fmaxf(top, part(k)[rows * D + 2 * r]);
+    for (int w = LANES / 2; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    constexpr int kUnroll = N >= 16 ? 2 : N >= 8 ? 4 : 8;
+#pragma unroll kUnroll
+    for (int k = 0; k < n; ++k) {
+      const float2 ml = *reinterpret_cast<const float2*>(part(k) + rows * D + 2 * r);
+      const float* src = part(k) + r * D;
+      float x[N];
+      // (vectors of the lanes side by side)
+      constexpr int V = N < 4 ? N : 4;
 #pragma unroll
-    for (int e = 0; e < N; ++e) o[e] += ml.x == -INFINITY ? 0.0f : x[e] * f;
+      for (int v = 0; v < N; v += V) {
+        const float* from = src + v * LANES + lane * V;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(x + v) = *reinterpret_cast<const float4*>(from);
+        else if constexpr (V == 2) *reinterpret_cast<float2*>(x + v) = *reinterpret_cast<const float2*>(from);
+        else x[v] = *from;
+      }
+      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+      sum += ml.x == -INFINITY ? ml.y : ml.y * f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] += ml.x == -INFINITY ? 0.0f : x[e] * f;
+    }
+    if (n > 0) {
+      const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int64_t row = ((int64_t)rec.y * a.p.drafts + i) * a.p.q_heads + rec.z * a.group +
+                          (block * rows + r) - i * a.group;
+      constexpr int V = N < 4 ? N : 4;
+#pragma unroll
+      for (int v = 0; v < N; v += V) {
+        const int64_t to = row * D + v * LANES + lane * V;
+        if constexpr (V == 1) {
+          ((A*)a.p.out)[to] = from_f32<A>(o[v] * f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; e += 2) store2<A>(a.p.out, to + e, o[v + e] * f, o[v + e + 1] * f);
+        }
+      }
+      if (lane == 0 && a.p.lse) a.p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+    __syncwarp();
   }
-  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t row = ((int64_t)rec.y * a.p.drafts + i) * a.p.q_heads + rec.z * a.group +
-                      (block * rows + r) - i * a.group;
-#pragma unroll
-  for (int e = 0; e < N; ++e) ((A*)a.p.out)[row * D + lane * N + e] = from_f32<A>(o[e] * f);
-  if (lane == 0 && a.p.lse) a.p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 template <class A, int D>
-int launch_join(const Launch& a, unsigned grid, int rows, cudaStream_t st) {
+__global__ void __launch_bounds__(kJoinThreads, 2)
+    tree_join_kernel(const __grid_constant__ Launch a, const int rows, const int ctas) {
+  __shared__ int4 record[kMaxCtas];
+  __shared__ int first_cta[kMaxCtas], count[kJoinThreads / 32];
+  static_assert(kMaxCtas <= kJoinThreads, "a thread a record");
+  const int c = threadIdx.x, warp = c / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (*reinterpret_cast<const volatile uint32_t*>(a.status) != 0u) return;
+  // (in the same order in every CTA)
+  const int4 own = c < ctas ? a.records[c] : make_int4(0, 0, 0, 0);
+  const uint32_t vote = __ballot_sync(0xffffffffu, own.x > 0);
+  if (c % 32 == 0) count[warp] = __popc(vote);
+  __syncthreads();
+  int found = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    if (w < warp) before += count[w];
+    found += count[w];
+  }
+  if (own.x > 0) {
+    before += __popc(vote & ((1u << c % 32) - 1));
+    record[before] = own;
+    first_cta[before] = c;
+  }
+  __syncthreads();
+  const int all = found * rows, warps = gridDim.x * (kJoinThreads / 32);
+  const int at = blockIdx.x * (kJoinThreads / 32) + warp;
+  if (all <= warps)
+    join_rows<A, D, 32>(a, record, first_cta, all, rows, at, warps);
+  else
+    join_rows<A, D, 8>(a, record, first_cta, all, rows, 4 * at + c % 32 / 8, 4 * warps);
+}
+
+template <class A, int D>
+int launch_join(const Launch& a, unsigned grid, int rows, const DeviceInfo& dev, cudaStream_t st) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(grid, rows / kJoinRows);
-  config.blockDim = dim3(kJoinRows * 32);
+  config.gridDim = dim3(2 * dev.sm_count);
+  config.blockDim = dim3(kJoinThreads);
   config.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  if (cudaLaunchKernelEx(&config, tree_join_kernel<A, D>, a, rows) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&config, tree_join_kernel<A, D>, a, rows, (int)grid) != cudaSuccess) {
     cudaGetLastError();
     return CT_ERR_LAUNCH_FAILED;
   }

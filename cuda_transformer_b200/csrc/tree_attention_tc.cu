@@ -48,9 +48,7 @@ struct TcCfg {
 
 struct Bars {
   uint64_t full[12], empty[12];  // units
-  // of a buffer: S is there, the weights are, their product is in O (the rows' threads
-  // may be two products behind: one barrier's parity would not tell them apart)
-  uint64_t s_full[2], p_ready[2], pv_done[2];
+  uint64_t s_full[2], p_ready[2];  // of a buffer: S is there, the weights (and V) are
   uint64_t q_ready, q_free, last;  // q is there; its last product is done
   CtaCtl ctl;
   int bad[kBad];   // of a tile: a page out of range
@@ -216,7 +214,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int i = 0; i < 2; ++i) {
       mbar_init(B(bars.s_full[i]), 1);
       mbar_init(B(bars.p_ready[i]), 4);
-      mbar_init(B(bars.pv_done[i]), 1);
     }
     mbar_init(B(bars.q_ready), q_rows > 0 ? 1 : 4);
     mbar_init(B(bars.q_free), 1);
@@ -239,9 +236,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto next_part = [&]() {
     ++cur.head;
     more = enter<K>(a, cur, 0, row0);
-  };
-  auto wait = [&](const uint64_t& bar, uint32_t parity) {
-    return mbar_wait(smem_u32(&bar), parity, ctl, a.status);
   };
   auto warp_wait = [&](const uint64_t& bar, uint32_t parity) {
     return (bool)__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), parity, ctl, a.status));
@@ -323,7 +317,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (mbar_test_wait(B(bars.full[u % K::kUnits]), u / K::kUnits & 1)) break;
   } else if (warp == 5) {
     // ------------------------------------------------------------ products
-    if (lane == 0) {
+    // (all lanes wait: a warp of which only one does wakes later; lane 0 issues)
+    {
       constexpr uint32_t kIdescS = idesc_f16(K::kBf16, 128, K::kKeys, false);
       constexpr uint32_t kIdescO = idesc_f16(K::kBf16, 128, D, true);
       uint32_t unit = 0, j = 0, part = 0;
@@ -332,29 +327,28 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int T = cur.stop - cur.tile;
         auto issue_s = [&](int t) {
           const uint32_t n = k_unit(unit, t), u = n % K::kUnits, buf = (j + t) & 1;
-          ok = ok && wait(bars.full[u], n / K::kUnits & 1);
+          ok = ok && warp_wait(bars.full[u], n / K::kUnits & 1);
           if (!ok) return;
           tc_fence_after();
+          if (lane != 0) return;
           const uint32_t k = ring + u * K::kUnit;
 #pragma unroll
           for (int s = 0; s < D / 16; ++s)
             umma_f16_ss(tmem + K::kS + K::kKeys * buf,
                         sdesc_kmajor(q_smem + s / 4 * (K::kRows * 128) + s % 4 * 32),
                         sdesc_kmajor(k + s / 4 * (K::kKeys * 128) + s % 4 * 32), kIdescS, s > 0);
-          umma_commit(B(bars.empty[u]));
           umma_commit(B(bars.s_full[buf]));
           if (t == T - 1) umma_commit(B(bars.q_free));
         };
-        ok = ok && wait(bars.q_ready, part & 1);
+        ok = ok && warp_wait(bars.q_ready, part & 1);
         issue_s(0);
         for (int t = 0; t < T && ok; ++t) {
           if (t + 1 < T) issue_s(t + 1);
           const uint32_t n = v_unit(unit, t, T), u = n % K::kUnits, buf = (j + t) & 1;
-          ok = ok && wait(bars.full[u], n / K::kUnits & 1) &&
-               wait(bars.p_ready[buf], (j + t) >> 1 & 1);
+          ok = ok && warp_wait(bars.p_ready[buf], (j + t) >> 1 & 1);
           if (!ok) break;
           tc_fence_after();
-          if (!*(volatile int*)&bars.skip[buf]) {
+          if (lane == 0 && !*(volatile int*)&bars.skip[buf]) {
             const uint32_t v = ring + u * K::kUnit;
 #pragma unroll
             for (int s = 0; s < K::kKeys / 16; ++s)
@@ -362,15 +356,16 @@ __global__ void __launch_bounds__(kThreads, 2)
                           sdesc(v + s * 2048, K::kKeys * 128, 1024, 2), kIdescO,
                           s > 0 || t % K::kFlush != 0);
           }
-          umma_commit(B(bars.empty[u]));
-          umma_commit(B(bars.pv_done[buf]));
+          if (lane == 0) umma_commit(B(bars.empty[u]));
+          __syncwarp();
         }
         unit += 2 * T;
         j += T;
         ++part;
         if (ok) next_part();
       }
-      umma_commit(B(bars.last));
+      if (lane == 0) umma_commit(B(bars.last));
+      __syncwarp();
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(B(bars.last), 0))
         if (globaltimer_ns() - t0 > CT_WAIT_TIMEOUT_NS) break;
@@ -385,6 +380,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     auto arrive = [&](const uint64_t& bar) {
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar));
+    };
+    // weights V of the part's tile t is in O (its V is free then; the rows' threads may
+    // be two products behind: the parity of a barrier a buffer would not tell)
+    auto product_done = [&](int t, int T) {
+      const uint32_t n = v_unit(unit, t, T);
+      return warp_wait(bars.empty[n % K::kUnits], n / K::kUnits & 1);
     };
     uint2 kept = make_uint2(0u, 0u);  // the row's mask
     auto load_q = [&]() {
@@ -410,6 +411,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t buf = j & 1;
         const bool fresh = t % K::kFlush == 0;  // O holds nothing yet
         if (!(ok = warp_wait(bars.s_full[buf], j >> 1 & 1))) break;
+        if (tid == 0) mbar_arrive(B(bars.empty[k_unit(unit, t) % K::kUnits]));  // K has been read
         if (!active) {
           arrive(bars.p_ready[buf]);
           continue;
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const float f = old == -INFINITY ? 0.0f : ex2(old - base);
           sum = old == -INFINITY ? sum : sum * f;
           if (!fresh) {
-            if (!(ok = warp_wait(bars.pv_done[(j - 1) & 1], (j - 1) >> 1 & 1))) break;
+            if (!(ok = product_done(t - 1, T))) break;
             tc_fence_after();
 #pragma unroll 1
             for (int d = 0; d < D; d += 32) {
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           fence_proxy_async_smem();
           dirty = __any_sync(0xffffffffu, dirty);
           if (dirty) {  // (rare) the tile's O without the tensor core
-            if (!fresh && !(ok = warp_wait(bars.pv_done[(j - 1) & 1], (j - 1) >> 1 & 1))) break;
+            if (!fresh && !(ok = product_done(t - 1, T))) break;
             tc_fence_after();
             float each[K::kKeys];
 #pragma unroll
@@ -500,13 +502,17 @@ __global__ void __launch_bounds__(kThreads, 2)
             add_tile<K>(lanes, each, sees[0], sees[1], v, rows, fresh);
           }
         }
+        if (warp == 0 && !masked) {  // (the issuing thread waits for the weights only)
+          const uint32_t n = v_unit(unit, t, T);
+          if (!(ok = warp_wait(bars.full[n % K::kUnits], n / K::kUnits & 1))) break;
+        }
         if (lane == 0) *(volatile int*)&bars.skip[buf] = dirty;
         tmem_wait_st();
         tc_fence_before();
         arrive(bars.p_ready[buf]);
         if ((t + 1) % K::kFlush == 0 && t + 1 < T) {
           // O moves to FP32 sums in this part's slot
-          if (!(ok = warp_wait(bars.pv_done[buf], j >> 1 & 1))) break;
+          if (!(ok = product_done(t, T))) break;
           tc_fence_after();
           const float f = has_flushed && flushed > -INFINITY ? ex2(flushed - base) : 0.0f;
 #pragma unroll 1
@@ -531,12 +537,12 @@ __global__ void __launch_bounds__(kThreads, 2)
           has_flushed = true;
         }
       }
-      unit += 2 * T;
       if (!ok) break;
       // the next part's q (S of the last tile is there: q has been read)
       next_part();
       if (more) load_q();
-      if (!(ok = warp_wait(bars.pv_done[(j - 1) & 1], (j - 1) >> 1 & 1))) break;
+      if (!(ok = product_done(T - 1, T))) break;
+      unit += 2 * T;
       tc_fence_after();
       const bool whole = part0 == 0 && T == tiles;
       if (active) {
@@ -626,7 +632,7 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
                                                                       q_rows);
   rc = check_launch();
   if (rc != CT_OK || a.whole) return rc;
-  return launch_join<typename K::A, K::D>(a, grid, slot_rows, st);
+  return launch_join<typename K::A, K::D>(a, grid, slot_rows, dev, st);
 }
 
 }  // namespace
