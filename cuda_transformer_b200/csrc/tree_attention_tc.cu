@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 4) {
     // ------------------------------------------------------------ producer
     uint32_t unit = 0, tile_count = 0, part = 0;
-    const int row = lane * a.box;  // lane's box of a tile
+    // boxes of a tile, tiles whose boxes' pages are looked up together; lane's box
+    const int boxes = K::kKeys / a.box, batch = 32 / boxes, row = lane * a.box;
     bool ok = true;
     auto page_of = [&](int position, int& slot) {
       const int index = a.page_shift >= 0 ? position >> a.page_shift : position / p.kv.page_size;
@@ -257,19 +258,24 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
     while (more && ok) {
       const int len = cur.context + cur.drafts, T = cur.stop - cur.tile;
-      auto look_up = [&](int t) {
-        const int position = (cur.tile + t) * K::kKeys + row;
-        int slot;
-        return t < T && row < K::kKeys && position < len
-                   ? p.kv.table[cur.b * p.kv.table_s + page_of(position, slot)] : -1;
+      // The pages of 32 boxes at a time (`batch` tiles from base on, and those before).
+      int base = 0, page_now = -1, slot_now = 0, page_old = -1, slot_old = 0;
+      auto look_up = [&](int t0) {
+        const int t = t0 + lane / boxes, position = (cur.tile + t) * K::kKeys + lane % boxes * a.box;
+        const bool in = t < T && position < len;
+        const int index = page_of(position, slot_now);
+        page_now = in ? p.kv.table[cur.b * p.kv.table_s + index] : -1;
       };
-      auto fetch = [&](int t, int page, bool is_k) {
+      auto fetch = [&](int t, bool is_k) {
         const int u = unit % K::kUnits;
+        const bool old = t < base;
+        const int from = (t - (old ? base - batch : base)) * boxes + lane % boxes;
+        const int page = __shfl_sync(0xffffffffu, old ? page_old : page_now, from);
+        const int slot = __shfl_sync(0xffffffffu, old ? slot_old : slot_now, from);
         if (unit >= K::kUnits)
           ok = ok && warp_wait(bars.empty[u], (unit / K::kUnits - 1) & 1);
         if (!ok) return;
-        const int position = (cur.tile + t) * K::kKeys + row;
-        const bool in = row < K::kKeys && position < len;
+        const bool in = lane < boxes && (cur.tile + t) * K::kKeys + row < len;
         const bool fine = in && page >= 0 && page < p.kv.pages;
         const uint32_t vote = __ballot_sync(0xffffffffu, fine);
         const bool bad = __any_sync(0xffffffffu, in && !fine);
@@ -279,8 +285,6 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         __syncwarp();
         if (fine) {
-          int slot;
-          page_of(position, slot);
           const CUtensorMap* map = is_k ? &k_map : &v_map;
 #pragma unroll
           for (int h = 0; h < K::kParts; ++h)
@@ -289,7 +293,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         ++unit;
       };
-      int now = look_up(0), next = look_up(1);
+      look_up(0);
+      fetch(0, true);
       if (q_rows > 0) {  // q_rows rows of whole tokens, as rows (token, head) of the box
         if (part > 0) ok = ok && warp_wait(bars.q_free, (part - 1) & 1);
         if (ok && lane == 0) {
@@ -300,13 +305,17 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         ++part;
       }
-      fetch(0, now, true);
       for (int t = 0; t < T && ok; ++t) {
-        const int after = look_up(t + 2);
-        if (t + 1 < T) fetch(t + 1, next, true);
-        fetch(t, now, false);
-        now = next;
-        next = after;
+        if (t + 1 < T) {
+          if (t + 1 == base + batch) {
+            page_old = page_now;
+            slot_old = slot_now;
+            base += batch;
+            look_up(base);
+          }
+          fetch(t + 1, true);
+        }
+        fetch(t, false);
       }
       tile_count += T;
       if (ok) next_part();
