@@ -196,7 +196,11 @@ class Generator:
             raise ValueError(f"{max(n, room)} tokens are more than max_len, {self.max_len}")
         self.release(dst)
         pairs = self.pool.fork(src, dst, n)
-        self.pool.reserve(dst, max(n, room))
+        try:
+            self.pool.reserve(dst, max(n, room))
+        except (RuntimeError, ValueError):
+            self.release(dst)
+            raise
         if pairs:
             pages = torch.tensor(pairs, dtype=torch.int32, device=self.history.device)
             ops.kv_copy_pages_([c for pair in self.caches for c in pair], pages[:, 0], pages[:, 1])
@@ -307,12 +311,13 @@ class Generator:
         take it, depths int32 [n] its nodes' distances from node 0) and returns
         the logits after each [batch, n, vocab].  The nodes' keys and values
         are in the cache behind the sequence, in their order; `keep_path` says
-        which of them stay.  The sequences' pages must have room for n tokens."""
+        which of them stay.  The sequences' pages must have room for n tokens
+        (else: NaN).  A negative node 0 ends its sequence, as in `step`."""
         batch, n = tokens.shape
+        self.live &= tokens[:, 0] >= 0
         at = torch.arange(n, dtype=torch.int32, device=tokens.device)
-        live = (self.live & (tokens[:, 0] >= 0))[:, None]
-        context = torch.where(live[:, 0], self.lens, -1)
-        slots = torch.where(live, self.lens[:, None] + at, -1).flatten()
+        context = torch.where(self.live, self.lens, -1)
+        slots = torch.where(self.live[:, None], self.lens[:, None] + at, -1).flatten()
         places = (self.lens[:, None] + depths).clamp(max=self.max_len - 1).flatten()
         ids = torch.arange(batch, dtype=torch.int32, device=tokens.device).repeat_interleave(n)
 

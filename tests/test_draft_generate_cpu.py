@@ -100,3 +100,15 @@ def test_forks_are_checked():
             gen.fork(0, dst, room)
     with pytest.raises(ValueError):
         gen.generate_drafted([torch.zeros(1, dtype=torch.int64)], 4)
+
+
+def test_a_fork_without_room_leaves_nothing_behind():
+    gen = generator(2, 12, 3)
+    gen.pool.reserve(0, 12)
+    gen.counts[0] = 4
+    while len(gen.pool.free) > 1:  # (one page: for the copy, not for more)
+        gen.pool.free.pop()
+    with pytest.raises(RuntimeError):
+        gen.fork(0, 1, 12)
+    assert gen.pool.owned[1] == [] and len(gen.pool.free) == 1 and gen.counts[1] == 0
+    assert gen.pool.users[gen.pool.owned[0][0]] == 1

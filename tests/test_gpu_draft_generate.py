@@ -110,3 +110,25 @@ def test_commands(cuda_device, capsys, monkeypatch):
         generate_case.main()
         line = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
         assert line["value"] > 0 and line.get("below_best_logit", 0.0) <= 4e-5
+
+
+def test_a_negative_root_ends_its_sequence(cuda_device):
+    """Its history, its length and its cache stay as they were; the others go on."""
+    _, prompts, gen = setup()
+    for b, p in enumerate(prompts):
+        gen.prompt(b, p, p.numel() + 8)
+    before, history = gen.lens.clone(), gen.history.clone()
+    tokens = torch.tensor([[1, 2], [-1, 2], [3, 4]], device="cuda")
+    node = torch.arange(2, dtype=torch.int32, device="cuda")
+    parents = (node - 1).expand(3, 2)
+    mask = (2 ** (node + 1) - 1).int()[None, :, None].expand(3, 2, 1)
+    caches = [c.clone() for pair in gen.caches for c in pair]
+    gen.step_drafts(tokens, parents, mask, node)
+    path = node.expand(3, 2).contiguous()
+    gen.keep_path(tokens, path, torch.tensor([2, 1, 1], dtype=torch.int32, device="cuda"))
+    assert gen.live.tolist() == [True, False, True]
+    assert (gen.lens - before).tolist() == [2, 0, 1]
+    assert torch.equal(gen.history[1], history[1])
+    pages = gen.pool.owned[1]
+    for c, old in zip([c for pair in gen.caches for c in pair], caches):
+        assert torch.equal(c[pages], old[pages])
