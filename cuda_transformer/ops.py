@@ -470,7 +470,9 @@ def kv_compact_(caches: list[Tensor], block_table: Tensor, context_lens: Tensor,
     j < counts[b].  keep (int32 [batch, n]) ascends along a row; context_lens,
     counts: int32 [batch].  verify_drafts gives path and counts to pass here;
     any other choice of tokens to keep is made the same way.  A move without a
-    place in the cache is left out."""
+    place in the cache is left out.  No cache may be in the list twice or
+    overlap another, and sequences must not share the pages that are written
+    (kv_copy_pages_ gives a fork its own)."""
     _kv_compact(caches, block_table, context_lens, keep, counts)
 
 

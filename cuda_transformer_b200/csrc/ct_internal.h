@@ -275,7 +275,6 @@ struct VerifyDrafts {
   int64_t batch, drafts, vocab;
   int dtype;
 };
-constexpr int64_t kMostDrafts = 1024;  // nodes of a tree that verify_drafts takes
 int launch_verify_drafts(const VerifyDrafts& p, const DeviceInfo& dev, cudaStream_t st);
 // Several caches of one shape, [page, kv_head, slot, head_dim]; the most that
 // one launch takes.

@@ -546,7 +546,8 @@ int ct_verify_drafts(const void* target, const int64_t target_stride[2],
  * keep[b][1] < ... (ct_verify_drafts' path); a move is left out when its page is
  * out of range, and when keep[b][j] <= j (it is in its place).  Where they do not
  * ascend, the moved rows' values mean nothing.  Two sequences must not share the
- * pages that are written.  No reference counterpart. */
+ * pages that are written; no cache may overlap another (the same one twice is
+ * refused).  No reference counterpart. */
 int ct_kv_compact(void* const* caches, const int64_t* cache_strides, int64_t caches_n,
                   const int32_t* block_table, int64_t table_stride,
                   const int32_t* context_lens, const int32_t* keep, int64_t keep_ld,

@@ -123,6 +123,13 @@ def test_move_refusals():
         assert copy(**kw) == want, kw
 
 
+def test_one_cache_twice_is_refused():
+    """Moving it up twice at once would lose tokens."""
+    one = (ctypes.c_void_p * 3)(256, 512, 256)
+    assert compact(caches=one, strides=strides(3), n=3) == BAD
+    assert compact(caches=one, strides=strides(3), n=3, pages=0) == cb.CT_OK
+
+
 def test_append_refusals_with_angles():
     """ct_kv_append_ex checks what ct_kv_append checks."""
     S3 = (ctypes.c_int64 * 3)(64, 64, 1)
