@@ -23,7 +23,7 @@
 // that type for the product and summed unrounded.
 //
 // Measured (device): 16 chains of 5 on 12 heads of 64 with FP32 activations over a BF16
-// cache of 4096 to 16384 tokens: 92 us, 5.6 TB/s of K and V; with a product a term
+// cache of 3500 to 4096 tokens: 92 us, 5.4 TB/s of K and V; with a product a term
 // instead of two terms a product, two CTAs an SM, 114.  4 trees of 10 on 6 heads of 64
 // over up to 256 tokens, FP32: 12 us, of which the launch and one pass through the
 // latencies are most.
