@@ -37,6 +37,7 @@ __device__ __forceinline__ float ex2(float x) {
 struct Launch {
   TreeAttention p;
   int group, blocks;    // query heads of a key/value head; row blocks of an item
+  int block0;           // of this launch: the first of them
   int group_shift;      // log2 of group, -1 when it is no power of two
   int shares;
   bool whole;           // an item a CTA: none is split
@@ -86,7 +87,7 @@ struct Cursor {
 };
 
 // The item at (c.b, c.head), `within` units into it, or the next one there is that
-// has rows behind row0.
+// has rows behind row0.  All lanes of a warp.
 template <class K>
 __device__ __forceinline__ bool enter(const Launch& a, Cursor& c, int64_t within, int row0) {
   while (c.left > 0 && c.b < a.p.batch) {
@@ -95,6 +96,18 @@ __device__ __forceinline__ bool enter(const Launch& a, Cursor& c, int64_t within
       ++c.b;
       c.head = 0;
       within = 0;
+      // the next that is there, 32 looked at at once: batches may be padded (2 sequences
+      // in 256 places 25 us, one place after the other 48)
+      if (s.tiles == 0)
+        for (; c.b < a.p.batch; c.b += 32) {
+          const int64_t b = c.b + threadIdx.x % 32;
+          const uint32_t there =
+              __ballot_sync(0xffffffffu, b < a.p.batch && sequence<K>(a.p, b).tiles > 0);
+          if (there) {
+            c.b += __ffs(there) - 1;
+            break;
+          }
+        }
       continue;
     }
     const int64_t units = s.tiles + K::kItemCost;
@@ -267,7 +280,8 @@ __device__ __forceinline__ void join_rows(const Launch& a, const int4* record, c
   for (; at - (int)(threadIdx.x % 32) / LANES < all; at += step) {
     const bool in = at < all;
     const int4 rec = record[in ? at / rows : 0];
-    const int cta = first_cta[in ? at / rows : 0], block = cta % a.blocks, r = at % rows;
+    const int cta = first_cta[in ? at / rows : 0], r = at % rows;
+    const int block = a.block0 + cta % a.blocks;
     const int i = token_of(a, block * rows + r);
     const int n = in && i < rec.w ? rec.x : 0;
     // the first part ends its CTA's share, the others begin theirs

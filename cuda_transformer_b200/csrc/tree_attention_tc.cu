@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   CtaCtl* const ctl = &bars.ctl;
   const TreeAttention& p = a.p;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int share = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks;
+  const int share = blockIdx.x / a.blocks, block = a.block0 + blockIdx.x % a.blocks;
   const int row0 = block * K::kRows;  // row r: token (row0 + r) / group, head (row0 + r) % group
   const uint32_t q_smem = smem_u32(shared), ring = q_smem + K::kQBytes;
   auto B = [](const uint64_t& x) { return smem_u32(&x); };
@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   }
   __syncwarp();
-  if (!bars.raised) write_rows_not_there<K>(p);
+  if (!bars.raised && a.block0 == 0) write_rows_not_there<K>(p);
   tc_fence_before();
   __syncthreads();
   if (warp == 5) {
@@ -643,30 +643,38 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
   int rc = allow_shared<tree_attention_tc_kernel<K>>(smem_bytes<K>(), dev);
   if (rc != CT_OK) return rc;
   const int64_t rows = p.drafts * a.group, items = p.batch * p.kv_heads;
-  a.blocks = (int)((rows + K::kRows - 1) / K::kRows);
+  const int blocks = (int)((rows + K::kRows - 1) / K::kRows);
   int ctas = 2 * dev.sm_count;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   a.whole = p.kv.max_pages * p.kv.page_size <= K::kWholeTokens;
-  const int64_t shares = a.whole ? items : ctas / a.blocks;
-  if (shares * a.blocks >= 1ll << 31) return CT_ERR_INVALID_ARGUMENT;
-  a.shares = (int)shares;
   CUtensorMap k_map{}, v_map{};
   make_maps(a, &k_map, &v_map, K::kKeys);
   if (a.box == 0) return kNoTc;
   // q by TMA where a block's rows are whole tokens
   CUtensorMap q_map{};
-  int q_rows = a.blocks == 1 ? (int)rows : K::kRows % a.group == 0 ? K::kRows : 0;
+  int q_rows = blocks == 1 ? (int)rows : K::kRows % a.group == 0 ? K::kRows : 0;
   if (!a.q_vectors || a.negative || q_rows == 0 ||
       make_tmap_pages(&q_map, p.q, p.act_dtype, p.batch, p.drafts, p.q_heads, K::D, p.qs, a.group,
                       q_rows / a.group) != CT_OK)
     q_rows = 0;
   const int slot_rows = rows >= K::kRows ? K::kRows : (int)(rows + 15) / 16 * 16;
-  const unsigned grid = (unsigned)(shares * a.blocks);
-  tree_attention_tc_kernel<K><<<grid, kThreads, smem_bytes<K>(), st>>>(a, k_map, v_map, q_map, slot_rows,
-                                                                      q_rows);
-  rc = check_launch();
-  if (rc != CT_OK || a.whole) return rc;
-  return launch_join<typename K::A, K::D>(a, grid, slot_rows, dev, st);
+  // a part of the blocks a launch where they are more than half the CTAs of a wave (a
+  // piece of a prompt, 4096 tokens over 4096, 32 and 8 heads of 128: 1.58 ms; all by the
+  // warps of tree_attention.cu 3.90)
+  const int launches = a.whole ? 1 : (blocks + ctas / 2 - 1) / (ctas / 2);
+  a.blocks = (blocks + launches - 1) / launches;
+  const int64_t shares = a.whole ? items : ctas / a.blocks;
+  if (shares * a.blocks >= 1ll << 31) return CT_ERR_INVALID_ARGUMENT;
+  a.shares = (int)shares;
+  for (a.block0 = 0; a.block0 < blocks; a.block0 += a.blocks) {
+    const unsigned grid = (unsigned)(shares * a.blocks);
+    tree_attention_tc_kernel<K><<<grid, kThreads, smem_bytes<K>(), st>>>(a, k_map, v_map, q_map,
+                                                                        slot_rows, q_rows);
+    rc = check_launch();
+    if (rc == CT_OK && !a.whole) rc = launch_join<typename K::A, K::D>(a, grid, slot_rows, dev, st);
+    if (rc != CT_OK) return rc;
+  }
+  return CT_OK;
 }
 
 }  // namespace
@@ -679,7 +687,7 @@ namespace tree {
 int launch_tc(const TreeAttention& p, const DeviceInfo& dev, cudaStream_t st) {
   const int64_t rows = p.drafts * (p.q_heads / p.kv_heads);
   if (p.act_dtype != p.kv.dtype || p.kv.dtype == CT_DTYPE_F32 || p.head_dim == 32 || rows <= 16 ||
-      p.kv.page_size % 8 != 0 || rows > 64 * dev.sm_count)
+      p.kv.page_size % 8 != 0)
     return kNoTc;
   const Launch a = begin_launch(p, dev);
   if (p.kv.dtype == CT_DTYPE_BF16)

@@ -203,6 +203,37 @@ def test_attention_sequences_that_take_no_part(cuda_device, ops):
     check(q[:1], k, v, table[:1], [16], [4], None, 16, (out[:1], lse[:1]), 0.125)
 
 
+@pytest.mark.parametrize("there", [[0, 299], [31, 32, 33, 290], [64], [5, 150, 151, 298, 299], []])
+@pytest.mark.parametrize("n,cache", [(4, F32), (5, F16), (24, BF16)])
+def test_attention_in_padded_batches(cuda_device, ops, there, n, cache):
+    """300 places for sequences of which few are there, far apart (some long enough to be
+    split); the others' table rows name no pages."""
+    context = [-1] * 300
+    for i, b in enumerate(there):
+        context[b] = (1900, 3, 0, 700, 65)[i]
+    g = gen(n)
+    k, v, table = make_cache([max(c, 0) + n if c >= 0 else 0 for c in context], 2, 64, 16, cache,
+                             "token", g)
+    table = torch.where(ints(context)[:, None] >= 0, table, -1)
+    if table.shape[1] < 121:  # a table that is split
+        table = torch.nn.functional.pad(table, (0, 121 - table.shape[1]), value=-1)
+    q = torch.randn(300, n, 4, 64, generator=g, device="cuda").to(cache)
+    got = ops.tree_attention(q, k, v, table, ints(context))
+    check(q, k, v, table, context, [n] * 300, None, 16, got, 0.125)
+
+
+@pytest.mark.parametrize("act,cache,dim", [(BF16, BF16, 64), (F16, F16, 128), (F32, F16, 64)])
+@pytest.mark.parametrize("n,context", [(300, [600, 40]), (602, [500])])
+def test_attention_of_more_rows_than_a_wave(cuda_device, ops, act, cache, dim, n, context):
+    """A piece of a prompt on 64 heads that share one: 150 and 301 blocks of 128 rows."""
+    g = gen(n)
+    k, v, table = make_cache([c + n for c in context], 1, dim, 16, cache, "head", g)
+    table = torch.nn.functional.pad(table, (0, 4), value=-1)
+    q = torch.randn(len(context), n, 64, dim, generator=g, device="cuda").to(act)
+    got = ops.tree_attention(q, k, v, table, ints(context))
+    check(q, k, v, table, context, [n] * len(context), None, 16, got, dim ** -0.5)
+
+
 @pytest.mark.parametrize("n", [5, 40])
 def test_attention_bad_lengths_and_pages(cuda_device, ops, n):
     """A length beyond the table, a page outside the cache: NaN in that sequence's rows
