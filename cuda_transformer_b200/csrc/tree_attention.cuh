@@ -266,18 +266,23 @@ __device__ __forceinline__ void write_rows_not_there(const TreeAttention& p) {
 // Joins the partials of split items.  Every CTA collects the records (most CTAs of the
 // first kernel leave one where sequences are short, few where one is long), so that
 // the rows there are can be dealt out evenly: a row a warp while that keeps all rows
-// on the way at once, four rows a warp when there are many.
+// on the way at once, 4 or 16 warps a row when there are few (one sequence of 60,000
+// tokens, 16 heads on one of 64, 8 drafts: 27 us, a warp a row 51), four rows a warp when
+// there are many.
 constexpr int kJoinThreads = 512;
 
-// Rows at, at + step, ... of the split items, LANES lanes a row.
-template <class A, int D, int LANES>
+// Rows at, at + step, ... of the split items, LANES lanes a row; with W > 1, W warps of
+// the CTA that take turns at its parts and meet in shared memory.
+template <class A, int D, int LANES, int W = 1>
 __device__ __forceinline__ void join_rows(const Launch& a, const int4* record, const int* first_cta,
-                                          int all, int rows, int at, int step) {
+                                          int all, int rows, int at, int step,
+                                          float (*meet)[D + 1] = nullptr) {
   constexpr int N = D / LANES;  // dims of a lane
-  const int lane = threadIdx.x % LANES;
+  const int lane = threadIdx.x % LANES, warp = threadIdx.x / 32;
   const int64_t each = partial_floats(rows, D);
-  // (all rows of a warp go through the same number of steps)
-  for (; at - (int)(threadIdx.x % 32) / LANES < all; at += step) {
+  static_assert(W == 1 || LANES == 32, "");
+  // (all rows of a warp, or of the CTA, go through the same number of steps)
+  for (; at - (W > 1 ? warp / W : (int)(threadIdx.x % 32) / LANES) < all; at += step) {
     const bool in = at < all;
     const int4 rec = record[in ? at / rows : 0];
     const int cta = first_cta[in ? at / rows : 0], r = at % rows;
@@ -293,7 +298,7 @@ __device__ __forceinline__ void join_rows(const Launch& a, const int4* record, c
     for (int w = LANES / 2; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
     constexpr int kUnroll = N >= 16 ? 2 : N >= 8 ? 4 : 8;
 #pragma unroll kUnroll
-    for (int k = 0; k < n; ++k) {
+    for (int k = W > 1 ? warp % W : 0; k < n; k += W) {
       const float2 ml = *reinterpret_cast<const float2*>(part(k) + rows * D + 2 * r);
       const float* src = part(k) + r * D;
       float x[N];
@@ -310,6 +315,22 @@ __device__ __forceinline__ void join_rows(const Launch& a, const int4* record, c
       sum += ml.x == -INFINITY ? ml.y : ml.y * f;
 #pragma unroll
       for (int e = 0; e < N; ++e) o[e] += ml.x == -INFINITY ? 0.0f : x[e] * f;
+    }
+    if constexpr (W > 1) {
+      __syncthreads();
+      if (warp % W) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) meet[warp][e * 32 + lane] = o[e];
+        if (lane == 0) meet[warp][D] = sum;
+      }
+      __syncthreads();
+      if (warp % W) continue;
+#pragma unroll
+      for (int w = 1; w < W; ++w) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] += meet[warp + w][e * 32 + lane];
+        sum += meet[warp + w][D];
+      }
     }
     if (n > 0) {
       const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -332,7 +353,9 @@ __device__ __forceinline__ void join_rows(const Launch& a, const int4* record, c
   }
 }
 
-template <class A, int D>
+// FEW: there cannot be more than 4 rows a CTA.  (One kernel for both took 2 us longer
+// where rows are many.)
+template <class A, int D, bool FEW>
 __global__ void __launch_bounds__(kJoinThreads, 2)
     tree_join_kernel(const __grid_constant__ Launch a, const int rows, const int ctas) {
   __shared__ int4 record[kMaxCtas];
@@ -360,7 +383,13 @@ __global__ void __launch_bounds__(kJoinThreads, 2)
   __syncthreads();
   const int all = found * rows, warps = gridDim.x * (kJoinThreads / 32);
   const int at = blockIdx.x * (kJoinThreads / 32) + warp;
-  if (all <= warps)
+  if constexpr (FEW) {
+    __shared__ float meet[kJoinThreads / 32][D + 1];
+    if (all <= (int)gridDim.x)
+      join_rows<A, D, 32, 16>(a, record, first_cta, all, rows, at / 16, warps / 16, meet);
+    else
+      join_rows<A, D, 32, 4>(a, record, first_cta, all, rows, at / 4, warps / 4, meet);
+  } else if (all <= warps)
     join_rows<A, D, 32>(a, record, first_cta, all, rows, at, warps);
   else
     join_rows<A, D, 8>(a, record, first_cta, all, rows, 4 * at + c % 32 / 8, 4 * warps);
@@ -377,7 +406,11 @@ int launch_join(const Launch& a, unsigned grid, int rows, const DeviceInfo& dev,
   attr.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  if (cudaLaunchKernelEx(&config, tree_join_kernel<A, D>, a, rows, (int)grid) != cudaSuccess) {
+  // (an item is split into blocks of rows, and no more of them end than there are CTAs)
+  const int64_t items = a.p.batch * a.p.kv_heads * a.blocks;
+  const bool few = (items < grid ? items : grid) * rows <= 4 * (int64_t)config.gridDim.x;
+  if (cudaLaunchKernelEx(&config, few ? tree_join_kernel<A, D, true> : tree_join_kernel<A, D, false>, a,
+                         rows, (int)grid) != cudaSuccess) {
     cudaGetLastError();
     return CT_ERR_LAUNCH_FAILED;
   }
