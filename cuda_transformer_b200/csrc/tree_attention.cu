@@ -24,8 +24,8 @@
 //
 // Measured (device): 16 chains of 5 on 12 heads of 64 with FP32 activations over a BF16
 // cache of 3500 to 4096 tokens: 92 us, 5.4 TB/s of K and V; with a product a term
-// instead of two terms a product, two CTAs an SM, 114.  4 trees of 10 on 6 heads of 64
-// over up to 256 tokens, FP32: 12 us, of which the launch and one pass through the
+// instead of two terms a product, two CTAs an SM, 114.  8 trees of 8 on 6 heads of 64 over
+// up to 248 tokens, FP32: 12.5 us, of which the launch and one pass through the
 // latencies are most.
 #include <cfloat>
 
