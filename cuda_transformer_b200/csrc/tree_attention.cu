@@ -19,8 +19,8 @@
 //
 // Roundings: FP32 activations over 16-bit caches are split into 16-bit terms, three
 // for BF16 and two for f16 (22 bits and more), and so are the weights; FP32 caches run
-// as two TF32 terms each way (22 bits).  16-bit activations: the weights are rounded to
-// that type for the product and summed unrounded.
+// as two TF32 terms each way (22 bits).  16-bit activations: the weights in two terms of
+// that type (16 bits and more), as in paged_attention; they are summed unrounded.
 //
 // Measured (device): 16 chains of 5 on 12 heads of 64 with FP32 activations over a BF16
 // cache of 3500 to 4096 tokens: 92 us, 5.4 TB/s of K and V; with a product a term
@@ -63,14 +63,16 @@ struct Cfg {
   static constexpr int kHalf = WK == 4 ? 4096 : 8192;
   static constexpr int kKeys = kHalf / kRowBytes < 128 ? kHalf / kRowBytes : 128;
   // Keys that a warp's scores are formed of at a time.
-  static constexpr int kMost = F32ACT && D == 128 ? 16 : 32;
+  static constexpr int kMost = (F32ACT || MT > 1) && D == 128 ? 16 : 32;
   static constexpr int kBlock = kKeys < kMost ? kKeys : kMost;
   static constexpr int NT = kBlock / 8;
   static constexpr int kTileBytes = kKeys * kRowBytes;  // K or V
   // 16-bit terms of q and of the weights (FP32 activations: 22 bits and more).
   static constexpr int kTerms = kF32 || !F32ACT ? 1 : kBf16 ? 3 : 2;
+  static constexpr int kWTerms = kF32 ? 1 : F32ACT ? kTerms : 2;
   // (packed: pairs of terms, 16 rows each)
   static constexpr int kQTiles = kPack ? (kTerms + 1) / 2 : kTerms;
+  static constexpr int kWTiles = kPack ? (kWTerms + 1) / 2 : kWTerms;
   static constexpr int kQRows = kPack && !kF32 ? 16 : kRows;
   static constexpr int kQBytes = kQTiles * kQRows * kRowBytes;
   static constexpr int kJoinDims = 32;
@@ -712,17 +714,17 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
                 o[m][n][e] += K::kPack ? acc[m][e] + acc[m][2 + e] : acc[m][e];
           }
         } else {
-          uint32_t w[MT][NT / 2][K::kQTiles][4];
+          uint32_t w[MT][NT / 2][K::kWTiles][4];
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int ks = 0; ks < NT / 2; ++ks)
 #pragma unroll
-              for (int t = 0; t < K::kQTiles; ++t)
+              for (int t = 0; t < K::kWTiles; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   if constexpr (K::kPack) {  // rows 0-7 and 8-15: two terms
-                    w[m][ks][t][j] = 2 * t + j % 2 >= K::kTerms
+                    w[m][ks][t][j] = 2 * t + j % 2 >= K::kWTerms
                                          ? 0u
                                          : take_term<C>(s[m][2 * ks + j / 2][0], s[m][2 * ks + j / 2][1]);
                   } else {
@@ -745,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
 #pragma unroll
               for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int t = 0; t < K::kQTiles; ++t) {
+                for (int t = 0; t < K::kWTiles; ++t) {
                   mma_next<C>(ks + t == 0, acc[m][0], w[m][ks][t], v[0], v[1]);
                   mma_next<C>(ks + t == 0, acc[m][1], w[m][ks][t], v[2], v[3]);
                 }

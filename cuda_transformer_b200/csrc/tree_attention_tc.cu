@@ -9,14 +9,16 @@
 //
 // A CTA has up to 128 rows, which are the lanes of Tensor Memory, and goes through
 // its share in tiles of 64 keys: S = Q K^T (128 x 64) into one of two buffers, a
-// thread a row forms the weights and writes them over S as the 16-bit operand of
-// O += P V (128 x D).  Two CTAs an SM overlap each other's latencies, and S of the
+// thread a row forms the weights and writes them over S as the 16-bit operands (two
+// terms) of O += P V (128 x D).  Two CTAs an SM overlap each other's latencies, and S of the
 // next tile is formed while the weights of this one are.  Warps 0-3 have the rows,
 // warp 4 fetches pages by TMA, warp 5 issues the products.
 //
-// Roundings: the weights are rounded to the cache's type for the product and are
-// summed unrounded; the base of a row's exponents may lie below its maximum by a
-// factor of 2^kMaxSlack, which changes no relative rounding.
+// Roundings: the weights are two terms of the cache's type for the products (16 bits
+// and more) and are summed unrounded; the base of a row's exponents may lie below its
+// maximum by a factor of 2^kMaxSlack, which changes no relative rounding.  One term
+// would leave O with the rounding of every weight (bf16 0.0021 to 0.0024 of O where the
+// output's own rounding is 0.0017), a step over one token with paged_attention would not.
 //
 // Measured (device): one tree of 64 on 32 and 8 heads of 128 over 131,072 tokens,
 // BF16, 256 rows an item: 155 us, 3.47 TB/s and 888 TFLOP/s of products.  A tile of a
@@ -58,10 +60,10 @@ struct TcCfg {
   // one head 45, 45, 47, 48.
   static constexpr int kItemCost = 4;
   static constexpr int kMinShare = kItemCost + 2;
-  // Tiles whose products may pile up in Tensor Memory: the tensor core cuts its sums
-  // off, by 2^-24 at most each time, so after 512 products O moves to FP32 sums in
-  // the workspace.
-  static constexpr int kFlush = 128;
+  // Tiles whose products (8 each) may pile up in Tensor Memory: the tensor core cuts
+  // its sums off, by 2^-24 at most each time, so after 512 products O moves to FP32
+  // sums in the workspace.
+  static constexpr int kFlush = 64;
   // f16 weights reach up to 2^14 instead of 1, clear of the subnormals.
   static constexpr float kBelow = kBf16 ? 0.0f : 8.0f;
   // Tables of at most so many tokens are not split (as in tree_attention.cu).  Not
@@ -111,6 +113,18 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, 
       : "memory");
 }
 
+// The high term of two weights (x in the low half): the 16-bit numbers at or below them,
+// so that what is left is positive too.
+template <class C>
+__device__ __forceinline__ uint32_t high2(float x, float y) {
+  if constexpr (std::is_same<C, __nv_bfloat16>::value) {
+    return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632u);
+  } else {
+    uint32_t w;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+    return w;
+  }
+}
 template <class C>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
   if constexpr (std::is_same<C, __nv_bfloat16>::value) {
@@ -146,6 +160,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+// What `high`, high2(x, y), leaves of x and y.
+template <class C>
+__device__ __forceinline__ uint32_t low2(float x, float y, uint32_t high) {
+  float2 h;
+  if constexpr (std::is_same<C, __nv_bfloat16>::value)
+    h = make_float2(__uint_as_float(high << 16), __uint_as_float(high & 0xffff0000u));
+  else
+    h = __half22float2(*reinterpret_cast<const __half2*>(&high));
+  const float2 rest = parts(fma2(pair(h.x, h.y), pair(-1.0f, -1.0f), pair(x, y)));
+  return pack2<C>(rest.x, rest.y);
 }
 // Whether one of the two 16-bit values of w is not finite.
 template <class C>
@@ -386,9 +411,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             const uint32_t v = ring + u * K::kUnit;
 #pragma unroll
             for (int s = 0; s < K::kKeys / 16; ++s)
-              umma_f16_ts(tmem, tmem + K::kS + K::kKeys * buf + 8 * s,
-                          sdesc(v + s * 2048, K::kKeys * 128, 1024, 2), kIdescO,
-                          s > 0 || t % K::kFlush != 0);
+#pragma unroll
+              for (int term = 0; term < 2; ++term)
+                umma_f16_ts(tmem, tmem + K::kS + K::kKeys * buf + K::kKeys / 2 * term + 8 * s,
+                            sdesc(v + s * 2048, K::kKeys * 128, 1024, 2), kIdescO,
+                            s + term > 0 || t % K::kFlush != 0);
           }
           if (lane == 0) umma_commit(B(bars.empty[u]));
           __syncwarp();
@@ -502,11 +529,16 @@ __global__ void __launch_bounds__(kThreads, 2)
           part_sum[e % 4] = add2(part_sum[e % 4], pair(x, y));
           s[e / 16][e % 16 * 2] = x;
           s[e / 16][e % 16 * 2 + 1] = y;
-          w[e] = __uint_as_float(pack2<C>(x, y));
+          w[e] = __uint_as_float(high2<C>(x, y));
         }
         const float2 both = parts(add2(add2(part_sum[0], part_sum[1]), add2(part_sum[2], part_sum[3])));
         sum += both.x + both.y;
         tmem_st32(lanes + K::kS + K::kKeys * buf, w);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          w[e] = __uint_as_float(low2<C>(s[e / 16][e % 16 * 2], s[e / 16][e % 16 * 2 + 1],
+                                         __float_as_uint(w[e])));
+        tmem_st32(lanes + K::kS + K::kKeys * buf + 32, w);
         bool dirty = false;
         if (masked) {
           // V behind the last token counts as zero (a weight of 0 would leave its
