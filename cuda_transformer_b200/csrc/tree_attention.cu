@@ -18,7 +18,8 @@
 // layout of Q K^T is the operand's of P V.
 //
 // Roundings: FP32 activations over 16-bit caches are split into 16-bit terms, three
-// for BF16 and two for f16 (22 bits and more), and so are the weights; FP32 caches run
+// for BF16 and two for f16 (22 bits and more; a row of q is brought into f16's range by
+// a power of two first, as in paged_attention), and so are the weights; FP32 caches run
 // as two TF32 terms each way (22 bits).  16-bit activations: the weights in two terms of
 // that type (16 bits and more), as in paged_attention; they are summed unrounded.
 //
@@ -70,6 +71,8 @@ struct Cfg {
   // 16-bit terms of q and of the weights (FP32 activations: 22 bits and more).
   static constexpr int kTerms = kF32 || !F32ACT ? 1 : kBf16 ? 3 : 2;
   static constexpr int kWTerms = kF32 ? 1 : F32ACT ? kTerms : 2;
+  // Rows of q have factors of their own (load_rows).
+  static constexpr bool kRowScale = F32ACT && !kF32 && !kBf16;
   // (packed: pairs of terms, 16 rows each)
   static constexpr int kQTiles = kPack ? (kTerms + 1) / 2 : kTerms;
   static constexpr int kWTiles = kPack ? (kWTerms + 1) / 2 : kWTerms;
@@ -217,10 +220,13 @@ __device__ __forceinline__ uint32_t chunk_pos(int r, int c) {
 }
 
 // A part's q into shared memory: rows of 16-byte chunks as the cache's type, or its
-// terms one behind the other; and the rows' first mask words.
+// terms one behind the other; and the rows' first mask words.  f16 terms hold the row
+// times a power of two that brings its largest element to 2^14 .. 2^15, so that large
+// ones do not overflow and what falls below f16's range is below 2^-38 of the largest;
+// row_scale is what undoes it.
 template <class K>
 __device__ __forceinline__ void load_rows(const Launch& a, const Cursor& c, int row0, char* shared,
-                                       uint2* mask_words) {
+                                       uint2* mask_words, float* row_scale) {
   using C = typename K::C;
   using A = typename K::A;
   constexpr int D = K::D, kEight = D / 8;
@@ -267,6 +273,20 @@ __device__ __forceinline__ void load_rows(const Launch& a, const Cursor& c, int 
         *reinterpret_cast<uint4*>(x + 4) = in[k][kWords - 1];
 #pragma unroll
         for (int y = 0; y < 8; ++y) x[y] = a.negative ? -x[y] : x[y];
+        if constexpr (K::kRowScale) {  // (kEight lanes side by side have a row)
+          float top = 0.0f;
+#pragma unroll
+          for (int y = 0; y < 8; ++y)
+            if (fabsf(x[y]) < INFINITY) top = fmaxf(top, fabsf(x[y]));
+#pragma unroll
+          for (int w = 1; w < kEight; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          int power = 15;
+          frexpf(top, &power);
+          power = top == 0.0f ? 0 : 15 - power < 120 ? 15 - power : 120;  // 2^+-power are normal
+#pragma unroll
+          for (int y = 0; y < 8; ++y) x[y] *= __int_as_float((127 + power) << 23);
+          if (d == 0) row_scale[r] = __int_as_float((127 - power) << 23);
+        }
         if constexpr (K::kF32) {
           *reinterpret_cast<float4*>(shared + chunk_pos<K::kRowBytes, K::kRows>(r, d / 4)) =
               *reinterpret_cast<float4*>(x);
@@ -339,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
       reinterpret_cast<float(*)[K::WK][K::kRows]>(shared + K::kJoinBytes);
   __shared__ Finder finder;
   __shared__ uint2 mask_words[K::kRows];
+  __shared__ float row_scale[K::kRowScale ? K::kRows : 1];
   __shared__ alignas(8) uint64_t full[K::WK][K::kStages], empty[K::WK][K::kStages];
   __shared__ int stage_bad[K::WK][K::kStages];
   __shared__ CtaCtl ctl;
@@ -448,14 +469,13 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
     next.tile += wk;
     to_own_tile();
   }
-  if (more) load_rows<K>(a, cur, row0, shared, mask_words);
+  if (more) load_rows<K>(a, cur, row0, shared, mask_words, row_scale);
   if (leader) {
 #pragma unroll 1
     for (int s = 0; s < K::kStages && more_in; ++s) copy_in();
   }
 
   // ---- the parts of items
-  const float c2 = a.c2;
   while (more) {
     const int context = cur.context, drafts = cur.drafts;
     const int64_t b = cur.b;
@@ -476,6 +496,20 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
     }
     // a thread's rows: warp_row + 16 m + lane / 4, and 8 below
     const int warp_row = wr * 16 * MT;
+    float row_c2[K::kRowScale ? MT : 1][K::kRowScale ? H : 1];
+    if constexpr (K::kRowScale) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const float x = fabsf(p.scale) * kLog2e * row_scale[warp_row + 16 * m + lane / 4 + 8 * h];
+          row_c2[m][h] = x < FLT_MIN ? FLT_MIN : x;  // (as a.c2)
+        }
+    }
+    auto c2_of = [&](int m, int h) {
+      if constexpr (K::kRowScale) return row_c2[m][h];
+      else return a.c2;
+    };
     auto seen = [&](int r, int position) {
       return seen_from(p, mask_words[r], b, token_of(a, row0 + r), position - context, drafts);
     };
@@ -639,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
             for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[m][n][2 * h], s[m][n][2 * h + 1]));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            top[m][h] = t * c2 - K::kBelow;
+            top[m][h] = t * c2_of(m, h) - K::kBelow;
             raise = raise || top[m][h] > base[m][h] + kMaxSlack;
           }
         if (__any_sync(0xffffffffu, raise)) {
@@ -667,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int e = 2 * h; e < 2 * h + 2; ++e) {
-                s[m][n][e] = ex2(__fmaf_rn(s[m][n][e], c2, -from));
+                s[m][n][e] = ex2(__fmaf_rn(s[m][n][e], c2_of(m, h), -from));
                 sum[m][h] += s[m][n][e];
               }
           }
@@ -906,7 +940,7 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
     __syncthreads();  // (the join has been read, q may be written)
     ++cur.head;
     more = enter<K>(a, cur, 0, row0);
-    if (more) load_rows<K>(a, cur, row0, shared, mask_words);
+    if (more) load_rows<K>(a, cur, row0, shared, mask_words, row_scale);
   }
   write_rows_not_there<K>(p);
   // after a wait that ran out: copies still on the way end before the memory is
