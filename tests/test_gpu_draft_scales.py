@@ -45,3 +45,31 @@ def test_an_infinite_query_is_its_rows_alone(cuda_device, ops):  # noqa: F811
     assert out[1, 2, 1].isnan().all()
     out[1, 2, 1] = want[1, 2, 1]
     assert torch.equal(out, want) and want.isfinite().all()
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("n,heads,kv,dim,page", [(24, 8, 2, 64, 16), (9, 6, 2, 128, 24),
+                                                 (40, 5, 1, 128, 8), (33, 16, 2, 64, 64),
+                                                 (4, 6, 2, 64, 16), (30, 4, 4, 64, 5)])
+def test_scales_of_16_bit_activations(cuda_device, ops, kind, n, heads, kv, dim, page):  # noqa: F811
+    """A negative, a zero and a large scale (scores of hundreds, one key far above the
+    rest, late and early), a query that is read element by element: on tcgen05 and on
+    the warps' products."""
+    q, k, v, table, bits = case(n, heads, kv, dim, page, kind, n + dim)
+    for b, j in ((0, 290), (2, 3)):
+        k[int(table[b, j // page]), :, j % page] = 3 * q[b, 2, ::heads // kv].to(kind)
+    q, mask = q.to(kind), pack(bits)
+    args = (k, v, table, ints(CONTEXTS), None, mask)
+    for scale in (dim ** -0.5, 1.0, -0.3, 0.0, 4.0):
+        got = ops.tree_attention(q, *args, scale)
+        check(q, k, v, table, CONTEXTS, [n] * 3, bits, page, got, scale)
+        if scale < 0:  # only q's sign turns
+            other = ops.tree_attention(-q, *args, -scale)
+            assert all(torch.equal(a, b) for a, b in zip(got, other))
+        if scale in (dim ** -0.5, 0.0):
+            norm_check(q, k, v, table, CONTEXTS, [n] * 3, bits, page, got[0], scale)
+        turned = q.transpose(2, 3).contiguous().transpose(2, 3)
+        shifted = torch.nn.functional.pad(q, (3, 0))[..., 3:]
+        for view in (turned, shifted):
+            again = ops.tree_attention(view, *args, scale)
+            assert all(torch.equal(a, b) for a, b in zip(got, again))
