@@ -73,6 +73,8 @@ struct Cfg {
   static constexpr int kWTerms = kF32 ? 1 : F32ACT ? kTerms : 2;
   // Rows of q have factors of their own (load_rows).
   static constexpr bool kRowScale = F32ACT && !kF32 && !kBf16;
+  // All terms of the weights are positive (take_weights).
+  static constexpr bool kPositive = !kRowScale;
   // (packed: pairs of terms, 16 rows each)
   static constexpr int kQTiles = kPack ? (kTerms + 1) / 2 : kTerms;
   static constexpr int kWTiles = kPack ? (kWTerms + 1) / 2 : kWTerms;
@@ -167,10 +169,20 @@ __device__ __forceinline__ void mma_next(bool first, float (&c)[4], const uint32
 }
 // What is left of x beside the TF32 value that the tensor core makes of it (it
 // drops the 13 low bits), rounded to nearest once it drops its own (without the half
-// step errors all point one way: 1.2e-6 of O, with it 7e-7).  What is left of an
-// infinity or a NaN may come out as anything; the value itself stays.
+// step errors all point one way: 1.2e-6 of O, with it 7e-7).  An infinity leaves -0:
+// inf - inf is 0x7fffffff, which the half step turns over.
 __device__ __forceinline__ uint32_t low_tf32(uint32_t x) {
   return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)) + 0x1000u;
+}
+// Infinite cached values.  Terms of the weights that share a sum are positive, all of
+// them, so that an infinite value times them is that infinity, not NaN.  Where low terms
+// may be 0 or negative (f16 with FP32 activations) they have a sum of their own, which
+// counts where the first terms' is finite.
+__device__ __forceinline__ uint32_t low_weight(uint32_t x) {
+  return __float_as_uint(fmaxf(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u), FLT_MIN)) + 0x1000u;
+}
+__device__ __forceinline__ float with_rest(float first, float rest) {
+  return fabsf(first) < INFINITY ? first + rest : first;
 }
 // The next 16-bit term of x and y (x in the low half); x and y keep the rest.
 template <class C>
@@ -185,6 +197,27 @@ __device__ __forceinline__ uint32_t take_term(float& x, float& y) {
     const __half2 h = __floats2half2_rn(x, y);
     w = *reinterpret_cast<const uint32_t*>(&h);
     const float2 f = __half22float2(h);
+    x -= f.x;
+    y -= f.y;
+  }
+  return w;
+}
+// The next term of weights x and y, of which `left` follow: positive where K::kPositive
+// says so.  It is cut off then, f16's from 2^-10 less (what follows is 0 all the same
+// for weights below 2^-14, 2^-22 of the largest; 21 bits).
+template <class K>
+__device__ __forceinline__ uint32_t take_weights(float& x, float& y, int left) {
+  using C = typename K::C;
+  if (!K::kPositive || left == 0) return take_term<C>(x, y);
+  uint32_t w;
+  if constexpr (K::kBf16) {
+    w = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632u);
+    x = fmaxf(x - __uint_as_float(w << 16), FLT_MIN);
+    y = fmaxf(y - __uint_as_float(w & 0xffff0000u), FLT_MIN);
+  } else {
+    constexpr float kBelowOne = 1.0f - 0x1p-10f;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y * kBelowOne), "f"(x * kBelowOne));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
     x -= f.x;
     y -= f.y;
   }
@@ -728,14 +761,15 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
               for (int m = 0; m < MT; ++m) {
                 if constexpr (K::kPack) {
                   const uint32_t w0 = __float_as_uint(s[m][ks][0]), w1 = __float_as_uint(s[m][ks][1]);
-                  const uint32_t w[4] = {w0, low_tf32(w0), w1, low_tf32(w1)};
+                  const uint32_t w[4] = {w0, low_weight(w0), w1, low_weight(w1)};
                   mma_next<C>(ks == 0, acc[m], w, v[0], v[1]);
                   mma<C>(acc[m], w, vl[0], vl[1]);
                   continue;
                 }
                 const uint32_t w[4] = {__float_as_uint(s[m][ks][0]), __float_as_uint(s[m][ks][2]),
                                        __float_as_uint(s[m][ks][1]), __float_as_uint(s[m][ks][3])};
-                const uint32_t wl[4] = {low_tf32(w[0]), low_tf32(w[1]), low_tf32(w[2]), low_tf32(w[3])};
+                const uint32_t wl[4] = {low_weight(w[0]), low_weight(w[1]), low_weight(w[2]),
+                                        low_weight(w[3])};
                 mma_next<C>(ks == 0, acc[m], w, v[0], v[1]);
                 mma<C>(acc[m], wl, v[0], v[1]);
                 mma<C>(acc[m], w, vl[0], vl[1]);
@@ -758,17 +792,21 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   if constexpr (K::kPack) {  // rows 0-7 and 8-15: two terms
-                    w[m][ks][t][j] = 2 * t + j % 2 >= K::kWTerms
-                                         ? 0u
-                                         : take_term<C>(s[m][2 * ks + j / 2][0], s[m][2 * ks + j / 2][1]);
+                    const int term = 2 * t + j % 2;  // (of three: the fourth is next to nothing)
+                    w[m][ks][t][j] = term >= K::kWTerms
+                                         ? 0x00800080u
+                                         : take_weights<K>(s[m][2 * ks + j / 2][0],
+                                                           s[m][2 * ks + j / 2][1], K::kWTerms - 1 - term);
                   } else {
-                    w[m][ks][t][j] = take_term<C>(s[m][2 * ks + j / 2][j % 2 * 2],
-                                                  s[m][2 * ks + j / 2][j % 2 * 2 + 1]);
+                    w[m][ks][t][j] = take_weights<K>(s[m][2 * ks + j / 2][j % 2 * 2],
+                                                     s[m][2 * ks + j / 2][j % 2 * 2 + 1],
+                                                     K::kWTerms - 1 - t);
                   }
                 }
 #pragma unroll
           for (int n = 0; n < D / 16; ++n) {
-            float acc[MT][2][4];
+            constexpr bool kApart = !K::kPositive && !K::kPack;
+            float acc[MT][2][4], others[kApart ? MT : 1][2][4];
 #pragma unroll
             for (int ks = 0; ks < NT / 2; ++ks) {
               uint32_t v[4];
@@ -781,18 +819,30 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
 #pragma unroll
               for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int t = 0; t < K::kWTiles; ++t) {
-                  mma_next<C>(ks + t == 0, acc[m][0], w[m][ks][t], v[0], v[1]);
-                  mma_next<C>(ks + t == 0, acc[m][1], w[m][ks][t], v[2], v[3]);
-                }
+                for (int t = 0; t < K::kWTiles; ++t)
+#pragma unroll
+                  for (int j = 0; j < 2; ++j) {
+                    if constexpr (kApart) {
+                      if (t > 0) {
+                        mma_next<C>(ks == 0, others[m][j], w[m][ks][t], v[2 * j], v[2 * j + 1]);
+                        continue;
+                      }
+                    }
+                    mma_next<C>(ks + t == 0, acc[m][j], w[m][ks][t], v[2 * j], v[2 * j + 1]);
+                  }
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
               for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 2 * H; ++e)
-                  o[m][2 * n + j][e] += K::kPack ? acc[m][j][e] + acc[m][j][2 + e] : acc[m][j][e];
+                for (int e = 0; e < 2 * H; ++e) {
+                  const float first = acc[m][j][e];
+                  if constexpr (kApart) o[m][2 * n + j][e] += with_rest(first, others[m][j][e]);
+                  else if constexpr (!K::kPack) o[m][2 * n + j][e] += first;
+                  else if constexpr (K::kPositive) o[m][2 * n + j][e] += first + acc[m][j][2 + e];
+                  else o[m][2 * n + j][e] += with_rest(first, acc[m][j][2 + e]);
+                }
           }
         }
         if (dirty) {  // infinities and NaN, for the rows that see their token

@@ -113,18 +113,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, 
       : "memory");
 }
 
-// The high term of two weights (x in the low half): the 16-bit numbers at or below them,
-// so that what is left is positive too.
-template <class C>
-__device__ __forceinline__ uint32_t high2(float x, float y) {
-  if constexpr (std::is_same<C, __nv_bfloat16>::value) {
-    return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632u);
-  } else {
-    uint32_t w;
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
-    return w;
-  }
-}
 template <class C>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
   if constexpr (std::is_same<C, __nv_bfloat16>::value) {
@@ -161,15 +149,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// What `high`, high2(x, y), leaves of x and y.
+// The two terms of weights x and y (x in the low half).  Both are positive, so that an
+// infinite cached value times them is that infinity, not NaN: high2 cuts off, f16 what is
+// 2^-10 less (low terms of weights below 2^-14, 2^-22 of the largest, may be 0 even so),
+// and low2 of bf16 takes 2^-23 of the weight on top.
+template <class C>
+__device__ __forceinline__ uint32_t high2(float x, float y) {
+  if constexpr (std::is_same<C, __nv_bfloat16>::value) {
+    return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632u);
+  } else {
+    constexpr float kBelowOne = 1.0f - 0x1p-10f;
+    const float2 f = parts(fma2(pair(x, y), pair(kBelowOne, kBelowOne), pair(0.0f, 0.0f)));
+    uint32_t w;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(f.y), "f"(f.x));
+    return w;
+  }
+}
 template <class C>
 __device__ __forceinline__ uint32_t low2(float x, float y, uint32_t high) {
-  float2 h;
-  if constexpr (std::is_same<C, __nv_bfloat16>::value)
-    h = make_float2(__uint_as_float(high << 16), __uint_as_float(high & 0xffff0000u));
-  else
-    h = __half22float2(*reinterpret_cast<const __half2*>(&high));
-  const float2 rest = parts(fma2(pair(h.x, h.y), pair(-1.0f, -1.0f), pair(x, y)));
+  float2 rest;
+  if constexpr (std::is_same<C, __nv_bfloat16>::value) {
+    constexpr float kAboveOne = 1.0f + 0x1p-23f;
+    rest = parts(fma2(pair(x, y), pair(kAboveOne, kAboveOne),
+                      pair(-__uint_as_float(high << 16), -__uint_as_float(high & 0xffff0000u))));
+  } else {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&high));
+    rest = parts(fma2(pair(h.x, h.y), pair(-1.0f, -1.0f), pair(x, y)));
+  }
   return pack2<C>(rest.x, rest.y);
 }
 // Whether one of the two 16-bit values of w is not finite.

@@ -484,9 +484,12 @@ size_t ct_tree_attention_workspace_size(int64_t drafts, int64_t q_heads, int64_t
  * rows of a sequence with a negative context_lens[b] (it takes no part) give O = 0
  * and LSE = -inf; a length beyond max_pages * page_size, or a page out of range,
  * gives NaN in the rows that are there.  What slots past the last new token hold
- * has no effect (they may be fetched with the others of their page).  A cached value that is not finite reaches the rows that see its token:
- * a key with a score of -inf has no weight, scores of +inf or NaN make their row
- * NaN, and values that are not finite make their element of O infinite or NaN.
+ * has no effect (they may be fetched with the others of their page).  Cached values
+ * that are not finite reach the rows that see their token, by the formula: a key
+ * with a score of -inf has no weight, a score of +inf or NaN makes its row NaN, an
+ * infinite value makes its element of O infinite, or NaN where its key has no
+ * weight.  (Weights below 2^-120 of the largest may count as none, those over an
+ * f16 cache below 2^-22.)
  * The workspace (16-byte aligned) needs no clearing and must not be used by
  * another call that can run concurrently.  Deterministic.  No reference
  * counterpart (the reference keeps no cache). */
