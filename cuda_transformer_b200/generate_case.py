@@ -125,7 +125,9 @@ class Generator:
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)  # tokens in the history
         self.prompt_lens = torch.zeros_like(self.lens)
         self.live = torch.zeros(batch, dtype=torch.bool, device=device)  # takes part in steps
-        self.counts = [0] * batch  # the host's count of the tokens; 0: none begun
+        # The host's counts of the tokens (0: none begun).  keep_path adds up to _ahead
+        # tokens that they lack; a graph that holds one does so unseen.
+        self.counts, self._ahead, self._captured = [0] * batch, 0, False
 
     def _embed(self, idx, positions):
         x = self.model.tok(idx)
@@ -189,6 +191,7 @@ class Generator:
     def fork(self, src: int, dst: int, room: int = 0) -> None:
         """Sequence dst begins as src is now (its tokens and their cached keys
         and values); `room`: tokens to reserve pages for."""
+        self._count()
         n = self.counts[src]
         if n == 0 or src == dst:
             raise ValueError(f"sequence {src} cannot be forked into {dst}")
@@ -213,14 +216,32 @@ class Generator:
         current lengths) and returns the logits after them [batch, vocab]
         (those of sequences that take no part mean nothing).  A negative token
         ends its sequence; its pages stay until `release`.  No host
-        synchronisation.  A sequence without room for it is a ValueError."""
+        synchronisation, unless room is short after `keep_path`: then the
+        lengths are read back.  A sequence without room for it is a ValueError."""
         self._take_room()
         return self._step(idx)
 
+    def _count(self) -> None:
+        """Brings the host's counts up to the device's."""
+        if self._ahead or self._captured:
+            self.counts = [have if n else 0 for n, have in zip(self.counts, self.lens.tolist())]
+            self._ahead = 0
+
+    def _need_room(self, more: int) -> None:
+        if self._captured:
+            self._count()
+        while True:
+            full = [seq for seq, n in enumerate(self.counts) if n and n + self._ahead + more > min(
+                self.max_len, len(self.pool.owned[seq]) * self.pool.page_size)]
+            if full and not self._ahead:
+                raise ValueError(f"sequence {full[0]} has no room for {more} more tokens after its "
+                                 f"{self.counts[full[0]]}")
+            if not full:
+                return
+            self._count()
+
     def _take_room(self) -> None:
-        for seq, n in enumerate(self.counts):
-            if n and n >= min(self.max_len, len(self.pool.owned[seq]) * self.pool.page_size):
-                raise ValueError(f"sequence {seq} has no room for a token after its {n}")
+        self._need_room(1)
         self.counts = [n + 1 if n else 0 for n in self.counts]
 
     @torch.no_grad()
@@ -335,7 +356,11 @@ class Generator:
     @torch.no_grad()
     def keep_path(self, tokens: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> None:
         """The nodes of `path` (verify_drafts') join their sequences, in the
-        cache and in the history."""
+        cache and in the history.  How many, the host learns when it has to
+        know (`fork`)."""
+        self._ahead += path.shape[1]
+        if path.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._captured = True
         counts = torch.where(self.live, counts, 0)
         ops.kv_compact_([c for pair in self.caches for c in pair], self.pool.table, self.lens, path,
                         counts)
@@ -399,8 +424,8 @@ class Generator:
             steps += 1
             for seq, (row, count) in enumerate(zip(found.tolist(), counts.tolist())):
                 if not ended[seq]:
-                    self.counts[seq] += count
                     made[seq].extend(row[:count])
+        self._count()
         filled = [(m + [-1] * new)[:new] for m in made]
         return torch.tensor(filled, device=device), steps
 

@@ -1,0 +1,86 @@
+"""What the host knows of a generator's sequences while drafts are kept on the device: CPU
+tests (the operators that move what the cache holds are stand-ins)."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def moved(monkeypatch):
+    """Calls of the cache operators, by name."""
+    from cuda_transformer_b200 import generate_case
+
+    calls = []
+    monkeypatch.setattr(generate_case.ops, "kv_compact_", lambda caches, *a: calls.append(("compact",) + a))
+    monkeypatch.setattr(generate_case.ops, "kv_copy_pages_",
+                        lambda caches, src, dst: calls.append(("copy", src.tolist(), dst.tolist())))
+    return calls
+
+
+def generator(batch=2, max_len=48, page=4, **kw):
+    from cuda_transformer_b200.generate_case import Generator
+    from cuda_transformer_b200.gpt_case import GPT
+
+    return Generator(GPT(1, 64, 2, max_len, 10), batch, max_len, page, **kw)
+
+
+def begin(gen, seq, tokens, room):
+    """As `prompt` leaves a sequence."""
+    gen.pool.reserve(seq, room)
+    gen.history[seq, :tokens] = torch.arange(tokens)
+    gen.lens[seq] = gen.prompt_lens[seq] = gen.counts[seq] = tokens
+    gen.live[seq] = True
+
+
+def keep(gen, counts, n=None):
+    """keep_path of a chain's first counts[b] nodes."""
+    n = n or max(counts)
+    at = torch.arange(n, dtype=torch.int32)
+    counts = torch.tensor(counts, dtype=torch.int32)
+    path = torch.where(at < counts[:, None], at, -1)
+    gen.keep_path(torch.arange(n).expand(len(counts), n) + 5, path, counts)
+
+
+def test_a_fork_after_kept_drafts_has_all_of_them(moved):
+    """Pages of what the sequence holds now, not of what the host counted before."""
+    gen = generator()
+    begin(gen, 0, 5, 40)
+    keep(gen, [5, 0])
+    assert gen.lens.tolist() == [10, 0]
+    gen.fork(0, 1, 40)
+    assert gen.lens.tolist() == [10, 10] and gen.counts == [10, 10]
+    assert gen.pool.owned[1][:2] == gen.pool.owned[0][:2]  # two full pages
+    assert moved[-1] == ("copy", [gen.pool.owned[0][2]], [gen.pool.owned[1][2]])
+    assert gen.history[1, :10].tolist() == gen.history[0, :10].tolist()
+
+
+def step(gen):
+    """What a step does to the lengths."""
+    gen._take_room()
+    gen.lens += gen.live
+
+
+def test_a_step_after_kept_drafts_looks_for_room(moved):
+    """Where the most that drafts can have added leaves none, what they did add counts."""
+    gen = generator()
+    begin(gen, 0, 5, 8)
+    keep(gen, [3, 0])
+    with pytest.raises(ValueError):  # 8 of 8
+        step(gen)
+    gen.release(0)
+    begin(gen, 1, 3, 8)
+    keep(gen, [0, 2], 8)
+    for _ in range(3):
+        step(gen)
+    with pytest.raises(ValueError):
+        step(gen)
+    assert gen.lens.tolist() == gen.counts == [0, 8]
+
+
+def test_sequences_that_take_no_part_keep_their_counts(moved):
+    gen = generator()
+    begin(gen, 0, 5, 20)
+    begin(gen, 1, 7, 20)
+    gen.live[1] = False
+    keep(gen, [3, 3])
+    gen._count()
+    assert gen.lens.tolist() == gen.counts == [8, 7]
