@@ -324,7 +324,6 @@ class Generator:
         fine = (best >= 0)[:, :, None] & (places < lens[:, :, None])
         return torch.cat([root[:, None], torch.where(fine.flatten(1), tokens, -1)], 1)
 
-    @torch.no_grad()
     def step_drafts(self, tokens: torch.Tensor, parents: torch.Tensor, mask: torch.Tensor,
                     depths: torch.Tensor) -> torch.Tensor:
         """Feeds every sequence the nodes of a tree (tokens int64 [batch, n],
@@ -332,8 +331,16 @@ class Generator:
         take it, depths int32 [n] its nodes' distances from node 0) and returns
         the logits after each [batch, n, vocab].  The nodes' keys and values
         are in the cache behind the sequence, in their order; `keep_path` says
-        which of them stay.  The sequences' pages must have room for n tokens
-        (else: NaN).  A negative node 0 ends its sequence, as in `step`."""
+        which of them stay.  A sequence without room for n tokens is a
+        ValueError (in a graph, whose replays the host does not see: NaN).  A
+        negative node 0 ends its sequence, as in `step`."""
+        if not (tokens.is_cuda and torch.cuda.is_current_stream_capturing()):
+            self._need_room(tokens.shape[1])
+        return self._step_drafts(tokens, parents, mask, depths)
+
+    @torch.no_grad()
+    def _step_drafts(self, tokens, parents, mask, depths):
+        """The device's part of a drafted step."""
         batch, n = tokens.shape
         self.live &= tokens[:, 0] >= 0
         at = torch.arange(n, dtype=torch.int32, device=tokens.device)
@@ -362,6 +369,7 @@ class Generator:
         if path.is_cuda and torch.cuda.is_current_stream_capturing():
             self._captured = True
         counts = torch.where(self.live, counts, 0)
+        counts = torch.minimum(counts, self.max_len - self.lens)  # (what has no column)
         ops.kv_compact_([c for pair in self.caches for c in pair], self.pool.table, self.lens, path,
                         counts)
         at = torch.arange(path.shape[1], device=path.device)
@@ -416,7 +424,7 @@ class Generator:
                 break
             self.live &= ~torch.tensor(ended, device=device)
             tokens = self.look_up_drafts(root, depth, branches)
-            logits = self.step_drafts(tokens, parents, mask, depths)
+            logits = self._step_drafts(tokens, parents, mask, depths)
             found, path, counts = ops.verify_drafts(scores(logits), tokens, parents,
                                                     uniform=uniform())
             self.keep_path(tokens, path, counts)

@@ -84,3 +84,32 @@ def test_sequences_that_take_no_part_keep_their_counts(moved):
     keep(gen, [3, 3])
     gen._count()
     assert gen.lens.tolist() == gen.counts == [8, 7]
+
+
+def test_kept_drafts_stay_within_the_longest_length(moved):
+    """max_len is no multiple of the page: pages have places behind it, the history has not."""
+    gen = generator(2, 10, 4)
+    begin(gen, 0, 5, 10)  # 12 places
+    begin(gen, 1, 10, 10)
+    keep(gen, [7, 3])
+    assert gen.lens.tolist() == [10, 10]
+    assert moved[-1][-1].tolist() == [5, 0]
+    assert gen.history[0].tolist() == [0, 1, 2, 3, 4, 5, 6, 7, 8, 9]
+    assert gen.history[1].tolist() == list(range(10))
+
+
+def test_drafts_without_room_are_refused(moved):
+    """Before anything runs: in the sequence's pages, and within the longest length."""
+    gen = generator(2, 10, 4)
+    node = torch.arange(4, dtype=torch.int32)
+    tree = (torch.zeros(2, 4, dtype=torch.int64), node - 1, None, node)
+    for tokens, room in ((5, 8), (7, 10)):
+        begin(gen, 1, tokens, room)
+        with pytest.raises(ValueError):
+            gen.step_drafts(*tree)
+        assert gen.live.tolist() == [False, True]
+        gen.release(1)
+    begin(gen, 1, 3, 8)
+    keep(gen, [0, 2])
+    with pytest.raises(ValueError):
+        gen.step_drafts(*tree)
