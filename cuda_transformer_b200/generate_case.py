@@ -384,7 +384,9 @@ class Generator:
         without processing (with a temperature: distributed alike), and the
         number of steps that it took.  Each step feeds a tree of looked-up
         tokens; max_len has to hold branches * depth tokens more than the
-        prompts and the new ones.  A sequence that has no next token ends: -1."""
+        prompts and the new ones.  A sequence that has no next token ends: -1.
+        The others go on from there: they hold all of their tokens but the
+        last, which the next `step` feeds."""
         if len(prompts) != self.batch:
             raise ValueError(f"{len(prompts)} prompts for {self.batch} sequences")
         device = self.history.device
@@ -410,6 +412,7 @@ class Generator:
             return logits if temperature == 0.0 else ops.cuda_softmax(logits / temperature)
 
         logits = self._prompts(prompts, new + n)
+        begun = list(self.counts)
         # the first token: a tree of its root alone
         u = uniform()
         root = ops.verify_drafts(scores(logits[:, None]), torch.zeros_like(self.lens)[:, None].long(),
@@ -433,7 +436,12 @@ class Generator:
             for seq, (row, count) in enumerate(zip(found.tolist(), counts.tolist())):
                 if not ended[seq]:
                     made[seq].extend(row[:count])
-        self._count()
+        # what came after the last token goes out again (no row reads it)
+        there = [(m + [-1]).index(-1) for m in made]
+        fed = [n + min(t, max(new - 1, 0)) for n, t in zip(begun, there)]
+        self.lens.copy_(torch.tensor(fed, dtype=torch.int32))
+        self.live.copy_(torch.tensor([t >= new for t in there]))
+        self.counts, self._ahead = fed, 0
         filled = [(m + [-1] * new)[:new] for m in made]
         return torch.tensor(filled, device=device), steps
 

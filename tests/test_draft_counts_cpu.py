@@ -113,3 +113,41 @@ def test_drafts_without_room_are_refused(moved):
     keep(gen, [0, 2])
     with pytest.raises(ValueError):
         gen.step_drafts(*tree)
+
+
+def test_generated_sequences_end_alike(moved, monkeypatch):
+    """Whichever of them had its tokens first: each holds its tokens but the last and goes
+    on; one that ended before does not."""
+    from cuda_transformer_b200 import generate_case
+
+    gen = generator(4, 48, 4)
+
+    def prompts(prompts, room):
+        for b, t in enumerate(prompts):
+            begin(gen, b, t.numel(), t.numel() + room)
+        return torch.zeros(4, 10)
+
+    # what is found a step: 5 tokens at once, one by one, none after two, none at all
+    found = [[[1], [1], [1], [-1]],
+             [[2, 3, 4, 5, 6], [2, -1, -1, -1, -1], [2, -1, -1, -1, -1], [9, 9, 9, 9, 9]],
+             [[9] * 5, [3] + [-1] * 4, [-1] * 5, [9] * 5]]
+    kept = [[1, 1, 1, 1], [5, 1, 1, 5], [5, 1, 1, 5]]
+    steps = iter(zip(found, kept))
+
+    def verify(target, tokens, *a, **kw):
+        new, counts = next(steps)
+        n = tokens.shape[1]
+        at = torch.arange(n, dtype=torch.int32)
+        counts = torch.tensor(counts, dtype=torch.int32)
+        return (torch.tensor(new)[:, :n], torch.where(at < counts[:, None], at, -1), counts)
+
+    monkeypatch.setattr(gen, "_prompts", prompts)
+    monkeypatch.setattr(gen, "_step_drafts", lambda *a: torch.zeros(4, 5, 10))
+    monkeypatch.setattr(generate_case.ops, "verify_drafts", verify)
+    tokens, steps = gen.generate_drafted([torch.zeros(n) for n in (3, 4, 5, 6)], 3, 4)
+    assert tokens.tolist() == [[1, 2, 3], [1, 2, 3], [1, 2, -1], [-1, -1, -1]] and steps == 2
+    assert gen.live.tolist() == [True, True, False, False]
+    assert gen.lens.tolist() == gen.counts == [5, 6, 7, 6]
+    step(gen)
+    gen._count()
+    assert gen.lens.tolist() == [6, 7, 7, 6]

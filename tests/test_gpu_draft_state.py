@@ -42,3 +42,23 @@ def test_a_fork_after_kept_drafts(cuda_device, rotary):
         logits = gen.step(torch.tensor(idx, device="cuda"))
         for seq in (0, 2):
             assert (logits[seq] - whole(model, gen, seq, rotary)).abs().max().item() <= 2e-5
+
+
+@pytest.mark.parametrize("rotary", [False, True])
+@pytest.mark.parametrize("depth,branches", [(4, 1), (3, 2)])
+def test_going_on_after_drafted_generation(cuda_device, rotary, depth, branches):
+    """The last tokens are fed next, then others; a fork goes on as well.  Sequences that
+    had all of their tokens earlier than others are among them."""
+    model, prompts, gen = setup(rotary=rotary)
+    tokens, _ = gen.generate_drafted(prompts, 16, depth, branches)
+    assert gen.live.all()
+    for b, p in enumerate(prompts):
+        assert gen.history[b, :int(gen.lens[b])].tolist() == p.tolist() + tokens[b, :-1].tolist()
+    for idx in (tokens[:, -1], torch.tensor([5, 9, 2], device="cuda")):
+        logits = gen.step(idx)
+        for seq in range(3):
+            assert (logits[seq] - whole(model, gen, seq, rotary)).abs().max().item() <= 2e-5
+    gen.fork(1, 0, 45)
+    logits = gen.step(torch.tensor([8, 7, 6], device="cuda"))
+    for seq in range(3):
+        assert (logits[seq] - whole(model, gen, seq, rotary)).abs().max().item() <= 2e-5
