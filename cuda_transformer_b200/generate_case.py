@@ -266,6 +266,11 @@ class Generator:
         x = self._embed(idx.clamp(min=0), at).unsqueeze(0)
         return self._logits(self._blocks(x, attend))
 
+    def _probabilities(self, logits: torch.Tensor, temperature: float) -> torch.Tensor:
+        # (bounded: +inf, as a bias can make it, takes all of the softmax)
+        top = torch.finfo(torch.float32).max
+        return ops.cuda_softmax((logits / temperature).clamp_(max=top))
+
     @torch.no_grad()
     def choose(self, logits: torch.Tensor, temperature: float = 0.0, uniform=None,
                **processing) -> torch.Tensor:
@@ -280,9 +285,7 @@ class Generator:
             best, idx = logits.max(-1)
             there = best > float("-inf")  # (false for NaN too)
         else:
-            # (bounded: +inf, as a bias can make it, takes all of the softmax)
-            top = torch.finfo(torch.float32).max
-            probs = ops.cuda_softmax((logits / temperature).clamp_(max=top).unsqueeze(0))[0]
+            probs = self._probabilities(logits.unsqueeze(0), temperature)[0]
             # the first token whose running sum passes the number; a scan's sums can
             # step up by a rounding at a token of probability 0, which has no say
             upto = torch.where(probs > 0, probs.cumsum(-1), 0.0)
@@ -409,7 +412,7 @@ class Generator:
             return torch.rand(self.batch, n, generator=g, device=device) if temperature else None
 
         def scores(logits):  # what verify_drafts takes: scores, or probabilities
-            return logits if temperature == 0.0 else ops.cuda_softmax(logits / temperature)
+            return logits if temperature == 0.0 else self._probabilities(logits, temperature)
 
         logits = self._prompts(prompts, new + n)
         begun = list(self.counts)

@@ -62,3 +62,26 @@ def test_going_on_after_drafted_generation(cuda_device, rotary, depth, branches)
     logits = gen.step(torch.tensor([8, 7, 6], device="cuda"))
     for seq in range(3):
         assert (logits[seq] - whole(model, gen, seq, rotary)).abs().max().item() <= 2e-5
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0, 1e-39])
+def test_an_infinite_logit_is_drawn(cuda_device, temperature):
+    """As in steps of one token; a temperature that makes logits infinite likewise."""
+    model, prompts, gen = setup()
+    if temperature < 1e-30:
+        with torch.no_grad():
+            model.lm_head_bias[7] = 100.0
+    else:
+        with torch.no_grad():
+            model.lm_head_bias[7] = torch.inf
+    tokens, _ = gen.generate_drafted(prompts, 6, 2, 2, temperature=temperature)
+    if temperature == 1e-39:  # (1 / 1e-39 is beyond FP32: all positive logits are bounded, and drawn alike)
+        from cuda_transformer_b200.generate_case import whole_sequence_logits
+
+        for b, p in enumerate(prompts):
+            seq = torch.cat([p, tokens[b]])
+            for t in range(6):
+                ref = whole_sequence_logits(model, seq[:p.numel() + t])
+                assert tokens[b, t] >= 0 and ref[tokens[b, t]] > 0
+    else:
+        assert (tokens == 7).all()
