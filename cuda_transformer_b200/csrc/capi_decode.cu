@@ -74,11 +74,11 @@ int check_sizes(int64_t caches_n, int64_t kv_heads, int64_t head_dim, int64_t pa
 // checked before the first; distinct: one that is there twice is refused.
 template <class P, class F>
 int for_caches(P& p, void* const* caches, const int64_t* strides, int64_t n, int64_t kv_heads,
-               int64_t pages, int64_t page_size, bool distinct, F&& launch) {
+               int64_t head_dim, int64_t pages, int64_t page_size, bool distinct, F&& launch) {
   const int64_t sizes[3] = {pages, kv_heads, page_size};
   for (int64_t c = 0; c < n; ++c) {
     if (pages > 0 && !caches[c]) return CT_ERR_INVALID_ARGUMENT;
-    if (strides[4 * c + 3] != 1) return CT_ERR_UNSUPPORTED_LAYOUT;
+    if (head_dim > 1 && strides[4 * c + 3] != 1) return CT_ERR_UNSUPPORTED_LAYOUT;
     for (int i = 0; i < 3; ++i)
       if (stride_of(sizes[i], strides[4 * c + i]) < 0) return CT_ERR_UNSUPPORTED_LAYOUT;
   }
@@ -415,7 +415,7 @@ int ct_kv_compact(void* const* caches, const int64_t* cache_strides, int64_t cac
   p.head_dim = (int)head_dim;
   p.dtype = cache_dtype;
   // (what is there twice would be moved twice, by threads that do not wait for each other)
-  return for_caches(p, caches, cache_strides, caches_n, kv_heads, pages, page_size, true,
+  return for_caches(p, caches, cache_strides, caches_n, kv_heads, head_dim, pages, page_size, true,
                     [&](const DeviceInfo& dev) {
                       return launch_kv_compact(p, dev, reinterpret_cast<cudaStream_t>(stream));
                     });
@@ -439,7 +439,7 @@ int ct_kv_copy_pages(void* const* caches, const int64_t* cache_strides, int64_t 
   p.page_size = (int)page_size;
   p.head_dim = (int)head_dim;
   p.dtype = cache_dtype;
-  return for_caches(p, caches, cache_strides, caches_n, kv_heads, pages, page_size, false,
+  return for_caches(p, caches, cache_strides, caches_n, kv_heads, head_dim, pages, page_size, false,
                     [&](const DeviceInfo& dev) {
                       return launch_kv_copy_pages(p, dev, reinterpret_cast<cudaStream_t>(stream));
                     });

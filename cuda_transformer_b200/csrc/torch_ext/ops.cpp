@@ -781,7 +781,7 @@ CacheTensors cache_tensors(at::TensorList caches) {
     check_on(t, caches[0], caches[0].scalar_type(), "caches");
     TORCH_CHECK(t.dim() == 4 && t.sizes() == caches[0].sizes(),
                 "caches must be [pages, kv_heads, page_size, hs] of equal shape");
-    TORCH_CHECK(t.stride(3) == 1, "caches must have unit stride along hs");
+    TORCH_CHECK(t.stride(3) == 1 || t.size(3) <= 1, "caches must have unit stride along hs");
     c.base.push_back(t.data_ptr());
     for (int i = 0; i < 4; ++i) c.strides.push_back(t.stride(i));
   }

@@ -130,6 +130,14 @@ def test_one_cache_twice_is_refused():
     assert compact(caches=one, strides=strides(3), n=3, pages=0) == cb.CT_OK
 
 
+def test_strides_of_single_elements_are_not_looked_at():
+    """A head dim of one element has any stride."""
+    one = dict(dim=1, pages=0, strides=strides(2, (64, 32, 8, 7)))
+    assert compact(**one) == copy(**one) == cb.CT_OK
+    two = dict(one, dim=2)
+    assert compact(**two) == copy(**two) == LAYOUT
+
+
 def test_append_refusals_with_angles():
     """ct_kv_append_ex checks what ct_kv_append checks."""
     S3 = (ctypes.c_int64 * 3)(64, 64, 1)

@@ -718,3 +718,19 @@ def test_append_with_other_angles(cuda_device, ops, interleaved, act, cache):
     # without a rotation the angles are not looked at
     ops.kv_append_(kc, vc, k, v, table, slots, seq_ids=seq, rotary_positions=angles)
     assert torch.equal(kc[3, :, 3], k[5].to(cache))
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_moves_of_single_elements(cuda_device, ops, kind):
+    """A head dim of one, cut out of a wider row: its stride means nothing."""
+    g = gen(31)
+    wide = [torch.randint(0, 251, (6, 2, 4, 8), generator=g, device="cuda").to(kind) for _ in range(2)]
+    want = [w.clone() for w in wide]
+    caches = [w[..., 3::8] for w in wide]
+    assert caches[0].shape[3] == 1 and caches[0].stride(3) == 8
+    for w in want:
+        w[5, ..., 3] = w[1, ..., 3]
+        w[0, :, 1, 3] = w[0, :, 2, 3]
+    ops.kv_copy_pages_(caches, ints([1]), ints([5]))
+    ops.kv_compact_(caches, ints([[0]]), ints([0]), ints([[0, 2]]), ints([2]))
+    assert all(torch.equal(w, x) for w, x in zip(wide, want))
