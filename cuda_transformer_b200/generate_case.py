@@ -392,14 +392,17 @@ class Generator:
         last, which the next `step` feeds."""
         if len(prompts) != self.batch:
             raise ValueError(f"{len(prompts)} prompts for {self.batch} sequences")
+        if depth < 0 or branches < 0:
+            raise ValueError(f"drafts of {branches} branches of {depth} tokens")
         device = self.history.device
         n = 1 + branches * depth
+        span = max(depth, 1)  # (a tree may be its root alone)
         node = torch.arange(n, dtype=torch.int32, device=device)
-        first = (node - 1) % depth == 0
+        first = (node - 1) % span == 0
         parents = torch.where(node == 0, -1, torch.where(first, 0, node - 1))
-        depths = torch.where(node == 0, 0, (node - 1) % depth + 1).int()
+        depths = torch.where(node == 0, 0, (node - 1) % span + 1).int()
         # a node sees the root and its branch up to itself
-        alike = (node[:, None] - 1) // depth == (node - 1) // depth
+        alike = (node[:, None] - 1) // span == (node - 1) // span
         sees = (node == 0) | (alike & (node <= node[:, None]) & (node[:, None] > 0))
         words = torch.nn.functional.pad(sees, (0, -n % 32)).unflatten(1, (-1, 32)).long()
         words = (words << torch.arange(32, device=device)).sum(-1)

@@ -151,3 +151,36 @@ def test_generated_sequences_end_alike(moved, monkeypatch):
     step(gen)
     gen._count()
     assert gen.lens.tolist() == [6, 7, 7, 6]
+
+
+@pytest.mark.parametrize("depth,branches", [(0, 1), (0, 3), (4, 0)])
+def test_generation_with_drafts_of_no_tokens(moved, monkeypatch, depth, branches):
+    """A tree of its root alone is a step of one token; fewer than none are refused."""
+    from cuda_transformer_b200 import generate_case
+
+    gen = generator()
+
+    def prompts(prompts, room):
+        for b, t in enumerate(prompts):
+            begin(gen, b, t.numel(), t.numel() + room)
+        return torch.zeros(2, 10)
+
+    def verify(target, tokens, *a, **kw):
+        assert tokens.shape == (2, 1)
+        ones = torch.ones(2, dtype=torch.int32)
+        return tokens + 1, torch.zeros(2, 1, dtype=torch.int32), ones
+
+    def step(tokens, parents, mask, depths):
+        assert parents.tolist() == [[-1]] * 2 and mask.tolist() == [[[1]]] * 2
+        assert depths.tolist() == [0]
+        return torch.zeros(2, 1, 10)
+
+    monkeypatch.setattr(gen, "_prompts", prompts)
+    monkeypatch.setattr(gen, "_step_drafts", step)
+    monkeypatch.setattr(generate_case.ops, "verify_drafts", verify)
+    some = [torch.zeros(3), torch.zeros(4)]
+    tokens, steps = gen.generate_drafted(some, 3, depth, branches)
+    assert tokens.tolist() == [[1, 2, 3]] * 2 and steps == 2
+    for bad in ((-1, 2), (2, -1)):
+        with pytest.raises(ValueError):
+            gen.generate_drafted(some, 3, *bad)
