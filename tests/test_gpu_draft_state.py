@@ -85,3 +85,36 @@ def test_an_infinite_logit_is_drawn(cuda_device, temperature):
                 assert tokens[b, t] >= 0 and ref[tokens[b, t]] > 0
     else:
         assert (tokens == 7).all()
+
+
+def test_captured_drafted_steps(cuda_device):
+    """A graph's drafted steps go unseen by the host: a fork and a step read the lengths."""
+    model, prompts, gen = setup()
+    for b in (0, 2):
+        gen.prompt(b, prompts[b], prompts[b].numel() + 30)
+    tokens = (torch.arange(12, device="cuda") * 5 % 65).view(3, 4)
+    path, counts = path_of([4, 0, 2], 4)
+
+    def drafted():
+        logits = gen.step_drafts(tokens, *chain(3, 4))
+        gen.keep_path(tokens, path, counts)
+        return logits
+
+    drafted()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = drafted()
+    for _ in range(3):
+        graph.replay()
+    for b, row in ((0, 3), (2, 1)):
+        assert (logits[b, row] - whole(model, gen, b, False)).abs().max().item() <= 2e-5
+    gen.fork(0, 1, 24)
+    assert gen.counts == gen.lens.tolist() == [17, 17, 17]
+    for _ in range(7):
+        out = gen.step(torch.tensor([3, 4, 5], device="cuda"))
+        for b in range(3):
+            assert (out[b] - whole(model, gen, b, False)).abs().max().item() <= 2e-5
+    with pytest.raises(ValueError):  # the fork's 24
+        gen.release(0)
+        for _ in range(8):
+            gen.step(torch.tensor([3, 4, 5], device="cuda"))
