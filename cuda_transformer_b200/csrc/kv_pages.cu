@@ -7,9 +7,11 @@
 // where rows are not aligned to that, one element.
 //
 // Measured (device): the kept quarter of 64 trees of 16, 24 caches of 8 heads of 128,
-// BF16: 8 us; every other one of 4 x 8192 tokens, 8 caches of 32 heads of 64: 249 us,
-// 4.2 TB/s of what has to move (the kept tokens are 128 bytes of each 256, and DRAM's
-// unit is 64); 512 pages of 16 tokens, 24 caches: 127 us.
+// BF16: 8 us; a random half of 4 x 8192 tokens, 8 caches of 32 heads of 64: 248 us, 4.3
+// TB/s of what has to move, and DRAM moves nothing else (0.54 GB read, 0.48 written while
+// it runs): threads wait for their loads and for the lists.  The same caches with the
+// first token dropped, which is one chain a sequence: 4.4 ms (the bytes take 0.33), the first
+// 4, 64, 512: 2.8, 2.0, 0.43.  512 pages of 16 tokens, 24 caches: 127 us.
 #include "decode_common.cuh"
 
 namespace ct {

@@ -23,9 +23,11 @@
 // as two TF32 terms each way (22 bits).  16-bit activations: the weights in two terms of
 // that type (16 bits and more), as in paged_attention; they are summed unrounded.
 //
-// Measured (device): 16 chains of 5 on 12 heads of 64 with FP32 activations over a BF16
-// cache of 3500 to 4096 tokens: 92 us, 5.4 TB/s of K and V; with a product a term
-// instead of two terms a product, two CTAs an SM, 114.  8 trees of 8 on 6 heads of 64 over
+// Measured (device): 16 chains of up to 5 on 32 heads of 64 with FP32 activations over a
+// BF16 cache of 3500 to 4096 tokens: 90 us, 5.5 TB/s of K and V; with a product a term
+// instead of two terms a product, two CTAs an SM, 114.  FP32 on FP32, 8 sequences of 2000
+// tokens on 32 and 8 heads of 128, 8, 32 and 128 rows: 39, 73 and 240 us for 20 us of
+// bytes (three products for one; the tensor pipe is busy 41 % of the last).  8 trees of 8 on 6 heads of 64 over
 // up to 248 tokens, FP32: 12.5 us, of which the launch and one pass through the
 // latencies are most.
 #include <cfloat>
@@ -99,9 +101,9 @@ struct Cfg {
   static constexpr int kMinShare = kItemCost + 2 * WK;
   // Tables of at most so many tokens are not split (an item a CTA, and no join): the
   // longer, the cheaper a token.  Not split / split, us: 8 sequences of 750 tokens on
-  // 32 and 8 heads of 128, BF16, 4 drafts 21.9 / 23.7, of 980 26.6 / 24.4; FP32, 8
-  // drafts on 6 heads of 64, 480 tokens 16.5 / 22.6, 980 26.7 / 24.6; 64 drafts, 300
-  // tokens 41 / 47, 600 61 / 57.
+  // 32 and 8 heads of 128, BF16, 4 drafts 21.0 / 23.1, of 980 25.6 / 23.5; FP32, 8
+  // drafts on 6 heads of 64, 480 tokens 15.8 / 21.8, 980 26.1 / 24.0; 64 drafts, 300
+  // tokens 38 / 44, 600 64 / 58.
   static constexpr int64_t kWholeTokens = !F32ACT ? 768 : kF32 && !kPack ? 256 : 512;
   // f16 weights reach up to 2^14 instead of 1, clear of the subnormals.
   static constexpr float kBelow = !kF32 && !kBf16 ? 8.0f : 0.0f;

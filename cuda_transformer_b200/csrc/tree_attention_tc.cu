@@ -21,13 +21,14 @@
 // output's own rounding is 0.0017), a step over one token with paged_attention would not.
 //
 // Measured (device): one tree of 64 on 32 and 8 heads of 128 over 131,072 tokens,
-// BF16, 256 rows an item: 155 us, 3.47 TB/s and 888 TFLOP/s of products.  A tile of a
-// CTA takes about 1850 cycles, of which the softmax needs 1400 and the issuing of
-// products 1540; loads alone take 114 us, everything but the softmax 152, everything
-// but the products 128.  Tried there and slower, the same state 165: eight warps with
-// the rows 189, tiles of 128 keys with one S 201, one CTA an SM with two groups of
-// warps that alternate 170, with 256 rows that share the keys 214.  64 trees of 16
-// over 300 to 2048 tokens: 58 us.
+// BF16, 256 rows an item: 195 us, 2.8 TB/s, in bursts; 234 in a stream of such calls, where
+// the power limit takes the clock to 1.48 GHz.  A tile of a CTA takes about 2600 cycles,
+// the tensor pipe is busy 58 % of them.  With one term of the weights, 155 us, it took
+// about 1850, of which the softmax needed 1400 and the issuing of products 1540; loads
+// alone took 114 us, everything but the softmax 152, everything but the products 128.
+// Tried then and slower, the same state 165: eight warps with the rows 189, tiles of 128
+// keys with one S 201, one CTA an SM with two groups of warps that alternate 170, with
+// 256 rows that share the keys 214.  64 trees of 16 over 16 to 4096 tokens: 58 us.
 #include "tree_attention.cuh"
 
 namespace ct {
@@ -56,8 +57,8 @@ struct TcCfg {
   // Two CTAs' 512 columns of Tensor Memory: O, then two buffers of S.
   static constexpr int kColumns = 256, kS = 128;
   // What an item costs beside its tiles, in tiles; units of a share at least.  2, 4,
-  // 6, 9: 64 trees of 16 over 300 to 2048 tokens 62, 58, 62, 67 us, 32 of up to 33 on
-  // one head 45, 45, 47, 48.
+  // 6, 9: 64 trees of 16 over 16 to 4096 tokens 61, 58, 61, 67 us, 32 of up to 33 on
+  // one head 44, 43, 43, 46.
   static constexpr int kItemCost = 4;
   static constexpr int kMinShare = kItemCost + 2;
   // Tiles whose products (8 each) may pile up in Tensor Memory: the tensor core cuts
@@ -67,8 +68,8 @@ struct TcCfg {
   // f16 weights reach up to 2^14 instead of 1, clear of the subnormals.
   static constexpr float kBelow = kBf16 ? 0.0f : 8.0f;
   // Tables of at most so many tokens are not split (as in tree_attention.cu).  Not
-  // split / split, us: 8 sequences on 32 and 8 heads of 128, 16 drafts, 480 tokens 16.5
-  // / 22.6, 750 22.5 / 22.7, 980 26.7 / 24.5.
+  // split / split, us: 8 sequences on 32 and 8 heads of 128, 16 drafts, 480 tokens 16.3
+  // / 21.5, 750 21.3 / 22.6, 980 26.3 / 23.9.
   static constexpr int64_t kWholeTokens = 768;
   static_assert(kWholeTokens / kKeys < kFlush, "no sums in the workspace");
 };
@@ -697,8 +698,8 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
     q_rows = 0;
   const int slot_rows = rows >= K::kRows ? K::kRows : (int)(rows + 15) / 16 * 16;
   // a part of the blocks a launch where they are more than half the CTAs of a wave (a
-  // piece of a prompt, 4096 tokens over 4096, 32 and 8 heads of 128: 1.58 ms; all by the
-  // warps of tree_attention.cu 3.90)
+  // piece of a prompt, 4096 tokens over 4096, 32 and 8 heads of 128: 1.70 ms; all by the
+  // warps of tree_attention.cu 5.02)
   const int launches = a.whole ? 1 : (blocks + ctas / 2 - 1) / (ctas / 2);
   a.blocks = (blocks + launches - 1) / launches;
   const int64_t shares = a.whole ? items : ctas / a.blocks;
@@ -720,8 +721,8 @@ int launch(Launch a, const DeviceInfo& dev, cudaStream_t st) {
 namespace tree {
 
 // From 17 rows on: below, the products on half-empty tiles lose to those of the warps
-// (tree_attention.cu).  Warps / here, us, 32 sequences of 2048 tokens, 32 and 8 heads:
-// of 128, 16 rows 60 / 60, 24 79 / 62, 64 112 / 66; of 64, 16 rows 38 / 45, 24 47 / 45.
+// (tree_attention.cu), or gain little.  Warps / here, us, 32 sequences of 2048 tokens, 32 and 8 heads:
+// of 128, 16 rows 61 / 58, 24 96 / 60, 64 140 / 65; of 64, 16 rows 38 / 47, 24 51 / 47.
 int launch_tc(const TreeAttention& p, const DeviceInfo& dev, cudaStream_t st) {
   const int64_t rows = p.drafts * (p.q_heads / p.kv_heads);
   if (p.act_dtype != p.kv.dtype || p.kv.dtype == CT_DTYPE_F32 || p.head_dim == 32 || rows <= 16 ||
