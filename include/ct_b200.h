@@ -488,7 +488,7 @@ size_t ct_tree_attention_workspace_size(int64_t drafts, int64_t q_heads, int64_t
  * that are not finite reach the rows that see their token, by the formula: a key
  * with a score of -inf has no weight, a score of +inf or NaN makes its row NaN, an
  * infinite value makes its element of O infinite, or NaN where its key has no
- * weight.  (Weights below 2^-120 of the largest may count as none, those over an
+ * weight.  (Weights below 2^-100 of the largest may count as none, those over an
  * f16 cache below 2^-22.)
  * The workspace (16-byte aligned) needs no clearing and must not be used by
  * another call that can run concurrently.  Deterministic.  No reference

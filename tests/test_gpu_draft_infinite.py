@@ -89,3 +89,25 @@ def test_infinite_values(cuda_device, ops, act, cache, dim, n, heads, kv):  # no
     assert out[:, :n // 2, :, 7].isfinite().all() and out[..., dim // 2].isnan().all()
     out[..., [5, 7, dim - 2, dim // 2]] = want[0][..., [5, 7, dim - 2, dim // 2]]
     check(q, k, clean, table, CONTEXTS, [n] * 3, None, PAGE, (out, lse), dim ** -0.5)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("n,heads,kv", SHAPES)
+def test_infinite_values_of_small_weight(cuda_device, ops, act, cache, dim, n, heads, kv):  # noqa: F811
+    """Weights down to 2^-98 of the largest (2^-21 over an f16 cache) still count."""
+    least = -(21 if cache == torch.float16 else 98) * math.log(2)
+    k, v, table, q = infinite_case(act, cache, n, heads, kv, dim, dim)
+    k.zero_()
+    q.zero_()
+    q[..., 3] = 1.0
+    for b, c in enumerate(CONTEXTS):
+        for i in range(min(c - 1, 31)):  # token 1 + i: dim i
+            at = slot(table, b, 1 + i + (c // 2 if c > 60 else 0))
+            k[at][..., 3] = least * (i + 1) / 32
+            v[at][..., i] = math.inf if i % 2 else -math.inf
+    out, lse = ops.tree_attention(q, k, v, table, ints(CONTEXTS), scale=1.0)
+    for b, c in enumerate(CONTEXTS):
+        m = min(c - 1, 31)
+        assert (out[b, ..., 1:m:2] == math.inf).all() and (out[b, ..., 0:m:2] == -math.inf).all()
+        assert out[b, ..., m:].isfinite().all() and lse[b].isfinite().all()
