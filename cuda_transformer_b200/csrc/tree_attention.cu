@@ -176,12 +176,15 @@ __device__ __forceinline__ void mma_next(bool first, float (&c)[4], const uint32
 __device__ __forceinline__ uint32_t low_tf32(uint32_t x) {
   return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)) + 0x1000u;
 }
-// Infinite cached values.  Terms of the weights that share a sum are positive, all of
-// them, so that an infinite value times them is that infinity, not NaN.  Where low terms
-// may be 0 or negative (f16 with FP32 activations) they have a sum of their own, which
-// counts where the first terms' is finite.
+// Infinite cached values.  Terms of a weight that share a sum are positive, all of them
+// (those of a weight of 0 are 0), so that an infinite value times them is that infinity,
+// not NaN.  Where low terms may be 0 or negative (f16 with FP32 activations) they have a
+// sum of their own, which counts where the first terms' is finite.
+__device__ __forceinline__ float positive_rest(float x, float high) {
+  return fmaxf(x - high, fminf(x, FLT_MIN));
+}
 __device__ __forceinline__ uint32_t low_weight(uint32_t x) {
-  return __float_as_uint(fmaxf(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u), FLT_MIN)) + 0x1000u;
+  return __float_as_uint(positive_rest(__uint_as_float(x), __uint_as_float(x & 0xffffe000u))) + 0x1000u;
 }
 __device__ __forceinline__ float with_rest(float first, float rest) {
   return fabsf(first) < INFINITY ? first + rest : first;
@@ -214,8 +217,8 @@ __device__ __forceinline__ uint32_t take_weights(float& x, float& y, int left) {
   uint32_t w;
   if constexpr (K::kBf16) {
     w = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632u);
-    x = fmaxf(x - __uint_as_float(w << 16), FLT_MIN);
-    y = fmaxf(y - __uint_as_float(w & 0xffff0000u), FLT_MIN);
+    x = positive_rest(x, __uint_as_float(w << 16));
+    y = positive_rest(y, __uint_as_float(w & 0xffff0000u));
   } else {
     constexpr float kBelowOne = 1.0f - 0x1p-10f;
     asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y * kBelowOne), "f"(x * kBelowOne));
@@ -796,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, K::kCtas)
                   if constexpr (K::kPack) {  // rows 0-7 and 8-15: two terms
                     const int term = 2 * t + j % 2;  // (of three: the fourth is next to nothing)
                     w[m][ks][t][j] = term >= K::kWTerms
-                                         ? 0x00800080u
+                                         ? __vminu2(w[m][ks][0][j], 0x00800080u)
                                          : take_weights<K>(s[m][2 * ks + j / 2][0],
                                                            s[m][2 * ks + j / 2][1], K::kWTerms - 1 - term);
                   } else {

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from .test_gpu_decode import TYPES, gen, make_cache
-from .test_gpu_draft import check, ints, ops  # noqa: F401
+from .test_gpu_draft import check, ints, ops, pack  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +111,22 @@ def test_infinite_values_of_small_weight(cuda_device, ops, act, cache, dim, n, h
         m = min(c - 1, 31)
         assert (out[b, ..., 1:m:2] == math.inf).all() and (out[b, ..., 0:m:2] == -math.inf).all()
         assert out[b, ..., m:].isfinite().all() and lse[b].isfinite().all()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("n,heads,kv", SHAPES[1:])
+def test_large_values_that_are_not_seen(cuda_device, ops, act, cache, n, heads, kv):  # noqa: F811
+    """The largest numbers of the type, under drafted tokens that only themselves see, and
+    under context tokens whose scores are -inf, leave the other rows bit for bit alone."""
+    k, v, table, q = infinite_case(act, cache, n, heads, kv, 64, 7)
+    bits = torch.eye(n, dtype=torch.bool, device="cuda").repeat(3, 1, 1)
+    bits[:, 1] = False  # row 1 sees the context alone
+    for b, c in enumerate(CONTEXTS):
+        k[slot(table, b, c // 2)][..., 3] = -math.inf
+    want = ops.tree_attention(q, k, v, table, ints(CONTEXTS), mask=pack(bits))
+    for b, c in enumerate(CONTEXTS):
+        v[slot(table, b, c // 2)] = torch.finfo(cache).max
+        for i in range(2, n):
+            v[slot(table, b, c + i)] = torch.finfo(cache).max * (-1) ** (i // 2)
+    out, lse = ops.tree_attention(q, k, v, table, ints(CONTEXTS), mask=pack(bits))
+    assert torch.equal(out[:, :2], want[0][:, :2]) and torch.equal(lse, want[1])
